@@ -175,6 +175,105 @@ int pyc_hip_gelu_dispatch(const char* symbol, size_t n, const void* x, void* y, 
 int pyc_hip_layernorm_dispatch(const char* symbol, int rows, int D, float eps, const void* x, const void* gamma,
                                const void* beta, void* y, void* stream);
 
+/* The paged 8-bit key/value cache (no reference counterpart: the reference
+ * holds no state between runs). A block holds block_size tokens of every kv head:
+ *   k [num_blocks][kv_heads][block_size][head_dim]  e4m3fn codes,
+ *   v [num_blocks][kv_heads][head_dim][block_size]  e4m3fn codes (a channel's
+ *     tokens run on: the operand of the product over tokens, as it is),
+ *   k_scale, v_scale [num_blocks][kv_heads] fp32: an element is code * scale.
+ * A block's codes are dense; k_block_stride and v_block_stride are the bytes
+ * from a block to the next (at least kv_heads * block_size * head_dim, multiples
+ * of 16; k and v on 16-byte boundaries). block_size 16, 32, 64 or 128, head_dim 64
+ * or 128, num_blocks * block_size < 2^31. Slot s is token s % block_size of block
+ * s / block_size. */
+typedef struct {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t k_block_stride;
+    int64_t v_block_stride;
+    int num_blocks;
+    int kv_heads;
+    int block_size;
+    int head_dim;
+} pyc_hip_kv_cache;
+
+/* The plan of one serving step, made on the device from what B requests hold in
+ * the cache (cached[b] tokens, their blocks in table[b][0 ..]) and what they bring
+ * (fresh[b] tokens; negative: the request is over). table is [B][width], rows
+ * table_stride apart; free_list[0 .. free_count[0]) is a stack of free blocks of
+ * room for free_capacity. In order of b:
+ *  - a request that is over pushes its ceil(cached / block_size) blocks;
+ *  - then fresh[b] > 0 is granted if cached + fresh fits the table row and
+ *    needs no new block or the stack holds the new blocks of all that was asked up
+ *    to and with b, and if all tokens asked up to and with b are at most `tokens`
+ *    (what does not fit its row counts as not asked);
+ *  - granted requests pop their new blocks into their table rows.
+ * Outputs: lens[b] = cached + granted (0 when over); q_offsets[B + 1], where each
+ * request's granted tokens begin; for each token its slot and its position in the
+ * request, -1 behind the last one up to `tokens`; free_after[0], the blocks left.
+ * A refused request keeps its length and its blocks, and has no tokens in the step.
+ * Entries of table and free_list that are not pushed or popped stay as they are.
+ * lens may be cached, free_after may be free_count; with neither, the call can be
+ * made again. B >= 1, width >= 1, tokens >= 0, block_size as above,
+ * width * block_size < 2^31. Symbol "hip_kv_plan". 0, -1 (bad argument, nothing
+ * launched), -2 (HIP error). */
+int pyc_hip_kv_plan_dispatch(
+    const char* symbol, int B, int width, int64_t table_stride, int block_size, int tokens,
+    const int32_t* cached, const int32_t* fresh, int32_t* table,
+    int32_t* free_list, int free_capacity, const int32_t* free_count,
+    int32_t* lens, int32_t* q_offsets, int32_t* slots, int32_t* positions, int32_t* free_after,
+    void* stream);
+
+/* Keys and values of a step into the cache: row t of k and v (kv_heads x
+ * head_dim dense, rows k_stride and v_stride elements apart) goes to slot slots[t];
+ * a slot outside the cache (-1) is skipped. For a block and head with new rows, a
+ * their largest finite magnitude and s_new the smallest power of two with a <= 448
+ * s_new, at least 2^-100, its scale becomes
+ *   s_new               where the block's first slot is written: the block
+ *                       starts anew, what it held counts as gone,
+ *   max(old, s_new)     else; codes already there are re-rounded to it (with an
+ *                       old scale that is not finite and positive: s_new, and the
+ *                       codes stay).
+ * code = e4m3(x * (1 / scale)), to nearest even; infinities and NaN become NaN.
+ * The rows of one block have to stand together in slots, as the plan lays them
+ * out, and no slot may come twice; otherwise which of the rows a block keeps is
+ * undefined. k and v on 16-byte boundaries, strides multiples of 8 and at least
+ * kv_heads * head_dim. 0 <= tokens < 2^24. Symbols "hip_kv_append_bf16",
+ * "hip_kv_append_f16". 0, -1, -2 as above. */
+int pyc_hip_kv_append_dispatch(
+    const char* symbol, const pyc_hip_kv_cache* cache, int tokens,
+    const void* k, int64_t k_stride, const void* v, int64_t v_stride, const int32_t* slots,
+    void* stream);
+
+/* Attention of a step's tokens over the cache. Request b has rows q_offsets[b] ..
+ * q_offsets[b + 1] - 1 of q and o (q_heads x head_dim dense, rows q_stride and
+ * o_stride elements apart) and lens[b] tokens in the blocks table[b][..], the
+ * step's own last among them; with n rows, row i sees keys j <= lens[b] - n + i:
+ *   o = sum_j softmax_j(scale q.k_j) v_j,  head h reading kv head h / (q_heads / kv_heads).
+ * One token each is decoding; more are draft tokens or a prompt chunk; a batch may
+ * mix them. fp32 softmax and sums. A row without a key
+ * (or with -infinity for every score) is zero; keys of a block id outside the cache
+ * count as absent; rows outside every request stay as they are.
+ * max_q: no request has more rows (what is past it is left); max_len: the longest
+ * of lens if known, else 0 (how the work is split goes by it, results do not but for
+ * the order of sums). workspace: pyc_hip_kv_attention_workspace bytes on a 16-byte
+ * boundary, zero before its first call and left zeroed where that matters: for one
+ * call at a time (calls that may overlap need one each). q_heads a multiple of
+ * kv_heads; q, o on 16-byte boundaries, strides multiples of 8, o overlapping
+ * nothing. 0 <= tokens < 2^24. Symbols "hip_kv_attention_bf16",
+ * "hip_kv_attention_f16". 0, -1, -2 as above. */
+int pyc_hip_kv_attention_dispatch(
+    const char* symbol, const pyc_hip_kv_cache* cache, int B, int tokens, int q_heads, int max_q, int max_len,
+    const void* q, int64_t q_stride, const int32_t* table, int64_t table_stride, int width,
+    const int32_t* lens, const int32_t* q_offsets, void* o, int64_t o_stride, float scale,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that a call of up to B requests and max_q rows each needs
+ * (0: bad arguments). Host only. */
+size_t pyc_hip_kv_attention_workspace(int B, int q_heads, int kv_heads, int head_dim, int max_q);
+
 /* Device properties the bench and the registry report. */
 typedef struct {
     char gcn_arch[64];       /* e.g. "gfx950:sramecc+:xnack-" */
@@ -225,7 +324,7 @@ int pyc_hip_kernel_resources_query(const char* symbol, pyc_hip_kernel_resources*
 
 /* Number of kernel symbols compiled into this library for op_key
  * ("matmul", "attention", "conv2d", "matmul_w8a16", "matmul_w8a16_chain",
- * "gelu", "layernorm"), independent of the
+ * "gelu", "layernorm", "kv_plan", "kv_append", "kv_attention"), independent of the
  * registry's state. */
 int pyc_hip_kernel_symbol_count(const char* op_key);
 

@@ -57,6 +57,15 @@ def _declare(L: C.CDLL) -> None:
     L.pyc_hip_gelu_dispatch.restype = I
     L.pyc_hip_layernorm_dispatch.argtypes = [S, I, I, F, P, P, P, P, P]
     L.pyc_hip_layernorm_dispatch.restype = I
+    I64 = C.c_int64
+    L.pyc_hip_kv_plan_dispatch.argtypes = [S, I, I, I64, I, I, P, P, P, P, I, P, P, P, P, P, P, P]
+    L.pyc_hip_kv_plan_dispatch.restype = I
+    L.pyc_hip_kv_append_dispatch.argtypes = [S, P, I, P, I64, P, I64, P, P]
+    L.pyc_hip_kv_append_dispatch.restype = I
+    L.pyc_hip_kv_attention_dispatch.argtypes = [S, P, I, I, I, I, I, P, I64, P, I64, I, P, P, P, I64, F, P, Z, P]
+    L.pyc_hip_kv_attention_dispatch.restype = I
+    L.pyc_hip_kv_attention_workspace.argtypes = [I, I, I, I, I]
+    L.pyc_hip_kv_attention_workspace.restype = Z
     L.pyc_hip_device_query.argtypes = [C.POINTER(abi.DeviceInfo)]
     L.pyc_hip_device_query.restype = I
     L.pyc_hip_kernel_resources_query.argtypes = [S, C.POINTER(abi.KernelResources)]
@@ -250,6 +259,153 @@ def layernorm(x, y, gamma=None, beta=None, eps: float = 1e-5, stream=None) -> No
                                             _ptr(x), _ptr(gamma) if gamma is not None else None,
                                             _ptr(beta) if beta is not None else None, _ptr(y),
                                             _stream(stream)), "layernorm")
+
+
+class KvCache:
+    """The paged 8-bit key/value cache over four tensors of the caller: k
+    [blocks, kv heads, block size, head dim] and v [blocks, kv heads, head dim,
+    block size], e4m3 codes as uint8 (or float8_e4m3fn), k_scale and v_scale
+    [blocks, kv heads] float32. Blocks may lie apart (stride 0 of k and v); each
+    is dense. Holds the tensors, allocates nothing."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+        if k.dim() != 4 or v.dim() != 4 or tuple(v.shape) != (k.shape[0], k.shape[1], k.shape[3], k.shape[2]):
+            raise PycError(f"kv cache: k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+        blocks, heads, size, dim = k.shape
+        for t in (k, v):
+            if t.dtype not in (torch.uint8, torch.float8_e4m3fn) or (blocks > 0 and not t[0].is_contiguous()):
+                raise PycError("kv cache: k and v are e4m3 codes with dense blocks")
+        for t in (k_scale, v_scale):
+            if t.dtype != torch.float32 or tuple(t.shape) != (blocks, heads) or not t.is_contiguous():
+                raise PycError("kv cache: the scales are dense float32 [blocks, kv heads]")
+        if len({t.device for t in (k, v, k_scale, v_scale)}) != 1:
+            raise PycError("kv cache: its tensors are on different devices")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = k.get_device()
+        self.kv_heads, self.block_size, self.head_dim = heads, size, dim
+        self.struct = abi.KvCache(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), k.stride(0) if blocks > 1 else k.numel(),
+                                  v.stride(0) if blocks > 1 else v.numel(), blocks, heads, size, dim)
+        self.ref = C.addressof(self.struct)
+
+
+def _kv_ints(what: str, device: int, *tensors) -> None:
+    """Refuses index tensors that the kernels would read as something else."""
+    import torch
+    for t in tensors:
+        if t.dtype is not torch.int32 or t.get_device() != device or not t.is_contiguous():
+            raise PycError(f"{what}: index tensors are dense int32 on the call's device")
+
+
+def _kv_table(what: str, device: int, table) -> None:
+    import torch
+    if table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != device or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise PycError(f"{what}: the block table is int32 [requests, width] with dense rows, on the call's device")
+
+
+def _kv_device(what: str, device: int) -> None:
+    import torch
+    if device < 0 or device != torch.cuda.current_device():
+        raise PycError(f"{what}: the tensors are not on the current device")
+
+
+def _kv_rows(what: str, t, cache: KvCache, heads: int) -> str:
+    """Checks [tokens, heads, head dim] rows; the symbol's suffix of their type."""
+    import torch
+    suffix = {torch.bfloat16: "bf16", torch.float16: "f16"}.get(t.dtype)
+    if suffix is None or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.head_dim or \
+            t.get_device() != cache.device or t.stride(2) != 1 or (heads > 1 and t.stride(1) != cache.head_dim):
+        raise PycError(f"{what}: rows are bf16 or f16 [tokens, {heads}, {cache.head_dim}] with dense heads, on the "
+                       "cache's device")
+    return suffix
+
+
+def _kv_row_stride(t) -> int:
+    return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1] * t.shape[2])
+
+
+def kv_plan(cached, fresh, table, free_list, free_count, block_size: int, lens, q_offsets, slots, positions,
+            free_after, stream=None) -> None:
+    """The plan of one serving step (pyc_hip_kv_plan_dispatch): cached, fresh
+    [B] (a negative fresh ends its request), table [B, width], the stack of free
+    blocks free_list with free_count [1]; writes lens [B], q_offsets [B + 1], slots
+    and positions [tokens], free_after [1]. All int32. lens may be cached and
+    free_after may be free_count."""
+    B, device = cached.shape[0], cached.get_device()
+    _kv_device("kv plan", device)
+    _kv_table("kv plan", device, table)
+    _kv_ints("kv plan", device, cached, fresh, free_list, free_count, lens, q_offsets, slots, positions, free_after)
+    if fresh.numel() != B or table.shape[0] != B or lens.numel() != B or q_offsets.numel() != B + 1 or \
+            slots.numel() != positions.numel() or free_count.numel() != 1 or free_after.numel() != 1:
+        raise PycError("kv plan: sizes do not match")
+    _check(lib().pyc_hip_kv_plan_dispatch(b"hip_kv_plan", B, table.shape[1], table.stride(0) if B > 1 else table.shape[1],
+                                          block_size, slots.numel(), _ptr(cached), _ptr(fresh), _ptr(table),
+                                          _ptr(free_list), free_list.numel(), _ptr(free_count), _ptr(lens),
+                                          _ptr(q_offsets), _ptr(slots), _ptr(positions), _ptr(free_after),
+                                          _stream(stream)), "kv plan")
+
+
+def kv_append(k, v, slots, cache: KvCache, stream=None) -> None:
+    """A step's keys and values [tokens, kv heads, head dim] (rows may be parts of
+    wider ones) into the cache's slots (pyc_hip_kv_append_dispatch); slots [tokens]
+    int32, -1: skipped."""
+    suffix = _kv_rows("kv append", k, cache, cache.kv_heads)
+    if _kv_rows("kv append", v, cache, cache.kv_heads) != suffix or v.shape[0] != k.shape[0] or \
+            slots.numel() != k.shape[0]:
+        raise PycError("kv append: k, v and slots do not match")
+    _kv_device("kv append", cache.device)
+    _kv_ints("kv append", cache.device, slots)
+    _check(lib().pyc_hip_kv_append_dispatch(_b("hip_kv_append_" + suffix), cache.ref, k.shape[0], _ptr(k),
+                                            _kv_row_stride(k), _ptr(v), _kv_row_stride(v), _ptr(slots),
+                                            _stream(stream)), "kv append")
+
+
+def kv_attention_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int, max_q: int):
+    """A zeroed workspace for kv_attention calls of up to `batch` requests with up
+    to max_q tokens each, on the current device; for one call at a time."""
+    import torch
+    n = lib().pyc_hip_kv_attention_workspace(batch, q_heads, kv_heads, head_dim, max_q)
+    if n == 0:
+        raise PycError("kv attention workspace: bad sizes")
+    return torch.zeros(n, dtype=torch.uint8, device="cuda")
+
+
+def kv_attention(q, cache: KvCache, table, lens, q_offsets, o, scale: float, max_q: int, max_len: int = 0,
+                 workspace=None, stream=None) -> None:
+    """o = attention of the rows q [tokens, q heads, head dim] over the cache
+    (pyc_hip_kv_attention_dispatch): table [B, width], lens [B] and q_offsets [B + 1]
+    as kv_plan leaves them; max_q: no request has more tokens in the step; max_len: the
+    longest of lens, if known. Without a workspace (kv_attention_workspace) one is
+    made for the call."""
+    tokens, heads = q.shape[0], q.shape[1]
+    suffix = _kv_rows("kv attention", q, cache, heads)
+    if _kv_rows("kv attention", o, cache, heads) != suffix or o.shape[0] != tokens:
+        raise PycError("kv attention: q and o do not match")
+    B, device = lens.shape[0], cache.device
+    _kv_device("kv attention", device)
+    _kv_table("kv attention", device, table)
+    _kv_ints("kv attention", device, lens, q_offsets)
+    if table.shape[0] != B or q_offsets.numel() != B + 1:
+        raise PycError("kv attention: table, lens and q_offsets do not match")
+    if B == 0 or tokens == 0:
+        return
+    at = _stream(stream)
+    if workspace is None:
+        import contextlib
+
+        import torch
+        # made and cleared on the call's stream, so that it is other work's only after the call
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(torch.cuda.ExternalStream(at)):
+            workspace = kv_attention_workspace(B, heads, cache.kv_heads, cache.head_dim, max_q)
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        raise PycError("kv attention: the workspace is dense, on the cache's device")
+    _check(lib().pyc_hip_kv_attention_dispatch(_b("hip_kv_attention_" + suffix), cache.ref, B, tokens, heads, max_q,
+                                               max_len, _ptr(q), _kv_row_stride(q), _ptr(table),
+                                               table.stride(0) if B > 1 else table.shape[1], table.shape[1],
+                                               _ptr(lens), _ptr(q_offsets), _ptr(o), _kv_row_stride(o), scale,
+                                               _ptr(workspace), workspace.numel() * workspace.element_size(), at),
+           "kv attention")
 
 
 def device_info() -> abi.DeviceInfo:

@@ -274,6 +274,22 @@ class KernelResources(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    """pyc_hip_kv_cache (pyc/hip_backend.h)."""
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("k_block_stride", C.c_int64),
+        ("v_block_stride", C.c_int64),
+        ("num_blocks", C.c_int),
+        ("kv_heads", C.c_int),
+        ("block_size", C.c_int),
+        ("head_dim", C.c_int),
+    ]
+
+
 CPU_EXECUTOR_FN = C.CFUNCTYPE(C.c_int, C.POINTER(IrModule), C.POINTER(Tensor), C.c_size_t,
                               C.POINTER(Tensor), C.c_size_t, C.c_void_p)
 

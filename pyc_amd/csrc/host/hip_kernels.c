@@ -64,10 +64,22 @@ int pyc_hip_w8a16_chain_launch_noalloc(int M, int nsteps, const void* X, const v
 int pyc_hip_gelu_launch(int dtype, size_t n, const void* x, void* y, void* stream);
 int pyc_hip_layernorm_launch(int dtype, int rows, int D, float eps, const void* x, const void* gamma,
                              const void* beta, void* y, void* stream);
+int pyc_hip_kv_plan_launch(int B, int width, int64_t table_stride, int bs, int tokens, const int32_t* cached,
+                           const int32_t* fresh, int32_t* table, int32_t* free_list, int free_cap,
+                           const int32_t* free_count, int32_t* lens, int32_t* q_offsets, int32_t* slots,
+                           int32_t* positions, int32_t* free_after, void* stream);
+int pyc_hip_kv_append_launch(int is_bf16, const pyc_hip_kv_cache* cache, int tokens, const void* k, int64_t k_stride,
+                             const void* v, int64_t v_stride, const int32_t* slots, void* stream);
+size_t pyc_hip_kv_attention_workspace_bytes(int B, int hq, int hk, int d, int max_q);
+int pyc_hip_kv_attention_launch(int is_bf16, const pyc_hip_kv_cache* cache, int B, int tokens, int hq, int max_q,
+                                int max_len, const void* q, int64_t q_stride, const int32_t* table,
+                                int64_t table_stride, int width, const int32_t* lens, const int32_t* q_offsets,
+                                void* o, int64_t o_stride, float scale, void* workspace, void* stream);
 
 /* ---------------------------------------------------------------- variant table */
 
-enum { VK_GEMM = 1, VK_ATTN = 2, VK_CONV = 3, VK_W8 = 4, VK_ELT = 5, VK_CHAIN = 6 };
+enum { VK_GEMM = 1, VK_ATTN = 2, VK_CONV = 3, VK_W8 = 4, VK_ELT = 5, VK_CHAIN = 6, VK_KV_PLAN = 7, VK_KV_APPEND = 8,
+       VK_KV_ATTN = 9 };
 enum { VT_BF16 = 1, VT_F16 = 2, VT_F32 = 3 };
 /* conv2d paths (hip_variant.tile of a VK_CONV entry) */
 enum { CONV_AUTO = 0, CONV_PERSIST = -1, CONV_TILED = 1 };
@@ -136,6 +148,12 @@ static const hip_variant k_variants[] = {
     {"layernorm", "hip_layernorm_f32", VK_ELT, VT_F32, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
     {"layernorm", "hip_layernorm_bf16", VK_ELT, VT_BF16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
     {"layernorm", "hip_layernorm_f16", VK_ELT, VT_F16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    /* the paged 8-bit key/value cache (no reference counterpart) */
+    {"kv_plan", "hip_kv_plan", VK_KV_PLAN, VT_F32, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    {"kv_append", "hip_kv_append_bf16", VK_KV_APPEND, VT_BF16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    {"kv_append", "hip_kv_append_f16", VK_KV_APPEND, VT_F16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    {"kv_attention", "hip_kv_attention_bf16", VK_KV_ATTN, VT_BF16, 0, 0, 0, 100, 3, PYC_KERNEL_WORKLOAD_ANY},
+    {"kv_attention", "hip_kv_attention_f16", VK_KV_ATTN, VT_F16, 0, 0, 0, 100, 3, PYC_KERNEL_WORKLOAD_ANY},
 };
 
 #define N_VARIANTS (sizeof(k_variants) / sizeof(k_variants[0]))
@@ -172,6 +190,12 @@ static int variant_kinfo(const hip_variant* v, pyc_hip_kinfo* ki) {
         case VK_ELT:
             return pyc_hip_kinfo_eltwise(strcmp(v->op_key, "gelu") == 0 ? 0 : 1,
                                          v->dtype == VT_F32 ? 0 : bf ? 1 : 2, ki);
+        case VK_KV_PLAN:
+            return pyc_hip_kinfo_kv_plan(ki);
+        case VK_KV_APPEND:
+            return pyc_hip_kinfo_kv_append(bf, ki);
+        case VK_KV_ATTN:
+            return pyc_hip_kinfo_kv_attention(bf, ki);
         default:
             return -1;
     }
@@ -658,6 +682,102 @@ int pyc_hip_layernorm_dispatch(const char* symbol, int rows, int D, float eps, c
     return pyc_hip_layernorm_launch(elt_dtype(v), rows, D, eps, x, gamma, beta, y, stream);
 }
 
+/* ---------------------------------------------------------------- paged 8-bit key/value cache */
+
+#define KV_MAX_TOKENS (1 << 24)
+
+static int kv_block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128; }
+
+static int kv_cache_ok(const pyc_hip_kv_cache* c) {
+    int64_t dense;
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || c->num_blocks <= 0 || c->kv_heads <= 0 ||
+        c->kv_heads > 65535 || !kv_block_size_ok(c->block_size) || (c->head_dim != 64 && c->head_dim != 128)) {
+        return 0;
+    }
+    if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) != 0 || (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) != 0) {
+        return 0;
+    }
+    dense = (int64_t)c->kv_heads * c->block_size * c->head_dim;
+    if (c->k_block_stride < dense || c->v_block_stride < dense || ((c->k_block_stride | c->v_block_stride) & 15) != 0) {
+        return 0;
+    }
+    return (int64_t)c->num_blocks * c->block_size <= 0x7FFFFFFFLL;
+}
+
+/* Rows of `heads` x `d` half elements that the kernels read and write 16 bytes at a time. */
+static int kv_rows_ok(const void* p, int64_t stride, int heads, int d) {
+    return p && ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && stride >= (int64_t)heads * d;
+}
+
+int pyc_hip_kv_plan_dispatch(const char* symbol, int B, int width, int64_t table_stride, int block_size, int tokens,
+                             const int32_t* cached, const int32_t* fresh, int32_t* table, int32_t* free_list,
+                             int free_capacity, const int32_t* free_count, int32_t* lens, int32_t* q_offsets,
+                             int32_t* slots, int32_t* positions, int32_t* free_after, void* stream) {
+    if (!find_variant(symbol, VK_KV_PLAN) || B <= 0 || width <= 0 || table_stride < width || tokens < 0 ||
+        free_capacity < 0 || !kv_block_size_ok(block_size) || (int64_t)width * block_size > 0x7FFFFFFFLL) {
+        return -1;
+    }
+    if (!cached || !fresh || !table || (free_capacity > 0 && !free_list) || !free_count || !lens || !q_offsets ||
+        (tokens > 0 && (!slots || !positions)) || !free_after) {
+        return -1;
+    }
+    return pyc_hip_kv_plan_launch(B, width, table_stride, block_size, tokens, cached, fresh, table, free_list,
+                                  free_capacity, free_count, lens, q_offsets, slots, positions, free_after, stream);
+}
+
+int pyc_hip_kv_append_dispatch(const char* symbol, const pyc_hip_kv_cache* cache, int tokens, const void* k,
+                               int64_t k_stride, const void* v, int64_t v_stride, const int32_t* slots,
+                               void* stream) {
+    const hip_variant* var = find_variant(symbol, VK_KV_APPEND);
+    if (!var || !kv_cache_ok(cache) || tokens < 0 || tokens >= KV_MAX_TOKENS) {
+        return -1;
+    }
+    if (tokens == 0) {
+        return 0;
+    }
+    if (!slots || !kv_rows_ok(k, k_stride, cache->kv_heads, cache->head_dim) ||
+        !kv_rows_ok(v, v_stride, cache->kv_heads, cache->head_dim)) {
+        return -1;
+    }
+    return pyc_hip_kv_append_launch(var->dtype == VT_BF16, cache, tokens, k, k_stride, v, v_stride, slots, stream);
+}
+
+size_t pyc_hip_kv_attention_workspace(int B, int q_heads, int kv_heads, int head_dim, int max_q) {
+    if (B <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128) ||
+        max_q <= 0 || max_q >= KV_MAX_TOKENS || (int64_t)B * q_heads > 0x7FFFFFFFLL) {
+        return 0;
+    }
+    return pyc_hip_kv_attention_workspace_bytes(B, q_heads, kv_heads, head_dim, max_q);
+}
+
+int pyc_hip_kv_attention_dispatch(const char* symbol, const pyc_hip_kv_cache* cache, int B, int tokens, int q_heads,
+                                  int max_q, int max_len, const void* q, int64_t q_stride, const int32_t* table,
+                                  int64_t table_stride, int width, const int32_t* lens, const int32_t* q_offsets,
+                                  void* o, int64_t o_stride, float scale, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    const hip_variant* var = find_variant(symbol, VK_KV_ATTN);
+    size_t need;
+    if (!var || !kv_cache_ok(cache) || B < 0 || tokens < 0 || tokens >= KV_MAX_TOKENS || q_heads <= 0 ||
+        q_heads % cache->kv_heads != 0 || max_len < 0) {
+        return -1;
+    }
+    if (B == 0 || tokens == 0) {
+        return 0;
+    }
+    need = pyc_hip_kv_attention_workspace(B, q_heads, cache->kv_heads, cache->head_dim, max_q);
+    if (need == 0 || !workspace || ((uintptr_t)workspace & 15) != 0 || workspace_bytes < need) {
+        return -1;
+    }
+    if (!table || width <= 0 || table_stride < width || (int64_t)width * cache->block_size > 0x7FFFFFFFLL || !lens ||
+        !q_offsets || !(scale == scale) || !kv_rows_ok(q, q_stride, q_heads, cache->head_dim) ||
+        !kv_rows_ok(o, o_stride, q_heads, cache->head_dim)) {
+        return -1;
+    }
+    return pyc_hip_kv_attention_launch(var->dtype == VT_BF16, cache, B, tokens, q_heads, max_q, max_len, q, q_stride,
+                                       table, table_stride, width, lens, q_offsets, o, o_stride, scale, workspace,
+                                       stream);
+}
+
 /* ---------------------------------------------------------------- registry */
 
 static pyc_mutex g_registry_init_lock = PYC_MUTEX_INIT;
@@ -689,7 +809,8 @@ void pyc_cutlass_registry_init(void) {
                 d.estimated_occupancy = (double)ki.waves_per_simd / 8.0;
                 d.shared_mem_bytes = ki.lds_bytes;
             }
-            d.tensor_core_eligible = v->kind != VK_ELT;  /* GELU/LayerNorm: VALU only */
+            /* GELU/LayerNorm and the cache's plan and append: VALU only */
+            d.tensor_core_eligible = v->kind != VK_ELT && v->kind != VK_KV_PLAN && v->kind != VK_KV_APPEND;
             d.reg_pressure_class = v->reg_class;
             d.preferred_workload_family = v->workload;
             d.preferred_hardware_family = PYC_KERNEL_HARDWARE_CDNA4;

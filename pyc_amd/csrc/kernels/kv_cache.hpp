@@ -1,0 +1,45 @@
+// kv_cache.hpp — the paged 8-bit key/value cache as its kernels see it.
+//
+// Keys   [blocks][kv heads][bs][D]  e4m3: a token's D codes run on.
+// Values [blocks][kv heads][D][bs]  e4m3: a channel's tokens run on, so that 16
+// tokens of one channel are one 16-byte load and, as they are, the operand
+// of O^T = V^T P^T: the product over tokens needs no transposition anywhere.
+// Scales [blocks][kv heads] fp32, one for keys and one for values.
+#pragma once
+
+#include "common.hpp"
+#include "pyc/ir.h"
+#include "pyc/hip_backend.h"
+
+namespace pyc {
+
+struct KvCache {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t k_stride, v_stride;  // bytes from a block to the next
+    int blocks, heads, bs, d;
+};
+
+inline KvCache kv_cache_of(const pyc_hip_kv_cache* c) {
+    return KvCache{(uint8_t*)c->k,    (uint8_t*)c->v,    c->k_scale,    c->v_scale,  c->k_block_stride,
+                   c->v_block_stride, c->num_blocks, c->kv_heads, c->block_size, c->head_dim};
+}
+
+// e4m3 to bf16 or f16, two codes a conversion, both exact (4 significant bits,
+// exponents -9 .. 8); 8 codes in two words.
+__device__ inline u32x4 fp8x8_to_half8(uint32_t lo, uint32_t hi, bf16_t) {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
+}
+__device__ inline u32x4 fp8x8_to_half8(uint32_t lo, uint32_t hi, f16_t) {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true))};
+}
+
+}  // namespace pyc

@@ -1,0 +1,311 @@
+"""GPU: attention over the paged 8-bit cache (pyc_hip_kv_attention_dispatch)
+against kv_util.attention_ref in 64 bits. An output may be off by what
+attention_ref derives (scores, sums and the rounding of P) plus half a step of the
+output's type; f16's step does not go below 2^-24."""
+import numpy as np
+import pytest
+
+import pyc_amd
+from tests import kv_util
+from tests.kv_util import DT, HALF
+
+pytestmark = pytest.mark.gpu
+
+
+def _tables(lens, bs, blocks, seed, width=None):
+    r = np.random.default_rng(seed)
+    ids = r.permutation(blocks)
+    need = [kv_util.ceil_div(n, bs) for n in lens]
+    width = width or max(max(need), 1)
+    t = np.full((len(lens), width), -1, np.int64)  # what is not a request's is no block
+    at = 0
+    for b, n in enumerate(need):
+        t[b, :n] = ids[at:at + n]
+        at += n
+    return t
+
+
+class Call:
+    """A batch: lens (the step's tokens among them), counts of tokens."""
+
+    def __init__(self, torch, dtype, hq, hk, d, bs, lens, counts, seed=0, gain=1.0, blocks=None, width=None):
+        self.torch, self.dtype, self.d = torch, dtype, d
+        need = sum(kv_util.ceil_div(n, bs) for n in lens)
+        self.blocks = blocks or need + 1
+        self.cache = kv_util.random_cache(self.blocks, hk, bs, d, seed + 1)
+        self.table = torch.from_numpy(_tables(lens, bs, self.blocks, seed, width)).to(torch.int32)
+        self.lens = torch.tensor(lens, dtype=torch.int32)
+        self.offsets = torch.tensor([0] + np.cumsum(counts).tolist(), dtype=torch.int32)
+        self.max_q = max(max(counts), 1)
+        g = torch.Generator().manual_seed(seed + 2)
+        self.q = (torch.randn((max(int(sum(counts)), 1), hq, d), generator=g) * gain).to(DT[dtype])
+        self.scale = d ** -0.5
+
+    def handle(self):
+        return pyc_amd.KvCache(*(self.cache[n].cuda() for n in ("k", "v", "k_scale", "v_scale")))
+
+    def run(self, max_len=0, max_q=None, fill=7.0, workspace=None):
+        torch = self.torch
+        o = torch.full(self.q.shape, fill, dtype=self.q.dtype, device="cuda")
+        pyc_amd.kv_attention(self.q.cuda(), self.handle(), self.table.cuda(), self.lens.cuda(), self.offsets.cuda(), o,
+                             self.scale, max_q or self.max_q, max_len=max_len, workspace=workspace)
+        torch.cuda.synchronize()
+        return o.cpu()
+
+    def check(self, got, max_q=1 << 30, fill=7.0):
+        torch = self.torch
+        ref, bound, done = kv_util.attention_ref(self.q, self.cache, self.table, self.lens, self.offsets, self.scale, max_q,
+                                                 torch.full(self.q.shape, fill))
+        g = got.double()
+        same_nan = torch.equal(torch.isnan(g), torch.isnan(ref))
+        assert same_nan, "NaN in other places"
+        room = bound * (1 + HALF[self.dtype]) + HALF[self.dtype] * ref.abs() + 2.0 ** -24
+        off = torch.where(torch.isnan(ref), torch.zeros_like(ref), (g - ref).abs() - room)
+        assert bool((off <= 0).all()), (float(off.max()), int((off > 0).sum()))
+        left = torch.equal(got[~done], torch.full_like(got, fill)[~done])
+        assert left, "rows of nobody were written"
+        return ref
+
+    def go(self, **kw):
+        got = self.run(**kw)
+        self.check(got, kw.get("max_q") or 1 << 30)
+        return got
+
+
+HEADS = [(1, 1), (4, 4), (8, 2), (32, 8), (12, 12), (16, 1), (40, 8), (24, 1)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hk", HEADS)
+def test_single_tokens(gpu, dtype, d, hq, hk):
+    """Decoding: lengths around 0, a chunk of 16, a tile of 64 and a block."""
+    lens = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 200, 0, 513]
+    Call(gpu, dtype, hq, hk, d, 16 if d == 128 else 32, lens, [1] * len(lens), seed=hq).go()
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64, 128])
+@pytest.mark.parametrize("d", [64, 128])
+def test_blocks(gpu, bs, d):
+    lens = [bs - 1, bs, bs + 1, 3 * bs + 7, 70, 1000]
+    Call(gpu, "bf16", 8, 2, d, bs, lens, [1] * 6, seed=bs, width=90).go()
+    Call(gpu, "f16", 8, 2, d, bs, lens, [3, 1, 5, 2, 4, 7], seed=bs).go()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (4, 4, 64), (16, 1, 64), (5, 5, 128)])
+@pytest.mark.parametrize("n", [2, 3, 4, 5, 8, 15, 16, 17, 33])
+def test_draft_tokens(gpu, dtype, hq, hk, d, n):
+    """A few tokens a request: rows of several tokens and heads share a tile."""
+    lens = [n, n + 1, 64, 65 + n, 300, 129]
+    counts = [n, max(1, n - 1), 1, n, n, max(1, n // 2)]
+    Call(gpu, dtype, hq, hk, d, 16, lens, counts, seed=n).go()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,d,bs", [(8, 2, 128, 16), (4, 4, 64, 64), (6, 2, 128, 32), (8, 1, 64, 128)])
+def test_prompt_chunks(gpu, dtype, hq, hk, d, bs):
+    """Chunks of prompts, with and without a cached beginning, whose rows and keys
+    end inside tiles, beside requests that bring one token or none."""
+    lens = [100, 257, 500, 128, 333, 64, 90]
+    counts = [100, 130, 67, 128, 1, 64, 0]
+    Call(gpu, dtype, hq, hk, d, bs, lens, counts, seed=bs).go()
+
+
+def test_long_chunk(gpu):
+    Call(gpu, "bf16", 8, 2, 128, 16, [1500, 900], [700, 513], seed=3).go()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_long_axis(gpu, dtype):
+    """Few rows over long contexts: the work is split along the keys."""
+    for hint in (0, 20001):
+        Call(gpu, dtype, 8, 2, 128, 64, [20001, 3, 9000], [1, 1, 2], seed=5, width=400).go(max_len=hint)
+
+
+@pytest.mark.parametrize("hint", [0, 1, 100, 5000, 1 << 30])
+def test_hint_is_only_a_hint(gpu, hint):
+    Call(gpu, "bf16", 8, 2, 128, 16, [5000, 17, 800], [1, 1, 1], seed=6).go(max_len=hint)
+
+
+def test_many_requests(gpu):
+    r = np.random.default_rng(0)
+    lens = r.integers(0, 150, 700).tolist()
+    Call(gpu, "bf16", 2, 1, 64, 16, lens, [1] * 700, seed=7).go()
+
+
+@pytest.mark.parametrize("gain", [0.01, 8.0, 40.0])
+def test_flat_and_peaked(gpu, gain):
+    """Scores from almost equal to a single key taking all."""
+    for dtype in ("bf16", "f16"):
+        Call(gpu, dtype, 8, 2, 128, 16, [777, 90], [1, 40], seed=8, gain=gain).go()
+
+
+def test_rows_without_keys(gpu):
+    """More tokens than keys: the first rows see nothing and are zero; a request
+    without keys, rows between and behind requests."""
+    torch = gpu
+    c = Call(torch, "bf16", 4, 2, 64, 16, [3, 0, 40, 0], [5, 2, 1, 70], seed=9)
+    c.go()
+    c = Call(torch, "bf16", 4, 2, 64, 16, [30, 0, 40], [5, 2, 1], seed=9)
+    c.q = torch.cat([c.q, c.q])  # rows behind the last request
+    c.go()
+
+
+def test_rows_past_max_q(gpu):
+    """max_q smaller than a request's tokens: its first rows as ever, the others left."""
+    c = Call(gpu, "bf16", 8, 2, 128, 16, [100, 60], [9, 3], seed=10)
+    c.go(max_q=4)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [6, 1, 20], [40, 90, 3]])
+def test_garbage_in_masked_places(gpu, dtype, counts):
+    """NaN codes behind a request's last token, NaN and infinite scales and NaN
+    codes in blocks that are nobody's: no trace of them."""
+    torch = gpu
+    lens = [70, 100, 45]
+    c = Call(torch, dtype, 8, 2, 64, 32, lens, counts, seed=11, blocks=20)
+    c.go()
+    used = set()
+    for b, n in enumerate(lens):
+        ids = c.table[b, :kv_util.ceil_div(n, 32)].tolist()
+        used |= set(ids)
+        c.cache["k"][ids[-1], :, n % 32 or 32:, :] = 0x7F
+        c.cache["v"][ids[-1], :, :, n % 32 or 32:] = 0xFF
+    for i in set(range(20)) - used:
+        c.cache["k"][i], c.cache["v"][i] = 0x7F, 0x7F
+        c.cache["k_scale"][i], c.cache["v_scale"][i] = float("nan"), float("inf")
+    c.go()
+
+
+@pytest.mark.parametrize("counts", [[3, 5], [40, 70]])
+def test_nan_that_some_rows_see(gpu, counts):
+    """A NaN code of a value among the step's own tokens: NaN in that channel for
+    the rows that see the token, nothing for the rows before it; a NaN key makes
+    its rows NaN."""
+    torch = gpu
+    lens = [80, 130]
+    c = Call(torch, "bf16", 4, 2, 64, 16, lens, counts, seed=12)
+    at = lens[0] - counts[0] + 1  # the second token of the first request
+    c.cache["v"][c.table[0, at // 16], 1, 5, at % 16] = 0x7F
+    ref = c.check(c.run())
+    assert bool(torch.isnan(ref[1:counts[0], 2:, 5]).all()) and not bool(torch.isnan(ref[0]).any())
+    at = lens[1] - counts[1] + 2
+    c.cache["k"][c.table[1, at // 16], 0, at % 16, 7] = 0x7F
+    ref = c.check(c.run())
+    first = counts[0]
+    assert bool(torch.isnan(ref[first + 2:, :2]).all()) and not bool(torch.isnan(ref[first:first + 2]).any())
+
+
+def test_nan_query(gpu):
+    """A NaN in one row of q stays in that row and head."""
+    torch = gpu
+    c = Call(torch, "bf16", 8, 2, 64, 16, [50, 60], [1, 9], seed=13)
+    c.q[4, 3, 9] = float("nan")
+    ref = c.check(c.run())
+    assert int(torch.isnan(ref).sum()) == 64
+
+
+def test_blocks_outside_the_cache(gpu):
+    """Ids outside the cache: their keys count as absent; with none left, zero."""
+    torch = gpu
+    c = Call(torch, "bf16", 8, 2, 64, 16, [80, 40, 16], [1, 2, 1], seed=14)
+    c.table[0, 1], c.table[0, 4], c.table[1, 0], c.table[2, 0] = -1, c.blocks, 1 << 30, -(1 << 31)
+    c.go()
+
+
+def test_lengths_outside_the_table(gpu):
+    """A length past the table's row is the row's, a negative one nothing; offsets
+    past the rows of q end with them."""
+    torch = gpu
+    c = Call(torch, "bf16", 4, 1, 64, 16, [48, 20, 33], [1, 1, 1], seed=15)
+    c.table[0] = torch.tensor([0, 1, 2], dtype=torch.int32)
+    c.lens[0], c.lens[1] = 5000, -3
+    c.go()
+    o = torch.full(c.q.shape, 7.0, dtype=c.q.dtype, device="cuda")
+    pyc_amd.kv_attention(c.q.cuda(), c.handle(), c.table.cuda(), c.lens.cuda(),
+                         torch.tensor([-5, 2, 1000, 900], dtype=torch.int32).cuda(), o, c.scale, 4)
+    torch.cuda.synchronize()
+
+
+def test_strided_rows_and_blocks(gpu):
+    """q as a part of a fused projection, o as a part of a wider row, blocks that
+    lie apart, a table that is part of a wider one."""
+    torch = gpu
+    c = Call(torch, "bf16", 4, 2, 64, 16, [70, 33], [2, 1], seed=16)
+    whole = c.run()
+    wide = torch.randn((3, 8, 64), device="cuda").to(torch.bfloat16)
+    wide[:, :4] = c.q.cuda()
+    out = torch.full((3, 6, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    n = 2 * 16 * 64
+    room = torch.full((c.blocks, 2 * n + 32), 0x7F, dtype=torch.uint8, device="cuda")
+    k, v = room[:, :n].unflatten(1, (2, 16, 64)), room[:, n + 16:2 * n + 16].unflatten(1, (2, 64, 16))
+    k.copy_(c.cache["k"])
+    v.copy_(c.cache["v"])
+    h = pyc_amd.KvCache(k, v, c.cache["k_scale"].cuda(), c.cache["v_scale"].cuda())
+    t = torch.full((2, 12), -1, dtype=torch.int32, device="cuda")
+    t[:, :5] = c.table.cuda()
+    pyc_amd.kv_attention(wide[:, :4], h, t[:, :5], c.lens.cuda(), c.offsets.cuda(), out[:, 2:], c.scale, 2)
+    torch.cuda.synchronize()
+    assert torch.equal(out[:, 2:].cpu(), whole) and bool((out[:, :2] == 7.0).all())
+
+
+def test_far_blocks(gpu):
+    """Blocks past 2^32 bytes from the cache's beginning."""
+    torch = gpu
+    c = Call(torch, "bf16", 4, 1, 64, 16, [90], [1], seed=17, blocks=6)
+    far = [torch.empty(6 << 30, dtype=torch.uint8, device="cuda").as_strided((6, 1) + s, (1 << 30, 1024) + t)
+           for s, t in (((16, 64), (64, 1)), ((64, 16), (16, 1)))]
+    far[0].copy_(c.cache["k"])
+    far[1].copy_(c.cache["v"])
+    h = pyc_amd.KvCache(far[0], far[1], c.cache["k_scale"].cuda(), c.cache["v_scale"].cuda())
+    o = torch.empty(c.q.shape, dtype=c.q.dtype, device="cuda")
+    pyc_amd.kv_attention(c.q.cuda(), h, c.table.cuda(), c.lens.cuda(), c.offsets.cuda(), o, c.scale, 1)
+    torch.cuda.synchronize()
+    c.check(o.cpu())
+
+
+def test_workspace_kept_and_made(gpu):
+    """A kept workspace over calls of different shapes, and one made for the call:
+    the same results, bit for bit, each time."""
+    torch = gpu
+    ws = pyc_amd.kv_attention_workspace(8, 32, 8, 128, 64)
+    for lens, counts, hq, hk, d in (([3000, 10], [1, 1], 32, 8, 128), ([200] * 8, [5] * 8, 8, 8, 64),
+                                    ([4000], [64], 16, 4, 128), ([3000, 10], [1, 1], 32, 8, 128)):
+        c = Call(torch, "bf16", hq, hk, d, 16, lens, counts, seed=18)
+        a = c.run(workspace=ws)
+        assert torch.equal(a, c.run()) and torch.equal(a, c.run(workspace=ws))
+        c.check(a)
+
+
+def test_short_workspace_is_refused(gpu):
+    torch = gpu
+    c = Call(torch, "bf16", 8, 2, 64, 16, [80], [1], seed=19)
+    with pytest.raises(pyc_amd.PycError):
+        c.run(workspace=torch.zeros(8, dtype=torch.uint8, device="cuda"))
+
+
+def test_other_stream(gpu):
+    """On a stream of its own, as torch's current one and as an argument."""
+    torch = gpu
+    c = Call(torch, "bf16", 8, 2, 128, 16, [900, 40], [1, 3], seed=20)
+    ref = c.run()
+    s = torch.cuda.Stream()
+    args = (c.q.cuda(), c.handle(), c.table.cuda(), c.lens.cuda(), c.offsets.cuda())
+    o = torch.empty((2,) + tuple(c.q.shape), dtype=c.q.dtype, device="cuda")
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        pyc_amd.kv_attention(*args, o[0], c.scale, 3)
+    pyc_amd.kv_attention(*args, o[1], c.scale, 3, stream=s.cuda_stream)
+    s.synchronize()
+    assert torch.equal(o[0].cpu(), ref) and torch.equal(o[1].cpu(), ref)
+
+
+def test_resources_match_the_code_object(gpu):
+    """What the registry says of the cache's kernels against the loaded code object."""
+    for sym in ("hip_kv_plan", "hip_kv_append_bf16", "hip_kv_append_f16", "hip_kv_attention_bf16", "hip_kv_attention_f16"):
+        r = pyc_amd.kernel_resources(sym)
+        assert r.device == 1 and r.lds_bytes == r.attr_lds_bytes and r.attr_max_threads >= r.threads, sym
+        assert r.waves_per_simd == r.attr_blocks_per_cu * (r.threads // 64) / 4, (sym, r.waves_per_simd, r.attr_blocks_per_cu)
+        assert r.attr_scratch_bytes == 0, sym
