@@ -11,19 +11,19 @@
 // there is one rounding, the same for a token alone and in its prompt, and a
 // block whose scale grows loses only what falls below the code's normal range.
 //
-// The tokens of one block stand together in the slot map; the wave that finds
-// the first of them owns the block for its head.
+// The tokens of one block stand together in the slot map; the workgroup that finds
+// the first of them owns the block for its heads. A wave has one chunk of 16 slots
+// of one head (a block of 128 slots is eight waves'), which it holds in registers from
+// one read of the rows: maximum, across the block's waves through LDS, then the
+// codes. Keys go out as they came, 8 codes a lane; values are transposed in
+// LDS, so that a channel's 16 tokens leave as one 16-byte store, merged with the
+// codes that are there when the chunk is not all new.
 #include "kv_cache.hpp"
 
 namespace pyc {
 
-constexpr int kAppendWaves = 4;
 constexpr int kMinExp = -100;
-
-__device__ inline uint8_t to_e4m3(float x) {
-    return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xff);
-}
-__device__ inline float from_e4m3(uint8_t c) { return __builtin_amdgcn_cvt_f32_fp8((int)c, 0); }
+constexpr int kChunk = 16;
 
 // The smallest power of two s >= 2^-100 with a <= 448 s (a finite, >= 0). a = m
 // 2^x with 1 <= m < 2 and 448 = 1.75 * 2^8.
@@ -34,70 +34,198 @@ __device__ inline float append_scale(float a) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-__device__ inline float append_finite(float x) {
-    const float m = fabsf(x);
-    return m <= 3.402823466e38f ? m : 0.f;
+__device__ inline bool append_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Four floats as codes, in one word.
+__device__ inline uint32_t pack_e4m3(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+// The codes of a word times f (below 1: the block's scale grew).
+__device__ inline uint32_t shrink_e4m3(uint32_t w, float f) {
+    return pack_e4m3(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * f, __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * f,
+                     __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * f, __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * f);
 }
 
-// One block of one head, keys (VALUES false) or values: rows t0 .. t0 + n - 1
-// of x go to the offsets that slots[] says.
-template <typename T, bool VALUES>
-__device__ inline void append_block(const uint16_t* x, int64_t x_stride, const int32_t* slots, int t0, int n,
-                                    uint8_t* codes, float* scale, int bs, int D) {
-    const int lane = threadIdx.x & (kWave - 1);
-    float a = 0.f;
-    bool starts = false;
-    for (int i = 0; i < n; ++i) {
-        const uint16_t* row = x + (int64_t)(t0 + i) * x_stride;
-        for (int d = lane; d < D; d += kWave) a = fmaxf(a, append_finite(elem<T>::to_f32(row[d])));
-        starts |= slots[t0 + i] % bs == 0;
-    }
+template <typename T> __device__ inline float half_at(const u32x4& w, int j) {
+    return elem<T>::to_f32((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+}
+
+struct AppendArgs {
+    KvCache c;
+    int tokens, span;
+    const uint16_t* k;
+    const uint16_t* v;
+    int64_t k_stride, v_stride;
+    const int32_t* slots;
+};
+
+// Orders a wave's LDS accesses for its other lanes.
+__device__ inline void lds_wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+typedef uint32_t __attribute__((may_alias)) word;
+typedef uint16_t __attribute__((may_alias)) half_word;
+
+// S: waves (chunks) of a block.
+template <typename T, int D, int S>
+__global__ void __launch_bounds__((S > 4 ? S : 4) * kWave) kv_append_kernel(AppendArgs a) {
+    constexpr int WAVES = S > 4 ? S : 4;
+    constexpr int HEADS = WAVES / S;        // heads of a workgroup
+    constexpr int LANES = D / 8;            // lanes of a row, 8 channels each
+    constexpr int RPL = kChunk * LANES / kWave;  // rows of a lane: slots RPL * (lane / LANES) ..
+    constexpr int PITCH = kChunk + 4;       // bytes of a channel in the transposition, off the banks' stride
+    __shared__ int where[WAVES][kChunk];    // row of x in each slot of the wave's chunk, -1: none
+    __shared__ uint32_t tile[WAVES][D * PITCH / 4];
+    __shared__ float most[WAVES];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int chunk = wave % S, h = blockIdx.y * HEADS + wave / S;
+    const bool values = blockIdx.z != 0, live = h < a.c.heads;
+    const int bs = kChunk * S;
+    const int64_t last = (int64_t)a.c.blocks * bs;
+    auto slot_of = [&](int i) { return i >= 0 && i < a.tokens ? a.slots[i] : -1; };
+    auto block_of = [&](int s) { return s >= 0 && s < last ? s / bs : -1; };
+    // Lane l looks at row t0 - 1 + l; the rows 1 .. span of these that begin a block are this workgroup's.
+    const int t0 = blockIdx.x * a.span;
+    const int my_slot = slot_of(t0 - 1 + lane), my_block = block_of(my_slot), before = __shfl_up(my_block, 1);
+    uint64_t first = __ballot(lane >= 1 && lane <= a.span && my_block >= 0 && my_block != before);
+    for (; first; first &= first - 1) {
+        const int i = __builtin_ctzll(first), t = t0 - 1 + i;
+        const int blk = __builtin_amdgcn_readlane(my_block, i);
+        // The block's rows: lane l's (and, of long blocks, another 64 behind them).
+        bool starts;
+        {
+            int x0 = lane - i, s0 = my_slot, s1 = -1;  // row t + x0
+            if constexpr (S > 2) {                     // a span and a block do not fit 64 lanes
+                x0 = lane;
+                s0 = slot_of(t + lane);
+                if constexpr (S > 4) s1 = slot_of(t + kWave + lane);
+            }
+            const uint64_t m0 = __ballot(block_of(s0) == blk) >> (S > 2 ? 0 : i), m1 = __ballot(block_of(s1) == blk);
+            int n = ~m0 ? __builtin_ctzll(~m0) : kWave + (~m1 ? __builtin_ctzll(~m1) : kWave);
+            n = min(n, bs);
+            if (lane < kChunk) where[wave][lane] = -1;
+            lds_wave_fence();
+            const bool in0 = x0 >= 0 && x0 < n, in1 = S > 4 && kWave + lane < n;
+            const int o0 = s0 % bs - kChunk * chunk, o1 = s1 % bs - kChunk * chunk;
+            if (in0 && o0 >= 0 && o0 < kChunk) where[wave][o0] = t + x0;
+            if (in1 && o1 >= 0 && o1 < kChunk) where[wave][o1] = t + kWave + lane;
+            starts = __any((in0 && s0 % bs == 0) || (in1 && s1 % bs == 0));
+        }
+        lds_wave_fence();
+        const int r = lane / LANES, c = lane % LANES;
+        const uint16_t* x = values ? a.v : a.k;
+        const int64_t stride = values ? a.v_stride : a.k_stride;
+        int row[RPL];
+        u32x4 w[RPL];
+        float mx = 0.f;
+        bool all = true;
 #pragma unroll
-    for (int w = 1; w < kWave; w *= 2) a = fmaxf(a, __shfl_xor(a, w));
-    const float old = *scale;
-    float s = append_scale(a);
-    const bool had = old > 0.f && old <= 3.402823466e38f;  // a scale that means something
-    if (!starts && had && old > s) s = old;
-    if (!starts && had && s > old) {
-        const float f = old / s;
-        for (int i = lane; i < bs * D; i += kWave) codes[i] = to_e4m3(from_e4m3(codes[i]) * f);
-        __threadfence_block();  // the new codes below go on top of these
-    }
-    const float inv = 1.0f / s;
-    for (int i = 0; i < n; ++i) {
-        const uint16_t* row = x + (int64_t)(t0 + i) * x_stride;
-        const int off = slots[t0 + i] % bs;
-        for (int d = lane; d < D; d += kWave) {
-            const float v = elem<T>::to_f32(row[d]);
-            const float y = fabsf(v) <= 3.402823466e38f ? v * inv : __builtin_nanf("");
-            codes[VALUES ? d * bs + off : off * D + d] = to_e4m3(y);
+        for (int i = 0; i < RPL; ++i) {
+            row[i] = live ? where[wave][RPL * r + i] : -1;
+            all &= row[i] >= 0;
+            w[i] = u32x4{0, 0, 0, 0};
+            if (row[i] >= 0) w[i] = *reinterpret_cast<const u32x4*>(x + row[i] * stride + (int64_t)h * D + 8 * c);
+        }
+        const int64_t at = (int64_t)blk * a.c.heads + min(h, a.c.heads - 1);
+        float* scale = (values ? a.c.v_scale : a.c.k_scale) + at;
+        const float old = *scale;
+#pragma unroll
+        for (int i = 0; i < RPL; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = fabsf(half_at<T>(w[i], j));
+                mx = append_finite(y) ? fmaxf(mx, y) : mx;
+            }
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
+        if constexpr (S > 1) {
+            asm volatile("" ::"v"(old));  // it is here before another wave may store the new scale
+            __syncthreads();              // and the last block's maxima are read
+            if (lane == 0) most[wave] = mx;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < S; ++i) mx = fmaxf(mx, most[wave - chunk + i]);
+        }
+        float s = append_scale(mx);
+        const bool had = old > 0.f && append_finite(old);  // a scale that means something
+        if (!starts && had) s = fmaxf(s, old);
+        const bool grow = !starts && had && s > old;
+        const float f = grow ? old / s : 1.f, inv = 1.0f / s;
+        if (!live) continue;
+        if (chunk == 0 && lane == 0 && s != old) *scale = s;
+        auto scaled = [&](int i, int j) {
+            const float y = half_at<T>(w[i], j);
+            return append_finite(y) ? y * inv : __builtin_nanf("");
+        };
+        if (!values) {
+            uint8_t* dst = a.c.k + blk * a.c.k_stride + ((int64_t)h * bs + kChunk * chunk + RPL * r) * D + 8 * c;
+#pragma unroll
+            for (int i = 0; i < RPL; ++i) {
+                u32x2 out;
+                if (row[i] >= 0) {
+                    out[0] = pack_e4m3(scaled(i, 0), scaled(i, 1), scaled(i, 2), scaled(i, 3));
+                    out[1] = pack_e4m3(scaled(i, 4), scaled(i, 5), scaled(i, 6), scaled(i, 7));
+                } else {
+                    if (!grow) continue;
+                    out = *reinterpret_cast<const u32x2*>(dst + i * D);
+                    out[0] = shrink_e4m3(out[0], f);
+                    out[1] = shrink_e4m3(out[1], f);
+                }
+                *reinterpret_cast<u32x2*>(dst + i * D) = out;
+            }
+        } else {
+            // slots RPL r .. of channel 8 c + j, as one word (or half of one)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint8_t* to = (uint8_t*)tile[wave] + (8 * c + j) * PITCH + RPL * r;
+                if constexpr (RPL == 4) {
+                    *(word*)to = pack_e4m3(scaled(0, j), scaled(1, j), scaled(2, j), scaled(3, j));
+                } else {
+                    *(half_word*)to = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(scaled(0, j), scaled(1, j), 0, false);
+                }
+            }
+            lds_wave_fence();
+            const bool whole = __all(all);
+            u32x4 keep{0, 0, 0, 0};  // bytes of a chunk that stay
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i)
+                    if (where[wave][i] < 0) keep[i >> 2] |= 0xffu << (8 * (i & 3));
+            }
+            const bool none = (keep[0] & keep[1] & keep[2] & keep[3]) == 0xffffffffu;
+            if (!none || grow) {
+                uint8_t* dst = a.c.v + blk * a.c.v_stride + ((int64_t)h * D + lane) * bs + kChunk * chunk;
+#pragma unroll
+                for (int i = 0; i < D / kWave; ++i) {
+                    u32x4* at16 = reinterpret_cast<u32x4*>(dst + (int64_t)kWave * i * bs);
+                    const uint32_t* from = tile[wave] + (lane + kWave * i) * (PITCH / 4);
+                    u32x4 out{from[0], from[1], from[2], from[3]};
+                    if (!whole) {
+                        u32x4 there = *at16;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (grow) there[e] = shrink_e4m3(there[e], f);
+                            out[e] = (out[e] & ~keep[e]) | (there[e] & keep[e]);
+                        }
+                    }
+                    *at16 = out;
+                }
+            }
         }
     }
-    if (lane == 0 && s != old) *scale = s;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kAppendWaves* kWave) kv_append_kernel(KvCache c, int tokens, const uint16_t* k,
-                                                                       int64_t k_stride, const uint16_t* v,
-                                                                       int64_t v_stride, const int32_t* slots) {
-    const int t = blockIdx.x, h = blockIdx.y * kAppendWaves + threadIdx.x / kWave;
-    if (h >= c.heads) return;
-    const int64_t last = (int64_t)c.blocks * c.bs;
-    auto block_of = [&](int i) {
-        const int s = i >= 0 && i < tokens ? slots[i] : -1;
-        return s >= 0 && s < last ? s / c.bs : -1;
-    };
-    const int blk = block_of(t);
-    if (blk < 0 || block_of(t - 1) == blk) return;
-    int n = 1;
-    while (block_of(t + n) == blk) ++n;
-    const int64_t at = (int64_t)blk * c.heads + h, hd = (int64_t)h * c.bs * c.d;
-    if (blockIdx.z == 0)
-        append_block<T, false>(k + (int64_t)h * c.d, k_stride, slots, t, n, c.k + blk * c.k_stride + hd, c.k_scale + at,
-                               c.bs, c.d);
-    else
-        append_block<T, true>(v + (int64_t)h * c.d, v_stride, slots, t, n, c.v + blk * c.v_stride + hd, c.v_scale + at,
-                              c.bs, c.d);
+template <typename T, int D> static const void* append_kernel_of(int bs) {
+    return bs == 16   ? reinterpret_cast<const void*>(&kv_append_kernel<T, D, 1>)
+           : bs == 32 ? reinterpret_cast<const void*>(&kv_append_kernel<T, D, 2>)
+           : bs == 64 ? reinterpret_cast<const void*>(&kv_append_kernel<T, D, 4>)
+                      : reinterpret_cast<const void*>(&kv_append_kernel<T, D, 8>);
+}
+static const void* append_kernel_of(int is_bf16, int d, int bs) {
+    return d == 128 ? (is_bf16 ? append_kernel_of<bf16_t, 128>(bs) : append_kernel_of<f16_t, 128>(bs))
+                    : (is_bf16 ? append_kernel_of<bf16_t, 64>(bs) : append_kernel_of<f16_t, 64>(bs));
 }
 
 }  // namespace pyc
@@ -106,26 +234,26 @@ extern "C" int pyc_hip_kv_append_launch(int is_bf16, const pyc_hip_kv_cache* cac
                                         int64_t k_stride, const void* v, int64_t v_stride, const int32_t* slots,
                                         void* stream) {
     using namespace pyc;
-    const KvCache c = kv_cache_of(cache);
-    const dim3 grid(tokens, (c.heads + kAppendWaves - 1) / kAppendWaves, 2), block(kAppendWaves * kWave);
-    hipStream_t s = (hipStream_t)stream;
-    if (is_bf16)
-        hipLaunchKernelGGL(kv_append_kernel<bf16_t>, grid, block, 0, s, c, tokens, (const uint16_t*)k, k_stride,
-                           (const uint16_t*)v, v_stride, slots);
-    else
-        hipLaunchKernelGGL(kv_append_kernel<f16_t>, grid, block, 0, s, c, tokens, (const uint16_t*)k, k_stride,
-                           (const uint16_t*)v, v_stride, slots);
-    return hipGetLastError() == hipSuccess ? 0 : -2;
+    AppendArgs a{kv_cache_of(cache), tokens, 1, (const uint16_t*)k, (const uint16_t*)v, k_stride, v_stride, slots};
+    // A workgroup for every row where that gives up to 16 k waves (most rows begin no
+    // block and their waves end at once), else for up to 16 rows in a row.
+    const int S = a.c.bs / kChunk, waves = S > 4 ? S : 4, per = waves / S;
+    const unsigned hy = (unsigned)((a.c.heads + per - 1) / per);
+    while (a.span < kChunk && (double)tokens / a.span * hy * 2 * waves > 16384.0) a.span *= 2;
+    void* args[] = {&a};
+    const hipError_t e = hipLaunchKernel(append_kernel_of(is_bf16, a.c.d, a.c.bs),
+                                         dim3((unsigned)((tokens + a.span - 1) / a.span), hy, 2), dim3(waves * kWave),
+                                         args, 0, (hipStream_t)stream);
+    return e == hipSuccess && hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
 extern "C" int pyc_hip_kinfo_kv_append(int is_bf16, pyc_hip_kinfo* out) {
     using namespace pyc;
     if (!out) return -1;
-    out->fn = is_bf16 ? reinterpret_cast<const void*>(&kv_append_kernel<bf16_t>)
-                      : reinterpret_cast<const void*>(&kv_append_kernel<f16_t>);
-    out->name = "kv_append_kernel";
-    out->lds_bytes = 0;
-    out->threads = kAppendWaves * kWave;
-    out->waves_per_simd = 8;
+    out->fn = append_kernel_of(is_bf16, 128, 16);
+    out->name = "kv_append_kernel<128, 1>";
+    out->lds_bytes = 4 * (kChunk * sizeof(int) + 128 * (kChunk + 4));
+    out->threads = 4 * kWave;
+    out->waves_per_simd = is_bf16 ? 6 : 8;
     return 0;
 }
