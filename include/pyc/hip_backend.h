@@ -216,8 +216,8 @@ typedef struct {
  * A refused request keeps its length and its blocks, and has no tokens in the step.
  * Entries of table and free_list that are not pushed or popped stay as they are.
  * lens may be cached, free_after may be free_count; with neither, the call can be
- * made again. B >= 1, width >= 1, tokens >= 0, block_size as above,
- * width * block_size < 2^31. Symbol "hip_kv_plan". 0, -1 (bad argument, nothing
+ * made again. B >= 1, width >= 1, 0 <= tokens < 2^24, block_size as above,
+ * width * block_size < 2^31 - 255. Symbol "hip_kv_plan". 0, -1 (bad argument, nothing
  * launched), -2 (HIP error). */
 int pyc_hip_kv_plan_dispatch(
     const char* symbol, int B, int width, int64_t table_stride, int block_size, int tokens,

@@ -714,7 +714,8 @@ int pyc_hip_kv_plan_dispatch(const char* symbol, int B, int width, int64_t table
                              int free_capacity, const int32_t* free_count, int32_t* lens, int32_t* q_offsets,
                              int32_t* slots, int32_t* positions, int32_t* free_after, void* stream) {
     if (!find_variant(symbol, VK_KV_PLAN) || B <= 0 || width <= 0 || table_stride < width || tokens < 0 ||
-        free_capacity < 0 || !kv_block_size_ok(block_size) || (int64_t)width * block_size > 0x7FFFFFFFLL) {
+        tokens >= KV_MAX_TOKENS || free_capacity < 0 || !kv_block_size_ok(block_size) ||
+        (int64_t)width * block_size > 0x7FFFFF00LL) {
         return -1;
     }
     if (!cached || !fresh || !table || (free_capacity > 0 && !free_list) || !free_count || !lens || !q_offsets ||
@@ -768,8 +769,8 @@ int pyc_hip_kv_attention_dispatch(const char* symbol, const pyc_hip_kv_cache* ca
     if (need == 0 || !workspace || ((uintptr_t)workspace & 15) != 0 || workspace_bytes < need) {
         return -1;
     }
-    if (!table || width <= 0 || table_stride < width || (int64_t)width * cache->block_size > 0x7FFFFFFFLL || !lens ||
-        !q_offsets || !(scale == scale) || !kv_rows_ok(q, q_stride, q_heads, cache->head_dim) ||
+    if (!table || width <= 0 || table_stride < width || (int64_t)width * cache->block_size > 0x7FFFFF00LL ||
+        (double)B * cache->kv_heads * width * cache->block_size >= 0x1p56 || !lens || !q_offsets || !(scale == scale) || !kv_rows_ok(q, q_stride, q_heads, cache->head_dim) ||
         !kv_rows_ok(o, o_stride, q_heads, cache->head_dim)) {
         return -1;
     }

@@ -9,49 +9,64 @@
 //   the new blocks are popped in request order; lens, q_offsets (exclusive sum
 //   of the granted tokens), and per token its position and slot
 //   table[b][pos / bs] * bs + pos % bs.
-// Whole numbers only: three prefix sums over the requests and one lookup per token.
+// Whole numbers only: prefix sums over the requests, in one workgroup, and one lookup
+// per token. Latency bounds it: a handful of dependent loads and stores of a few
+// hundred nanoseconds each. So everything that can be known is loaded at once, blocks
+// move a wave at a time, a step whose requests bring a token each writes it from the
+// request's own thread, and many tokens get a launch over all CUs.
 #include "common.hpp"
 
 namespace pyc {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / kWave;
+constexpr uint32_t kPlanMost = 0x7fffffffu;  // sums stop here: more than there is of anything
 
 struct PlanSum {
-    int64_t blocks, tokens;
+    uint32_t blocks, tokens;
 };
+__device__ inline PlanSum plan_add(PlanSum a, PlanSum b) {
+    return PlanSum{min(a.blocks + b.blocks, kPlanMost), min(a.tokens + b.tokens, kPlanMost)};
+}
 
 // Inclusive sum over the workgroup's threads; `all` is the sum of all of them.
 __device__ inline PlanSum plan_scan(PlanSum v, PlanSum* all, PlanSum* waves) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n = blockDim.x / kWave;
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
-        const int64_t b = __shfl_up(v.blocks, d), t = __shfl_up(v.tokens, d);
-        if (lane >= d) {
-            v.blocks += b;
-            v.tokens += t;
-        }
+        const PlanSum x{(uint32_t)__shfl_up((int)v.blocks, d), (uint32_t)__shfl_up((int)v.tokens, d)};
+        if (lane >= d) v = plan_add(v, x);
+    }
+    if (n == 1) {
+        *all = PlanSum{(uint32_t)__shfl((int)v.blocks, kWave - 1), (uint32_t)__shfl((int)v.tokens, kWave - 1)};
+        return v;
     }
     __syncthreads();  // the last use of `waves`
     if (lane == kWave - 1) waves[wave] = v;
     __syncthreads();
     PlanSum before{0, 0};
     *all = PlanSum{0, 0};
-    for (int w = 0; w < kPlanWaves; ++w) {
-        if (w < wave) {
-            before.blocks += waves[w].blocks;
-            before.tokens += waves[w].tokens;
-        }
-        all->blocks += waves[w].blocks;
-        all->tokens += waves[w].tokens;
+    for (int w = 0; w < n; ++w) {
+        if (w < wave) before = plan_add(before, waves[w]);
+        *all = plan_add(*all, waves[w]);
     }
-    v.blocks += before.blocks;
-    v.tokens += before.tokens;
-    return v;
+    return plan_add(v, before);
+}
+
+// The workgroup's threads' bits, or-ed.
+__device__ inline uint32_t plan_vote(uint32_t bits, uint32_t* votes) {
+    const int n = blockDim.x / kWave;
+    uint32_t mine = (__any(bits & 1) ? 1u : 0u) | (__any(bits & 2) ? 2u : 0u);
+    if (n == 1) return mine;
+    __syncthreads();  // the last use of `votes`
+    if ((threadIdx.x & (kWave - 1)) == 0) votes[threadIdx.x / kWave] = mine;
+    __syncthreads();
+    for (int w = 0; w < n; ++w) mine |= votes[w];
+    return mine;
 }
 
 struct PlanArgs {
-    int B, width, bs, tokens, free_cap;
+    int B, width, bs, shift, tokens, free_cap;  // bs == 1 << shift
     const int32_t* cached;
     const int32_t* fresh;
     int32_t* table;
@@ -65,91 +80,145 @@ struct PlanArgs {
     int32_t* free_after;
 };
 
-// Slot and position of token t: the request is the last one whose offset is <= t.
-__device__ inline void plan_token(const PlanArgs& a, int t, int total) {
-    int slot = -1, pos = -1;
-    if (t < total) {
-        int lo = 0, hi = a.B;  // q_offsets[lo] <= t < q_offsets[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.q_offsets[mid] <= t) lo = mid;
-            else hi = mid;
-        }
-        // the request was granted: its length now, less its tokens behind this one
-        pos = a.lens[lo] - (a.q_offsets[lo + 1] - t);
-        slot = a.table[lo * a.table_stride + pos / a.bs] * a.bs + pos % a.bs;
+// Slot and position of token t < q_offsets[B]: the request is the last one whose
+// offset is <= t (offsets in LDS or global memory).
+__device__ inline void plan_token(const PlanArgs& a, const int32_t* offsets, const int32_t* lens, int t) {
+    int lo = 0, hi = a.B;  // offsets[lo] <= t < offsets[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (offsets[mid] <= t) lo = mid;
+        else hi = mid;
     }
-    a.slots[t] = slot;
+    // the request was granted: its length now, less its tokens behind this one
+    const int pos = lens[lo] - (offsets[lo + 1] - t);
+    a.slots[t] = a.table[lo * a.table_stride + (pos >> a.shift)] * a.bs + (pos & (a.bs - 1));
     a.positions[t] = pos;
+}
+
+// f(thread, j, k) for every j < count of every thread of the workgroup, k counting
+// them all; `end` is the inclusive sum of count over the threads. Counts of up to two
+// everywhere (`few`): each thread does its own, else all are dealt out.
+constexpr uint32_t kPlanFew = 2;
+template <typename F>
+__device__ inline void plan_each(bool few, uint32_t count, uint32_t end, uint32_t all, uint32_t* s_end, F f) {
+    if (few) {
+        for (uint32_t j = 0; j < count; ++j) f((int)threadIdx.x, j, end - count + j);
+        return;
+    }
+    __syncthreads();  // the last use of s_end
+    s_end[threadIdx.x] = end;
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k < all; k += blockDim.x) {
+        int lo = 0, hi = (int)blockDim.x - 1;  // the first thread whose end is past k
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s_end[mid] > k) hi = mid;
+            else lo = mid + 1;
+        }
+        f(lo, k - (lo ? s_end[lo - 1] : 0u), k);
+    }
 }
 
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a, int with_tokens) {
     __shared__ PlanSum waves[kPlanWaves];
-    const int tid = threadIdx.x;
-    const int64_t cap_tokens = (int64_t)a.width * a.bs;
-    const int64_t F = min(max(a.free_count[0], 0), a.free_cap);
-    auto held = [&](int b) { return min((int64_t)max(a.cached[b], 0), cap_tokens); };
-
-    // Ended requests give their blocks back.
-    int64_t pushed = 0;
-    for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
-        const int b = b0 + tid;
-        int64_t back = 0;
-        if (b < a.B && a.fresh[b] < 0) back = (held(b) + a.bs - 1) / a.bs;
-        PlanSum all;
-        const PlanSum end = plan_scan(PlanSum{back, 0}, &all, waves);
-        for (int64_t j = 0; j < back; ++j) {
-            const int64_t at = F + pushed + end.blocks - back + j;
-            if (at < a.free_cap) a.free_list[at] = a.table[b * a.table_stride + j];
-        }
-        pushed += all.blocks;
-    }
-    const int64_t top = min(F + pushed, (int64_t)a.free_cap);
-    __syncthreads();  // the pushed entries are read below
+    __shared__ uint32_t votes[kPlanWaves];
+    __shared__ int32_t s_offsets[kPlanThreads + 4], s_lens[kPlanThreads], s_have[kPlanThreads];
+    __shared__ uint32_t s_end[kPlanThreads];
+    const int tid = threadIdx.x, T = blockDim.x;
+    const int cap_tokens = a.width * a.bs;
+    const uint32_t F = (uint32_t)min(max(a.free_count[0], 0), a.free_cap);
 
     PlanSum asked{0, 0}, given{0, 0};
-    for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
-        const int b = b0 + tid;
-        int64_t have_tokens = 0, ask = 0, need = 0, have = 0;
-        int f = 0;
+    uint32_t top = F;
+    bool long_asks = false;
+    auto load = [&](int b, int* held, int* fresh, int* block) {
+        *held = *fresh = *block = 0;
         if (b < a.B) {
-            f = a.fresh[b];
-            have_tokens = held(b);
-            have = (have_tokens + a.bs - 1) / a.bs;
-            if (f > 0 && have_tokens + f <= cap_tokens) {
-                ask = f;
-                need = (have_tokens + f + a.bs - 1) / a.bs - have;
-            }
+            *held = min(max(a.cached[b], 0), cap_tokens);
+            *fresh = a.fresh[b];
+            *block = a.table[b * a.table_stride + min(*held >> a.shift, a.width - 1)];
+        }
+    };
+    int held, fresh, block;  // block: the entry that the next token falls into
+    load(tid, &held, &fresh, &block);
+    // Ended requests give their blocks back. (A first request is looked at before
+    // any sum: most steps have none that ends.)
+    for (int b0 = 0; b0 < a.B; b0 += T) {
+        const int b = b0 + tid, f = b0 == 0 ? fresh : b < a.B ? a.fresh[b] : 0;
+        if (!plan_vote(f < 0, votes)) continue;
+        uint32_t back = 0;
+        if (f < 0) back = (uint32_t)((b0 == 0 ? held : min(max(a.cached[b], 0), cap_tokens)) + a.bs - 1) >> a.shift;
+        PlanSum all;
+        const PlanSum end = plan_scan(PlanSum{back, 0}, &all, waves);
+        plan_each(false, back, end.blocks, all.blocks, s_end, [&](int i, uint32_t j, uint32_t k) {
+            if (top + k < (uint32_t)a.free_cap) a.free_list[top + k] = a.table[(b0 + i) * a.table_stride + j];
+        });
+        top = min(top + all.blocks, (uint32_t)a.free_cap);
+    }
+    if (top != F) __syncthreads();  // the pushed entries are read below
+
+    for (int b0 = 0; b0 < a.B; b0 += T) {
+        const int b = b0 + tid;
+        if (b0 != 0) load(b, &held, &fresh, &block);
+        const int have = (int)((uint32_t)(held + a.bs - 1) >> a.shift);
+        uint32_t ask = 0, need = 0;
+        if (fresh > 0 && fresh <= cap_tokens - held) {
+            ask = (uint32_t)fresh;
+            need = (((uint32_t)held + ask + a.bs - 1) >> a.shift) - have;
         }
         PlanSum all;
-        const PlanSum end = plan_scan(PlanSum{need, ask}, &all, waves);
-        const bool granted = ask > 0 && (need == 0 || asked.blocks + end.blocks <= top) &&
-                             asked.tokens + end.tokens <= a.tokens;
-        asked.blocks += all.blocks;
-        asked.tokens += all.tokens;
-        if (!granted) ask = need = 0;
-        const PlanSum mine = plan_scan(PlanSum{need, ask}, &all, waves);
-        for (int64_t j = 0; j < need; ++j)
-            a.table[b * a.table_stride + have + j] = a.free_list[top - 1 - (given.blocks + mine.blocks - need + j)];
-        if (b < a.B) {
-            a.lens[b] = f < 0 ? 0 : (int)(have_tokens + ask);
-            a.q_offsets[b] = (int)(given.tokens + mine.tokens - ask);
+        PlanSum end = plan_add(asked, plan_scan(PlanSum{need, ask}, &all, waves));
+        const bool refused = ask > 0 && ((need > 0 && end.blocks > top) || end.tokens > (uint32_t)a.tokens);
+        asked = plan_add(asked, all);
+        if (plan_vote(refused, votes)) {
+            if (refused) ask = need = 0;
+            end = plan_add(given, plan_scan(PlanSum{need, ask}, &all, waves));
+        } else {
+            end = plan_add(given, PlanSum{end.blocks - (asked.blocks - all.blocks), end.tokens - (asked.tokens - all.tokens)});
         }
-        given.blocks += all.blocks;
-        given.tokens += all.tokens;
+        const uint32_t first = end.tokens - ask, pop = top - 1 - (end.blocks - need);  // its first token and new block
+        if (need > 0 && have == held >> a.shift) block = a.free_list[pop];
+        const uint32_t vote = plan_vote((ask > 1 ? 1 : 0) | (need > kPlanFew ? 2 : 0), votes);
+        long_asks |= (vote & 1) != 0;
+        s_have[tid] = have;  // read behind plan_each's barriers, or by this thread
+        plan_each(!(vote & 2), need, end.blocks - given.blocks, all.blocks, s_end, [&](int i, uint32_t j, uint32_t k) {
+            a.table[(b0 + i) * a.table_stride + s_have[i] + j] = a.free_list[top - 1 - (given.blocks + k)];
+        });
+        given = plan_add(given, all);
+        if (b < a.B) {
+            const int len = fresh < 0 ? 0 : held + (int)ask;
+            a.lens[b] = len;
+            a.q_offsets[b] = (int)first;
+            if (a.B <= T) {
+                s_lens[tid] = len;
+                s_offsets[tid] = (int)first;
+            }
+            if (with_tokens && !long_asks && ask == 1) {
+                a.slots[first] = block * a.bs + (held & (a.bs - 1));
+                a.positions[first] = held;
+            }
+        }
     }
+    const int total = (int)given.tokens;
     if (tid == 0) {
-        a.q_offsets[a.B] = (int)given.tokens;
+        a.q_offsets[a.B] = total;
+        s_offsets[a.B <= T ? a.B : 0] = total;
         a.free_after[0] = (int)(top - given.blocks);
     }
     if (!with_tokens) return;
-    __syncthreads();  // lens, q_offsets and the table are read below
-    for (int t = tid; t < a.tokens; t += kPlanThreads) plan_token(a, t, (int)given.tokens);
+    if (long_asks) {
+        __syncthreads();  // lens, offsets and the table are read below
+        const bool near = a.B <= T;
+        for (int t = tid; t < total; t += T) plan_token(a, near ? s_offsets : a.q_offsets, near ? s_lens : a.lens, t);
+    }
+    for (int t = total + tid; t < a.tokens; t += T) a.slots[t] = a.positions[t] = -1;
 }
 
 __global__ void __launch_bounds__(256) kv_slots_kernel(PlanArgs a) {
     const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t < a.tokens) plan_token(a, t, a.q_offsets[a.B]);
+    if (t >= a.tokens) return;
+    if (t < a.q_offsets[a.B]) plan_token(a, a.q_offsets, a.lens, t);
+    else a.slots[t] = a.positions[t] = -1;
 }
 
 }  // namespace pyc
@@ -159,11 +228,15 @@ extern "C" int pyc_hip_kv_plan_launch(int B, int width, int64_t table_stride, in
                                       int free_cap, const int32_t* free_count, int32_t* lens, int32_t* q_offsets,
                                       int32_t* slots, int32_t* positions, int32_t* free_after, void* stream) {
     using namespace pyc;
-    const PlanArgs a{B,          width,     bs,        tokens,     free_cap, cached,    fresh,     table,
-                     table_stride, free_list, free_count, lens,     q_offsets, slots, positions, free_after};
+    const PlanArgs a{B,      width,        bs,        __builtin_ctz(bs), tokens, free_cap,  cached, fresh,
+                     table,  table_stride, free_list, free_count,        lens,   q_offsets, slots,  positions,
+                     free_after};
     hipStream_t s = (hipStream_t)stream;
+    // One workgroup looks up 4096 tokens in about the time of another launch.
     const int one = tokens <= 4 * kPlanThreads;
-    hipLaunchKernelGGL(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, one);
+    int threads = kWave;
+    while (threads < kPlanThreads && (threads < B || (one && 4 * threads < tokens))) threads *= 2;
+    hipLaunchKernelGGL(kv_plan_kernel, dim3(1), dim3(threads), 0, s, a, one);
     if (!one) hipLaunchKernelGGL(kv_slots_kernel, dim3((tokens + 255) / 256), dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
@@ -173,7 +246,7 @@ extern "C" int pyc_hip_kinfo_kv_plan(pyc_hip_kinfo* out) {
     if (!out) return -1;
     out->fn = reinterpret_cast<const void*>(&kv_plan_kernel);
     out->name = "kv_plan_kernel";
-    out->lds_bytes = sizeof(PlanSum) * kPlanWaves;
+    out->lds_bytes = (sizeof(PlanSum) + sizeof(uint32_t)) * kPlanWaves + sizeof(int32_t) * (4 * kPlanThreads + 4);
     out->threads = kPlanThreads;
     out->waves_per_simd = 4;
     return 0;
