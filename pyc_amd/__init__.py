@@ -289,40 +289,30 @@ class KvCache:
         self.ref = C.addressof(self.struct)
 
 
-def _kv_ints(what: str, device: int, *tensors) -> None:
-    """Refuses index tensors that the kernels would read as something else."""
+_kv_env = None  # (torch.int32, the current device's index, symbol suffixes), made at the first call
+
+
+def _make_kv_env():
     import torch
-    for t in tensors:
-        if t.dtype is not torch.int32 or t.get_device() != device or not t.is_contiguous():
-            raise PycError(f"{what}: index tensors are dense int32 on the call's device")
+    global _kv_env
+    torch.cuda.is_available()
+    device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _kv_env = (torch.int32, device, {torch.bfloat16: b"bf16", torch.float16: b"f16"})
+    return _kv_env
 
 
-def _kv_table(what: str, device: int, table) -> None:
-    import torch
-    if table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != device or \
-            (table.shape[1] > 1 and table.stride(1) != 1):
-        raise PycError(f"{what}: the block table is int32 [requests, width] with dense rows, on the call's device")
+def _kv_refuse(what: str, why: str):
+    raise PycError(f"{what}: {why}")
 
 
-def _kv_device(what: str, device: int) -> None:
-    import torch
-    if device < 0 or device != torch.cuda.current_device():
-        raise PycError(f"{what}: the tensors are not on the current device")
-
-
-def _kv_rows(what: str, t, cache: KvCache, heads: int) -> str:
-    """Checks [tokens, heads, head dim] rows; the symbol's suffix of their type."""
-    import torch
-    suffix = {torch.bfloat16: "bf16", torch.float16: "f16"}.get(t.dtype)
-    if suffix is None or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.head_dim or \
-            t.get_device() != cache.device or t.stride(2) != 1 or (heads > 1 and t.stride(1) != cache.head_dim):
-        raise PycError(f"{what}: rows are bf16 or f16 [tokens, {heads}, {cache.head_dim}] with dense heads, on the "
-                       "cache's device")
-    return suffix
-
-
-def _kv_row_stride(t) -> int:
-    return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1] * t.shape[2])
+def _kv_rows(what: str, t, cache: KvCache, heads: int, suffixes):
+    """Checks [tokens, heads, head dim] rows: (symbol suffix of their type, tokens, row stride)."""
+    suffix, shape, stride = suffixes.get(t.dtype), t.shape, t.stride()
+    if suffix is None or len(shape) != 3 or shape[1] != heads or shape[2] != cache.head_dim or stride[2] != 1 or \
+            (stride[1] != cache.head_dim and heads > 1) or t.get_device() != cache.device:
+        _kv_refuse(what, f"rows are bf16 or f16 [tokens, {heads}, {cache.head_dim}] with dense heads, on the cache's device")
+    n = shape[0]
+    return suffix, n, stride[0] if n > 1 else heads * cache.head_dim
 
 
 def kv_plan(cached, fresh, table, free_list, free_count, block_size: int, lens, q_offsets, slots, positions,
@@ -332,33 +322,45 @@ def kv_plan(cached, fresh, table, free_list, free_count, block_size: int, lens, 
     blocks free_list with free_count [1]; writes lens [B], q_offsets [B + 1], slots
     and positions [tokens], free_after [1]. All int32. lens may be cached and
     free_after may be free_count."""
-    B, device = cached.shape[0], cached.get_device()
-    _kv_device("kv plan", device)
-    _kv_table("kv plan", device, table)
-    _kv_ints("kv plan", device, cached, fresh, free_list, free_count, lens, q_offsets, slots, positions, free_after)
-    if fresh.numel() != B or table.shape[0] != B or lens.numel() != B or q_offsets.numel() != B + 1 or \
-            slots.numel() != positions.numel() or free_count.numel() != 1 or free_after.numel() != 1:
-        raise PycError("kv plan: sizes do not match")
-    _check(lib().pyc_hip_kv_plan_dispatch(b"hip_kv_plan", B, table.shape[1], table.stride(0) if B > 1 else table.shape[1],
-                                          block_size, slots.numel(), _ptr(cached), _ptr(fresh), _ptr(table),
-                                          _ptr(free_list), free_list.numel(), _ptr(free_count), _ptr(lens),
-                                          _ptr(q_offsets), _ptr(slots), _ptr(positions), _ptr(free_after),
-                                          _stream(stream)), "kv plan")
+    i32, current, _ = _kv_env or _make_kv_env()
+    device = cached.get_device()
+    if device < 0 or device != current():
+        _kv_refuse("kv plan", "the tensors are not on the current device")
+    for t in (cached, fresh, free_list, free_count, lens, q_offsets, slots, positions, free_after):
+        if t.dtype is not i32 or t.get_device() != device or not t.is_contiguous():
+            _kv_refuse("kv plan", "index tensors are dense int32 on the call's device")
+    B, tokens, shape, stride = cached.numel(), slots.numel(), table.shape, table.stride()
+    if len(shape) != 2 or shape[0] != B or table.dtype is not i32 or table.get_device() != device or \
+            (stride[1] != 1 and shape[1] > 1):
+        _kv_refuse("kv plan", "the block table is int32 [requests, width] with dense rows, on the call's device")
+    if fresh.numel() != B or lens.numel() != B or q_offsets.numel() != B + 1 or positions.numel() != tokens or \
+            free_count.numel() != 1 or free_after.numel() != 1:
+        _kv_refuse("kv plan", "sizes do not match")
+    rc = (_lib or lib()).pyc_hip_kv_plan_dispatch(
+        b"hip_kv_plan", B, shape[1], stride[0] if B > 1 else shape[1], block_size, tokens, cached.data_ptr(),
+        fresh.data_ptr(), table.data_ptr(), free_list.data_ptr(), free_list.numel(), free_count.data_ptr(), lens.data_ptr(),
+        q_offsets.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_after.data_ptr(), _stream(stream))
+    if rc != 0:
+        _check(rc, "kv plan")
 
 
 def kv_append(k, v, slots, cache: KvCache, stream=None) -> None:
     """A step's keys and values [tokens, kv heads, head dim] (rows may be parts of
     wider ones) into the cache's slots (pyc_hip_kv_append_dispatch); slots [tokens]
     int32, -1: skipped."""
-    suffix = _kv_rows("kv append", k, cache, cache.kv_heads)
-    if _kv_rows("kv append", v, cache, cache.kv_heads) != suffix or v.shape[0] != k.shape[0] or \
-            slots.numel() != k.shape[0]:
-        raise PycError("kv append: k, v and slots do not match")
-    _kv_device("kv append", cache.device)
-    _kv_ints("kv append", cache.device, slots)
-    _check(lib().pyc_hip_kv_append_dispatch(_b("hip_kv_append_" + suffix), cache.ref, k.shape[0], _ptr(k),
-                                            _kv_row_stride(k), _ptr(v), _kv_row_stride(v), _ptr(slots),
-                                            _stream(stream)), "kv append")
+    i32, current, suffixes = _kv_env or _make_kv_env()
+    suffix, tokens, k_stride = _kv_rows("kv append", k, cache, cache.kv_heads, suffixes)
+    v_suffix, v_tokens, v_stride = _kv_rows("kv append", v, cache, cache.kv_heads, suffixes)
+    if v_suffix is not suffix or v_tokens != tokens or slots.numel() != tokens:
+        _kv_refuse("kv append", "k, v and slots do not match")
+    if slots.dtype is not i32 or slots.get_device() != cache.device or not slots.is_contiguous():
+        _kv_refuse("kv append", "index tensors are dense int32 on the call's device")
+    if cache.device < 0 or cache.device != current():
+        _kv_refuse("kv append", "the tensors are not on the current device")
+    rc = (_lib or lib()).pyc_hip_kv_append_dispatch(b"hip_kv_append_" + suffix, cache.ref, tokens, k.data_ptr(), k_stride,
+                                                    v.data_ptr(), v_stride, slots.data_ptr(), _stream(stream))
+    if rc != 0:
+        _check(rc, "kv append")
 
 
 def kv_attention_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int, max_q: int):
@@ -378,16 +380,22 @@ def kv_attention(q, cache: KvCache, table, lens, q_offsets, o, scale: float, max
     as kv_plan leaves them; max_q: no request has more tokens in the step; max_len: the
     longest of lens, if known. Without a workspace (kv_attention_workspace) one is
     made for the call."""
-    tokens, heads = q.shape[0], q.shape[1]
-    suffix = _kv_rows("kv attention", q, cache, heads)
-    if _kv_rows("kv attention", o, cache, heads) != suffix or o.shape[0] != tokens:
-        raise PycError("kv attention: q and o do not match")
-    B, device = lens.shape[0], cache.device
-    _kv_device("kv attention", device)
-    _kv_table("kv attention", device, table)
-    _kv_ints("kv attention", device, lens, q_offsets)
-    if table.shape[0] != B or q_offsets.numel() != B + 1:
-        raise PycError("kv attention: table, lens and q_offsets do not match")
+    i32, current, suffixes = _kv_env or _make_kv_env()
+    heads, device = q.shape[1], cache.device
+    suffix, tokens, q_stride = _kv_rows("kv attention", q, cache, heads, suffixes)
+    o_suffix, o_tokens, o_stride = _kv_rows("kv attention", o, cache, heads, suffixes)
+    if o_suffix is not suffix or o_tokens != tokens:
+        _kv_refuse("kv attention", "q and o do not match")
+    for t in (lens, q_offsets):
+        if t.dtype is not i32 or t.get_device() != device or not t.is_contiguous():
+            _kv_refuse("kv attention", "index tensors are dense int32 on the call's device")
+    B, shape, stride = lens.numel(), table.shape, table.stride()
+    if len(shape) != 2 or shape[0] != B or table.dtype is not i32 or table.get_device() != device or \
+            (stride[1] != 1 and shape[1] > 1) or q_offsets.numel() != B + 1:
+        _kv_refuse("kv attention", "the block table is int32 [requests, width] with dense rows, lens [requests] and "
+                                   "q_offsets [requests + 1] go with it, on the call's device")
+    if device < 0 or device != current():
+        _kv_refuse("kv attention", "the tensors are not on the current device")
     if B == 0 or tokens == 0:
         return
     at = _stream(stream)
@@ -399,13 +407,13 @@ def kv_attention(q, cache: KvCache, table, lens, q_offsets, o, scale: float, max
         with contextlib.nullcontext() if stream is None else torch.cuda.stream(torch.cuda.ExternalStream(at)):
             workspace = kv_attention_workspace(B, heads, cache.kv_heads, cache.head_dim, max_q)
     elif workspace.get_device() != device or not workspace.is_contiguous():
-        raise PycError("kv attention: the workspace is dense, on the cache's device")
-    _check(lib().pyc_hip_kv_attention_dispatch(_b("hip_kv_attention_" + suffix), cache.ref, B, tokens, heads, max_q,
-                                               max_len, _ptr(q), _kv_row_stride(q), _ptr(table),
-                                               table.stride(0) if B > 1 else table.shape[1], table.shape[1],
-                                               _ptr(lens), _ptr(q_offsets), _ptr(o), _kv_row_stride(o), scale,
-                                               _ptr(workspace), workspace.numel() * workspace.element_size(), at),
-           "kv attention")
+        _kv_refuse("kv attention", "the workspace is dense, on the cache's device")
+    rc = (_lib or lib()).pyc_hip_kv_attention_dispatch(
+        b"hip_kv_attention_" + suffix, cache.ref, B, tokens, heads, max_q, max_len, q.data_ptr(), q_stride,
+        table.data_ptr(), stride[0] if B > 1 else shape[1], shape[1], lens.data_ptr(), q_offsets.data_ptr(), o.data_ptr(),
+        o_stride, scale, workspace.data_ptr(), workspace.nbytes, at)
+    if rc != 0:
+        _check(rc, "kv attention")
 
 
 def device_info() -> abi.DeviceInfo:

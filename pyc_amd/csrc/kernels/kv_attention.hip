@@ -389,16 +389,11 @@ __device__ inline int attn_locate(const AttnArgs& a, int most_rows, int64_t u, i
     }
     return -1;
 }
-// Piece w of W: units u(w) .. u(w + 1) - 1. No product here passes 64 bits: there
-// are fewer than 2^12 pieces.
-__device__ inline int64_t piece_begin(int64_t total, int W, int w) {
-    return total / W * w + total % W * w / W;
-}
-__device__ inline int piece_of(int64_t total, int W, int64_t u) {
-    int w = (int)min((int64_t)(W - 1), u / max(total / W, (int64_t)1));  // not too early
-    while (piece_begin(total, W, w) > u) --w;
-    return w;
-}
+// Piece w of W begins at floor(total w / W). There are fewer than 2^12 pieces and
+// 2^50 units: no product passes 64 bits.
+__device__ inline int64_t piece_begin(int64_t total, int W, int w) { return total * w / W; }
+// The last piece that begins at or before u.
+__device__ inline int piece_of(int64_t total, int W, int64_t u) { return (int)(((u + 1) * W - 1) / total); }
 
 constexpr int kSplitWaves = 4;
 
