@@ -23,7 +23,10 @@
 // `len` (or of a block id outside the cache) have their value codes cleared, and
 // where a row may not see a token that others see, a NaN code is taken out of the
 // product and put back by a product of indicators.
+#include <type_traits>
+
 #include "kv_cache.hpp"
+#include "lds_dma.hpp"
 
 namespace pyc {
 
@@ -64,7 +67,7 @@ __device__ inline uint32_t pack_half2(float lo, float hi, bf16_t) {
 // Bit 7 of every byte that is a NaN code.
 __device__ inline uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// Rows per request up to which the split kernel takes it; the others go to kv_attn_kernel.
+// Requests of up to most_rows rows are the split kernel's; the others go to kv_chunk_kernel.
 struct AttnSplit {
     int most_rows;
     float* part;       // two partial results for each wave
@@ -490,19 +493,411 @@ __global__ void __launch_bounds__(32 * kJoinParts) kv_join_kernel(AttnArgs a, At
     }
 }
 
-// Requests of more rows than the split kernel takes: a wave for 16 of them.
+// ---------------------------------------------------------------------------
+// Requests of many rows (prompt chunks): matrix work. A workgroup has 128 rows of a
+// request and kv head; its 8 waves are 4 times 32 rows and two groups that take the
+// tiles of 64 keys in turn and join at the end. On v_mfma_f32_32x32x16, as above:
+// S^T = K Q^T with the keys of a tile ordered so that a lane ends with 16 keys of one
+// chunk of each half tile, O^T += V^T P^T with P as it is. A group's tiles come by
+// LDS-DMA, as codes, into a ring of three. The two groups are one phase apart: while a
+// wave of one runs matrix instructions (phase M: the scores of its next tile and the
+// products of this one, and the conversion of both operands' codes), the wave of the
+// other that shares its SIMD runs its softmax (phase V).
+constexpr int kChunkRows = 128;
+constexpr int kChunkRing = 3;
+constexpr int kChunkThreads = 512;
+constexpr size_t chunk_lds_bytes(int d) {  // rings, raw values, flags; maxima and sums to join
+    return (size_t)2 * kChunkRing * 2 * 64 * d + 4 * 64 * d + 64 + 8 * 32 * 2 * sizeof(float);
+}
+
+__device__ inline f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x16& c, bf16_t) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ inline f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x16& c, f16_t) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Row tiles of a request in the chunk kernel.
+__device__ inline int chunk_tiles(const AttnReq& r, int from_rows) {
+    return r.rows > from_rows ? (r.rows + kChunkRows - 1) / kChunkRows : 0;
+}
+
+// The reference m of a row is its maximum over the first tile that shows it a key,
+// raised only when a later tile's sum of p passes 2^14: p stays far from
+// overflow in bf16 (whose exponents are fp32's), and the common path has no maximum.
+constexpr float kChunkSumMax = 16384.0f;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kWave) kv_attn_kernel(AttnArgs a, int from_rows) {
-    const int r0 = 16 * blockIdx.x, h = blockIdx.y;
-    for (int b = blockIdx.z; b < a.B; b += gridDim.z) {
-        const AttnReq r = attn_request(a, b);
-        if (r0 >= r.rows || r.rows <= from_rows) continue;
-        AttnWave<T, D, 1> w;
-        w.begin(a, r, h, r0);
-        // keys that the tile's last row sees
-        const int last = min(r0 + 15, r.rows - 1) / a.G, end = max(0, r.len - r.n + last + 1);
-        w.run(a, r, b, h, 0, (end + 63) / 64);
-        w.store(a, r, h, r0);
+__global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, int from_rows) {
+    constexpr int KC = D / 16;            // 16-byte chunks of a key's row in LDS
+    constexpr int KK = D / 32;            // pairs of k steps of S
+    constexpr int DT = D / 32;            // 32-channel tiles of O^T
+    constexpr int TILE = 64 * D;          // bytes of one operand of a tile
+    constexpr int DMA = TILE / (4 * 1024);  // wave loads of an operand for each of a group's waves
+    constexpr bool SPLIT = __is_same(T, f16_t);
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * kChunkRing * 2 * TILE];
+    // Value tiles that hold a NaN code, as they came, and which waves' parts of them
+    // are there; [group][tile % 2]. In the ring NaN codes are 0: the product then says
+    // nothing of them, and nan_values gives the NaN to the rows that see them.
+    __shared__ __attribute__((aligned(16))) uint8_t raw[4][TILE];
+    __shared__ __attribute__((aligned(16))) int with_nan[4][4];
+    __shared__ float joint[8][32][2];
+    static_assert(sizeof(ring) + sizeof(raw) + sizeof(with_nan) + sizeof(joint) == chunk_lds_bytes(D), "registered LDS figure");
+    static_assert(8 * 64 * (DT / 2) * 64 <= (int)sizeof(ring), "room to join in");
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int grp = wave >> 2, wr = wave & 3, l32 = lane & 31, hh = lane >> 5, bs = a.c.bs;
+
+    // The part: blockIdx.x counts (request, row tile from the last, head).
+    int b = -1, h = 0, rt = 0;
+    {
+        int64_t u = blockIdx.x, base = 0;
+        for (int b0 = 0; b0 < a.B && b < 0; b0 += kWave) {
+            const int i = b0 + lane;
+            const int64_t mine =
+                i < a.B ? (int64_t)chunk_tiles(attn_request(a, i), from_rows) * a.c.heads : 0;
+            int64_t end = mine;
+#pragma unroll
+            for (int d = 1; d < kWave; d *= 2) {
+                const int64_t x = __shfl_up(end, d);
+                if (lane >= d) end += x;
+            }
+            const uint64_t past = __ballot(base + end > u);
+            if (past) {
+                const int i2 = __builtin_ctzll(past);
+                const int v = (int)(u - base - __shfl(end - mine, i2));
+                b = b0 + i2;
+                h = v % a.c.heads;
+                rt = (int)(__shfl(mine, i2) / a.c.heads) - 1 - v / a.c.heads;
+            }
+            base += __shfl(end, kWave - 1);
+        }
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    h = __builtin_amdgcn_readfirstlane(h);
+    rt = __builtin_amdgcn_readfirstlane(rt);
+    if (b < 0) return;
+    const AttnReq r = attn_request(a, b);
+    const int r0 = rt * kChunkRows, w0 = r0 + 32 * wr;  // the part's first row, the wave's
+    const int keys = max(0, r.len - r.n + min(r0 + kChunkRows - 1, r.rows - 1) / a.G + 1);  // that its last row sees
+    const int n = (keys + 127) / 128;  // tiles of each group (the last of group 1 may have no key)
+
+    // Q and what each row sees.
+    const int row = w0 + l32;
+    const bool live = row < r.rows;
+    const int limit = live ? r.len - r.n + row / a.G : r.len - 1;
+    u32x4 q[2 * KK];
+    {
+        const int i = live ? row / a.G : 0, qh = live ? row % a.G : 0;
+        const uint16_t* src = a.q + (int64_t)(r.first + i) * a.q_stride + (int64_t)(h * a.G + qh) * D + 16 * hh;
+#pragma unroll
+        for (int k = 0; k < KK; ++k)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) q[2 * k + u] = *reinterpret_cast<const u32x4*>(src + 32 * k + 8 * u);
+    }
+
+    // Blocks and scales of 16 of the group's tiles: lane l has chunk l % 4 of tile l / 4.
+    auto pages = [&](int j0) {
+        const int64_t key = 64 * (2 * ((int64_t)j0 + (lane >> 2)) + grp) + 16 * (lane & 3);
+        AttnPages p;
+        p.id = -1;
+        if (key < r.len) p.id = a.table[b * a.table_stride + key / bs];
+        if (p.id < 0 || p.id >= a.c.blocks) p.id = -1;
+        const int64_t at = (int64_t)max(p.id, 0) * a.c.heads + h;
+        p.sk = a.c.k_scale[at] * a.scale_log2;
+        p.sv = a.c.v_scale[at];
+        return p;
+    };
+    const uint32_t lds0 = (uint32_t)(uintptr_t)&ring[0] + (uint32_t)(grp * kChunkRing * 2 * TILE);
+    // LDS row m of a half tile holds key 16 (m / 4 % 2) + 4 (m / 8) + m % 4 of it; rows
+    // are swizzled by 16-byte chunks so that 16 lanes reading one chunk of 16 rows
+    // touch every bank once (rows of 128 bytes: c ^ m / 2 % 8, of 64: c ^ m / 4 % 4).
+    auto swz = [](int row64, int m, int c) { return row64 ? c ^ ((m >> 2) & 3) : c ^ ((m >> 1) & 7); };
+    auto issue = [&](const AttnPages& p, int j) {  // tile j of the group into its slot
+        // made opaque, so that the addresses are formed here instead of held over the loop
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int tile = 2 * j + grp, t4 = 4 * (j & 15);
+        const uint32_t slot = lds0 + (uint32_t)((j % kChunkRing) * 2 * TILE);
+#pragma unroll
+        for (int x = 0; x < DMA; ++x) {
+            const int i = wr + 4 * x;
+            const int m = i * (1024 / D) + ln / KC, c = swz(D == 64, m, ln % KC), m32 = m & 31;
+            const int key = (m & 32) + 16 * ((m32 >> 2) & 1) + 4 * (m32 >> 3) + (m32 & 3);
+            const int id = max(__shfl(p.id, t4 + (key >> 4)), 0);
+            lds_dma_b128(a.c.k + id * a.c.k_stride + ((int64_t)h * bs + ((64 * tile + key) & (bs - 1))) * D + 16 * c,
+                         slot + (uint32_t)(1024 * i));
+        }
+#pragma unroll
+        for (int x = 0; x < DMA; ++x) {
+            const int i = wr + 4 * x;
+            const int d = 16 * i + ln / 4, c = swz(1, d, ln & 3);
+            const int id = max(__shfl(p.id, t4 + c), 0);
+            lds_dma_b128(a.c.v + id * a.c.v_stride + ((int64_t)h * D + d) * bs + ((64 * tile + 16 * c) & (bs - 1)),
+                         slot + (uint32_t)(TILE + 1024 * i));
+        }
+    };
+
+    f32x16 o[DT], s[2];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    u32x4 hi[4], lo[4];  // P^T: [2 e + u], half tile e, its keys 8 u .. of each lane half
+    AttnPages pg = pages(0), nx = pg;  // of the tile whose softmax is next; of the tiles 16 on
+    if (n > 16) nx = pages(16);
+
+    // This wave's part of tile j's values, which has landed: NaN codes out of it.
+    auto check_values = [&](int j) {
+        uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
+        u32x4 w[DMA];
+        uint32_t bad = 0;
+#pragma unroll
+        for (int x = 0; x < DMA; ++x) {
+            w[x] = *reinterpret_cast<const u32x4*>(mine + 1024 * (wr + 4 * x));
+            bad |= nan_codes(w[x][0]) | nan_codes(w[x][1]) | nan_codes(w[x][2]) | nan_codes(w[x][3]);
+        }
+        const bool any = __any(bad != 0);
+        if (lane == 0) with_nan[2 * grp + (j & 1)][wr] = any;
+        if (!any) return;
+#pragma unroll
+        for (int x = 0; x < DMA; ++x) {
+            *reinterpret_cast<u32x4*>(raw[2 * grp + (j & 1)] + 1024 * (wr + 4 * x) + 16 * lane) = w[x];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) w[x][y] &= ~((nan_codes(w[x][y]) >> 7) * 0xffu);
+            *reinterpret_cast<u32x4*>(mine + 1024 * (wr + 4 * x)) = w[x];
+        }
+    };
+    // NaN codes among tile j's values: NaN sums for the rows that see them, by a product of indicators.
+    auto nan_values = [&](int j, const int (&seen)[2]) {
+        const int which = 2 * grp + (j & 1);
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e) {
+            u32x4 one[2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                one[i >> 2][i & 3] = (2 * i < seen[e] ? 0x3f80u : 0u) | (2 * i + 1 < seen[e] ? 0x3f800000u : 0u);
+#pragma unroll
+            for (int k = 0; k < DT; ++k) {
+                u32x4 w = *reinterpret_cast<const u32x4*>(raw[which] + (32 * k + l32) * 64 + 16 * swz(1, l32, 2 * e + hh));
+                if (!with_nan[which][(2 * k + (l32 >> 4)) & 3]) w = u32x4{0, 0, 0, 0};  // the part is not there
+#pragma unroll
+                for (int x = 0; x < 4; ++x) w[x] = (nan_codes(w[x]) >> 7) * 0x38u;  // 1.0
+                f32x16 hit;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) hit[i] = 0.f;
+                hit = mfma32x32x16(fp8x8_to_half8(w[0], w[1], bf16_t{}), one[0], hit, bf16_t{});
+                hit = mfma32x32x16(fp8x8_to_half8(w[2], w[3], bf16_t{}), one[1], hit, bf16_t{});
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[k][i] = hit[i] > 0.f ? __builtin_nanf("") : o[k][i];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+
+    // One M phase: S of tile js and O += P V of tile jp (if DP).
+    auto m_phase = [&](auto dp_tag, int js, int jp) {
+        constexpr bool DP = decltype(dp_tag)::value;
+        uint32_t so_k = (uint32_t)((grp * kChunkRing + js % kChunkRing) * 2 * TILE);
+        uint32_t so_v = (uint32_t)((grp * kChunkRing + jp % kChunkRing) * 2 * TILE + TILE);
+        asm volatile("" : "+s"(so_k), "+s"(so_v));
+        const uint8_t* ks = ring + so_k;
+        const uint8_t* vs = ring + so_v;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[e][i] = 0.f;
+        u32x4 kf[2], vf[2];
+        auto load = [&](int st, int x) {
+            const int e = st / KK, k = st % KK;
+            kf[x] = *reinterpret_cast<const u32x4*>(ks + (32 * e + l32) * D + 16 * swz(D == 64, l32, 2 * k + hh));
+            if constexpr (DP) vf[x] = *reinterpret_cast<const u32x4*>(vs + (32 * k + l32) * 64 + 16 * swz(1, l32, 2 * e + hh));
+        };
+        load(0, 0);
+#pragma unroll
+        for (int st = 0; st < 2 * KK; ++st) {
+            const int e = st / KK, k = st % KK;
+            if (st + 1 < 2 * KK) load(st + 1, (st + 1) & 1);
+            const u32x4 kw = kf[st & 1];
+            s[e] = mfma32x32x16(fp8x8_to_half8(kw[0], kw[1], T{}), q[2 * k], s[e], T{});
+            s[e] = mfma32x32x16(fp8x8_to_half8(kw[2], kw[3], T{}), q[2 * k + 1], s[e], T{});
+            if constexpr (DP) {
+                const u32x4 w = vf[st & 1];
+                const u32x4 v0 = fp8x8_to_half8(w[0], w[1], bf16_t{}), v1 = fp8x8_to_half8(w[2], w[3], bf16_t{});
+                o[k] = mfma32x32x16(v0, hi[2 * e], o[k], bf16_t{});
+                o[k] = mfma32x32x16(v1, hi[2 * e + 1], o[k], bf16_t{});
+                if constexpr (SPLIT) {
+                    o[k] = mfma32x32x16(v0, lo[2 * e], o[k], bf16_t{});
+                    o[k] = mfma32x32x16(v1, lo[2 * e + 1], o[k], bf16_t{});
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // The softmax of tile j, whose scores are in s: P into hi (and lo).
+    auto v_phase = [&](int j) {
+        const int key0 = 64 * (2 * j + grp), t4 = 4 * (j & 15) + hh;
+        float sk[2], sv[2];
+        int seen[2];
+        bool part = false;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            sk[e] = __shfl(pg.sk, t4 + 2 * e);
+            sv[e] = __shfl(pg.sv, t4 + 2 * e);
+            const int id = __shfl(pg.id, t4 + 2 * e), key = key0 + 32 * e + 16 * hh;
+            seen[e] = id < 0 ? 0 : min(min(r.len, limit + 1) - key, 16);
+            part |= seen[e] < 16;
+        }
+        const bool clean = !__any(part);
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[e][i] = fmaf(s[e][i], sk[e], -ref);
+        if (!clean) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[e][i] = i < seen[e] ? s[e][i] : -INFINITY;
+        }
+        auto exponentiate = [&]() {  // P, and the sum of p
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(s[e][i]), p1 = __builtin_amdgcn_exp2f(s[e][i + 1]);
+                    sum[0] += p0;
+                    sum[1] += p1;
+                    float x0 = p0 * sv[e], x1 = p1 * sv[e];
+                    if (!clean) {  // sv may be anything
+                        x0 = i < seen[e] ? x0 : 0.f;
+                        x1 = i + 1 < seen[e] ? x1 : 0.f;
+                    }
+                    const uint32_t w = pack_half2(x0, x1, bf16_t{});
+                    hi[2 * e + (i >> 3)][(i & 7) >> 1] = w;
+                    if constexpr (SPLIT)
+                        lo[2 * e + (i >> 3)][(i & 7) >> 1] = pack_half2(
+                            x0 - __uint_as_float(w << 16), x1 - __uint_as_float(w & 0xffff0000u), bf16_t{});
+                }
+            return sum[0] + sum[1];
+        };
+        float sum = exponentiate();
+        const bool fresh = m == -INFINITY && (seen[0] > 0 || seen[1] > 0);
+        if (__any(fresh || !(sum <= kChunkSumMax))) {
+            // both lane halves of a row move together
+            float mx = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[0][i]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[1][i]);
+            const float mo = __shfl_xor(mx, 32), so = __shfl_xor(sum, 32);
+            mx = __builtin_elementwise_maximum(mx, mo);  // of the row, above ref
+            const bool move = mx != -INFINITY && (m == -INFINITY || !(sum <= kChunkSumMax) || !(so <= kChunkSumMax));
+            const float shift = move ? mx : 0.f, keep = __builtin_amdgcn_exp2f(-shift);
+            if (m != -INFINITY) {
+                l *= keep;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[t][i] *= keep;
+            }
+            if (move) m = ref + shift;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[e][i] -= shift;
+            sum = exponentiate();
+        }
+        l += sum;
+        const int* nan = with_nan[2 * grp + (j & 1)];
+        if (__builtin_amdgcn_readfirstlane(nan[0] | nan[1] | nan[2] | nan[3])) nan_values(j, seen);
+    };
+
+    if (n > 0) {
+        issue(pg, 0);
+        if (n > 1) {
+            issue(pg, 1);
+            wait_vmem_le<2 * DMA>();  // the first tile's own part landed ...
+        } else {
+            wait_vmem_le<0>();
+        }
+        check_values(0);
+        __syncthreads();                // ... and every wave's
+        if (grp == 1) __syncthreads();  // group 1 is one phase behind
+        m_phase(std::false_type{}, 0, 0);
+        __syncthreads();
+        v_phase(0);
+        wait_vmem_le<0>();
+        if (n > 1) check_values(1);
+        __syncthreads();
+        for (int k = 0; k < n; ++k) {
+            // The wave in its M phase goes first: the softmax of the SIMD's other wave
+            // takes the cycles that its matrix instructions leave. (The last S is of
+            // a tile that does not exist: whatever its slot holds, nobody reads it.)
+            __builtin_amdgcn_s_setprio(2);
+            if (k + 2 < n) issue(((k + 2) & 15) < 2 && k + 2 >= 16 ? nx : pg, k + 2);
+            m_phase(std::true_type{}, k + 1, k);
+            __builtin_amdgcn_s_setprio(0);
+            __syncthreads();
+            if (k + 1 < n) {
+                if (((k + 1) & 15) == 0) {
+                    pg = nx;
+                    if (k + 17 < n) nx = pages(k + 17);
+                }
+                v_phase(k + 1);
+                wait_vmem_le<0>();  // tile k + 2 landed
+                if (k + 2 < n) check_values(k + 2);
+                __syncthreads();
+            }
+        }
+        if (grp == 0) __syncthreads();
+    }
+    __syncthreads();  // the rings are free
+
+    // Join: group g ends with channels 32 t .. of t in its half.
+    {
+        l += __shfl_xor(l, 32);
+        if (hh == 0) {
+            joint[wave][l32][0] = m;
+            joint[wave][l32][1] = l;
+        }
+        f32x4* give = reinterpret_cast<f32x4*>(ring) + (size_t)wave * (DT / 2) * 4 * kWave + lane;
+#pragma unroll
+        for (int t = 0; t < DT / 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x16& x = o[t];
+                const f32x16& y = o[DT / 2 + t];
+                give[(4 * t + i) * kWave] =
+                    grp == 0 ? f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]}
+                             : f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+            }
+        __syncthreads();
+        const float m2 = joint[wave ^ 4][l32][0], l2 = joint[wave ^ 4][l32][1];
+        const float mx = __builtin_elementwise_maximum(m, m2), ref = mx == -INFINITY ? 0.f : mx;
+        const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(m2 - ref);
+        const float inv = mx == -INFINITY ? 0.f : 1.0f / (l * f + l2 * g);
+        const f32x4* take = reinterpret_cast<const f32x4*>(ring) + (size_t)(wave ^ 4) * (DT / 2) * 4 * kWave + lane;
+        uint16_t* dst = a.o + (int64_t)(r.first + row / a.G) * a.o_stride + (int64_t)(h * a.G + row % a.G) * D +
+                        32 * (DT / 2) * grp + 4 * hh;
+#pragma unroll
+        for (int t = 0; t < DT / 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 y = take[(4 * t + i) * kWave];
+                float z[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mine = grp == 0 ? o[t][4 * i + e] : o[DT / 2 + t][4 * i + e];
+                    z[e] = (mine * f + y[e] * g) * inv;
+                }
+                u32x2 w;
+                w[0] = (uint32_t)elem<T>::from_f32(z[0]) | ((uint32_t)elem<T>::from_f32(z[1]) << 16);
+                w[1] = (uint32_t)elem<T>::from_f32(z[2]) | ((uint32_t)elem<T>::from_f32(z[3]) << 16);
+                if (live) *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * i) = w;
+            }
     }
 }
 
@@ -530,9 +925,13 @@ template <typename T, int D> static void launch_attention(const AttnArgs& a, flo
     else hipLaunchKernelGGL((kv_split_kernel<T, D, 4>), dim3(groups), block, 0, s, a, sp);
     hipLaunchKernelGGL((kv_join_kernel<T, D>), dim3(sp.most_rows, a.c.heads, zb), dim3(32 * kJoinParts), 0, s, a, sp,
                        groups * kSplitWaves);
-    if (rows > sp.most_rows)
-        hipLaunchKernelGGL((kv_attn_kernel<T, D>), dim3((unsigned)((rows + 15) / 16), a.c.heads, zb), dim3(kWave), 0, s,
-                           a, sp.most_rows);
+    if (rows > sp.most_rows) {
+        // row tiles: whole ones, and one more for each request that is large enough
+        const long all = (long)a.tokens * a.G, some = all / (sp.most_rows + 1);
+        const long tiles = all / kChunkRows + (some < a.B ? some : a.B);
+        hipLaunchKernelGGL((kv_chunk_kernel<T, D>), dim3((unsigned)(tiles * a.c.heads)), dim3(kChunkThreads), 0, s, a,
+                           sp.most_rows);
+    }
 }
 
 }  // namespace pyc

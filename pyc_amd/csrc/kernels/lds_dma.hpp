@@ -44,6 +44,15 @@ __device__ inline void lds_dma_buf_b128_nt_u(i32x4 rsrc, uint32_t voff, uint32_t
                  : "memory", "m0");
 }
 
+// The same from a 64-bit address for each lane, for data that no one descriptor
+// covers: lane i's 16 bytes at src land at lds_base + 16*i.
+__device__ inline void lds_dma_b128(const void* src, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(src)
+                 : "memory", "m0");
+}
+
 // Raw buffer descriptor (CDNA layout): 48-bit base, stride 0, byte count,
 // 32-bit data format. Every field is wave-uniform.
 __device__ inline i32x4 make_buf_rsrc(const void* base, uint32_t bytes) {
