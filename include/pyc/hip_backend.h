@@ -183,7 +183,7 @@ int pyc_hip_layernorm_dispatch(const char* symbol, int rows, int D, float eps, c
  *   k_scale, v_scale [num_blocks][kv_heads] fp32: an element is code * scale.
  * A block's codes are dense; k_block_stride and v_block_stride are the bytes
  * from a block to the next (at least kv_heads * block_size * head_dim, multiples
- * of 16; k and v on 16-byte boundaries). block_size 16, 32, 64 or 128, head_dim 64
+ * of 16, below 2^31; k and v on 16-byte boundaries). block_size 16, 32, 64 or 128, head_dim 64
  * or 128, num_blocks * block_size < 2^31. Slot s is token s % block_size of block
  * s / block_size. */
 typedef struct {

@@ -698,7 +698,8 @@ static int kv_cache_ok(const pyc_hip_kv_cache* c) {
         return 0;
     }
     dense = (int64_t)c->kv_heads * c->block_size * c->head_dim;
-    if (c->k_block_stride < dense || c->v_block_stride < dense || ((c->k_block_stride | c->v_block_stride) & 15) != 0) {
+    if (c->k_block_stride < dense || c->v_block_stride < dense || ((c->k_block_stride | c->v_block_stride) & 15) != 0 ||
+        c->k_block_stride > 0x7FFFFFFFLL || c->v_block_stride > 0x7FFFFFFFLL) {
         return 0;
     }
     return (int64_t)c->num_blocks * c->block_size <= 0x7FFFFFFFLL;

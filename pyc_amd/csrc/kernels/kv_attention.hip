@@ -597,45 +597,48 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, 
     }
 
     // Blocks and scales of 16 of the group's tiles: lane l has chunk l % 4 of tile l / 4.
-    auto pages = [&](int j0) {
+    auto page_ids = [&](int j0) {
         const int64_t key = 64 * (2 * ((int64_t)j0 + (lane >> 2)) + grp) + 16 * (lane & 3);
-        AttnPages p;
-        p.id = -1;
-        if (key < r.len) p.id = a.table[b * a.table_stride + key / bs];
+        return key < r.len ? a.table[b * a.table_stride + key / bs] : -1;
+    };
+    auto page_scales = [&](AttnPages& p) {
         if (p.id < 0 || p.id >= a.c.blocks) p.id = -1;
         const int64_t at = (int64_t)max(p.id, 0) * a.c.heads + h;
-        p.sk = a.c.k_scale[at] * a.scale_log2;
+        p.sk = a.c.k_scale[at];
         p.sv = a.c.v_scale[at];
-        return p;
     };
     const uint32_t lds0 = (uint32_t)(uintptr_t)&ring[0] + (uint32_t)(grp * kChunkRing * 2 * TILE);
     // LDS row m of a half tile holds key 16 (m / 4 % 2) + 4 (m / 8) + m % 4 of it; rows
     // are swizzled by 16-byte chunks so that 16 lanes reading one chunk of 16 rows
     // touch every bank once (rows of 128 bytes: c ^ m / 2 % 8, of 64: c ^ m / 4 % 4).
     auto swz = [](int row64, int m, int c) { return row64 ? c ^ ((m >> 2) & 3) : c ^ ((m >> 1) & 7); };
-    auto issue = [&](const AttnPages& p, int j) {  // tile j of the group into its slot
-        // made opaque, so that the addresses are formed here instead of held over the loop
-        int ln = lane;
-        asm volatile("" : "+v"(ln));
-        const int tile = 2 * j + grp, t4 = 4 * (j & 15);
-        const uint32_t slot = lds0 + (uint32_t)((j % kChunkRing) * 2 * TILE);
+    // The loads of a tile are 2 DMA of this wave: x < DMA keys, else values. A lane's
+    // load x is at one place of a block in every tile (a group's tiles are 128 keys
+    // apart, whole blocks): `at` is that place in block 0, `from` the lane (times
+    // 4) of AttnPages with its chunk of tile 0.
+    uint64_t at[2 * DMA];
+    int from[2 * DMA];
 #pragma unroll
-        for (int x = 0; x < DMA; ++x) {
-            const int i = wr + 4 * x;
-            const int m = i * (1024 / D) + ln / KC, c = swz(D == 64, m, ln % KC), m32 = m & 31;
-            const int key = (m & 32) + 16 * ((m32 >> 2) & 1) + 4 * (m32 >> 3) + (m32 & 3);
-            const int id = max(__shfl(p.id, t4 + (key >> 4)), 0);
-            lds_dma_b128(a.c.k + id * a.c.k_stride + ((int64_t)h * bs + ((64 * tile + key) & (bs - 1))) * D + 16 * c,
-                         slot + (uint32_t)(1024 * i));
-        }
+    for (int x = 0; x < DMA; ++x) {
+        const int i = wr + 4 * x;
+        const int m = i * (1024 / D) + lane / KC, c = swz(D == 64, m, lane % KC), m32 = m & 31;
+        const int key = (m & 32) + 16 * ((m32 >> 2) & 1) + 4 * (m32 >> 3) + (m32 & 3);
+        at[x] = (uint64_t)(uintptr_t)a.c.k + ((int64_t)h * bs + ((64 * grp + key) & (bs - 1))) * D + 16 * c;
+        from[x] = 4 * (key >> 4);
+        const int d = 16 * i + lane / 4, vc = swz(1, d, lane & 3);
+        at[DMA + x] = (uint64_t)(uintptr_t)a.c.v + ((int64_t)h * D + d) * bs + ((64 * grp + 16 * vc) & (bs - 1));
+        from[DMA + x] = 4 * vc;
+    }
+    const uint32_t k_stride = (uint32_t)a.c.k_stride, v_stride = (uint32_t)a.c.v_stride;  // below 2^31
+    auto load_id = [&](int x, int ids, int j) { return __builtin_amdgcn_ds_bpermute(from[x] + 16 * (j & 15), ids); };
+    auto issue_one = [&](int x, int id, int in) {  // from block id into tile in's slot
+        const uint32_t slot = lds0 + (uint32_t)((in % kChunkRing) * 2 * TILE + 1024 * (wr + 4 * (x % DMA)));
+        const uint64_t src = at[x] + (uint64_t)(uint32_t)max(id, 0) * (x < DMA ? k_stride : v_stride);
+        lds_dma_b128((const void*)(uintptr_t)src, x < DMA ? slot : slot + TILE);
+    };
+    auto issue = [&](const AttnPages& p, int j) {
 #pragma unroll
-        for (int x = 0; x < DMA; ++x) {
-            const int i = wr + 4 * x;
-            const int d = 16 * i + ln / 4, c = swz(1, d, ln & 3);
-            const int id = max(__shfl(p.id, t4 + c), 0);
-            lds_dma_b128(a.c.v + id * a.c.v_stride + ((int64_t)h * D + d) * bs + ((64 * tile + 16 * c) & (bs - 1)),
-                         slot + (uint32_t)(TILE + 1024 * i));
-        }
+        for (int x = 0; x < 2 * DMA; ++x) issue_one(x, load_id(x, p.id, j), j);
     };
 
     f32x16 o[DT], s[2];
@@ -645,28 +648,58 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, 
         for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
     float m = -INFINITY, l = 0.f;
     u32x4 hi[4], lo[4];  // P^T: [2 e + u], half tile e, its keys 8 u .. of each lane half
-    AttnPages pg = pages(0), nx = pg;  // of the tile whose softmax is next; of the tiles 16 on
-    if (n > 16) nx = pages(16);
+    AttnPages pg, nx;  // of the tile whose softmax is next; of the tiles 16 on
+    pg.id = page_ids(0);
+    page_scales(pg);
+    nx = pg;
+    if (n > 16) {
+        nx.id = page_ids(16);
+        page_scales(nx);
+    }
+    // What the next softmax needs of its tile's two chunks of this lane.
+    float sk[2], sv[2];
+    int chunk_id[2];
+    auto take_scales = [&](int j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int lane4 = 16 * (j & 15) + 8 * e + 4 * hh;
+            sk[e] = __uint_as_float(__builtin_amdgcn_ds_bpermute(lane4, (int)__float_as_uint(pg.sk)));
+            sv[e] = __uint_as_float(__builtin_amdgcn_ds_bpermute(lane4, (int)__float_as_uint(pg.sv)));
+            chunk_id[e] = __builtin_amdgcn_ds_bpermute(lane4, pg.id);
+        }
+    };
+    u32x4 vf[2];  // value fragments; the first of a tile is read before its M phase
+    auto load_v = [&](int j, int st, int x) {
+        uint32_t so = (uint32_t)((grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE);
+        asm volatile("" : "+s"(so));
+        vf[x] = *reinterpret_cast<const u32x4*>(ring + so + (32 * (st % KK) + l32) * 64 + 16 * swz(1, l32, 2 * (st / KK) + hh));
+    };
 
-    // This wave's part of tile j's values, which has landed: NaN codes out of it.
-    auto check_values = [&](int j) {
-        uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
-        u32x4 w[DMA];
+    // This wave's part of tile j's values, which has landed: NaN codes out of it. (The
+    // tile's product is two barriers away.)
+    u32x4 part[DMA];
+    auto read_part = [&](int j) {
+        const uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
+#pragma unroll
+        for (int x = 0; x < DMA; ++x) part[x] = *reinterpret_cast<const u32x4*>(mine + 1024 * (wr + 4 * x));
+    };
+    auto check_part = [&](int j) {
         uint32_t bad = 0;
 #pragma unroll
-        for (int x = 0; x < DMA; ++x) {
-            w[x] = *reinterpret_cast<const u32x4*>(mine + 1024 * (wr + 4 * x));
-            bad |= nan_codes(w[x][0]) | nan_codes(w[x][1]) | nan_codes(w[x][2]) | nan_codes(w[x][3]);
-        }
-        const bool any = __any(bad != 0);
+        for (int x = 0; x < DMA; ++x)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) bad |= (part[x][y] & 0x7f7f7f7fu) + 0x01010101u;
+        const bool any = __any((bad & 0x80808080u) != 0);
         if (lane == 0) with_nan[2 * grp + (j & 1)][wr] = any;
         if (!any) return;
+        uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
 #pragma unroll
         for (int x = 0; x < DMA; ++x) {
-            *reinterpret_cast<u32x4*>(raw[2 * grp + (j & 1)] + 1024 * (wr + 4 * x) + 16 * lane) = w[x];
+            u32x4 w = part[x];
+            *reinterpret_cast<u32x4*>(raw[2 * grp + (j & 1)] + 1024 * (wr + 4 * x) + 16 * lane) = w;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) w[x][y] &= ~((nan_codes(w[x][y]) >> 7) * 0xffu);
-            *reinterpret_cast<u32x4*>(mine + 1024 * (wr + 4 * x)) = w[x];
+            for (int y = 0; y < 4; ++y) w[y] &= ~((nan_codes(w[y]) >> 7) * 0xffu);
+            *reinterpret_cast<u32x4*>(mine + 1024 * (wr + 4 * x)) = w;
         }
     };
     // NaN codes among tile j's values: NaN sums for the rows that see them, by a product of indicators.
@@ -696,32 +729,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, 
         }
     };
 
-    // One M phase: S of tile js and O += P V of tile jp (if DP).
-    auto m_phase = [&](auto dp_tag, int js, int jp) {
+    // One M phase: S of tile js and O += P V of tile jp (if DP); on its way the loads of
+    // tile ji are issued into tile in's slot (that of the tile before jp), the part of tile js
+    // that this wave loaded is checked, and the scales of js are taken.
+    auto m_phase = [&](auto dp_tag, int js, int jp, const AttnPages& pi, int ji, int in) {
         constexpr bool DP = decltype(dp_tag)::value;
+        constexpr int ST = 2 * KK;
         uint32_t so_k = (uint32_t)((grp * kChunkRing + js % kChunkRing) * 2 * TILE);
-        uint32_t so_v = (uint32_t)((grp * kChunkRing + jp % kChunkRing) * 2 * TILE + TILE);
-        asm volatile("" : "+s"(so_k), "+s"(so_v));
+        asm volatile("" : "+s"(so_k));
         const uint8_t* ks = ring + so_k;
-        const uint8_t* vs = ring + so_v;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[e][i] = 0.f;
-        u32x4 kf[2], vf[2];
-        auto load = [&](int st, int x) {
-            const int e = st / KK, k = st % KK;
-            kf[x] = *reinterpret_cast<const u32x4*>(ks + (32 * e + l32) * D + 16 * swz(D == 64, l32, 2 * k + hh));
-            if constexpr (DP) vf[x] = *reinterpret_cast<const u32x4*>(vs + (32 * k + l32) * 64 + 16 * swz(1, l32, 2 * e + hh));
+        u32x4 kf[2];
+        auto load_k = [&](int st, int x) {
+            kf[x] = *reinterpret_cast<const u32x4*>(ks + (32 * (st / KK) + l32) * D + 16 * swz(D == 64, l32, 2 * (st % KK) + hh));
         };
-        load(0, 0);
+        int ids[2 * DMA];
+        load_k(0, 0);
+        if constexpr (DP) {
 #pragma unroll
-        for (int st = 0; st < 2 * KK; ++st) {
+            for (int x = 0; x < 2 * DMA; ++x) ids[x] = load_id(x, pi.id, ji);
+        }
+#pragma unroll
+        for (int st = 0; st < ST; ++st) {
             const int e = st / KK, k = st % KK;
-            if (st + 1 < 2 * KK) load(st + 1, (st + 1) & 1);
-            const u32x4 kw = kf[st & 1];
-            s[e] = mfma32x32x16(fp8x8_to_half8(kw[0], kw[1], T{}), q[2 * k], s[e], T{});
-            s[e] = mfma32x32x16(fp8x8_to_half8(kw[2], kw[3], T{}), q[2 * k + 1], s[e], T{});
+            if (st + 1 < ST) {
+                load_k(st + 1, (st + 1) & 1);
+                if constexpr (DP) load_v(jp, st + 1, (st + 1) & 1);
+            }
+            if (st == ST / 2) read_part(js);
+            if (st == ST / 2 + 1) take_scales(js);
             if constexpr (DP) {
                 const u32x4 w = vf[st & 1];
                 const u32x4 v0 = fp8x8_to_half8(w[0], w[1], bf16_t{}), v1 = fp8x8_to_half8(w[2], w[3], bf16_t{});
@@ -732,66 +767,93 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, 
                     o[k] = mfma32x32x16(v1, lo[2 * e + 1], o[k], bf16_t{});
                 }
             }
+            const u32x4 kw = kf[st & 1];
+            f32x16 zero;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+            s[e] = mfma32x32x16(fp8x8_to_half8(kw[0], kw[1], T{}), q[2 * k], k == 0 ? zero : s[e], T{});
+            s[e] = mfma32x32x16(fp8x8_to_half8(kw[2], kw[3], T{}), q[2 * k + 1], s[e], T{});
+            if constexpr (DP) {
+                if (st >= 1 && st <= 2 * DMA) issue_one(st - 1, ids[st - 1], in);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
+        check_part(js);
     };
     // The softmax of tile j, whose scores are in s: P into hi (and lo).
     auto v_phase = [&](int j) {
-        const int key0 = 64 * (2 * j + grp), t4 = 4 * (j & 15) + hh;
-        float sk[2], sv[2];
+        const int key0 = 64 * (2 * j + grp);
         int seen[2];
-        bool part = false;
+        bool odd = false;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            sk[e] = __shfl(pg.sk, t4 + 2 * e);
-            sv[e] = __shfl(pg.sv, t4 + 2 * e);
-            const int id = __shfl(pg.id, t4 + 2 * e), key = key0 + 32 * e + 16 * hh;
-            seen[e] = id < 0 ? 0 : min(min(r.len, limit + 1) - key, 16);
-            part |= seen[e] < 16;
+            sk[e] *= a.scale_log2;
+            const int key = key0 + 32 * e + 16 * hh;
+            seen[e] = chunk_id[e] < 0 ? 0 : min(min(r.len, limit + 1) - key, 16);
+            odd |= seen[e] < 16 || !(sv[e] >= 0x1p-64f && sv[e] <= 0x1p64f);
         }
-        const bool clean = !__any(part);
+        // Nothing masked and ordinary scales: the value scale goes into the exponent,
+        // p sv = 2^(x + log2 sv), and out of the chunk's sum once. Else p is
+        // masked and multiplied.
+        const bool plain = !__any(odd);
         const float ref = m == -INFINITY ? 0.f : m;
+        float add[2], out[2];
+        if (plain) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                add[e] = __builtin_amdgcn_logf(sv[e]) - ref;
+                out[e] = __builtin_amdgcn_rcpf(sv[e]);
+            }
+        } else {
+            add[0] = add[1] = -ref;
+            out[0] = out[1] = 1.0f;
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[e][i] = fmaf(s[e][i], sk[e], -ref);
-        if (!clean) {
+            for (int i = 0; i < 16; ++i) s[e][i] = fmaf(s[e][i], sk[e], add[e]);
+        if (!plain) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[e][i] = i < seen[e] ? s[e][i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) {
+                    float x = i < seen[e] ? s[e][i] : -INFINITY;
+                    asm volatile("" : "+v"(x));  // keeps the masking inside this branch
+                    s[e][i] = x;
+                }
         }
-        auto exponentiate = [&]() {  // P, and the sum of p
-            float sum[2] = {0.f, 0.f};
+        auto pack = [&](int e, int i, float x0, float x1) {
+            const uint32_t w = pack_half2(x0, x1, bf16_t{});
+            hi[2 * e + (i >> 3)][(i & 7) >> 1] = w;
+            if constexpr (SPLIT)
+                lo[2 * e + (i >> 3)][(i & 7) >> 1] =
+                    pack_half2(x0 - __uint_as_float(w << 16), x1 - __uint_as_float(w & 0xffff0000u), bf16_t{});
+        };
+        auto exponentiate = [&]() {  // s becomes what is rounded to P; the sum of p
+            float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(s[e][i]), p1 = __builtin_amdgcn_exp2f(s[e][i + 1]);
-                    sum[0] += p0;
-                    sum[1] += p1;
-                    float x0 = p0 * sv[e], x1 = p1 * sv[e];
-                    if (!clean) {  // sv may be anything
-                        x0 = i < seen[e] ? x0 : 0.f;
-                        x1 = i + 1 < seen[e] ? x1 : 0.f;
-                    }
-                    const uint32_t w = pack_half2(x0, x1, bf16_t{});
-                    hi[2 * e + (i >> 3)][(i & 7) >> 1] = w;
-                    if constexpr (SPLIT)
-                        lo[2 * e + (i >> 3)][(i & 7) >> 1] = pack_half2(
-                            x0 - __uint_as_float(w << 16), x1 - __uint_as_float(w & 0xffff0000u), bf16_t{});
+                    sum[e][0] += p0;
+                    sum[e][1] += p1;
+                    pack(e, i, p0, p1);
                 }
-            return sum[0] + sum[1];
+            return (sum[0][0] + sum[0][1]) * out[0] + (sum[1][0] + sum[1][1]) * out[1];
         };
         float sum = exponentiate();
         const bool fresh = m == -INFINITY && (seen[0] > 0 || seen[1] > 0);
         if (__any(fresh || !(sum <= kChunkSumMax))) {
             // both lane halves of a row move together
-            float mx = s[0][0];
+            float mx = -INFINITY;
 #pragma unroll
-            for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[0][i]);
+            for (int e = 0; e < 2; ++e) {
+                float me = s[e][0];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[1][i]);
+                for (int i = 1; i < 16; ++i) me = __builtin_elementwise_maximum(me, s[e][i]);
+                mx = __builtin_elementwise_maximum(mx, me - (add[e] + ref));
+            }
             const float mo = __shfl_xor(mx, 32), so = __shfl_xor(sum, 32);
             mx = __builtin_elementwise_maximum(mx, mo);  // of the row, above ref
             const bool move = mx != -INFINITY && (m == -INFINITY || !(sum <= kChunkSumMax) || !(so <= kChunkSumMax));
@@ -810,6 +872,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, 
                 for (int i = 0; i < 16; ++i) s[e][i] -= shift;
             sum = exponentiate();
         }
+        if (!plain) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(s[e][i]), p1 = __builtin_amdgcn_exp2f(s[e][i + 1]);
+                    pack(e, i, i < seen[e] ? p0 * sv[e] : 0.f, i + 1 < seen[e] ? p1 * sv[e] : 0.f);  // sv may be anything
+                }
+        }
         l += sum;
         const int* nan = with_nan[2 * grp + (j & 1)];
         if (__builtin_amdgcn_readfirstlane(nan[0] | nan[1] | nan[2] | nan[3])) nan_values(j, seen);
@@ -823,38 +894,41 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, 
         } else {
             wait_vmem_le<0>();
         }
-        check_values(0);
         __syncthreads();                // ... and every wave's
         if (grp == 1) __syncthreads();  // group 1 is one phase behind
-        m_phase(std::false_type{}, 0, 0);
+        m_phase(std::false_type{}, 0, 0, pg, 0, 0);
         __syncthreads();
         v_phase(0);
         wait_vmem_le<0>();
-        if (n > 1) check_values(1);
+        load_v(0, 0, 0);
         __syncthreads();
         for (int k = 0; k < n; ++k) {
+            // The last tiles' M phases do as the others: load the last tile once more, into a
+            // slot that nobody reads, and compute an S of whatever its slot holds.
+            if (((k + 1) & 15) == 0) pg = nx;
+            const int ji = min(k + 2, n - 1);
+            AttnPages pi;
+            pi.id = (ji & 15) == 0 && ji > k + 1 ? nx.id : pg.id;
             // The wave in its M phase goes first: the softmax of the SIMD's other wave
-            // takes the cycles that its matrix instructions leave. (The last S is of
-            // a tile that does not exist: whatever its slot holds, nobody reads it.)
+            // takes the cycles that its matrix instructions leave.
             __builtin_amdgcn_s_setprio(2);
-            if (k + 2 < n) issue(((k + 2) & 15) < 2 && k + 2 >= 16 ? nx : pg, k + 2);
-            m_phase(std::true_type{}, k + 1, k);
+            m_phase(std::true_type{}, k + 1, k, pi, ji, k + 2);
             __builtin_amdgcn_s_setprio(0);
             __syncthreads();
             if (k + 1 < n) {
-                if (((k + 1) & 15) == 0) {
-                    pg = nx;
-                    if (k + 17 < n) nx = pages(k + 17);
-                }
+                // the next 16 tiles' blocks, then their scales: they have tiles' time to come
+                if (((k + 1) & 15) == 1 && (k & ~15) + 16 < n) nx.id = page_ids((k & ~15) + 16);
+                if (((k + 1) & 15) == 3) page_scales(nx);
                 v_phase(k + 1);
                 wait_vmem_le<0>();  // tile k + 2 landed
-                if (k + 2 < n) check_values(k + 2);
+                load_v(k + 1, 0, 0);
                 __syncthreads();
             }
         }
         if (grp == 0) __syncthreads();
     }
-    __syncthreads();  // the rings are free
+    wait_vmem_le<0>();  // no load into a ring is on its way
+    __syncthreads();    // the rings are free
 
     // Join: group g ends with channels 32 t .. of t in its half.
     {

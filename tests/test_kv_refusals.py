@@ -22,6 +22,7 @@ def _cache(**kw):
 
 BAD_CACHES = [dict(k=None), dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(k=P + 8), dict(v=P + 1),
               dict(k_scale=P + 2), dict(k_block_stride=2 * 16 * 64 - 16), dict(v_block_stride=2 * 16 * 64 + 8),
+              dict(k_block_stride=1 << 31), dict(v_block_stride=1 << 40),
               dict(num_blocks=0), dict(num_blocks=-1), dict(num_blocks=1 << 28), dict(kv_heads=0), dict(block_size=8),
               dict(block_size=48), dict(block_size=256), dict(head_dim=96), dict(head_dim=256)]
 
