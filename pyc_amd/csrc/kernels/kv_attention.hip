@@ -58,6 +58,15 @@ __device__ inline AttnReq attn_request(const AttnArgs& a, int b) {
     return r;
 }
 
+// Values that are the same in all lanes, into scalar registers.
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline int64_t uniform(int64_t x) {
+    return (int64_t)(((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
+}
+__device__ inline AttnReq uniform(const AttnReq& r) {
+    return AttnReq{uniform(r.len), uniform(r.n), uniform(r.first), uniform(r.rows)};
+}
+
 __device__ inline uint32_t pack_half2(float lo, float hi, bf16_t) {
     typedef __attribute__((ext_vector_type(2))) float f2;
     typedef __attribute__((ext_vector_type(2))) __bf16 h2;
@@ -66,13 +75,6 @@ __device__ inline uint32_t pack_half2(float lo, float hi, bf16_t) {
 
 // Bit 7 of every byte that is a NaN code.
 __device__ inline uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
-// Requests of up to most_rows rows are the split kernel's; the others go to kv_chunk_kernel.
-struct AttnSplit {
-    int most_rows;
-    float* part;       // two partial results for each wave
-    int64_t part_size; // floats of one: [most_rows][D] sums, then [most_rows][2] maximum and sum
-};
 
 // The blocks and scales of 16 tiles of 64 keys: lane l has chunk l % 4 of tile l / 4.
 struct AttnPages {
@@ -325,172 +327,341 @@ template <typename T, int D, int NT> struct AttnWave {
         }
     }
 
-    // A part of the rows' keys: sums, maximum and sum of p.
-    __device__ void store_part(const AttnReq& r, const AttnSplit& sp, int64_t slot) {
+    // A part of the rows' keys: sums in rows of D + 4 (off the banks' stride), maximum and sum of p.
+    __device__ void store_part(int live, float* sums, float* ml) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
-        float* dst = sp.part + slot * sp.part_size;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int row = 16 * n + (lane & 15);
             float sum = l[n];
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            if (row >= r.rows) continue;
+            if (row >= live) continue;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(dst + row * D + 16 * dt + 4 * g) = o[n][dt];
+            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(sums + row * (D + 4) + 16 * dt + 4 * g) = o[n][dt];
             if (g == 0) {
-                float* ml = dst + (int64_t)sp.most_rows * D + 2 * row;
-                ml[0] = m[n];
-                ml[1] = sum;
+                ml[2 * row] = m[n];
+                ml[2 * row + 1] = sum;
             }
         }
     }
 };
 
-// The split kernel's work: for every request of at most most_rows rows and every kv
-// head a run of tiles of 64 keys, all runs one after the other (request, head, tile),
-// cut into equal pieces, one for each wave. A run that falls into several pieces is
-// joined by kv_join_kernel.
-__device__ inline int attn_tiles(const AttnArgs& a, const AttnReq& r, int most_rows) {
+// ---------------------------------------------------------------------------
+// Requests of few rows (decoding, draft tokens): reading the cache is the work, so
+// it is cut evenly. A request of up to most_rows rows has, for every kv head and every
+// 16 NT rows, a run of tiles of 64 keys; all runs, one after the other, are cut into
+// one piece for each wave. What a wave finds of a run it leaves in LDS unless it has
+// all of it; the workgroup joins what its waves have of one run, and where a run goes
+// on in other workgroups, the last of these to be done joins all. Up to 256 short runs
+// get a workgroup each instead: then no run crosses one.
+struct AttnSplit {
+    int most_rows;
+    float* part;     // two results of every workgroup: [16 NT][D] sums, [16 NT][2] maximum and sum
+    uint32_t* done;  // for every run that workgroups share: how many are done; zero between calls
+};
+constexpr int kSplitGroups = 256;
+__host__ __device__ constexpr int split_waves(int nt) { return nt == 1 ? 8 : 4; }
+
+struct SplitPart {  // a part of a run in LDS
+    int b, h, rt, t0, t1, tiles, live, first;
+    int64_t begin;  // the run's first unit
+};
+template <int D, int NT> struct SplitShare {
+    static constexpr int WAVES = split_waves(NT), ROWS = 16 * NT;
+    float sums[2 * WAVES][ROWS][D + 4];
+    float ml[2 * WAVES][ROWS][2];
+    SplitPart part[2 * WAVES];
+    int last[2];
+};
+
+// Tiles of a request's runs (0: it is not the split kernel's), and its runs of a head.
+__device__ inline int split_tiles(const AttnArgs& a, const AttnReq& r, int most_rows) {
     if (r.rows <= 0 || r.rows > most_rows) return 0;
     const int end = r.len - r.n + r.rows / a.G;  // keys that the last row sees
     return max(1, end / 64 + (end % 64 > 0 ? 1 : 0));
 }
-__device__ inline int64_t attn_tiles64(const AttnArgs& a, int b, int most_rows) {
-    return b < a.B ? attn_tiles(a, attn_request(a, b), most_rows) : 0;
+template <int ROWS> __device__ inline void split_request(const AttnArgs& a, int b, int most_rows, int* tiles, int* runs) {
+    *tiles = *runs = 0;
+    if (b >= a.B) return;
+    const AttnReq r = attn_request(a, b);
+    *tiles = split_tiles(a, r, most_rows);
+    *runs = *tiles ? (r.rows + ROWS - 1) / ROWS : 0;
 }
 __device__ inline int64_t wave_sum(int64_t x) {
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
     return x;
 }
-__device__ inline int64_t attn_total(const AttnArgs& a, int most_rows) {
-    int64_t sum = 0;
-    for (int b0 = 0; b0 < a.B; b0 += kWave) sum += attn_tiles64(a, b0 + (threadIdx.x & 63), most_rows);
-    return wave_sum(sum) * a.c.heads;
+// 64-bit quotients are slow and rarely needed.
+__device__ inline uint64_t div_u64(uint64_t n, uint64_t d) {
+    return ((n | d) >> 32) == 0 ? (uint32_t)n / (uint32_t)d : n / d;
 }
-// The request that unit u (0 <= u < total) belongs to, and the units before it.
-__device__ inline int attn_locate(const AttnArgs& a, int most_rows, int64_t u, int64_t* before) {
-    const int lane = threadIdx.x & 63;
-    int64_t base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += kWave) {
-        const int64_t mine = attn_tiles64(a, b0 + lane, most_rows) * a.c.heads;
-        int64_t end = mine;
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const int64_t x = __shfl_up(end, d);
-            if (lane >= d) end += x;
-        }
-        end += base;
-        const uint64_t past = __ballot(end > u);
-        if (past) {
-            const int i = __builtin_ctzll(past);
-            *before = __shfl(end - mine, i);
-            return b0 + i;
-        }
-        base = __shfl(end, kWave - 1);
-    }
-    return -1;
+// Piece w of W begins at floor(total w / W); the last piece that begins at or before
+// u. There are fewer than 2^12 pieces and 2^50 units: no product passes 64 bits.
+__device__ inline int64_t piece_begin(int64_t total, int W, int w) { return (int64_t)div_u64((uint64_t)total * w, W); }
+__device__ inline int piece_of(int64_t total, int W, int64_t u) {
+    return (int)div_u64((uint64_t)(u + 1) * W - 1, (uint64_t)total);
 }
-// Piece w of W begins at floor(total w / W). There are fewer than 2^12 pieces and
-// 2^50 units: no product passes 64 bits.
-__device__ inline int64_t piece_begin(int64_t total, int W, int w) { return total * w / W; }
-// The last piece that begins at or before u.
-__device__ inline int piece_of(int64_t total, int W, int64_t u) { return (int)(((u + 1) * W - 1) / total); }
 
-constexpr int kSplitWaves = 4;
+template <typename T, int D> struct SplitRow {  // a row of results, D / 64 channels a lane
+    static constexpr int E = D / 64;
+    float x[E], m, l;
+    __device__ void store(const AttnArgs& a, const SplitPart& p, int row) const {
+        const int lane = threadIdx.x & 63, at = p.rt + row;  // row of the request and head
+        const float inv = m == -INFINITY ? 0.f : 1.0f / l;
+        uint16_t* dst = a.o + (int64_t)(p.first + at / a.G) * a.o_stride + (int64_t)(p.h * a.G + at % a.G) * D + E * lane;
+        if constexpr (E == 2)
+            *reinterpret_cast<uint32_t*>(dst) =
+                (uint32_t)elem<T>::from_f32(x[0] * inv) | ((uint32_t)elem<T>::from_f32(x[1] * inv) << 16);
+        else
+            *dst = elem<T>::from_f32(x[0] * inv);
+    }
+};
+__device__ inline uint64_t pack_floats(float a, float b) {
+    return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+}
+// Accesses to what workgroups on other XCDs read or wrote (their L2 caches are not coherent).
+__device__ inline void agent_store(uint64_t* p, uint64_t v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline uint64_t agent_load(const uint64_t* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float wave_max(float x) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) x = __builtin_elementwise_maximum(x, __shfl_xor(x, d));
+    return x;
+}
+__device__ inline float wave_sum(float x) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
+    return x;
+}
+__device__ inline float read_lane(float x, int i) {
+    return __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(x), i));
+}
+
+// Workgroup wg of `groups`.
+template <typename T, int D, int NT>
+__device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitShare<D, NT>& sh, int wg, int groups) {
+    constexpr int WAVES = split_waves(NT), ROWS = 16 * NT, E = D / 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    // All units (tiles of all runs), all runs, the longest run.
+    int tiles0, runs0;
+    split_request<ROWS>(a, lane, sp.most_rows, &tiles0, &runs0);
+    int64_t total = (int64_t)tiles0 * runs0, runs = runs0;
+    int longest = tiles0;
+    for (int b0 = kWave; b0 < a.B; b0 += kWave) {
+        int t, n;
+        split_request<ROWS>(a, b0 + lane, sp.most_rows, &t, &n);
+        total += (int64_t)t * n;
+        runs += n;
+        longest = max(longest, t);
+    }
+    total = uniform(wave_sum(total) * a.c.heads);
+    runs = uniform(wave_sum(runs) * a.c.heads);
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) longest = max(longest, __shfl_xor(longest, d));
+    const bool aligned = runs <= groups && uniform(longest) <= 2 * WAVES;
+    const int W = (int)min((int64_t)groups * WAVES, total);
+
+    // This wave's piece: `left` units from tile t0 of run (b, h, rt); unit u of all.
+    int64_t u = 0, left = 0, before = 0;
+    int b = 0, h = 0, rt = 0, t0 = 0, w = wg * WAVES + wave;
+    if (aligned) {
+        u = wg;  // a run here, counted below as a unit
+        left = wg < runs ? 1 : 0;
+    } else if (w < W) {
+        u = piece_begin(total, W, w);
+        left = piece_begin(total, W, w + 1) - u;
+    }
+    if (left > 0) {
+        int64_t base = 0;
+        for (int b0 = 0; b0 < a.B; b0 += kWave) {
+            int t = tiles0, n = runs0;
+            if (b0) split_request<ROWS>(a, b0 + lane, sp.most_rows, &t, &n);
+            const int64_t mine = (int64_t)n * (aligned ? 1 : t) * a.c.heads;
+            int64_t end = mine;
+#pragma unroll
+            for (int d = 1; d < kWave; d *= 2) {
+                const int64_t x = __shfl_up(end, d);
+                if (lane >= d) end += x;
+            }
+            end += base;
+            const uint64_t past = __ballot(end > u);
+            if (past) {
+                const int i = __builtin_ctzll(past);
+                before = __shfl(end - mine, i);
+                b = b0 + i;
+                break;
+            }
+            base = __shfl(end, kWave - 1);
+        }
+    }
+    b = uniform(b);
+    before = uniform(before);
+    AttnReq r = uniform(attn_request(a, b));
+    int tiles = split_tiles(a, r, sp.most_rows), n_rt = (r.rows + ROWS - 1) / ROWS;
+    if (left > 0) {
+        const int64_t v = u - before;
+        const int64_t run = aligned ? v : (int64_t)div_u64(v, tiles);
+        h = (int)div_u64(run, n_rt);
+        rt = (int)(run - (int64_t)h * n_rt);
+        if (aligned) {  // the workgroup's run, a piece for each wave
+            t0 = tiles * wave / WAVES;
+            left = tiles * (wave + 1) / WAVES - t0;
+            u = t0;  // not looked at again but for u - t0, the run's first unit
+        } else {
+            t0 = (int)(v - run * tiles);
+        }
+    }
+    h = uniform(h);
+    rt = uniform(rt);
+    t0 = uniform(t0);
+    u = uniform(u);
+    left = uniform(left);
+    if (lane < 2) sh.part[2 * wave + lane].t1 = 0;
+    while (left > 0) {
+        const int t1 = (int)min((int64_t)tiles, t0 + left);
+        AttnWave<T, D, NT> wv;
+        wv.begin(a, r, h, ROWS * rt);
+        wv.run(a, r, b, h, t0, t1);
+        if (t0 == 0 && t1 == tiles) {
+            wv.store(a, r, h, ROWS * rt);
+        } else {
+            const int at = 2 * wave + (t0 == 0 ? 1 : 0), live = min(r.rows - ROWS * rt, ROWS);
+            wv.store_part(live, &sh.sums[at][0][0], &sh.ml[at][0][0]);
+            if (lane == 0) sh.part[at] = SplitPart{b, h, ROWS * rt, t0, t1, tiles, live, r.first, u - t0};
+        }
+        u += t1 - t0;
+        left -= t1 - t0;
+        if (left <= 0) break;
+        t0 = 0;
+        if (++rt == n_rt) {
+            rt = 0;
+            if (++h == a.c.heads) {
+                h = 0;
+                do {
+                    r = uniform(attn_request(a, ++b));
+                    tiles = split_tiles(a, r, sp.most_rows);
+                } while (tiles == 0);  // ends: there are units left
+                n_rt = (r.rows + ROWS - 1) / ROWS;
+            }
+        }
+    }
+    __syncthreads();
+
+    // Join the parts in LDS. Lane i has part i's head: a part at 2 w + 1 begins a run,
+    // one at 2 w goes on with the part before it (of another workgroup, if it is the first).
+    SplitPart mine = sh.part[min(lane, 2 * WAVES - 1)];
+    if (lane >= 2 * WAVES) mine.t1 = 0;
+    const uint64_t have = __ballot(mine.t1 > 0);
+    uint64_t begins = __ballot(mine.t1 > 0 && (mine.t0 == 0 || (have & ((1ull << lane) - 1)) == 0));
+    int shared = 0;             // runs that go beyond this workgroup: at most its first and its last
+    int shared_at[2] = {0, 0};  // a part of each
+    for (uint64_t left_runs = begins; left_runs; left_runs &= left_runs - 1) {
+        const int i = __builtin_ctzll(left_runs);
+        const uint64_t later = left_runs & (left_runs - 1);
+        const uint64_t parts = have & (~0ull << i) & (later ? (1ull << __builtin_ctzll(later)) - 1 : ~0ull);
+        const int last = 63 - __builtin_clzll(parts);
+        const SplitPart& p = sh.part[i];
+        const bool whole = p.t0 == 0 && sh.part[last].t1 == p.tiles;
+        float* dst = sp.part + (2 * (int64_t)wg + (p.t0 == 0 ? 1 : 0)) * (ROWS * (D + 2));
+        for (int row = wave; row < p.live; row += WAVES) {
+            const bool in = (parts >> lane) & 1;
+            const int li = min(lane, 2 * WAVES - 1);
+            const float pm = in ? sh.ml[li][row][0] : -INFINITY, pl = in ? sh.ml[li][row][1] : 0.f;
+            SplitRow<T, D> o;
+            o.m = wave_max(pm);
+            const float wgt = __builtin_amdgcn_exp2f(pm - (o.m == -INFINITY ? 0.f : o.m));
+            o.l = wave_sum(in ? pl * wgt : 0.f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o.x[e] = 0.f;
+            for (uint64_t k = parts; k; k &= k - 1) {
+                const int j = __builtin_ctzll(k);
+                const float f = read_lane(wgt, j);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o.x[e] += f * sh.sums[j][row][E * lane + e];
+            }
+            if (whole) {
+                o.store(a, p, row);
+            } else {
+                if constexpr (E == 2)
+                    agent_store(reinterpret_cast<uint64_t*>(dst + row * D) + lane, pack_floats(o.x[0], o.x[1]));
+                else
+                    __hip_atomic_store(dst + row * D + lane, o.x[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (lane == 0) agent_store(reinterpret_cast<uint64_t*>(dst + ROWS * D) + row, pack_floats(o.m, o.l));
+            }
+        }
+        if (!whole) shared_at[shared++ & 1] = i;
+    }
+    if (shared == 0) return;
+    // Count the workgroup in; the last one of a run joins it.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores are where others see them
+    __syncthreads();
+    const int n_rt_most = (sp.most_rows + ROWS - 1) / ROWS;
+    if (threadIdx.x < shared) {
+        const SplitPart& p = sh.part[shared_at[threadIdx.x]];
+        const int w0 = piece_of(total, W, p.begin) / WAVES, w1 = piece_of(total, W, p.begin + p.tiles - 1) / WAVES;
+        uint32_t* done = sp.done + ((int64_t)p.b * a.c.heads + p.h) * n_rt_most + p.rt / ROWS;
+        const uint32_t before_me = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = before_me == (uint32_t)(w1 - w0);
+        if (last) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh.last[threadIdx.x] = last ? w1 - w0 + 1 : 0;
+        sh.part[shared_at[threadIdx.x]].t1 = w0;  // t1 has been used
+    }
+    __syncthreads();
+    for (int k = 0; k < shared; ++k) {
+        const int n = sh.last[k];
+        if (n == 0) continue;
+        const SplitPart& p = sh.part[shared_at[k]];
+        const int w0 = p.t1;
+        // workgroup w0 + i's result: of the run that it ends with, for the others the one they begin with
+        auto src = [&](int i) { return sp.part + (2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) * (ROWS * (D + 2)); };
+        for (int row = wave; row < p.live; row += WAVES) {
+            SplitRow<T, D> o;
+            o.m = -INFINITY;
+            o.l = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o.x[e] = 0.f;
+            for (int i0 = 0; i0 < n; i0 += kWave) {
+                const int cnt = min(n - i0, kWave), mi = min(i0 + lane, n - 1);
+                const uint64_t v = agent_load(reinterpret_cast<const uint64_t*>(src(mi) + ROWS * D) + row);
+                const bool in = lane < cnt;
+                const float pm = in ? __uint_as_float((uint32_t)v) : -INFINITY, pl = __uint_as_float((uint32_t)(v >> 32));
+                const float mx = __builtin_elementwise_maximum(o.m, wave_max(pm)), ref = mx == -INFINITY ? 0.f : mx;
+                const float keep = __builtin_amdgcn_exp2f(o.m - ref), wgt = __builtin_amdgcn_exp2f(pm - ref);
+                o.m = mx;
+                o.l = o.l * keep + wave_sum(in ? pl * wgt : 0.f);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o.x[e] *= keep;
+                for (int i = 0; i < cnt; i += 8) {
+                    uint64_t x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float* from = src(i0 + min(i + j, cnt - 1)) + row * D;
+                        if constexpr (E == 2) x[j] = agent_load(reinterpret_cast<const uint64_t*>(from) + lane);
+                        else
+                            x[j] = __float_as_uint(__hip_atomic_load(from + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float f = i + j < cnt ? read_lane(wgt, min(i + j, cnt - 1)) : 0.f;
+                        o.x[0] += f * __uint_as_float((uint32_t)x[j]);
+                        if constexpr (E == 2) o.x[1] += f * __uint_as_float((uint32_t)(x[j] >> 32));
+                    }
+                }
+            }
+            o.store(a, p, row);
+        }
+    }
+}
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kSplitWaves* kWave, NT == 1 ? 2 : 1) kv_split_kernel(AttnArgs a, AttnSplit sp) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int w = blockIdx.x * kSplitWaves + wave;
-    const int64_t total = attn_total(a, sp.most_rows);
-    const int W = (int)min((int64_t)gridDim.x * kSplitWaves, total);
-    if (w >= W) return;
-    int64_t u = piece_begin(total, W, w);
-    const int64_t end = piece_begin(total, W, w + 1);
-    int64_t before;
-    int b = __builtin_amdgcn_readfirstlane(attn_locate(a, sp.most_rows, u, &before));
-    if (b < 0) return;
-    AttnReq r = attn_request(a, b);
-    int tiles = attn_tiles(a, r, sp.most_rows);
-    int h = (int)((u - before) / tiles), t0 = (int)((u - before) % tiles);
-    for (;;) {
-        const int t1 = (int)min((int64_t)tiles, t0 + (end - u));
-        AttnWave<T, D, NT> wv;
-        wv.begin(a, r, h, 0);
-        wv.run(a, r, b, h, t0, t1);
-        if (t0 == 0 && t1 == tiles) wv.store(a, r, h, 0);
-        else wv.store_part(r, sp, 2 * (int64_t)w + (t0 == 0 ? 1 : 0));
-        u += t1 - t0;
-        if (u >= end) return;
-        t0 = 0;
-        if (++h == a.c.heads) {
-            h = 0;
-            do {
-                r = attn_request(a, ++b);
-                tiles = attn_tiles(a, r, sp.most_rows);
-            } while (tiles == 0);  // ends: there are units left
-        }
-    }
-}
-
-// Joins the parts of one row: thread 32 p + c takes channels D / 32 * c .. of parts p, p + 8, ...
-constexpr int kJoinParts = 8;
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * kJoinParts) kv_join_kernel(AttnArgs a, AttnSplit sp, int waves) {
-    constexpr int C = D / 32;
-    __shared__ float so[kJoinParts][D], sm[kJoinParts], sl[kJoinParts];
-    const int row = blockIdx.x, h = blockIdx.y, c = threadIdx.x & 31, p = threadIdx.x / 32;
-    const int64_t total = attn_total(a, sp.most_rows);
-    const int W = (int)min((int64_t)waves, total);
-    for (int b = blockIdx.z; b < a.B; b += gridDim.z) {
-        const AttnReq r = attn_request(a, b);
-        const int tiles = attn_tiles(a, r, sp.most_rows);
-        if (tiles == 0 || row >= r.rows) continue;
-        int64_t before = 0;
-        for (int b0 = 0; b0 < b; b0 += kWave) {
-            const int i = b0 + (threadIdx.x & 63);
-            before += i < b ? attn_tiles64(a, i, sp.most_rows) : 0;
-        }
-        before = wave_sum(before) * a.c.heads + (int64_t)h * tiles;
-        const int w0 = piece_of(total, W, before), w1 = piece_of(total, W, before + tiles - 1);
-        if (w0 == w1) continue;
-        float m = -INFINITY, l = 0.f, o[C];
-#pragma unroll
-        for (int i = 0; i < C; ++i) o[i] = 0.f;
-        for (int w = w0 + p; w <= w1; w += kJoinParts) {
-            const float* src = sp.part + (2 * (int64_t)w + (w == w0 ? 1 : 0)) * sp.part_size;
-            const float* ml = src + (int64_t)sp.most_rows * D + 2 * row;
-            const float pm = ml[0], pl = ml[1], mx = __builtin_elementwise_maximum(m, pm);
-            const float ref = mx == -INFINITY ? 0.f : mx;
-            const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(pm - ref);
-            m = mx;
-            l = l * f + pl * g;
-#pragma unroll
-            for (int i = 0; i < C; ++i) o[i] = o[i] * f + src[row * D + C * c + i] * g;
-        }
-#pragma unroll
-        for (int i = 0; i < C; ++i) so[p][C * c + i] = o[i];
-        if (c == 0) {
-            sm[p] = m;
-            sl[p] = l;
-        }
-        __syncthreads();
-        if (threadIdx.x < D) {
-            float mx = sm[0], sum = 0.f, x = 0.f;
-            for (int i = 1; i < kJoinParts; ++i) mx = __builtin_elementwise_maximum(mx, sm[i]);
-            const float ref = mx == -INFINITY ? 0.f : mx;
-            for (int i = 0; i < kJoinParts; ++i) {
-                const float g = __builtin_amdgcn_exp2f(sm[i] - ref);
-                sum += sl[i] * g;
-                x += so[i][threadIdx.x] * g;
-            }
-            a.o[(int64_t)(r.first + row / a.G) * a.o_stride + (int64_t)(h * a.G + row % a.G) * D + threadIdx.x] =
-                elem<T>::from_f32(mx == -INFINITY ? 0.f : x / sum);
-        }
-        __syncthreads();
-    }
+__global__ void __launch_bounds__(split_waves(NT) * kWave, 1) kv_split_kernel(AttnArgs a, AttnSplit sp) {
+    __shared__ SplitShare<D, NT> sh;
+    split_body<T, D, NT>(a, sp, sh, blockIdx.x, gridDim.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -506,10 +677,6 @@ __global__ void __launch_bounds__(32 * kJoinParts) kv_join_kernel(AttnArgs a, At
 constexpr int kChunkRows = 128;
 constexpr int kChunkRing = 3;
 constexpr int kChunkThreads = 512;
-constexpr size_t chunk_lds_bytes(int d) {  // rings, raw values, flags; maxima and sums to join
-    return (size_t)2 * kChunkRing * 2 * 64 * d + 4 * 64 * d + 64 + 8 * 32 * 2 * sizeof(float);
-}
-
 __device__ inline f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x16& c, bf16_t) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
@@ -527,31 +694,38 @@ __device__ inline int chunk_tiles(const AttnReq& r, int from_rows) {
 // overflow in bf16 (whose exponents are fp32's), and the common path has no maximum.
 constexpr float kChunkSumMax = 16384.0f;
 
+template <int D> struct ChunkShare {
+    static constexpr int TILE = 64 * D;
+    __attribute__((aligned(1024))) uint8_t ring[2 * kChunkRing * 2 * TILE];
+    // Value tiles that hold a NaN code, as they came, and which waves' parts of them
+    // are there; [group][tile % 2]. In the ring NaN codes are 0: the product then says
+    // nothing of them, and nan_values gives the NaN to the rows that see them.
+    __attribute__((aligned(16))) uint8_t raw[4][TILE];
+    __attribute__((aligned(16))) int with_nan[4][4];
+    float joint[8][32][2];
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, int from_rows) {
+__device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D>& sh, int part_index) {
     constexpr int KC = D / 16;            // 16-byte chunks of a key's row in LDS
     constexpr int KK = D / 32;            // pairs of k steps of S
     constexpr int DT = D / 32;            // 32-channel tiles of O^T
     constexpr int TILE = 64 * D;          // bytes of one operand of a tile
     constexpr int DMA = TILE / (4 * 1024);  // wave loads of an operand for each of a group's waves
     constexpr bool SPLIT = __is_same(T, f16_t);
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * kChunkRing * 2 * TILE];
-    // Value tiles that hold a NaN code, as they came, and which waves' parts of them
-    // are there; [group][tile % 2]. In the ring NaN codes are 0: the product then says
-    // nothing of them, and nan_values gives the NaN to the rows that see them.
-    __shared__ __attribute__((aligned(16))) uint8_t raw[4][TILE];
-    __shared__ __attribute__((aligned(16))) int with_nan[4][4];
-    __shared__ float joint[8][32][2];
-    static_assert(sizeof(ring) + sizeof(raw) + sizeof(with_nan) + sizeof(joint) == chunk_lds_bytes(D), "registered LDS figure");
+    auto& ring = sh.ring;
+    auto& raw = sh.raw;
+    auto& with_nan = sh.with_nan;
+    auto& joint = sh.joint;
     static_assert(8 * 64 * (DT / 2) * 64 <= (int)sizeof(ring), "room to join in");
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int grp = wave >> 2, wr = wave & 3, l32 = lane & 31, hh = lane >> 5, bs = a.c.bs;
 
-    // The part: blockIdx.x counts (request, row tile from the last, head).
+    // The part: part_index counts (request, row tile from the last, head).
     int b = -1, h = 0, rt = 0;
     {
-        int64_t u = blockIdx.x, base = 0;
+        int64_t u = part_index, base = 0;
         for (int b0 = 0; b0 < a.B && b < 0; b0 += kWave) {
             const int i = b0 + lane;
             const int64_t mine =
@@ -975,37 +1149,57 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, 
     }
 }
 
-constexpr int kSplitMost = 2048;  // waves: 8 on each of 256 CUs
+// A batch with requests of many rows: the first `parts` workgroups take parts of these,
+// the others split what the rest of the batch reads, on the CUs that are left.
+template <typename T, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, AttnSplit sp, int parts) {
+    static_assert(split_waves(1) * kWave == kChunkThreads, "one workgroup size");
+    union Share {
+        SplitShare<D, 1> split;
+        ChunkShare<D> chunk;
+    };
+    __shared__ Share sh;
+    if ((int)blockIdx.x < parts) chunk_body<T, D>(a, sp.most_rows, sh.chunk, blockIdx.x);
+    else split_body<T, D, 1>(a, sp, sh.split, blockIdx.x - parts, gridDim.x - parts);
+}
 
-// Rows that the split kernel takes per request, as 16s: all of them up to 64, else 16.
-static int split_tiles(long rows) { return rows <= 16 || rows > 64 ? 1 : rows <= 32 ? 2 : 4; }
+// Rows of a request that the split kernel takes, 16 NT of them a wave: all up to 64 at
+// NT = 2; of a batch with more, requests of up to 16 at NT = 1.
+constexpr int kSplitRows = 64;
+static int split_nt(long rows) { return rows <= 16 || rows > kSplitRows ? 1 : 2; }
+static long split_most_rows(long rows) { return rows <= kSplitRows ? rows : 16; }
+static long split_run_tiles(long rows) { return (split_most_rows(rows) + 16 * split_nt(rows) - 1) / (16 * split_nt(rows)); }
+// A workspace is the workgroups' results, in room for the largest of any call, then the
+// counters: these stay zero between calls whatever the calls' shapes.
+constexpr size_t kSplitPartBytes = (size_t)2 * kSplitGroups * 32 * (128 + 2) * sizeof(float);
 
-template <typename T, int D> static void launch_attention(const AttnArgs& a, float* part, int max_len, hipStream_t s) {
-    const long rows = (long)a.max_q * a.G;
-    const int nt = split_tiles(rows);
+template <typename T, int D> static void launch_attention(const AttnArgs& a, int max_q, void* workspace, int max_len,
+                                                           hipStream_t s) {
+    const long rows = (long)max_q * a.G, run_tiles = split_run_tiles(rows);  // as the workspace was made
+    const int nt = split_nt(rows), waves = split_waves(nt);
     AttnSplit sp;
-    sp.most_rows = (int)(rows < 16 * nt ? rows : 16 * nt);
-    sp.part = part;
-    sp.part_size = (int64_t)sp.most_rows * (D + 2);
+    sp.most_rows = (int)split_most_rows(rows);
+    sp.part = (float*)workspace;
+    sp.done = (uint32_t*)((char*)workspace + kSplitPartBytes);
+    // Workgroups of the split: for every wave a tile, for every run a workgroup, at most one on a CU.
     const long keys = max_len > 0 ? max_len : (long)a.width * a.c.bs;
-    const double units = (double)a.B * a.c.heads * (double)((keys + 63) / 64);
-    const int most = nt == 1 ? kSplitMost : kSplitMost / 2;
-    const int waves = units < most ? (int)units : most;
-    const int groups = (waves + kSplitWaves - 1) / kSplitWaves;
-    const unsigned zb = a.B < 65535 ? a.B : 65535;
-    const dim3 block(kSplitWaves * kWave);
-    if (nt == 1) hipLaunchKernelGGL((kv_split_kernel<T, D, 1>), dim3(groups), block, 0, s, a, sp);
-    else if (nt == 2) hipLaunchKernelGGL((kv_split_kernel<T, D, 2>), dim3(groups), block, 0, s, a, sp);
-    else hipLaunchKernelGGL((kv_split_kernel<T, D, 4>), dim3(groups), block, 0, s, a, sp);
-    hipLaunchKernelGGL((kv_join_kernel<T, D>), dim3(sp.most_rows, a.c.heads, zb), dim3(32 * kJoinParts), 0, s, a, sp,
-                       groups * kSplitWaves);
-    if (rows > sp.most_rows) {
-        // row tiles: whole ones, and one more for each request that is large enough
-        const long all = (long)a.tokens * a.G, some = all / (sp.most_rows + 1);
-        const long tiles = all / kChunkRows + (some < a.B ? some : a.B);
-        hipLaunchKernelGGL((kv_chunk_kernel<T, D>), dim3((unsigned)(tiles * a.c.heads)), dim3(kChunkThreads), 0, s, a,
-                           sp.most_rows);
+    const double runs = (double)a.B * a.c.heads * run_tiles, units = runs * (double)((keys + 63) / 64);
+    double groups = units / waves;
+    if (groups < runs) groups = runs;
+    const int split = groups < kSplitGroups ? (int)groups : kSplitGroups;
+    if (rows <= kSplitRows) {
+        if (nt == 1) hipLaunchKernelGGL((kv_split_kernel<T, D, 1>), dim3(split), dim3(waves * kWave), 0, s, a, sp);
+        else hipLaunchKernelGGL((kv_split_kernel<T, D, 2>), dim3(split), dim3(waves * kWave), 0, s, a, sp);
+        return;
     }
+    // Where most requests must have about max_q tokens, all are taken as chunks.
+    const bool chunks_only = 4.0 * a.tokens >= 3.0 * (double)a.B * max_q;
+    if (chunks_only) sp.most_rows = 0;
+    // Parts: whole ones, and one more for each request that is large enough.
+    const long all = (long)a.tokens * a.G, some = all / (sp.most_rows + 1);
+    const long parts = (all / kChunkRows + (some < a.B ? some : a.B)) * a.c.heads;
+    hipLaunchKernelGGL((kv_chunk_kernel<T, D>), dim3((unsigned)(parts + (chunks_only ? 0 : split))), dim3(kChunkThreads), 0,
+                       s, a, sp, (int)parts);
 }
 
 }  // namespace pyc
@@ -1013,9 +1207,8 @@ template <typename T, int D> static void launch_attention(const AttnArgs& a, flo
 extern "C" size_t pyc_hip_kv_attention_workspace_bytes(int B, int hq, int hk, int d, int max_q) {
     using namespace pyc;
     const long rows = (long)max_q * (hq / hk);
-    const int nt = split_tiles(rows);
-    const long most = rows < 16 * nt ? rows : 16 * nt;
-    return (size_t)2 * kSplitMost * most * (d + 2) * sizeof(float);
+    (void)d;
+    return kSplitPartBytes + ((size_t)B * hk * split_run_tiles(rows) * sizeof(uint32_t) + 15) / 16 * 16;
 }
 
 extern "C" int pyc_hip_kv_attention_launch(int is_bf16, const pyc_hip_kv_cache* cache, int B, int tokens, int hq,
@@ -1042,13 +1235,12 @@ extern "C" int pyc_hip_kv_attention_launch(int is_bf16, const pyc_hip_kv_cache* 
     a.o_stride = o_stride;
     a.scale_log2 = scale * 1.44269504088896340736f;
     hipStream_t s = (hipStream_t)stream;
-    float* part = (float*)workspace;
     if (a.c.d == 128) {
-        if (is_bf16) launch_attention<bf16_t, 128>(a, part, max_len, s);
-        else launch_attention<f16_t, 128>(a, part, max_len, s);
+        if (is_bf16) launch_attention<bf16_t, 128>(a, max_q, workspace, max_len, s);
+        else launch_attention<f16_t, 128>(a, max_q, workspace, max_len, s);
     } else {
-        if (is_bf16) launch_attention<bf16_t, 64>(a, part, max_len, s);
-        else launch_attention<f16_t, 64>(a, part, max_len, s);
+        if (is_bf16) launch_attention<bf16_t, 64>(a, max_q, workspace, max_len, s);
+        else launch_attention<f16_t, 64>(a, max_q, workspace, max_len, s);
     }
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
@@ -1059,8 +1251,8 @@ extern "C" int pyc_hip_kinfo_kv_attention(int is_bf16, pyc_hip_kinfo* out) {
     out->fn = is_bf16 ? reinterpret_cast<const void*>(&kv_split_kernel<bf16_t, 128, 1>)
                       : reinterpret_cast<const void*>(&kv_split_kernel<f16_t, 128, 1>);
     out->name = "kv_split_kernel<128, 1>";
-    out->lds_bytes = 0;
-    out->threads = kSplitWaves * kWave;
+    out->lds_bytes = sizeof(SplitShare<128, 1>);
+    out->threads = split_waves(1) * kWave;
     out->waves_per_simd = 2;
     return 0;
 }
