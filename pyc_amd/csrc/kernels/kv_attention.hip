@@ -67,6 +67,50 @@ __device__ inline AttnReq uniform(const AttnReq& r) {
     return AttnReq{uniform(r.len), uniform(r.n), uniform(r.first), uniform(r.rows)};
 }
 
+__device__ inline float read_lane(float x, int i) {
+    return __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(x), i));
+}
+__device__ inline int64_t read_lane(int64_t x, int i) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32) |
+                     (uint32_t)__builtin_amdgcn_readlane((int)x, i));
+}
+
+// Inclusive scan over the wave's lanes by DPP moves (a few cycles each where a
+// shuffle through the LDS takes 60): rows of 16 lanes by shifts of 1, 2, 4 and
+// 8, then lane 15 of the row before into rows 1 and 3, and lane 31 into rows 2 and 3.
+// A move gives `none` where there is no lane to take from.
+template <int CTRL, int ROWS> __device__ inline int dpp_move(int none, int x) {
+    return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> __device__ inline float dpp_move(float none, float x) {
+    return __int_as_float(dpp_move<CTRL, ROWS>(__float_as_int(none), __float_as_int(x)));
+}
+template <int CTRL, int ROWS> __device__ inline int64_t dpp_move(int64_t none, int64_t x) {
+    return (int64_t)(((uint64_t)(uint32_t)dpp_move<CTRL, ROWS>((int)(none >> 32), (int)(x >> 32)) << 32) |
+                     (uint32_t)dpp_move<CTRL, ROWS>((int)none, (int)x));
+}
+template <typename V, typename F> __device__ inline V wave_scan(V x, V none, F f) {
+    x = f(x, dpp_move<0x111, 0xf>(none, x));
+    x = f(x, dpp_move<0x112, 0xf>(none, x));
+    x = f(x, dpp_move<0x114, 0xf>(none, x));
+    x = f(x, dpp_move<0x118, 0xf>(none, x));
+    x = f(x, dpp_move<0x142, 0xa>(none, x));
+    x = f(x, dpp_move<0x143, 0xc>(none, x));
+    return x;
+}
+__device__ inline int64_t wave_prefix(int64_t x) {
+    return wave_scan(x, (int64_t)0, [](int64_t a, int64_t b) { return a + b; });
+}
+__device__ inline float wave_sum(float x) {
+    return read_lane(wave_scan(x, 0.f, [](float a, float b) { return a + b; }), 63);
+}
+__device__ inline float wave_max(float x) {
+    return read_lane(wave_scan(x, -INFINITY, [](float a, float b) { return __builtin_elementwise_maximum(a, b); }), 63);
+}
+__device__ inline int wave_max(int x) {
+    return __builtin_amdgcn_readlane(wave_scan(x, 0, [](int a, int b) { return max(a, b); }), 63);
+}
+
 __device__ inline uint32_t pack_half2(float lo, float hi, bf16_t) {
     typedef __attribute__((ext_vector_type(2))) float f2;
     typedef __attribute__((ext_vector_type(2))) __bf16 h2;
@@ -150,16 +194,21 @@ template <typename T, int D, int NT> struct AttnWave {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int t = 0; t < 4; ++t) s[n][t] = f32x4{0, 0, 0, 0};
+        // two products at a time: a sum's next term waits for the one before it
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; t += 2)
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                const u32x4 w = k[t * KC + c];
-                const u32x4 k0 = fp8x8_to_half8(w[0], w[1], T{}), k1 = fp8x8_to_half8(w[2], w[3], T{});
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    s[n][t] = mfma16x16x32(k0, q[n][2 * c], s[n][t], T{});
-                    s[n][t] = mfma16x16x32(k1, q[n][2 * c + 1], s[n][t], T{});
+                for (int u = 0; u < 2; ++u) {
+                    const u32x4 w0 = k[t * KC + c], w1 = k[(t + 1) * KC + c];
+                    const u32x4 k0 = fp8x8_to_half8(w0[2 * u], w0[2 * u + 1], T{});
+                    const u32x4 k1 = fp8x8_to_half8(w1[2 * u], w1[2 * u + 1], T{});
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        s[n][t] = mfma16x16x32(k0, q[n][2 * c + u], s[n][t], T{});
+                        s[n][t + 1] = mfma16x16x32(k1, q[n][2 * c + u], s[n][t + 1], T{});
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);  // else every code is converted first, into registers there are not
             }
@@ -223,15 +272,19 @@ template <typename T, int D, int NT> struct AttnWave {
         }
         if (masked) values_masked(valid, seen);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            const u32x4 v0 = fp8x8_to_half8(v[dt][0], v[dt][1], bf16_t{}), v1 = fp8x8_to_half8(v[dt][2], v[dt][3], bf16_t{});
+        for (int dt = 0; dt < DT; dt += 2) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                o[n][dt] = mfma16x16x32(v0, hi[n][0], o[n][dt], bf16_t{});
-                o[n][dt] = mfma16x16x32(v1, hi[n][1], o[n][dt], bf16_t{});
-                if constexpr (__is_same(T, f16_t)) {
-                    o[n][dt] = mfma16x16x32(v0, lo[n][0], o[n][dt], bf16_t{});
-                    o[n][dt] = mfma16x16x32(v1, lo[n][1], o[n][dt], bf16_t{});
+            for (int u = 0; u < 2; ++u) {
+                const u32x4 v0 = fp8x8_to_half8(v[dt][2 * u], v[dt][2 * u + 1], bf16_t{});
+                const u32x4 v1 = fp8x8_to_half8(v[dt + 1][2 * u], v[dt + 1][2 * u + 1], bf16_t{});
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    o[n][dt] = mfma16x16x32(v0, hi[n][u], o[n][dt], bf16_t{});
+                    o[n][dt + 1] = mfma16x16x32(v1, hi[n][u], o[n][dt + 1], bf16_t{});
+                    if constexpr (__is_same(T, f16_t)) {
+                        o[n][dt] = mfma16x16x32(v0, lo[n][u], o[n][dt], bf16_t{});
+                        o[n][dt + 1] = mfma16x16x32(v1, lo[n][u], o[n][dt + 1], bf16_t{});
+                    }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -381,18 +434,6 @@ __device__ inline int split_tiles(const AttnArgs& a, const AttnReq& r, int most_
     const int end = r.len - r.n + r.rows / a.G;  // keys that the last row sees
     return max(1, end / 64 + (end % 64 > 0 ? 1 : 0));
 }
-template <int ROWS> __device__ inline void split_request(const AttnArgs& a, int b, int most_rows, int* tiles, int* runs) {
-    *tiles = *runs = 0;
-    if (b >= a.B) return;
-    const AttnReq r = attn_request(a, b);
-    *tiles = split_tiles(a, r, most_rows);
-    *runs = *tiles ? (r.rows + ROWS - 1) / ROWS : 0;
-}
-__device__ inline int64_t wave_sum(int64_t x) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
-    return x;
-}
 // 64-bit quotients are slow and rarely needed.
 __device__ inline uint64_t div_u64(uint64_t n, uint64_t d) {
     return ((n | d) >> 32) == 0 ? (uint32_t)n / (uint32_t)d : n / d;
@@ -428,47 +469,44 @@ __device__ inline void agent_store(uint64_t* p, uint64_t v) {
 __device__ inline uint64_t agent_load(const uint64_t* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ inline float wave_max(float x) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) x = __builtin_elementwise_maximum(x, __shfl_xor(x, d));
-    return x;
-}
-__device__ inline float wave_sum(float x) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
-    return x;
-}
-__device__ inline float read_lane(float x, int i) {
-    return __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(x), i));
-}
-
 // Workgroup wg of `groups`.
 template <typename T, int D, int NT>
 __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitShare<D, NT>& sh, int wg, int groups) {
     constexpr int WAVES = split_waves(NT), ROWS = 16 * NT, E = D / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    // Lane i's request is the i-th of a batch's first 64; larger batches are looked at again.
+    const AttnReq near = lane < a.B ? attn_request(a, lane) : AttnReq{0, 0, 0, 0};
+    auto request = [&](int b) {
+        if (b >= kWave) return uniform(attn_request(a, b));
+        return AttnReq{__builtin_amdgcn_readlane(near.len, b), __builtin_amdgcn_readlane(near.n, b),
+                       __builtin_amdgcn_readlane(near.first, b), __builtin_amdgcn_readlane(near.rows, b)};
+    };
+    auto runs_of = [&](const AttnReq& r) { return (r.rows + ROWS - 1) / ROWS; };
+    auto work_of = [&](int b0, int* runs) {  // tiles and runs of request b0 + lane
+        const AttnReq r = b0 == 0 ? near : b0 + lane < a.B ? attn_request(a, b0 + lane) : AttnReq{0, 0, 0, 0};
+        const int t = split_tiles(a, r, sp.most_rows);
+        *runs = t ? runs_of(r) : 0;
+        return t;
+    };
     // All units (tiles of all runs), all runs, the longest run.
-    int tiles0, runs0;
-    split_request<ROWS>(a, lane, sp.most_rows, &tiles0, &runs0);
-    int64_t total = (int64_t)tiles0 * runs0, runs = runs0;
-    int longest = tiles0;
-    for (int b0 = kWave; b0 < a.B; b0 += kWave) {
-        int t, n;
-        split_request<ROWS>(a, b0 + lane, sp.most_rows, &t, &n);
+    int64_t total = 0, runs = 0;
+    int longest = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kWave) {
+        int n;
+        const int t = work_of(b0, &n);
         total += (int64_t)t * n;
         runs += n;
         longest = max(longest, t);
     }
-    total = uniform(wave_sum(total) * a.c.heads);
-    runs = uniform(wave_sum(runs) * a.c.heads);
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) longest = max(longest, __shfl_xor(longest, d));
-    const bool aligned = runs <= groups && uniform(longest) <= 2 * WAVES;
+    total = read_lane(wave_prefix(total), kWave - 1) * a.c.heads;
+    runs = read_lane(wave_prefix(runs), kWave - 1) * a.c.heads;
+    const bool aligned = runs <= groups && wave_max(longest) <= 2 * WAVES;
     const int W = (int)min((int64_t)groups * WAVES, total);
 
     // This wave's piece: `left` units from tile t0 of run (b, h, rt); unit u of all.
     int64_t u = 0, left = 0, before = 0;
-    int b = 0, h = 0, rt = 0, t0 = 0, w = wg * WAVES + wave;
+    int b = 0, h = 0, rt = 0, t0 = 0;
+    const int w = wg * WAVES + wave;
     if (aligned) {
         u = wg;  // a run here, counted below as a unit
         left = wg < runs ? 1 : 0;
@@ -479,30 +517,23 @@ __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitS
     if (left > 0) {
         int64_t base = 0;
         for (int b0 = 0; b0 < a.B; b0 += kWave) {
-            int t = tiles0, n = runs0;
-            if (b0) split_request<ROWS>(a, b0 + lane, sp.most_rows, &t, &n);
-            const int64_t mine = (int64_t)n * (aligned ? 1 : t) * a.c.heads;
-            int64_t end = mine;
-#pragma unroll
-            for (int d = 1; d < kWave; d *= 2) {
-                const int64_t x = __shfl_up(end, d);
-                if (lane >= d) end += x;
-            }
-            end += base;
+            int n;
+            const int t = work_of(b0, &n);
+            const int64_t mine = (int64_t)n * (aligned ? 1 : t) * a.c.heads, end = base + wave_prefix(mine);
             const uint64_t past = __ballot(end > u);
             if (past) {
                 const int i = __builtin_ctzll(past);
-                before = __shfl(end - mine, i);
+                before = read_lane(end - mine, i);
                 b = b0 + i;
                 break;
             }
-            base = __shfl(end, kWave - 1);
+            base = read_lane(end, kWave - 1);
         }
     }
     b = uniform(b);
     before = uniform(before);
-    AttnReq r = uniform(attn_request(a, b));
-    int tiles = split_tiles(a, r, sp.most_rows), n_rt = (r.rows + ROWS - 1) / ROWS;
+    AttnReq r = request(b);
+    int tiles = split_tiles(a, r, sp.most_rows), n_rt = runs_of(r);
     if (left > 0) {
         const int64_t v = u - before;
         const int64_t run = aligned ? v : (int64_t)div_u64(v, tiles);
@@ -543,10 +574,10 @@ __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitS
             if (++h == a.c.heads) {
                 h = 0;
                 do {
-                    r = uniform(attn_request(a, ++b));
+                    r = request(++b);
                     tiles = split_tiles(a, r, sp.most_rows);
                 } while (tiles == 0);  // ends: there are units left
-                n_rt = (r.rows + ROWS - 1) / ROWS;
+                n_rt = runs_of(r);
             }
         }
     }
@@ -725,26 +756,21 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     // The part: part_index counts (request, row tile from the last, head).
     int b = -1, h = 0, rt = 0;
     {
-        int64_t u = part_index, base = 0;
+        int64_t base = 0;
         for (int b0 = 0; b0 < a.B && b < 0; b0 += kWave) {
             const int i = b0 + lane;
             const int64_t mine =
                 i < a.B ? (int64_t)chunk_tiles(attn_request(a, i), from_rows) * a.c.heads : 0;
-            int64_t end = mine;
-#pragma unroll
-            for (int d = 1; d < kWave; d *= 2) {
-                const int64_t x = __shfl_up(end, d);
-                if (lane >= d) end += x;
-            }
-            const uint64_t past = __ballot(base + end > u);
+            const int64_t end = base + wave_prefix(mine);
+            const uint64_t past = __ballot(end > part_index);
             if (past) {
                 const int i2 = __builtin_ctzll(past);
-                const int v = (int)(u - base - __shfl(end - mine, i2));
+                const int v = (int)(part_index - read_lane(end - mine, i2));
                 b = b0 + i2;
                 h = v % a.c.heads;
-                rt = (int)(__shfl(mine, i2) / a.c.heads) - 1 - v / a.c.heads;
+                rt = (int)(read_lane(mine, i2) / a.c.heads) - 1 - v / a.c.heads;
             }
-            base += __shfl(end, kWave - 1);
+            base = read_lane(end, kWave - 1);
         }
     }
     b = __builtin_amdgcn_readfirstlane(b);
