@@ -67,37 +67,6 @@ __device__ inline AttnReq uniform(const AttnReq& r) {
     return AttnReq{uniform(r.len), uniform(r.n), uniform(r.first), uniform(r.rows)};
 }
 
-__device__ inline float read_lane(float x, int i) {
-    return __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(x), i));
-}
-__device__ inline int64_t read_lane(int64_t x, int i) {
-    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32) |
-                     (uint32_t)__builtin_amdgcn_readlane((int)x, i));
-}
-
-// Inclusive scan over the wave's lanes by DPP moves (a few cycles each where a
-// shuffle through the LDS takes 60): rows of 16 lanes by shifts of 1, 2, 4 and
-// 8, then lane 15 of the row before into rows 1 and 3, and lane 31 into rows 2 and 3.
-// A move gives `none` where there is no lane to take from.
-template <int CTRL, int ROWS> __device__ inline int dpp_move(int none, int x) {
-    return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS> __device__ inline float dpp_move(float none, float x) {
-    return __int_as_float(dpp_move<CTRL, ROWS>(__float_as_int(none), __float_as_int(x)));
-}
-template <int CTRL, int ROWS> __device__ inline int64_t dpp_move(int64_t none, int64_t x) {
-    return (int64_t)(((uint64_t)(uint32_t)dpp_move<CTRL, ROWS>((int)(none >> 32), (int)(x >> 32)) << 32) |
-                     (uint32_t)dpp_move<CTRL, ROWS>((int)none, (int)x));
-}
-template <typename V, typename F> __device__ inline V wave_scan(V x, V none, F f) {
-    x = f(x, dpp_move<0x111, 0xf>(none, x));
-    x = f(x, dpp_move<0x112, 0xf>(none, x));
-    x = f(x, dpp_move<0x114, 0xf>(none, x));
-    x = f(x, dpp_move<0x118, 0xf>(none, x));
-    x = f(x, dpp_move<0x142, 0xa>(none, x));
-    x = f(x, dpp_move<0x143, 0xc>(none, x));
-    return x;
-}
 __device__ inline int64_t wave_prefix(int64_t x) {
     return wave_scan(x, (int64_t)0, [](int64_t a, int64_t b) { return a + b; });
 }
@@ -414,14 +383,15 @@ struct AttnSplit {
     uint32_t* done;  // for every run that workgroups share: how many are done; zero between calls
 };
 constexpr int kSplitGroups = 256;
-__host__ __device__ constexpr int split_waves(int nt) { return nt == 1 ? 8 : 4; }
+// Two waves on a SIMD where their registers allow it.
+__host__ __device__ constexpr int split_waves(int nt, int d) { return nt == 1 || d == 64 ? 8 : 4; }
 
 struct SplitPart {  // a part of a run in LDS
     int b, h, rt, t0, t1, tiles, live, first;
     int64_t begin;  // the run's first unit
 };
 template <int D, int NT> struct SplitShare {
-    static constexpr int WAVES = split_waves(NT), ROWS = 16 * NT;
+    static constexpr int WAVES = split_waves(NT, D), ROWS = 16 * NT;
     float sums[2 * WAVES][ROWS][D + 4];
     float ml[2 * WAVES][ROWS][2];
     SplitPart part[2 * WAVES];
@@ -472,7 +442,7 @@ __device__ inline uint64_t agent_load(const uint64_t* p) {
 // Workgroup wg of `groups`.
 template <typename T, int D, int NT>
 __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitShare<D, NT>& sh, int wg, int groups) {
-    constexpr int WAVES = split_waves(NT), ROWS = 16 * NT, E = D / 64;
+    constexpr int WAVES = split_waves(NT, D), ROWS = 16 * NT, E = D / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     // Lane i's request is the i-th of a batch's first 64; larger batches are looked at again.
     const AttnReq near = lane < a.B ? attn_request(a, lane) : AttnReq{0, 0, 0, 0};
@@ -690,7 +660,7 @@ __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitS
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(split_waves(NT) * kWave, 1) kv_split_kernel(AttnArgs a, AttnSplit sp) {
+__global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel(AttnArgs a, AttnSplit sp) {
     __shared__ SplitShare<D, NT> sh;
     split_body<T, D, NT>(a, sp, sh, blockIdx.x, gridDim.x);
 }
@@ -1179,7 +1149,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
 // the others split what the rest of the batch reads, on the CUs that are left.
 template <typename T, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, AttnSplit sp, int parts) {
-    static_assert(split_waves(1) * kWave == kChunkThreads, "one workgroup size");
+    static_assert(split_waves(1, 128) * kWave == kChunkThreads, "one workgroup size");
     union Share {
         SplitShare<D, 1> split;
         ChunkShare<D> chunk;
@@ -1202,7 +1172,7 @@ constexpr size_t kSplitPartBytes = (size_t)2 * kSplitGroups * 32 * (128 + 2) * s
 template <typename T, int D> static void launch_attention(const AttnArgs& a, int max_q, void* workspace, int max_len,
                                                            hipStream_t s) {
     const long rows = (long)max_q * a.G, run_tiles = split_run_tiles(rows);  // as the workspace was made
-    const int nt = split_nt(rows), waves = split_waves(nt);
+    const int nt = split_nt(rows), waves = split_waves(nt, D);
     AttnSplit sp;
     sp.most_rows = (int)split_most_rows(rows);
     sp.part = (float*)workspace;
@@ -1278,7 +1248,7 @@ extern "C" int pyc_hip_kinfo_kv_attention(int is_bf16, pyc_hip_kinfo* out) {
                       : reinterpret_cast<const void*>(&kv_split_kernel<f16_t, 128, 1>);
     out->name = "kv_split_kernel<128, 1>";
     out->lds_bytes = sizeof(SplitShare<128, 1>);
-    out->threads = split_waves(1) * kWave;
+    out->threads = split_waves(1, 128) * kWave;
     out->waves_per_simd = 2;
     return 0;
 }

@@ -27,6 +27,38 @@ inline KvCache kv_cache_of(const pyc_hip_kv_cache* c) {
                    c->v_block_stride, c->num_blocks, c->kv_heads, c->block_size, c->head_dim};
 }
 
+__device__ inline float read_lane(float x, int i) {
+    return __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(x), i));
+}
+__device__ inline int64_t read_lane(int64_t x, int i) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32) |
+                     (uint32_t)__builtin_amdgcn_readlane((int)x, i));
+}
+
+// Inclusive scan over the wave's lanes by DPP moves (a few cycles each where a
+// shuffle through the LDS takes 60): rows of 16 lanes by shifts of 1, 2, 4 and
+// 8, then lane 15 of the row before into rows 1 and 3, and lane 31 into rows 2 and 3.
+// A move gives `none` where there is no lane to take from.
+template <int CTRL, int ROWS> __device__ inline int dpp_move(int none, int x) {
+    return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> __device__ inline float dpp_move(float none, float x) {
+    return __int_as_float(dpp_move<CTRL, ROWS>(__float_as_int(none), __float_as_int(x)));
+}
+template <int CTRL, int ROWS> __device__ inline int64_t dpp_move(int64_t none, int64_t x) {
+    return (int64_t)(((uint64_t)(uint32_t)dpp_move<CTRL, ROWS>((int)(none >> 32), (int)(x >> 32)) << 32) |
+                     (uint32_t)dpp_move<CTRL, ROWS>((int)none, (int)x));
+}
+template <typename V, typename F> __device__ inline V wave_scan(V x, V none, F f) {
+    x = f(x, dpp_move<0x111, 0xf>(none, x));
+    x = f(x, dpp_move<0x112, 0xf>(none, x));
+    x = f(x, dpp_move<0x114, 0xf>(none, x));
+    x = f(x, dpp_move<0x118, 0xf>(none, x));
+    x = f(x, dpp_move<0x142, 0xa>(none, x));
+    x = f(x, dpp_move<0x143, 0xc>(none, x));
+    return x;
+}
+
 // e4m3 to bf16 or f16, two codes a conversion, both exact (4 significant bits,
 // exponents -9 .. 8); 8 codes in two words.
 __device__ inline u32x4 fp8x8_to_half8(uint32_t lo, uint32_t hi, bf16_t) {

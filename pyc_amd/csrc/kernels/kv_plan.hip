@@ -14,7 +14,7 @@
 // hundred nanoseconds each. So everything that can be known is loaded at once, blocks
 // move a wave at a time, a step whose requests bring a token each writes it from the
 // request's own thread, and many tokens get a launch over all CUs.
-#include "common.hpp"
+#include "kv_cache.hpp"
 
 namespace pyc {
 
@@ -32,37 +32,38 @@ __device__ inline PlanSum plan_add(PlanSum a, PlanSum b) {
 // Inclusive sum over the workgroup's threads; `all` is the sum of all of them.
 __device__ inline PlanSum plan_scan(PlanSum v, PlanSum* all, PlanSum* waves) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n = blockDim.x / kWave;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const PlanSum x{(uint32_t)__shfl_up((int)v.blocks, d), (uint32_t)__shfl_up((int)v.tokens, d)};
-        if (lane >= d) v = plan_add(v, x);
-    }
+    auto add = [](int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, kPlanMost); };
+    v = PlanSum{(uint32_t)wave_scan((int)v.blocks, 0, add), (uint32_t)wave_scan((int)v.tokens, 0, add)};
     if (n == 1) {
-        *all = PlanSum{(uint32_t)__shfl((int)v.blocks, kWave - 1), (uint32_t)__shfl((int)v.tokens, kWave - 1)};
+        *all = PlanSum{(uint32_t)__builtin_amdgcn_readlane((int)v.blocks, kWave - 1),
+                       (uint32_t)__builtin_amdgcn_readlane((int)v.tokens, kWave - 1)};
         return v;
     }
     __syncthreads();  // the last use of `waves`
     if (lane == kWave - 1) waves[wave] = v;
     __syncthreads();
-    PlanSum before{0, 0};
-    *all = PlanSum{0, 0};
-    for (int w = 0; w < n; ++w) {
-        if (w < wave) before = plan_add(before, waves[w]);
-        *all = plan_add(*all, waves[w]);
-    }
-    return plan_add(v, before);
+    // every wave scans the waves' sums
+    PlanSum w = lane < n ? waves[lane] : PlanSum{0, 0};
+    w = PlanSum{(uint32_t)wave_scan((int)w.blocks, 0, add), (uint32_t)wave_scan((int)w.tokens, 0, add)};
+    auto at = [&](int i) {
+        return PlanSum{(uint32_t)__builtin_amdgcn_readlane((int)w.blocks, i),
+                       (uint32_t)__builtin_amdgcn_readlane((int)w.tokens, i)};
+    };
+    *all = at(kWave - 1);
+    const int uw = __builtin_amdgcn_readfirstlane(wave);
+    return uw ? plan_add(v, at(uw - 1)) : v;
 }
 
 // The workgroup's threads' bits, or-ed.
 __device__ inline uint32_t plan_vote(uint32_t bits, uint32_t* votes) {
     const int n = blockDim.x / kWave;
-    uint32_t mine = (__any(bits & 1) ? 1u : 0u) | (__any(bits & 2) ? 2u : 0u);
+    const uint32_t mine = (__any(bits & 1) ? 1u : 0u) | (__any(bits & 2) ? 2u : 0u);
     if (n == 1) return mine;
     __syncthreads();  // the last use of `votes`
     if ((threadIdx.x & (kWave - 1)) == 0) votes[threadIdx.x / kWave] = mine;
     __syncthreads();
-    for (int w = 0; w < n; ++w) mine |= votes[w];
-    return mine;
+    const uint32_t theirs = votes[min((int)(threadIdx.x & (kWave - 1)), n - 1)];
+    return (__any(theirs & 1) ? 1u : 0u) | (__any(theirs & 2) ? 2u : 0u);
 }
 
 struct PlanArgs {
@@ -95,27 +96,45 @@ __device__ inline void plan_token(const PlanArgs& a, const int32_t* offsets, con
     a.positions[t] = pos;
 }
 
-// f(thread, j, k) for every j < count of every thread of the workgroup, k counting
-// them all; `end` is the inclusive sum of count over the threads. Counts of up to two
-// everywhere (`few`): each thread does its own, else all are dealt out.
+// Moves one block id for every j < count of every thread of the workgroup: from(i, j,
+// k) to to(i, j, k), with i the thread and k counting all; `end` is the inclusive sum
+// of count over the threads. Counts of up to two everywhere (`few`): each thread
+// does its own, else all are dealt out, four to a thread at a time.
 constexpr uint32_t kPlanFew = 2;
-template <typename F>
-__device__ inline void plan_each(bool few, uint32_t count, uint32_t end, uint32_t all, uint32_t* s_end, F f) {
+template <typename From, typename To>
+__device__ inline void plan_move(bool few, uint32_t count, uint32_t end, uint32_t all, uint32_t* s_end, From from, To to) {
     if (few) {
-        for (uint32_t j = 0; j < count; ++j) f((int)threadIdx.x, j, end - count + j);
+        for (uint32_t j = 0; j < count; ++j) {
+            int32_t* dst = to((int)threadIdx.x, j, end - count + j);
+            if (dst) *dst = *from((int)threadIdx.x, j, end - count + j);
+        }
         return;
     }
+    const int T = (int)blockDim.x;
     __syncthreads();  // the last use of s_end
     s_end[threadIdx.x] = end;
     __syncthreads();
-    for (uint32_t k = threadIdx.x; k < all; k += blockDim.x) {
-        int lo = 0, hi = (int)blockDim.x - 1;  // the first thread whose end is past k
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (s_end[mid] > k) hi = mid;
-            else lo = mid + 1;
+    for (uint32_t k0 = threadIdx.x; k0 < all; k0 += 4 * T) {
+        int32_t id[4], *dst[4];
+        int i[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) i[x] = 0;
+        for (int step = T / 2; step > 0; step /= 2)  // the first thread whose end is past k
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (s_end[i[x] + step - 1] <= k0 + x * T) i[x] += step;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint32_t k = k0 + x * T;
+            dst[x] = nullptr;
+            if (k >= all) continue;
+            const uint32_t j = k - (i[x] ? s_end[i[x] - 1] : 0u);
+            dst[x] = to(i[x], j, k);
+            if (dst[x]) id[x] = *from(i[x], j, k);
         }
-        f(lo, k - (lo ? s_end[lo - 1] : 0u), k);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (dst[x]) *dst[x] = id[x];
     }
 }
 
@@ -150,9 +169,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a, int w
         if (f < 0) back = (uint32_t)((b0 == 0 ? held : min(max(a.cached[b], 0), cap_tokens)) + a.bs - 1) >> a.shift;
         PlanSum all;
         const PlanSum end = plan_scan(PlanSum{back, 0}, &all, waves);
-        plan_each(false, back, end.blocks, all.blocks, s_end, [&](int i, uint32_t j, uint32_t k) {
-            if (top + k < (uint32_t)a.free_cap) a.free_list[top + k] = a.table[(b0 + i) * a.table_stride + j];
-        });
+        plan_move(
+            false, back, end.blocks, all.blocks, s_end,
+            [&](int i, uint32_t j, uint32_t) { return a.table + (b0 + i) * a.table_stride + j; },
+            [&](int, uint32_t, uint32_t k) { return top + k < (uint32_t)a.free_cap ? a.free_list + top + k : nullptr; });
         top = min(top + all.blocks, (uint32_t)a.free_cap);
     }
     if (top != F) __syncthreads();  // the pushed entries are read below
@@ -180,10 +200,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a, int w
         if (need > 0 && have == held >> a.shift) block = a.free_list[pop];
         const uint32_t vote = plan_vote((ask > 1 ? 1 : 0) | (need > kPlanFew ? 2 : 0), votes);
         long_asks |= (vote & 1) != 0;
-        s_have[tid] = have;  // read behind plan_each's barriers, or by this thread
-        plan_each(!(vote & 2), need, end.blocks - given.blocks, all.blocks, s_end, [&](int i, uint32_t j, uint32_t k) {
-            a.table[(b0 + i) * a.table_stride + s_have[i] + j] = a.free_list[top - 1 - (given.blocks + k)];
-        });
+        s_have[tid] = have;  // read behind plan_move's barriers, or by this thread
+        plan_move(
+            !(vote & 2), need, end.blocks - given.blocks, all.blocks, s_end,
+            [&](int, uint32_t, uint32_t k) { return a.free_list + (top - 1 - (given.blocks + k)); },
+            [&](int i, uint32_t j, uint32_t) { return a.table + (b0 + i) * a.table_stride + s_have[i] + j; });
         given = plan_add(given, all);
         if (b < a.B) {
             const int len = fresh < 0 ? 0 : held + (int)ask;
@@ -214,10 +235,18 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a, int w
     for (int t = total + tid; t < a.tokens; t += T) a.slots[t] = a.positions[t] = -1;
 }
 
+// Many tokens: the search runs in LDS where the offsets fit.
+constexpr int kSlotsNear = 1024;
 __global__ void __launch_bounds__(256) kv_slots_kernel(PlanArgs a) {
+    __shared__ int32_t s_offsets[kSlotsNear + 1];
     const int t = blockIdx.x * 256 + threadIdx.x;
+    const bool near = a.B <= kSlotsNear;
+    if (near) {
+        for (int i = threadIdx.x; i <= a.B; i += 256) s_offsets[i] = a.q_offsets[i];
+        __syncthreads();
+    }
     if (t >= a.tokens) return;
-    if (t < a.q_offsets[a.B]) plan_token(a, a.q_offsets, a.lens, t);
+    if (t < (near ? s_offsets[a.B] : a.q_offsets[a.B])) plan_token(a, near ? s_offsets : a.q_offsets, a.lens, t);
     else a.slots[t] = a.positions[t] = -1;
 }
 
@@ -248,6 +277,6 @@ extern "C" int pyc_hip_kinfo_kv_plan(pyc_hip_kinfo* out) {
     out->name = "kv_plan_kernel";
     out->lds_bytes = (sizeof(PlanSum) + sizeof(uint32_t)) * kPlanWaves + sizeof(int32_t) * (4 * kPlanThreads + 4);
     out->threads = kPlanThreads;
-    out->waves_per_simd = 4;
+    out->waves_per_simd = 8;
     return 0;
 }
