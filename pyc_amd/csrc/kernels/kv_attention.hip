@@ -459,17 +459,22 @@ __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitS
         return t;
     };
     // All units (tiles of all runs), all runs, the longest run.
-    int64_t total = 0, runs = 0;
+    int64_t total = 0, runs = 0, units0 = 0, runs0 = 0;  // and the first 64 requests' prefix sums
     int longest = 0;
     for (int b0 = 0; b0 < a.B; b0 += kWave) {
         int n;
         const int t = work_of(b0, &n);
-        total += (int64_t)t * n;
-        runs += n;
+        const int64_t ut = wave_prefix((int64_t)t * n), rn = wave_prefix((int64_t)n);
+        if (b0 == 0) {
+            units0 = ut;
+            runs0 = rn;
+        }
+        total += read_lane(ut, kWave - 1);
+        runs += read_lane(rn, kWave - 1);
         longest = max(longest, t);
     }
-    total = read_lane(wave_prefix(total), kWave - 1) * a.c.heads;
-    runs = read_lane(wave_prefix(runs), kWave - 1) * a.c.heads;
+    total *= a.c.heads;
+    runs *= a.c.heads;
     const bool aligned = runs <= groups && wave_max(longest) <= 2 * WAVES;
     const int W = (int)min((int64_t)groups * WAVES, total);
 
@@ -487,13 +492,17 @@ __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitS
     if (left > 0) {
         int64_t base = 0;
         for (int b0 = 0; b0 < a.B; b0 += kWave) {
-            int n;
-            const int t = work_of(b0, &n);
-            const int64_t mine = (int64_t)n * (aligned ? 1 : t) * a.c.heads, end = base + wave_prefix(mine);
+            int64_t end = aligned ? runs0 : units0;
+            if (b0) {
+                int n;
+                const int t = work_of(b0, &n);
+                end = wave_prefix((int64_t)n * (aligned ? 1 : t));
+            }
+            end = base + end * a.c.heads;
             const uint64_t past = __ballot(end > u);
             if (past) {
                 const int i = __builtin_ctzll(past);
-                before = read_lane(end - mine, i);
+                before = i ? read_lane(end, i - 1) : base;
                 b = b0 + i;
                 break;
             }
@@ -579,11 +588,23 @@ __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitS
             o.l = wave_sum(in ? pl * wgt : 0.f);
 #pragma unroll
             for (int e = 0; e < E; ++e) o.x[e] = 0.f;
-            for (uint64_t k = parts; k; k &= k - 1) {
-                const int j = __builtin_ctzll(k);
-                const float f = read_lane(wgt, j);
+            for (uint64_t k = parts; k;) {  // four at a time: an LDS read takes longer than the rest
+                int j[4];
+                float f[4], x[4][E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) o.x[e] += f * sh.sums[j][row][E * lane + e];
+                for (int y = 0; y < 4; ++y) {
+                    j[y] = k ? __builtin_ctzll(k) : j[0];
+                    f[y] = k ? read_lane(wgt, j[y]) : 0.f;
+                    k &= k - 1;
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[y][e] = sh.sums[j[y]][row][E * lane + e];
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o.x[e] += f[y] * x[y][e];
             }
             if (whole) {
                 o.store(a, p, row);
@@ -628,7 +649,18 @@ __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitS
             for (int e = 0; e < E; ++e) o.x[e] = 0.f;
             for (int i0 = 0; i0 < n; i0 += kWave) {
                 const int cnt = min(n - i0, kWave), mi = min(i0 + lane, n - 1);
+                uint64_t x[8];
+                auto load = [&](int i) {  // results i .. i + 7 of the 64
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float* from = src(i0 + min(i + j, cnt - 1)) + row * D;
+                        if constexpr (E == 2) x[j] = agent_load(reinterpret_cast<const uint64_t*>(from) + lane);
+                        else
+                            x[j] = __float_as_uint(__hip_atomic_load(from + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                    }
+                };
                 const uint64_t v = agent_load(reinterpret_cast<const uint64_t*>(src(mi) + ROWS * D) + row);
+                load(0);  // while the weights are made
                 const bool in = lane < cnt;
                 const float pm = in ? __uint_as_float((uint32_t)v) : -INFINITY, pl = __uint_as_float((uint32_t)(v >> 32));
                 const float mx = __builtin_elementwise_maximum(o.m, wave_max(pm)), ref = mx == -INFINITY ? 0.f : mx;
@@ -638,14 +670,7 @@ __device__ inline void split_body(const AttnArgs& a, const AttnSplit& sp, SplitS
 #pragma unroll
                 for (int e = 0; e < E; ++e) o.x[e] *= keep;
                 for (int i = 0; i < cnt; i += 8) {
-                    uint64_t x[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float* from = src(i0 + min(i + j, cnt - 1)) + row * D;
-                        if constexpr (E == 2) x[j] = agent_load(reinterpret_cast<const uint64_t*>(from) + lane);
-                        else
-                            x[j] = __float_as_uint(__hip_atomic_load(from + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-                    }
+                    if (i) load(i);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float f = i + j < cnt ? read_lane(wgt, min(i + j, cnt - 1)) : 0.f;
