@@ -22,33 +22,14 @@
 
 namespace pyc {
 
-constexpr int kMinExp = -100;
 constexpr int kChunk = 16;
-
-// The smallest power of two s >= 2^-100 with a <= 448 s (a finite, >= 0). a = m
-// 2^x with 1 <= m < 2 and 448 = 1.75 * 2^8.
-__device__ inline float append_scale(float a) {
-    const uint32_t u = __float_as_uint(a);
-    int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-    e = max(e, kMinExp);
-    return __uint_as_float((uint32_t)(e + 127) << 23);
-}
 
 __device__ inline bool append_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-// Four floats as codes, in one word.
-__device__ inline uint32_t pack_e4m3(float a, float b, float c, float d) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
-}
 // The codes of a word times f (below 1: the block's scale grew).
 __device__ inline uint32_t shrink_e4m3(uint32_t w, float f) {
     return pack_e4m3(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * f, __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * f,
                      __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * f, __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * f);
-}
-
-template <typename T> __device__ inline float half_at(const u32x4& w, int j) {
-    return elem<T>::to_f32((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
 }
 
 struct AppendArgs {
@@ -148,7 +129,7 @@ __global__ void __launch_bounds__((S > 4 ? S : 4) * kWave) kv_append_kernel(Appe
 #pragma unroll
             for (int i = 0; i < S; ++i) mx = fmaxf(mx, most[wave - chunk + i]);
         }
-        float s = append_scale(mx);
+        float s = e4m3_scale(mx);
         const bool had = old > 0.f && append_finite(old);  // a scale that means something
         if (!starts && had) s = fmaxf(s, old);
         const bool grow = !starts && had && s > old;

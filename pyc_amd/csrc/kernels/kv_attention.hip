@@ -703,6 +703,7 @@ __global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel
 constexpr int kChunkRows = 128;
 constexpr int kChunkRing = 3;
 constexpr int kChunkThreads = 512;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 __device__ inline f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x16& c, bf16_t) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
@@ -781,14 +782,59 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     const int row = w0 + l32;
     const bool live = row < r.rows;
     const int limit = live ? r.len - r.n + row / a.G : r.len - 1;
-    u32x4 q[2 * KK];
+    // bf16: q = r (h + l / 16) with r a power of two for the row and h and l e4m3: 4 + 4
+    // of its 8 bits, exact down to 2^-14 of the row's largest element, below
+    // that to 2^-23 of it. The scores are then products of codes as they are, at twice
+    // the rate, and K needs no conversion. f16 has 11 bits: K is converted.
+    constexpr int K8 = D / 64;  // 64-channel steps of the code product
+    u32x4 q[SPLIT ? 2 * KK : 1];
+    i32x8 q8[SPLIT ? 1 : K8][2];
+    float q_scale = 1.f;
     {
         const int i = live ? row / a.G : 0, qh = live ? row % a.G : 0;
-        const uint16_t* src = a.q + (int64_t)(r.first + i) * a.q_stride + (int64_t)(h * a.G + qh) * D + 16 * hh;
+        const uint16_t* src = a.q + (int64_t)(r.first + i) * a.q_stride + (int64_t)(h * a.G + qh) * D;
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (int k = 0; k < KK; ++k)
+            for (int k = 0; k < KK; ++k)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) q[2 * k + u] = *reinterpret_cast<const u32x4*>(src + 32 * k + 8 * u);
+                for (int u = 0; u < 2; ++u)
+                    q[2 * k + u] = *reinterpret_cast<const u32x4*>(src + 32 * k + 16 * hh + 8 * u);
+        } else {
+            u32x4 w[K8][4];
+            float most = 0.f;
+#pragma unroll
+            for (int k = 0; k < K8; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    w[k][x] = *reinterpret_cast<const u32x4*>(src + 64 * k + 32 * hh + 8 * x);
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        const float v = fabsf(half_at<T>(w[k][x], y));
+                        most = v <= 3.402823466e38f ? fmaxf(most, v) : most;
+                    }
+                }
+            most = fmaxf(most, __shfl_xor(most, 32));
+            q_scale = e4m3_scale(most);
+            const float inv = 1.0f / q_scale;
+#pragma unroll
+            for (int k = 0; k < K8; ++k)
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {  // four channels
+                    float v[4], rest[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const float e = half_at<T>(w[k][x / 2], 4 * (x & 1) + y);
+                        v[y] = fabsf(e) <= 3.402823466e38f ? e * inv : __builtin_nanf("");
+                    }
+                    const int hi8 = (int)pack_e4m3(v[0], v[1], v[2], v[3]);
+                    rest[0] = v[0] - __builtin_amdgcn_cvt_f32_fp8(hi8, 0);
+                    rest[1] = v[1] - __builtin_amdgcn_cvt_f32_fp8(hi8, 1);
+                    rest[2] = v[2] - __builtin_amdgcn_cvt_f32_fp8(hi8, 2);
+                    rest[3] = v[3] - __builtin_amdgcn_cvt_f32_fp8(hi8, 3);
+                    q8[k][0][x] = hi8;
+                    q8[k][1][x] = (int)pack_e4m3(16.f * rest[0], 16.f * rest[1], 16.f * rest[2], 16.f * rest[3]);
+                }
+        }
     }
 
     // Blocks and scales of 16 of the group's tiles: lane l has chunk l % 4 of tile l / 4.
@@ -933,9 +979,18 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         uint32_t so_k = (uint32_t)((grp * kChunkRing + js % kChunkRing) * 2 * TILE);
         asm volatile("" : "+s"(so_k));
         const uint8_t* ks = ring + so_k;
-        u32x4 kf[2];
+        u32x4 kf[2][SPLIT ? 1 : 2];
         auto load_k = [&](int st, int x) {
-            kf[x] = *reinterpret_cast<const u32x4*>(ks + (32 * (st / KK) + l32) * D + 16 * swz(D == 64, l32, 2 * (st % KK) + hh));
+            if constexpr (SPLIT) {
+                kf[x][0] = *reinterpret_cast<const u32x4*>(ks + (32 * (st / KK) + l32) * D +
+                                                           16 * swz(D == 64, l32, 2 * (st % KK) + hh));
+            } else if (st % 2 == 0) {
+                const int e = st / 2 / K8, k = st / 2 % K8;
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    kf[st / 2 % 2][y] = *reinterpret_cast<const u32x4*>(ks + (32 * e + l32) * D +
+                                                                        16 * swz(D == 64, l32, 4 * k + 2 * hh + y));
+            }
         };
         int ids[2 * DMA];
         load_k(0, 0);
@@ -962,17 +1017,30 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                     o[k] = mfma32x32x16(v1, lo[2 * e + 1], o[k], bf16_t{});
                 }
             }
-            const u32x4 kw = kf[st & 1];
             f32x16 zero;
 #pragma unroll
             for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-            s[e] = mfma32x32x16(fp8x8_to_half8(kw[0], kw[1], T{}), q[2 * k], k == 0 ? zero : s[e], T{});
-            s[e] = mfma32x32x16(fp8x8_to_half8(kw[2], kw[3], T{}), q[2 * k + 1], s[e], T{});
+            if constexpr (SPLIT) {
+                const u32x4 kw = kf[st & 1][0];
+                s[e] = mfma32x32x16(fp8x8_to_half8(kw[0], kw[1], T{}), q[2 * k], k == 0 ? zero : s[e], T{});
+                s[e] = mfma32x32x16(fp8x8_to_half8(kw[2], kw[3], T{}), q[2 * k + 1], s[e], T{});
+            } else {
+                const int se = st / 2 / K8, sk8 = st / 2 % K8, piece = st % 2;
+                const u32x4 x = kf[st / 2 % 2][0], y = kf[st / 2 % 2][1];
+                const i32x8 kw{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+                // scales 2^0 and, for l, 2^-4 (exponent bytes 127 and 123)
+                s[se] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                    kw, q8[sk8][piece], sk8 == 0 && piece == 0 ? zero : s[se], 0, 0, 0, 0x7f7f7f7f, 0,
+                    piece ? 0x7b7b7b7b : 0x7f7f7f7f);
+            }
             if constexpr (DP) {
                 if (st >= 1 && st <= 2 * DMA) issue_one(st - 1, ids[st - 1], in);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        // used here: the compiler would move the products of S to the softmax, which
+        // alone needs them, and so into the other phase
+        asm volatile("" : "+v"(s[0]), "+v"(s[1]));
         check_part(js);
     };
     // The softmax of tile j, whose scores are in s: P into hi (and lo).
@@ -982,7 +1050,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         bool odd = false;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            sk[e] *= a.scale_log2;
+            sk[e] *= q_scale * a.scale_log2;
             const int key = key0 + 32 * e + 16 * hh;
             seen[e] = chunk_id[e] < 0 ? 0 : min(min(r.len, limit + 1) - key, 16);
             odd |= seen[e] < 16 || !(sv[e] >= 0x1p-64f && sv[e] <= 0x1p64f);

@@ -59,6 +59,26 @@ template <typename V, typename F> __device__ inline V wave_scan(V x, V none, F f
     return x;
 }
 
+constexpr int kMinExp = -100;
+// The smallest power of two s >= 2^-100 with a <= 448 s (a finite, >= 0). a = m
+// 2^x with 1 <= m < 2 and 448 = 1.75 * 2^8.
+__device__ inline float e4m3_scale(float a) {
+    const uint32_t u = __float_as_uint(a);
+    int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = max(e, kMinExp);
+    return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// Four floats as codes, in one word.
+__device__ inline uint32_t pack_e4m3(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+// Element j of 8 half-precision ones.
+template <typename T> __device__ inline float half_at(const u32x4& w, int j) {
+    return elem<T>::to_f32((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+}
+
 // e4m3 to bf16 or f16, two codes a conversion, both exact (4 significant bits,
 // exponents -9 .. 8); 8 codes in two words.
 __device__ inline u32x4 fp8x8_to_half8(uint32_t lo, uint32_t hi, bf16_t) {
