@@ -1077,13 +1077,16 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             for (int i = 0; i < 16; ++i) s[e][i] = fmaf(s[e][i], sk[e], add[e]);
         if (!plain) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+                int n_seen = seen[e];
+                asm volatile("" : "+v"(n_seen));  // keeps the comparisons inside this branch
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float x = i < seen[e] ? s[e][i] : -INFINITY;
-                    asm volatile("" : "+v"(x));  // keeps the masking inside this branch
+                    float x = i < n_seen ? s[e][i] : -INFINITY;
+                    asm volatile("" : "+v"(x));  // and the masking
                     s[e][i] = x;
                 }
+            }
         }
         auto pack = [&](int e, int i, float x0, float x1) {
             const uint32_t w = pack_half2(x0, x1, bf16_t{});
@@ -1137,12 +1140,15 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         }
         if (!plain) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+                int n_seen = seen[e];
+                asm volatile("" : "+v"(n_seen));
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(s[e][i]), p1 = __builtin_amdgcn_exp2f(s[e][i + 1]);
-                    pack(e, i, i < seen[e] ? p0 * sv[e] : 0.f, i + 1 < seen[e] ? p1 * sv[e] : 0.f);  // sv may be anything
+                    pack(e, i, i < n_seen ? p0 * sv[e] : 0.f, i + 1 < n_seen ? p1 * sv[e] : 0.f);  // sv may be anything
                 }
+            }
         }
         l += sum;
         const int* nan = with_nan[2 * grp + (j & 1)];
