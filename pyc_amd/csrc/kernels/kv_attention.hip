@@ -909,7 +909,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             chunk_id[e] = __builtin_amdgcn_ds_bpermute(lane4, pg.id);
         }
     };
-    u32x4 vf[2];  // value fragments; the first of a tile is read before its M phase
+    u32x4 vf[3];  // value fragments, read two steps ahead; a tile's first two before its M phase
     auto load_v = [&](int j, int st, int x) {
         uint32_t so = (uint32_t)((grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE);
         asm volatile("" : "+s"(so));
@@ -979,11 +979,13 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         uint32_t so_k = (uint32_t)((grp * kChunkRing + js % kChunkRing) * 2 * TILE);
         asm volatile("" : "+s"(so_k));
         const uint8_t* ks = ring + so_k;
-        u32x4 kf[2][SPLIT ? 1 : 2];
-        auto load_k = [&](int st, int x) {
+        // K fragments are read two steps before their products, which are two steps behind
+        // V's: a read takes longer than a step.
+        u32x4 kf[SPLIT ? 3 : 2][SPLIT ? 1 : 2];
+        auto load_k = [&](int st) {
             if constexpr (SPLIT) {
-                kf[x][0] = *reinterpret_cast<const u32x4*>(ks + (32 * (st / KK) + l32) * D +
-                                                           16 * swz(D == 64, l32, 2 * (st % KK) + hh));
+                kf[st % 3][0] = *reinterpret_cast<const u32x4*>(ks + (32 * (st / KK) + l32) * D +
+                                                                16 * swz(D == 64, l32, 2 * (st % KK) + hh));
             } else if (st % 2 == 0) {
                 const int e = st / 2 / K8, k = st / 2 % K8;
 #pragma unroll
@@ -993,45 +995,50 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             }
         };
         int ids[2 * DMA];
-        load_k(0, 0);
         if constexpr (DP) {
 #pragma unroll
             for (int x = 0; x < 2 * DMA; ++x) ids[x] = load_id(x, pi.id, ji);
         }
 #pragma unroll
-        for (int st = 0; st < ST; ++st) {
-            const int e = st / KK, k = st % KK;
-            if (st + 1 < ST) {
-                load_k(st + 1, (st + 1) & 1);
-                if constexpr (DP) load_v(jp, st + 1, (st + 1) & 1);
+        for (int st = 0; st < ST + 2; ++st) {
+            if (st < ST) load_k(st);
+            if constexpr (DP) {
+                if (st + 2 < ST) load_v(jp, st + 2, (st + 2) % 3);
             }
             if (st == ST / 2) read_part(js);
             if (st == ST / 2 + 1) take_scales(js);
             if constexpr (DP) {
-                const u32x4 w = vf[st & 1];
-                const u32x4 v0 = fp8x8_to_half8(w[0], w[1], bf16_t{}), v1 = fp8x8_to_half8(w[2], w[3], bf16_t{});
-                o[k] = mfma32x32x16(v0, hi[2 * e], o[k], bf16_t{});
-                o[k] = mfma32x32x16(v1, hi[2 * e + 1], o[k], bf16_t{});
-                if constexpr (SPLIT) {
-                    o[k] = mfma32x32x16(v0, lo[2 * e], o[k], bf16_t{});
-                    o[k] = mfma32x32x16(v1, lo[2 * e + 1], o[k], bf16_t{});
+                if (st < ST) {
+                    const int e = st / KK, k = st % KK;
+                    const u32x4 w = vf[st % 3];
+                    const u32x4 v0 = fp8x8_to_half8(w[0], w[1], bf16_t{}), v1 = fp8x8_to_half8(w[2], w[3], bf16_t{});
+                    o[k] = mfma32x32x16(v0, hi[2 * e], o[k], bf16_t{});
+                    o[k] = mfma32x32x16(v1, hi[2 * e + 1], o[k], bf16_t{});
+                    if constexpr (SPLIT) {
+                        o[k] = mfma32x32x16(v0, lo[2 * e], o[k], bf16_t{});
+                        o[k] = mfma32x32x16(v1, lo[2 * e + 1], o[k], bf16_t{});
+                    }
                 }
             }
             f32x16 zero;
 #pragma unroll
             for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-            if constexpr (SPLIT) {
-                const u32x4 kw = kf[st & 1][0];
-                s[e] = mfma32x32x16(fp8x8_to_half8(kw[0], kw[1], T{}), q[2 * k], k == 0 ? zero : s[e], T{});
-                s[e] = mfma32x32x16(fp8x8_to_half8(kw[2], kw[3], T{}), q[2 * k + 1], s[e], T{});
-            } else {
-                const int se = st / 2 / K8, sk8 = st / 2 % K8, piece = st % 2;
-                const u32x4 x = kf[st / 2 % 2][0], y = kf[st / 2 % 2][1];
-                const i32x8 kw{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-                // scales 2^0 and, for l, 2^-4 (exponent bytes 127 and 123)
-                s[se] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                    kw, q8[sk8][piece], sk8 == 0 && piece == 0 ? zero : s[se], 0, 0, 0, 0x7f7f7f7f, 0,
-                    piece ? 0x7b7b7b7b : 0x7f7f7f7f);
+            if (st >= 2) {
+                const int ss = st - 2;
+                if constexpr (SPLIT) {
+                    const int e = ss / KK, k = ss % KK;
+                    const u32x4 kw = kf[ss % 3][0];
+                    s[e] = mfma32x32x16(fp8x8_to_half8(kw[0], kw[1], T{}), q[2 * k], k == 0 ? zero : s[e], T{});
+                    s[e] = mfma32x32x16(fp8x8_to_half8(kw[2], kw[3], T{}), q[2 * k + 1], s[e], T{});
+                } else {
+                    const int se = ss / 2 / K8, sk8 = ss / 2 % K8, piece = ss % 2;
+                    const u32x4 x = kf[ss / 2 % 2][0], y = kf[ss / 2 % 2][1];
+                    const i32x8 kw{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+                    // scales 2^0 and, for l, 2^-4 (exponent bytes 127 and 123)
+                    s[se] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                        kw, q8[sk8][piece], sk8 == 0 && piece == 0 ? zero : s[se], 0, 0, 0, 0x7f7f7f7f, 0,
+                        piece ? 0x7b7b7b7b : 0x7f7f7f7f);
+                }
             }
             if constexpr (DP) {
                 if (st >= 1 && st <= 2 * DMA) issue_one(st - 1, ids[st - 1], in);
@@ -1170,6 +1177,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         v_phase(0);
         wait_vmem_le<0>();
         load_v(0, 0, 0);
+        load_v(0, 1, 1);
         __syncthreads();
         for (int k = 0; k < n; ++k) {
             // The last tiles' M phases do as the others: load the last tile once more, into a
@@ -1191,6 +1199,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 v_phase(k + 1);
                 wait_vmem_le<0>();  // tile k + 2 landed
                 load_v(k + 1, 0, 0);
+                load_v(k + 1, 1, 1);
                 __syncthreads();
             }
         }
