@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel
 // products of this one, and the conversion of both operands' codes), the wave of the
 // other that shares its SIMD runs its softmax (phase V).
 constexpr int kChunkRows = 128;
-constexpr int kChunkRing = 3;
+constexpr int kChunkRing = 4;
 constexpr int kChunkThreads = 512;
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 __device__ inline f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x16& c, bf16_t) {
@@ -724,11 +724,11 @@ constexpr float kChunkSumMax = 16384.0f;
 template <int D> struct ChunkShare {
     static constexpr int TILE = 64 * D;
     __attribute__((aligned(1024))) uint8_t ring[2 * kChunkRing * 2 * TILE];
-    // Value tiles that hold a NaN code, as they came, and which waves' parts of them
-    // are there; [group][tile % 2]. In the ring NaN codes are 0: the product then says
+    // Which codes of a value tile are NaN, a bit each, where a wave's part of it (with_nan)
+    // has any; [group][tile % 4]. In the ring these are 0: the product then says
     // nothing of them, and nan_values gives the NaN to the rows that see them.
-    __attribute__((aligned(16))) uint8_t raw[4][TILE];
-    __attribute__((aligned(16))) int with_nan[4][4];
+    __attribute__((aligned(16))) uint16_t nans[8][TILE / 16];
+    __attribute__((aligned(16))) int with_nan[8][4];
     float joint[8][32][2];
 };
 
@@ -741,7 +741,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     constexpr int DMA = TILE / (4 * 1024);  // wave loads of an operand for each of a group's waves
     constexpr bool SPLIT = __is_same(T, f16_t);
     auto& ring = sh.ring;
-    auto& raw = sh.raw;
+    auto& nans = sh.nans;
     auto& with_nan = sh.with_nan;
     auto& joint = sh.joint;
     static_assert(8 * 64 * (DT / 2) * 64 <= (int)sizeof(ring), "room to join in");
@@ -877,9 +877,9 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         const uint64_t src = at[x] + (uint64_t)(uint32_t)max(id, 0) * (x < DMA ? k_stride : v_stride);
         lds_dma_b128((const void*)(uintptr_t)src, x < DMA ? slot : slot + TILE);
     };
-    auto issue = [&](const AttnPages& p, int j) {
+    auto issue = [&](const AttnPages& p, int j, int in) {
 #pragma unroll
-        for (int x = 0; x < 2 * DMA; ++x) issue_one(x, load_id(x, p.id, j), j);
+        for (int x = 0; x < 2 * DMA; ++x) issue_one(x, load_id(x, p.id, j), in);
     };
 
     f32x16 o[DT], s[2];
@@ -917,7 +917,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     };
 
     // This wave's part of tile j's values, which has landed: NaN codes out of it. (The
-    // tile's product is two barriers away.)
+    // tile's softmax is behind the next barrier.)
     u32x4 part[DMA];
     auto read_part = [&](int j) {
         const uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
@@ -931,21 +931,26 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
 #pragma unroll
             for (int y = 0; y < 4; ++y) bad |= (part[x][y] & 0x7f7f7f7fu) + 0x01010101u;
         const bool any = __any((bad & 0x80808080u) != 0);
-        if (lane == 0) with_nan[2 * grp + (j & 1)][wr] = any;
+        if (lane == 0) with_nan[4 * grp + (j & 3)][wr] = any;
         if (!any) return;
         uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
 #pragma unroll
         for (int x = 0; x < DMA; ++x) {
             u32x4 w = part[x];
-            *reinterpret_cast<u32x4*>(raw[2 * grp + (j & 1)] + 1024 * (wr + 4 * x) + 16 * lane) = w;
+            uint32_t bits = 0;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) w[y] &= ~((nan_codes(w[y]) >> 7) * 0xffu);
+            for (int y = 0; y < 4; ++y) {
+                const uint32_t nan = nan_codes(w[y]) >> 7;
+                bits |= (nan * 0x01020408u >> 24) << (4 * y);
+                w[y] &= ~(nan * 0xffu);
+            }
+            nans[4 * grp + (j & 3)][64 * (wr + 4 * x) + lane] = (uint16_t)bits;
             *reinterpret_cast<u32x4*>(mine + 1024 * (wr + 4 * x)) = w;
         }
     };
     // NaN codes among tile j's values: NaN sums for the rows that see them, by a product of indicators.
     auto nan_values = [&](int j, const int (&seen)[2]) {
-        const int which = 2 * grp + (j & 1);
+        const int which = 4 * grp + (j & 3);
 #pragma unroll 1
         for (int e = 0; e < 2; ++e) {
             u32x4 one[2];
@@ -954,10 +959,11 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 one[i >> 2][i & 3] = (2 * i < seen[e] ? 0x3f80u : 0u) | (2 * i + 1 < seen[e] ? 0x3f800000u : 0u);
 #pragma unroll
             for (int k = 0; k < DT; ++k) {
-                u32x4 w = *reinterpret_cast<const u32x4*>(raw[which] + (32 * k + l32) * 64 + 16 * swz(1, l32, 2 * e + hh));
-                if (!with_nan[which][(2 * k + (l32 >> 4)) & 3]) w = u32x4{0, 0, 0, 0};  // the part is not there
+                uint32_t bits = nans[which][(32 * k + l32) * 4 + swz(1, l32, 2 * e + hh)];
+                if (!with_nan[which][(2 * k + (l32 >> 4)) & 3]) bits = 0;  // the part has none
+                u32x4 w;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) w[x] = (nan_codes(w[x]) >> 7) * 0x38u;  // 1.0
+                for (int x = 0; x < 4; ++x) w[x] = (((bits >> (4 * x)) & 15u) * 0x00204081u & 0x01010101u) * 0x38u;  // 1.0
                 f32x16 hit;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) hit[i] = 0.f;
@@ -970,10 +976,12 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         }
     };
 
-    // One M phase: S of tile js and O += P V of tile jp (if DP); on its way the loads of
-    // tile ji are issued into tile in's slot (that of the tile before jp), the part of tile js
-    // that this wave loaded is checked, and the scales of js are taken.
-    auto m_phase = [&](auto dp_tag, int js, int jp, const AttnPages& pi, int ji, int in) {
+    // One M phase: S of tile jp + 1 and O += P V of tile jp (if DP: from the second on); on
+    // its way the loads of tile ji are issued into the slot of tile jp + 3 (that of jp - 1),
+    // the part of tile jp + 2 that this wave loaded is checked, and the scales of jp + 1
+    // are taken.
+    auto m_phase = [&](auto dp_tag, int jp, int ids_of_ji, int ji) {
+        const int js = jp + 1;
         constexpr bool DP = decltype(dp_tag)::value;
         constexpr int ST = 2 * KK;
         uint32_t so_k = (uint32_t)((grp * kChunkRing + js % kChunkRing) * 2 * TILE);
@@ -997,7 +1005,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         int ids[2 * DMA];
         if constexpr (DP) {
 #pragma unroll
-            for (int x = 0; x < 2 * DMA; ++x) ids[x] = load_id(x, pi.id, ji);
+            for (int x = 0; x < 2 * DMA; ++x) ids[x] = load_id(x, ids_of_ji, ji);
         }
 #pragma unroll
         for (int st = 0; st < ST + 2; ++st) {
@@ -1005,7 +1013,9 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             if constexpr (DP) {
                 if (st + 2 < ST) load_v(jp, st + 2, (st + 2) % 3);
             }
-            if (st == ST / 2) read_part(js);
+            if constexpr (DP) {
+                if (st == ST / 2) read_part(jp + 2);
+            }
             if (st == ST / 2 + 1) take_scales(js);
             if constexpr (DP) {
                 if (st < ST) {
@@ -1041,14 +1051,14 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 }
             }
             if constexpr (DP) {
-                if (st >= 1 && st <= 2 * DMA) issue_one(st - 1, ids[st - 1], in);
+                if (st >= 1 && st <= 2 * DMA) issue_one(st - 1, ids[st - 1], jp + 3);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         // used here: the compiler would move the products of S to the softmax, which
         // alone needs them, and so into the other phase
         asm volatile("" : "+v"(s[0]), "+v"(s[1]));
-        check_part(js);
+        if constexpr (DP) check_part(jp + 2);
     };
     // The softmax of tile j, whose scores are in s: P into hi (and lo).
     auto v_phase = [&](int j) {
@@ -1158,50 +1168,48 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             }
         }
         l += sum;
-        const int* nan = with_nan[2 * grp + (j & 1)];
+        const int* nan = with_nan[4 * grp + (j & 3)];
         if (__builtin_amdgcn_readfirstlane(nan[0] | nan[1] | nan[2] | nan[3])) nan_values(j, seen);
     };
 
+    // One M phase and what comes with it; the last tiles' load the last tile once more, into
+    // slots that nobody reads, and compute an S of whatever its slot holds.
+    auto m_step = [&](int k) {
+        wait_vmem_le<0>();  // tile k + 2, issued a tile's time ago
+        if (((k + 1) & 15) == 0) pg = nx;
+        const int ji = min(k + 3, n - 1);
+        const int ids = ji > k + 1 && (ji >> 4) != ((k + 1) >> 4) ? nx.id : pg.id;
+        // The wave in its M phase goes first: the softmax of the SIMD's other wave takes
+        // the cycles that its matrix instructions leave.
+        __builtin_amdgcn_s_setprio(2);
+        m_phase(std::true_type{}, k, ids, ji);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto v_step = [&](int j) {
+        // the next 16 tiles' blocks, then their scales: they have tiles' time to come
+        if ((j & 15) == 1 && (j & ~15) + 16 < n) nx.id = page_ids((j & ~15) + 16);
+        if ((j & 15) == 3) page_scales(nx);
+        v_phase(j);
+        load_v(j, 0, 0);
+        load_v(j, 1, 1);
+    };
     if (n > 0) {
-        issue(pg, 0);
-        if (n > 1) {
-            issue(pg, 1);
-            wait_vmem_le<2 * DMA>();  // the first tile's own part landed ...
-        } else {
-            wait_vmem_le<0>();
-        }
-        __syncthreads();                // ... and every wave's
-        if (grp == 1) __syncthreads();  // group 1 is one phase behind
-        m_phase(std::false_type{}, 0, 0, pg, 0, 0);
+        for (int j = 0; j < 3; ++j) issue(pg, min(j, n - 1), j);
+        wait_vmem_le<2 * DMA>();  // tiles 0 and 1
+        read_part(0);
+        check_part(0);
+        read_part(1);
+        check_part(1);
         __syncthreads();
-        v_phase(0);
-        wait_vmem_le<0>();
-        load_v(0, 0, 0);
-        load_v(0, 1, 1);
-        __syncthreads();
+        m_phase(std::false_type{}, -1, 0, 0);
+        // A barrier a tile: group 0 passes it before, group 1 behind a product, so the groups
+        // stay half a tile apart and are free between. Behind it the tile that both
+        // waited for and checked is there, and the slot of the tile before is free.
         for (int k = 0; k < n; ++k) {
-            // The last tiles' M phases do as the others: load the last tile once more, into a
-            // slot that nobody reads, and compute an S of whatever its slot holds.
-            if (((k + 1) & 15) == 0) pg = nx;
-            const int ji = min(k + 2, n - 1);
-            AttnPages pi;
-            pi.id = (ji & 15) == 0 && ji > k + 1 ? nx.id : pg.id;
-            // The wave in its M phase goes first: the softmax of the SIMD's other wave
-            // takes the cycles that its matrix instructions leave.
-            __builtin_amdgcn_s_setprio(2);
-            m_phase(std::true_type{}, k + 1, k, pi, ji, k + 2);
-            __builtin_amdgcn_s_setprio(0);
-            __syncthreads();
-            if (k + 1 < n) {
-                // the next 16 tiles' blocks, then their scales: they have tiles' time to come
-                if (((k + 1) & 15) == 1 && (k & ~15) + 16 < n) nx.id = page_ids((k & ~15) + 16);
-                if (((k + 1) & 15) == 3) page_scales(nx);
-                v_phase(k + 1);
-                wait_vmem_le<0>();  // tile k + 2 landed
-                load_v(k + 1, 0, 0);
-                load_v(k + 1, 1, 1);
-                __syncthreads();
-            }
+            v_step(k);
+            if (grp == 0 && k > 0) __syncthreads();
+            m_step(k);
+            if (grp == 1) __syncthreads();
         }
         if (grp == 0) __syncthreads();
     }
