@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel
 // wave of one runs matrix instructions (phase M: the scores of its next tile and the
 // products of this one, and the conversion of both operands' codes), the wave of the
 // other that shares its SIMD runs its softmax (phase V).
-constexpr int kChunkRows = 128;
+constexpr int chunk_rows(int groups) { return 256 / groups; }
 constexpr int kChunkRing = 4;
 constexpr int kChunkThreads = 512;
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -712,8 +712,8 @@ __device__ inline f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x
 }
 
 // Row tiles of a request in the chunk kernel.
-__device__ inline int chunk_tiles(const AttnReq& r, int from_rows) {
-    return r.rows > from_rows ? (r.rows + kChunkRows - 1) / kChunkRows : 0;
+__device__ inline int chunk_tiles(const AttnReq& r, int from_rows, int part_rows) {
+    return r.rows > from_rows ? (r.rows + part_rows - 1) / part_rows : 0;
 }
 
 // The reference m of a row is its maximum over the first tile that shows it a key,
@@ -721,42 +721,48 @@ __device__ inline int chunk_tiles(const AttnReq& r, int from_rows) {
 // overflow in bf16 (whose exponents are fp32's), and the common path has no maximum.
 constexpr float kChunkSumMax = 16384.0f;
 
-template <int D> struct ChunkShare {
+template <int D, int GROUPS> struct ChunkShare {
     static constexpr int TILE = 64 * D;
-    __attribute__((aligned(1024))) uint8_t ring[2 * kChunkRing * 2 * TILE];
+    __attribute__((aligned(1024))) uint8_t ring[GROUPS * kChunkRing * 2 * TILE];
     // Which codes of a value tile are NaN, a bit each, where a wave's part of it (with_nan)
     // has any; [group][tile % 4]. In the ring these are 0: the product then says
     // nothing of them, and nan_values gives the NaN to the rows that see them.
-    __attribute__((aligned(16))) uint16_t nans[8][TILE / 16];
-    __attribute__((aligned(16))) int with_nan[8][4];
+    __attribute__((aligned(16))) uint16_t nans[4 * GROUPS][TILE / 16];
+    __attribute__((aligned(16))) int with_nan[4 * GROUPS][8 / GROUPS];
     float joint[8][32][2];
 };
 
-template <typename T, int D>
-__device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D>& sh, int part_index) {
+template <typename T, int D, int GROUPS>
+__device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D, GROUPS>& sh, int part_index) {
+    constexpr int ROWS = chunk_rows(GROUPS);
+    constexpr int LOADERS = 8 / GROUPS;   // waves that load a tile together
     constexpr int KC = D / 16;            // 16-byte chunks of a key's row in LDS
     constexpr int KK = D / 32;            // pairs of k steps of S
     constexpr int DT = D / 32;            // 32-channel tiles of O^T
     constexpr int TILE = 64 * D;          // bytes of one operand of a tile
-    constexpr int DMA = TILE / (4 * 1024);  // wave loads of an operand for each of a group's waves
+    constexpr int DMA = TILE / (LOADERS * 1024);  // wave loads of an operand for each of them
+    static_assert(DMA > 0, "each loads of both operands");
     constexpr bool SPLIT = __is_same(T, f16_t);
     auto& ring = sh.ring;
     auto& nans = sh.nans;
     auto& with_nan = sh.with_nan;
     auto& joint = sh.joint;
-    static_assert(8 * 64 * (DT / 2) * 64 <= (int)sizeof(ring), "room to join in");
+    static_assert(GROUPS == 1 || 8 * 64 * (DT / 2) * 64 <= (int)sizeof(ring), "room to join in");
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int grp = wave >> 2, wr = wave & 3, l32 = lane & 31, hh = lane >> 5, bs = a.c.bs;
+    const int phase = wave >> 2;                                 // which of a SIMD's two waves
+    const int grp = GROUPS == 2 ? phase : 0, wr = wave % LOADERS;  // whose tiles; place in the group
+    const int l32 = lane & 31, hh = lane >> 5, bs = a.c.bs;
 
     // The part: part_index counts (request, row tile from the last, head).
     int b = -1, h = 0, rt = 0;
+    AttnReq r{0, 0, 0, 0};
     {
         int64_t base = 0;
         for (int b0 = 0; b0 < a.B && b < 0; b0 += kWave) {
             const int i = b0 + lane;
-            const int64_t mine =
-                i < a.B ? (int64_t)chunk_tiles(attn_request(a, i), from_rows) * a.c.heads : 0;
+            const AttnReq near = i < a.B ? attn_request(a, i) : AttnReq{0, 0, 0, 0};
+            const int64_t mine = (int64_t)chunk_tiles(near, from_rows, ROWS) * a.c.heads;
             const int64_t end = base + wave_prefix(mine);
             const uint64_t past = __ballot(end > part_index);
             if (past) {
@@ -765,6 +771,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 b = b0 + i2;
                 h = v % a.c.heads;
                 rt = (int)(read_lane(mine, i2) / a.c.heads) - 1 - v / a.c.heads;
+                r = AttnReq{__builtin_amdgcn_readlane(near.len, i2), __builtin_amdgcn_readlane(near.n, i2),
+                            __builtin_amdgcn_readlane(near.first, i2), __builtin_amdgcn_readlane(near.rows, i2)};
             }
             base = read_lane(end, kWave - 1);
         }
@@ -773,95 +781,51 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     h = __builtin_amdgcn_readfirstlane(h);
     rt = __builtin_amdgcn_readfirstlane(rt);
     if (b < 0) return;
-    const AttnReq r = attn_request(a, b);
-    const int r0 = rt * kChunkRows, w0 = r0 + 32 * wr;  // the part's first row, the wave's
-    const int keys = max(0, r.len - r.n + min(r0 + kChunkRows - 1, r.rows - 1) / a.G + 1);  // that its last row sees
-    const int n = (keys + 127) / 128;  // tiles of each group (the last of group 1 may have no key)
+    r = uniform(r);
+    const int r0 = rt * ROWS, w0 = r0 + 32 * wr;  // the part's first row, the wave's
+    const int keys = max(0, r.len - r.n + min(r0 + ROWS - 1, r.rows - 1) / a.G + 1);  // that its last row sees
+    const int n = (keys + 64 * GROUPS - 1) / (64 * GROUPS);  // tiles of each group (the last of group 1 may have no key)
 
     // Q and what each row sees.
     const int row = w0 + l32;
     const bool live = row < r.rows;
     const int limit = live ? r.len - r.n + row / a.G : r.len - 1;
-    // bf16: q = r (h + l / 16) with r a power of two for the row and h and l e4m3: 4 + 4
-    // of its 8 bits, exact down to 2^-14 of the row's largest element, below
-    // that to 2^-23 of it. The scores are then products of codes as they are, at twice
-    // the rate, and K needs no conversion. f16 has 11 bits: K is converted.
-    constexpr int K8 = D / 64;  // 64-channel steps of the code product
-    u32x4 q[SPLIT ? 2 * KK : 1];
-    i32x8 q8[SPLIT ? 1 : K8][2];
-    float q_scale = 1.f;
-    {
-        const int i = live ? row / a.G : 0, qh = live ? row % a.G : 0;
-        const uint16_t* src = a.q + (int64_t)(r.first + i) * a.q_stride + (int64_t)(h * a.G + qh) * D;
-        if constexpr (SPLIT) {
-#pragma unroll
-            for (int k = 0; k < KK; ++k)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    q[2 * k + u] = *reinterpret_cast<const u32x4*>(src + 32 * k + 16 * hh + 8 * u);
-        } else {
-            u32x4 w[K8][4];
-            float most = 0.f;
-#pragma unroll
-            for (int k = 0; k < K8; ++k)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    w[k][x] = *reinterpret_cast<const u32x4*>(src + 64 * k + 32 * hh + 8 * x);
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        const float v = fabsf(half_at<T>(w[k][x], y));
-                        most = v <= 3.402823466e38f ? fmaxf(most, v) : most;
-                    }
-                }
-            most = fmaxf(most, __shfl_xor(most, 32));
-            q_scale = e4m3_scale(most);
-            const float inv = 1.0f / q_scale;
-#pragma unroll
-            for (int k = 0; k < K8; ++k)
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {  // four channels
-                    float v[4], rest[4];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float e = half_at<T>(w[k][x / 2], 4 * (x & 1) + y);
-                        v[y] = fabsf(e) <= 3.402823466e38f ? e * inv : __builtin_nanf("");
-                    }
-                    const int hi8 = (int)pack_e4m3(v[0], v[1], v[2], v[3]);
-                    rest[0] = v[0] - __builtin_amdgcn_cvt_f32_fp8(hi8, 0);
-                    rest[1] = v[1] - __builtin_amdgcn_cvt_f32_fp8(hi8, 1);
-                    rest[2] = v[2] - __builtin_amdgcn_cvt_f32_fp8(hi8, 2);
-                    rest[3] = v[3] - __builtin_amdgcn_cvt_f32_fp8(hi8, 3);
-                    q8[k][0][x] = hi8;
-                    q8[k][1][x] = (int)pack_e4m3(16.f * rest[0], 16.f * rest[1], 16.f * rest[2], 16.f * rest[3]);
-                }
-        }
-    }
-
     // Blocks and scales of 16 of the group's tiles: lane l has chunk l % 4 of tile l / 4.
     auto page_ids = [&](int j0) {
-        const int64_t key = 64 * (2 * ((int64_t)j0 + (lane >> 2)) + grp) + 16 * (lane & 3);
+        const int64_t key = 64 * (GROUPS * ((int64_t)j0 + (lane >> 2)) + grp) + 16 * (lane & 3);
         return key < r.len ? a.table[b * a.table_stride + key / bs] : -1;
     };
-    auto page_scales = [&](AttnPages& p) {
+    struct Pages : AttnPages {
+        float log_sv, inv_sv;
+        uint64_t plain;  // bit l: lane l's chunk is there and its value scale an ordinary one
+    };
+    auto page_scales = [&](Pages& p) {
         if (p.id < 0 || p.id >= a.c.blocks) p.id = -1;
         const int64_t at = (int64_t)max(p.id, 0) * a.c.heads + h;
         p.sk = a.c.k_scale[at];
         p.sv = a.c.v_scale[at];
     };
+    auto page_derive = [&](Pages& p) {
+        p.log_sv = __builtin_amdgcn_logf(p.sv);
+        p.inv_sv = __builtin_amdgcn_rcpf(p.sv);
+        p.plain = __ballot(p.id >= 0 && p.sv >= 0x1p-64f && p.sv <= 0x1p64f);
+    };
+    // every row of the wave sees all keys below this
+    const int open = w0 < r.rows ? min(r.len - r.n + w0 / a.G + 1, r.len) : r.len;
     const uint32_t lds0 = (uint32_t)(uintptr_t)&ring[0] + (uint32_t)(grp * kChunkRing * 2 * TILE);
     // LDS row m of a half tile holds key 16 (m / 4 % 2) + 4 (m / 8) + m % 4 of it; rows
     // are swizzled by 16-byte chunks so that 16 lanes reading one chunk of 16 rows
     // touch every bank once (rows of 128 bytes: c ^ m / 2 % 8, of 64: c ^ m / 4 % 4).
     auto swz = [](int row64, int m, int c) { return row64 ? c ^ ((m >> 2) & 3) : c ^ ((m >> 1) & 7); };
     // The loads of a tile are 2 DMA of this wave: x < DMA keys, else values. A lane's
-    // load x is at one place of a block in every tile (a group's tiles are 128 keys
-    // apart, whole blocks): `at` is that place in block 0, `from` the lane (times
-    // 4) of AttnPages with its chunk of tile 0.
+    // load x is at one place of a block in every tile: `at` is that place in block 0, `from`
+    // the lane (times 4) of AttnPages with its chunk of tile 0. (Two groups' tiles are
+    // 128 keys apart, whole blocks; one group's odd tiles are the second half of a block of 128.)
     uint64_t at[2 * DMA];
     int from[2 * DMA];
 #pragma unroll
     for (int x = 0; x < DMA; ++x) {
-        const int i = wr + 4 * x;
+        const int i = wr + LOADERS * x;
         const int m = i * (1024 / D) + lane / KC, c = swz(D == 64, m, lane % KC), m32 = m & 31;
         const int key = (m & 32) + 16 * ((m32 >> 2) & 1) + 4 * (m32 >> 3) + (m32 & 3);
         at[x] = (uint64_t)(uintptr_t)a.c.k + ((int64_t)h * bs + ((64 * grp + key) & (bs - 1))) * D + 16 * c;
@@ -872,15 +836,89 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     }
     const uint32_t k_stride = (uint32_t)a.c.k_stride, v_stride = (uint32_t)a.c.v_stride;  // below 2^31
     auto load_id = [&](int x, int ids, int j) { return __builtin_amdgcn_ds_bpermute(from[x] + 16 * (j & 15), ids); };
-    auto issue_one = [&](int x, int id, int in) {  // from block id into tile in's slot
-        const uint32_t slot = lds0 + (uint32_t)((in % kChunkRing) * 2 * TILE + 1024 * (wr + 4 * (x % DMA)));
-        const uint64_t src = at[x] + (uint64_t)(uint32_t)max(id, 0) * (x < DMA ? k_stride : v_stride);
+    const uint32_t odd = GROUPS == 1 && bs > 64 ? 64 : 0;  // keys
+    auto issue_one = [&](int x, int id, int j, int in) {  // of tile j, from block id into tile in's slot
+        const uint32_t slot = lds0 + (uint32_t)((in % kChunkRing) * 2 * TILE + 1024 * (wr + LOADERS * (x % DMA)));
+        const uint64_t src = at[x] + (uint64_t)(uint32_t)max(id, 0) * (x < DMA ? k_stride : v_stride) +
+                             (j & 1 ? (x < DMA ? odd * D : odd) : 0u);
         lds_dma_b128((const void*)(uintptr_t)src, x < DMA ? slot : slot + TILE);
     };
-    auto issue = [&](const AttnPages& p, int j, int in) {
+    auto issue = [&](const Pages& p, int j, int in) {
 #pragma unroll
-        for (int x = 0; x < 2 * DMA; ++x) issue_one(x, load_id(x, p.id, j), in);
+        for (int x = 0; x < 2 * DMA; ++x) issue_one(x, load_id(x, p.id, j), j, in);
     };
+
+    // bf16: q = r (h + l / 16) with r a power of two for the row and h and l e4m3: 4 + 4
+    // of its 8 bits, exact down to 2^-14 of the row's largest element, below
+    // that to 2^-23 of it. The scores are then products of codes as they are, at twice
+    // the rate, and K needs no conversion. f16 has 11 bits: K is converted.
+    constexpr int K8 = D / 64;  // 64-channel steps of the code product
+    u32x4 q[SPLIT ? 2 * KK : 1];
+    i32x8 q8[SPLIT ? 1 : K8][2];
+    float q_scale = 1.f;
+    // What the first products wait for, in this order: the blocks' ids and Q together, then
+    // the scales and the tiles, and Q's codes while the tiles come.
+    u32x4 w[SPLIT ? 1 : K8][4];
+    Pages pg, nx;  // of the tile whose softmax is next; of the tiles 16 on
+    pg.id = page_ids(0);
+    {
+        const int i = live ? row / a.G : 0, qh = live ? row % a.G : 0;
+        const uint16_t* src = a.q + (int64_t)(r.first + i) * a.q_stride + (int64_t)(h * a.G + qh) * D;
+        if constexpr (SPLIT) {
+#pragma unroll
+            for (int k = 0; k < KK; ++k)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) q[2 * k + u] = *reinterpret_cast<const u32x4*>(src + 32 * k + 16 * hh + 8 * u);
+#pragma unroll
+            for (int k = 0; k < 2 * KK; ++k) asm volatile("" : "+v"(q[k]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < K8; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) w[k][x] = *reinterpret_cast<const u32x4*>(src + 64 * k + 32 * hh + 8 * x);
+#pragma unroll
+            for (int k = 0; k < K8; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) asm volatile("" : "+v"(w[k][x]));
+        }
+    }
+    page_scales(pg);
+    nx = pg;
+    if (n > 0)
+        for (int j = 0; j < 3; ++j) issue(pg, min(j, n - 1), j);
+    if constexpr (!SPLIT) {
+        float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < K8; ++k)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    const float v = fabsf(half_at<T>(w[k][x], y));
+                    most = v <= 3.402823466e38f ? fmaxf(most, v) : most;
+                }
+        most = fmaxf(most, __shfl_xor(most, 32));
+        q_scale = e4m3_scale(most);
+        const float inv = 1.0f / q_scale;
+#pragma unroll
+        for (int k = 0; k < K8; ++k)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {  // four channels
+                float v[4], rest[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float e = half_at<T>(w[k][x / 2], 4 * (x & 1) + y);
+                    v[y] = fabsf(e) <= 3.402823466e38f ? e * inv : __builtin_nanf("");
+                }
+                const int hi8 = (int)pack_e4m3(v[0], v[1], v[2], v[3]);
+                rest[0] = v[0] - __builtin_amdgcn_cvt_f32_fp8(hi8, 0);
+                rest[1] = v[1] - __builtin_amdgcn_cvt_f32_fp8(hi8, 1);
+                rest[2] = v[2] - __builtin_amdgcn_cvt_f32_fp8(hi8, 2);
+                rest[3] = v[3] - __builtin_amdgcn_cvt_f32_fp8(hi8, 3);
+                q8[k][0][x] = hi8;
+                q8[k][1][x] = (int)pack_e4m3(16.f * rest[0], 16.f * rest[1], 16.f * rest[2], 16.f * rest[3]);
+            }
+    }
 
     f32x16 o[DT], s[2];
 #pragma unroll
@@ -889,31 +927,29 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
     float m = -INFINITY, l = 0.f;
     u32x4 hi[4], lo[4];  // P^T: [2 e + u], half tile e, its keys 8 u .. of each lane half
-    AttnPages pg, nx;  // of the tile whose softmax is next; of the tiles 16 on
-    pg.id = page_ids(0);
-    page_scales(pg);
-    nx = pg;
-    if (n > 16) {
-        nx.id = page_ids(16);
-        page_scales(nx);
-    }
     // What the next softmax needs of its tile's two chunks of this lane.
-    float sk[2], sv[2];
-    int chunk_id[2];
+    float sk[2], log_sv[2], inv_sv[2];
+    auto of_chunk = [&](int x, int j, int e) { return __builtin_amdgcn_ds_bpermute(16 * (j & 15) + 8 * e + 4 * hh, x); };
+    auto of_chunk_f = [&](float x, int j, int e) { return __int_as_float(of_chunk(__float_as_int(x), j, e)); };
     auto take_scales = [&](int j) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int lane4 = 16 * (j & 15) + 8 * e + 4 * hh;
-            sk[e] = __uint_as_float(__builtin_amdgcn_ds_bpermute(lane4, (int)__float_as_uint(pg.sk)));
-            sv[e] = __uint_as_float(__builtin_amdgcn_ds_bpermute(lane4, (int)__float_as_uint(pg.sv)));
-            chunk_id[e] = __builtin_amdgcn_ds_bpermute(lane4, pg.id);
+            sk[e] = of_chunk_f(pg.sk, j, e);
+            log_sv[e] = of_chunk_f(pg.log_sv, j, e);
+            inv_sv[e] = of_chunk_f(pg.inv_sv, j, e);
         }
     };
     u32x4 vf[3];  // value fragments, read two steps ahead; a tile's first two before its M phase
-    auto load_v = [&](int j, int st, int x) {
+    // A tile's values as this lane reads them: half tile e, made here so that the addresses
+    // are not held over the loop for every slot of the ring.
+    auto v_base = [&](int j, const uint8_t* (&vs)[2]) {
         uint32_t so = (uint32_t)((grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE);
         asm volatile("" : "+s"(so));
-        vf[x] = *reinterpret_cast<const u32x4*>(ring + so + (32 * (st % KK) + l32) * 64 + 16 * swz(1, l32, 2 * (st / KK) + hh));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) vs[e] = ring + so + l32 * 64 + 16 * swz(1, l32, 2 * e + hh);
+    };
+    auto load_v = [&](const uint8_t* const (&vs)[2], int st) {
+        vf[st % 3] = *reinterpret_cast<const u32x4*>(vs[st / KK] + 32 * (st % KK) * 64);
     };
 
     // This wave's part of tile j's values, which has landed: NaN codes out of it. (The
@@ -922,15 +958,18 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     auto read_part = [&](int j) {
         const uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
 #pragma unroll
-        for (int x = 0; x < DMA; ++x) part[x] = *reinterpret_cast<const u32x4*>(mine + 1024 * (wr + 4 * x));
+        for (int x = 0; x < DMA; ++x) part[x] = *reinterpret_cast<const u32x4*>(mine + 1024 * (wr + LOADERS * x));
     };
-    auto check_part = [&](int j) {
+    auto part_nans = [&]() {
         uint32_t bad = 0;
 #pragma unroll
         for (int x = 0; x < DMA; ++x)
 #pragma unroll
             for (int y = 0; y < 4; ++y) bad |= (part[x][y] & 0x7f7f7f7fu) + 0x01010101u;
-        const bool any = __any((bad & 0x80808080u) != 0);
+        return bad & 0x80808080u;
+    };
+    auto check_part = [&](int j, uint32_t bad) {
+        const bool any = __any(bad != 0);
         if (lane == 0) with_nan[4 * grp + (j & 3)][wr] = any;
         if (!any) return;
         uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
@@ -944,8 +983,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 bits |= (nan * 0x01020408u >> 24) << (4 * y);
                 w[y] &= ~(nan * 0xffu);
             }
-            nans[4 * grp + (j & 3)][64 * (wr + 4 * x) + lane] = (uint16_t)bits;
-            *reinterpret_cast<u32x4*>(mine + 1024 * (wr + 4 * x)) = w;
+            nans[4 * grp + (j & 3)][64 * (wr + LOADERS * x) + lane] = (uint16_t)bits;
+            *reinterpret_cast<u32x4*>(mine + 1024 * (wr + LOADERS * x)) = w;
         }
     };
     // NaN codes among tile j's values: NaN sums for the rows that see them, by a product of indicators.
@@ -960,7 +999,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
 #pragma unroll
             for (int k = 0; k < DT; ++k) {
                 uint32_t bits = nans[which][(32 * k + l32) * 4 + swz(1, l32, 2 * e + hh)];
-                if (!with_nan[which][(2 * k + (l32 >> 4)) & 3]) bits = 0;  // the part has none
+                if (!with_nan[which][(2 * k + (l32 >> 4)) % LOADERS]) bits = 0;  // the part has none
                 u32x4 w;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) w[x] = (((bits >> (4 * x)) & 15u) * 0x00204081u & 0x01010101u) * 0x38u;  // 1.0
@@ -1003,7 +1042,10 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             }
         };
         int ids[2 * DMA];
+        const uint8_t* vs[2];
+        uint32_t bad = 0;
         if constexpr (DP) {
+            v_base(jp, vs);
 #pragma unroll
             for (int x = 0; x < 2 * DMA; ++x) ids[x] = load_id(x, ids_of_ji, ji);
         }
@@ -1011,28 +1053,25 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         for (int st = 0; st < ST + 2; ++st) {
             if (st < ST) load_k(st);
             if constexpr (DP) {
-                if (st + 2 < ST) load_v(jp, st + 2, (st + 2) % 3);
-            }
-            if constexpr (DP) {
+                if (st + 2 < ST) load_v(vs, st + 2);
                 if (st == ST / 2) read_part(jp + 2);
             }
             if (st == ST / 2 + 1) take_scales(js);
-            if constexpr (DP) {
-                if (st < ST) {
-                    const int e = st / KK, k = st % KK;
-                    const u32x4 w = vf[st % 3];
-                    const u32x4 v0 = fp8x8_to_half8(w[0], w[1], bf16_t{}), v1 = fp8x8_to_half8(w[2], w[3], bf16_t{});
-                    o[k] = mfma32x32x16(v0, hi[2 * e], o[k], bf16_t{});
-                    o[k] = mfma32x32x16(v1, hi[2 * e + 1], o[k], bf16_t{});
-                    if constexpr (SPLIT) {
-                        o[k] = mfma32x32x16(v0, lo[2 * e], o[k], bf16_t{});
-                        o[k] = mfma32x32x16(v1, lo[2 * e + 1], o[k], bf16_t{});
+            // O's two products of a step wait for each other: S goes between them.
+            auto pv = [&](int u) {
+                if constexpr (DP) {
+                    if (st < ST) {
+                        const int e = st / KK, k = st % KK;
+                        const u32x4 w = vf[st % 3], v0 = fp8x8_to_half8(w[2 * u], w[2 * u + 1], bf16_t{});
+                        o[k] = mfma32x32x16(v0, hi[2 * e + u], o[k], bf16_t{});
+                        if constexpr (SPLIT) o[k] = mfma32x32x16(v0, lo[2 * e + u], o[k], bf16_t{});
                     }
                 }
-            }
+            };
             f32x16 zero;
 #pragma unroll
             for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+            pv(0);
             if (st >= 2) {
                 const int ss = st - 2;
                 if constexpr (SPLIT) {
@@ -1050,43 +1089,45 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                         piece ? 0x7b7b7b7b : 0x7f7f7f7f);
                 }
             }
+            pv(1);
             if constexpr (DP) {
-                if (st >= 1 && st <= 2 * DMA) issue_one(st - 1, ids[st - 1], jp + 3);
+                if (st == ST) bad = part_nans();
+            }
+            if constexpr (DP) {
+                if (st >= 1 && st <= 2 * DMA) issue_one(st - 1, ids[st - 1], ji, jp + 3);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         // used here: the compiler would move the products of S to the softmax, which
         // alone needs them, and so into the other phase
         asm volatile("" : "+v"(s[0]), "+v"(s[1]));
-        if constexpr (DP) check_part(jp + 2);
+        if constexpr (DP) check_part(jp + 2, bad);
     };
     // The softmax of tile j, whose scores are in s: P into hi (and lo).
     auto v_phase = [&](int j) {
-        const int key0 = 64 * (2 * j + grp);
-        int seen[2];
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            sk[e] *= q_scale * a.scale_log2;
-            const int key = key0 + 32 * e + 16 * hh;
-            seen[e] = chunk_id[e] < 0 ? 0 : min(min(r.len, limit + 1) - key, 16);
-            odd |= seen[e] < 16 || !(sv[e] >= 0x1p-64f && sv[e] <= 0x1p64f);
-        }
+        const int key0 = 64 * (GROUPS * j + grp);
         // Nothing masked and ordinary scales: the value scale goes into the exponent,
         // p sv = 2^(x + log2 sv), and out of the chunk's sum once. Else p is
         // masked and multiplied.
-        const bool plain = !__any(odd);
-        const float ref = m == -INFINITY ? 0.f : m;
-        float add[2], out[2];
-        if (plain) {
+        const bool plain = ((uint32_t)(pg.plain >> (4 * (j & 15))) & 15u) == 15u && key0 + 64 <= open;
+        const float ref = m == -INFINITY ? 0.f : m, factor = q_scale * a.scale_log2;
+        float add[2], out[2], sv[2];
+        int seen[2] = {16, 16};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            sk[e] *= factor;
+            add[e] = log_sv[e] - ref;
+            out[e] = inv_sv[e];
+        }
+        if (!plain) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                add[e] = __builtin_amdgcn_logf(sv[e]) - ref;
-                out[e] = __builtin_amdgcn_rcpf(sv[e]);
+                const int id = of_chunk(pg.id, j, e);
+                sv[e] = of_chunk_f(pg.sv, j, e);
+                seen[e] = id < 0 ? 0 : min(min(r.len, limit + 1) - (key0 + 32 * e + 16 * hh), 16);
+                add[e] = -ref;
+                out[e] = 1.0f;
             }
-        } else {
-            add[0] = add[1] = -ref;
-            out[0] = out[1] = 1.0f;
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -1169,7 +1210,10 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         }
         l += sum;
         const int* nan = with_nan[4 * grp + (j & 3)];
-        if (__builtin_amdgcn_readfirstlane(nan[0] | nan[1] | nan[2] | nan[3])) nan_values(j, seen);
+        int any_nan = nan[0];
+#pragma unroll
+        for (int i = 1; i < LOADERS; ++i) any_nan |= nan[i];
+        if (__builtin_amdgcn_readfirstlane(any_nan)) nan_values(j, seen);
     };
 
     // One M phase and what comes with it; the last tiles' load the last tile once more, into
@@ -1189,76 +1233,87 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         // the next 16 tiles' blocks, then their scales: they have tiles' time to come
         if ((j & 15) == 1 && (j & ~15) + 16 < n) nx.id = page_ids((j & ~15) + 16);
         if ((j & 15) == 3) page_scales(nx);
+        if ((j & 15) == 5) page_derive(nx);
         v_phase(j);
-        load_v(j, 0, 0);
-        load_v(j, 1, 1);
+        const uint8_t* vs[2];
+        v_base(j, vs);
+        load_v(vs, 0);
+        load_v(vs, 1);
     };
     if (n > 0) {
-        for (int j = 0; j < 3; ++j) issue(pg, min(j, n - 1), j);
         wait_vmem_le<2 * DMA>();  // tiles 0 and 1
+        page_derive(pg);
         read_part(0);
-        check_part(0);
+        check_part(0, part_nans());
         read_part(1);
-        check_part(1);
+        check_part(1, part_nans());
         __syncthreads();
         m_phase(std::false_type{}, -1, 0, 0);
-        // A barrier a tile: group 0 passes it before, group 1 behind a product, so the groups
+        // A barrier a tile: a SIMD's first wave passes it before, its second behind a product, so they
         // stay half a tile apart and are free between. Behind it the tile that both
         // waited for and checked is there, and the slot of the tile before is free.
         for (int k = 0; k < n; ++k) {
             v_step(k);
-            if (grp == 0 && k > 0) __syncthreads();
+            if (phase == 0 && k > 0) __syncthreads();
             m_step(k);
-            if (grp == 1) __syncthreads();
+            if (phase == 1) __syncthreads();
         }
-        if (grp == 0) __syncthreads();
+        if (phase == 0) __syncthreads();
     }
     wait_vmem_le<0>();  // no load into a ring is on its way
-    __syncthreads();    // the rings are free
 
-    // Join: group g ends with channels 32 t .. of t in its half.
-    {
-        l += __shfl_xor(l, 32);
-        if (hh == 0) {
-            joint[wave][l32][0] = m;
-            joint[wave][l32][1] = l;
-        }
-        f32x4* give = reinterpret_cast<f32x4*>(ring) + (size_t)wave * (DT / 2) * 4 * kWave + lane;
+    l += __shfl_xor(l, 32);
+    uint16_t* dst = a.o + (int64_t)(r.first + row / a.G) * a.o_stride + (int64_t)(h * a.G + row % a.G) * D + 4 * hh;
+    auto store = [&](int t, int i, float z0, float z1, float z2, float z3) {  // channels 32 t + 8 i + 4 hh ..
+        u32x2 w;
+        w[0] = (uint32_t)elem<T>::from_f32(z0) | ((uint32_t)elem<T>::from_f32(z1) << 16);
+        w[1] = (uint32_t)elem<T>::from_f32(z2) | ((uint32_t)elem<T>::from_f32(z3) << 16);
+        if (live) *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * i) = w;
+    };
+    if constexpr (GROUPS == 1) {
+        const float inv = m == -INFINITY ? 0.f : 1.0f / l;
 #pragma unroll
-        for (int t = 0; t < DT / 2; ++t)
+        for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x16& x = o[t];
-                const f32x16& y = o[DT / 2 + t];
-                give[(4 * t + i) * kWave] =
-                    grp == 0 ? f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]}
-                             : f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
-            }
-        __syncthreads();
-        const float m2 = joint[wave ^ 4][l32][0], l2 = joint[wave ^ 4][l32][1];
-        const float mx = __builtin_elementwise_maximum(m, m2), ref = mx == -INFINITY ? 0.f : mx;
-        const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(m2 - ref);
-        const float inv = mx == -INFINITY ? 0.f : 1.0f / (l * f + l2 * g);
-        const f32x4* take = reinterpret_cast<const f32x4*>(ring) + (size_t)(wave ^ 4) * (DT / 2) * 4 * kWave + lane;
-        uint16_t* dst = a.o + (int64_t)(r.first + row / a.G) * a.o_stride + (int64_t)(h * a.G + row % a.G) * D +
-                        32 * (DT / 2) * grp + 4 * hh;
-#pragma unroll
-        for (int t = 0; t < DT / 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 y = take[(4 * t + i) * kWave];
-                float z[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float mine = grp == 0 ? o[t][4 * i + e] : o[DT / 2 + t][4 * i + e];
-                    z[e] = (mine * f + y[e] * g) * inv;
-                }
-                u32x2 w;
-                w[0] = (uint32_t)elem<T>::from_f32(z[0]) | ((uint32_t)elem<T>::from_f32(z[1]) << 16);
-                w[1] = (uint32_t)elem<T>::from_f32(z[2]) | ((uint32_t)elem<T>::from_f32(z[3]) << 16);
-                if (live) *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * i) = w;
-            }
+            for (int i = 0; i < 4; ++i)
+                store(t, i, o[t][4 * i] * inv, o[t][4 * i + 1] * inv, o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv);
+        return;
     }
+    __syncthreads();  // the rings are free
+    // Join: group g ends with channels 32 t .. of t in its half.
+    if (hh == 0) {
+        joint[wave][l32][0] = m;
+        joint[wave][l32][1] = l;
+    }
+    f32x4* give = reinterpret_cast<f32x4*>(ring) + (size_t)wave * (DT / 2) * 4 * kWave + lane;
+#pragma unroll
+    for (int t = 0; t < DT / 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x16& x = o[t];
+            const f32x16& y = o[DT / 2 + t];
+            give[(4 * t + i) * kWave] = grp == 0 ? f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]}
+                                                 : f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+        }
+    __syncthreads();
+    const float m2 = joint[wave ^ 4][l32][0], l2 = joint[wave ^ 4][l32][1];
+    const float mx = __builtin_elementwise_maximum(m, m2), ref = mx == -INFINITY ? 0.f : mx;
+    const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(m2 - ref);
+    const float inv = mx == -INFINITY ? 0.f : 1.0f / (l * f + l2 * g);
+    const f32x4* take = reinterpret_cast<const f32x4*>(ring) + (size_t)(wave ^ 4) * (DT / 2) * 4 * kWave + lane;
+#pragma unroll
+    for (int t = 0; t < DT / 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 y = take[(4 * t + i) * kWave];
+            float z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float mine = grp == 0 ? o[t][4 * i + e] : o[DT / 2 + t][4 * i + e];
+                z[e] = (mine * f + y[e] * g) * inv;
+            }
+            store(grp * (DT / 2) + t, i, z[0], z[1], z[2], z[3]);
+        }
 }
 
 // A batch with requests of many rows: the first `parts` workgroups take parts of these,
@@ -1268,11 +1323,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, 
     static_assert(split_waves(1, 128) * kWave == kChunkThreads, "one workgroup size");
     union Share {
         SplitShare<D, 1> split;
-        ChunkShare<D> chunk;
+        ChunkShare<D, 2> chunk;
     };
     __shared__ Share sh;
-    if ((int)blockIdx.x < parts) chunk_body<T, D>(a, sp.most_rows, sh.chunk, blockIdx.x);
+    if ((int)blockIdx.x < parts) chunk_body<T, D, 2>(a, sp.most_rows, sh.chunk, blockIdx.x);
     else split_body<T, D, 1>(a, sp, sh.split, blockIdx.x - parts, gridDim.x - parts);
+}
+
+// A batch of long chunks only: parts of 256 rows.
+template <typename T, int D> __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunks_kernel(AttnArgs a) {
+    __shared__ ChunkShare<D, 1> sh;
+    chunk_body<T, D, 1>(a, 0, sh, blockIdx.x);
 }
 
 // Rows of a request that the split kernel takes, 16 NT of them a wave: all up to 64 at
@@ -1309,7 +1370,13 @@ template <typename T, int D> static void launch_attention(const AttnArgs& a, int
     if (chunks_only) sp.most_rows = 0;
     // Parts: whole ones, and one more for each request that is large enough.
     const long all = (long)a.tokens * a.G, some = all / (sp.most_rows + 1);
-    const long parts = (all / kChunkRows + (some < a.B ? some : a.B)) * a.c.heads;
+    auto parts_of = [&](int groups) { return (all / chunk_rows(groups) + (some < a.B ? some : a.B)) * a.c.heads; };
+    if constexpr (D == 128)
+        if (chunks_only && parts_of(2) > kSplitGroups) {
+            hipLaunchKernelGGL((kv_chunks_kernel<T, D>), dim3((unsigned)parts_of(1)), dim3(kChunkThreads), 0, s, a);
+            return;
+        }
+    const long parts = parts_of(2);
     hipLaunchKernelGGL((kv_chunk_kernel<T, D>), dim3((unsigned)(parts + (chunks_only ? 0 : split))), dim3(kChunkThreads), 0,
                        s, a, sp, (int)parts);
 }
