@@ -724,6 +724,9 @@ constexpr float kChunkSumMax = 16384.0f;
 template <int D, int GROUPS> struct ChunkShare {
     static constexpr int TILE = 64 * D;
     __attribute__((aligned(1024))) uint8_t ring[GROUPS * kChunkRing * 2 * TILE];
+    // One group: the values as bf16, converted once by the wave that loaded them. Channel
+    // rows of 64 keys, 16-byte chunks at c ^ row % 8. Two groups have no room for this.
+    __attribute__((aligned(1024))) uint16_t values[GROUPS == 1 ? kChunkRing * TILE : 1];
     // Which codes of a value tile are NaN, a bit each, where a wave's part of it (with_nan)
     // has any; [group][tile % 4]. In the ring these are 0: the product then says
     // nothing of them, and nan_values gives the NaN to the rows that see them.
@@ -742,6 +745,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     constexpr int TILE = 64 * D;          // bytes of one operand of a tile
     constexpr int DMA = TILE / (LOADERS * 1024);  // wave loads of an operand for each of them
     static_assert(DMA > 0, "each loads of both operands");
+    constexpr bool SHARED = GROUPS == 1;  // converted values in LDS
     constexpr bool SPLIT = __is_same(T, f16_t);
     auto& ring = sh.ring;
     auto& nans = sh.nans;
@@ -752,7 +756,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int phase = wave >> 2;                                 // which of a SIMD's two waves
     const int grp = GROUPS == 2 ? phase : 0, wr = wave % LOADERS;  // whose tiles; place in the group
-    const int l32 = lane & 31, hh = lane >> 5, bs = a.c.bs;
+    const int l32 = lane & 31, hh = lane >> 5, bs = a.c.bs, bs_log2 = __builtin_ctz(bs);
 
     // The part: part_index counts (request, row tile from the last, head).
     int b = -1, h = 0, rt = 0;
@@ -762,7 +766,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         for (int b0 = 0; b0 < a.B && b < 0; b0 += kWave) {
             const int i = b0 + lane;
             const AttnReq near = i < a.B ? attn_request(a, i) : AttnReq{0, 0, 0, 0};
-            const int64_t mine = (int64_t)chunk_tiles(near, from_rows, ROWS) * a.c.heads;
+            const int tiles = chunk_tiles(near, from_rows, ROWS);
+            const int64_t mine = (int64_t)tiles * a.c.heads;
             const int64_t end = base + wave_prefix(mine);
             const uint64_t past = __ballot(end > part_index);
             if (past) {
@@ -770,7 +775,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 const int v = (int)(part_index - read_lane(end - mine, i2));
                 b = b0 + i2;
                 h = v % a.c.heads;
-                rt = (int)(read_lane(mine, i2) / a.c.heads) - 1 - v / a.c.heads;
+                rt = __builtin_amdgcn_readlane(tiles, i2) - 1 - v / a.c.heads;
                 r = AttnReq{__builtin_amdgcn_readlane(near.len, i2), __builtin_amdgcn_readlane(near.n, i2),
                             __builtin_amdgcn_readlane(near.first, i2), __builtin_amdgcn_readlane(near.rows, i2)};
             }
@@ -793,7 +798,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     // Blocks and scales of 16 of the group's tiles: lane l has chunk l % 4 of tile l / 4.
     auto page_ids = [&](int j0) {
         const int64_t key = 64 * (GROUPS * ((int64_t)j0 + (lane >> 2)) + grp) + 16 * (lane & 3);
-        return key < r.len ? a.table[b * a.table_stride + key / bs] : -1;
+        return key < r.len ? a.table[b * a.table_stride + (key >> bs_log2)] : -1;
     };
     struct Pages : AttnPages {
         float log_sv, inv_sv;
@@ -929,6 +934,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     u32x4 hi[4], lo[4];  // P^T: [2 e + u], half tile e, its keys 8 u .. of each lane half
     // What the next softmax needs of its tile's two chunks of this lane.
     float sk[2], log_sv[2], inv_sv[2];
+    int any_nan = 0;  // lane x % LOADERS: NaN codes among the values that wave loaded
     auto of_chunk = [&](int x, int j, int e) { return __builtin_amdgcn_ds_bpermute(16 * (j & 15) + 8 * e + 4 * hh, x); };
     auto of_chunk_f = [&](float x, int j, int e) { return __int_as_float(of_chunk(__float_as_int(x), j, e)); };
     auto take_scales = [&](int j) {
@@ -938,18 +944,32 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             log_sv[e] = of_chunk_f(pg.log_sv, j, e);
             inv_sv[e] = of_chunk_f(pg.inv_sv, j, e);
         }
+        any_nan = with_nan[4 * grp + (j & 3)][lane % LOADERS];
     };
-    u32x4 vf[3];  // value fragments, read two steps ahead; a tile's first two before its M phase
+    // Value fragments, read two steps ahead; a tile's first two before its M phase.
+    u32x4 vf[3][SHARED ? 2 : 1];
     // A tile's values as this lane reads them: half tile e, made here so that the addresses
     // are not held over the loop for every slot of the ring.
     auto v_base = [&](int j, const uint8_t* (&vs)[2]) {
-        uint32_t so = (uint32_t)((grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE);
+        uint32_t so = (uint32_t)(SHARED ? j % kChunkRing * 2 * TILE : (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE);
         asm volatile("" : "+s"(so));
 #pragma unroll
-        for (int e = 0; e < 2; ++e) vs[e] = ring + so + l32 * 64 + 16 * swz(1, l32, 2 * e + hh);
+        for (int e = 0; e < 2; ++e)
+            if constexpr (SHARED) vs[e] = (const uint8_t*)sh.values + so + l32 * 128 + 16 * ((4 * e + 2 * hh) ^ (l32 & 7));
+            else vs[e] = ring + so + l32 * 64 + 16 * swz(1, l32, 2 * e + hh);
     };
+    const int other = (l32 & 1) ? -16 : 16;  // from a fragment's first chunk to its second
     auto load_v = [&](const uint8_t* const (&vs)[2], int st) {
-        vf[st % 3] = *reinterpret_cast<const u32x4*>(vs[st / KK] + 32 * (st % KK) * 64);
+        const uint8_t* p = vs[st / KK] + 32 * (st % KK) * (SHARED ? 128 : 64);
+        vf[st % 3][0] = *reinterpret_cast<const u32x4*>(p);
+        if constexpr (SHARED) vf[st % 3][1] = *reinterpret_cast<const u32x4*>(p + other);
+    };
+    auto put_values = [&](int j, int x, const u32x4& w) {  // this lane's chunk of codes into sh.values
+        const int d = 16 * (wr + LOADERS * x) + lane / 4, c = 2 * swz(1, d, lane & 3);
+        uint16_t* row = sh.values + j % kChunkRing * TILE + 64 * d;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<u32x4*>(row + 8 * ((c + u) ^ (d & 7))) = fp8x8_to_half8(w[2 * u], w[2 * u + 1], bf16_t{});
     };
 
     // This wave's part of tile j's values, which has landed: NaN codes out of it. (The
@@ -960,12 +980,14 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
 #pragma unroll
         for (int x = 0; x < DMA; ++x) part[x] = *reinterpret_cast<const u32x4*>(mine + 1024 * (wr + LOADERS * x));
     };
-    auto part_nans = [&]() {
+    auto part_nans = [&](int j) {
         uint32_t bad = 0;
 #pragma unroll
-        for (int x = 0; x < DMA; ++x)
+        for (int x = 0; x < DMA; ++x) {
+            if constexpr (SHARED) put_values(j, x, part[x]);  // and again should one be NaN
 #pragma unroll
             for (int y = 0; y < 4; ++y) bad |= (part[x][y] & 0x7f7f7f7fu) + 0x01010101u;
+        }
         return bad & 0x80808080u;
     };
     auto check_part = [&](int j, uint32_t bad) {
@@ -984,7 +1006,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 w[y] &= ~(nan * 0xffu);
             }
             nans[4 * grp + (j & 3)][64 * (wr + LOADERS * x) + lane] = (uint16_t)bits;
-            *reinterpret_cast<u32x4*>(mine + 1024 * (wr + LOADERS * x)) = w;
+            if constexpr (SHARED) put_values(j, x, w);
+            else *reinterpret_cast<u32x4*>(mine + 1024 * (wr + LOADERS * x)) = w;
         }
     };
     // NaN codes among tile j's values: NaN sums for the rows that see them, by a product of indicators.
@@ -1062,7 +1085,9 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 if constexpr (DP) {
                     if (st < ST) {
                         const int e = st / KK, k = st % KK;
-                        const u32x4 w = vf[st % 3], v0 = fp8x8_to_half8(w[2 * u], w[2 * u + 1], bf16_t{});
+                        u32x4 v0;
+                        if constexpr (SHARED) v0 = vf[st % 3][u];
+                        else v0 = fp8x8_to_half8(vf[st % 3][0][2 * u], vf[st % 3][0][2 * u + 1], bf16_t{});
                         o[k] = mfma32x32x16(v0, hi[2 * e + u], o[k], bf16_t{});
                         if constexpr (SPLIT) o[k] = mfma32x32x16(v0, lo[2 * e + u], o[k], bf16_t{});
                     }
@@ -1091,7 +1116,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             }
             pv(1);
             if constexpr (DP) {
-                if (st == ST) bad = part_nans();
+                if (st == ST) bad = part_nans(jp + 2);
             }
             if constexpr (DP) {
                 if (st >= 1 && st <= 2 * DMA) issue_one(st - 1, ids[st - 1], ji, jp + 3);
@@ -1154,17 +1179,26 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                     pack_half2(x0 - __uint_as_float(w << 16), x1 - __uint_as_float(w & 0xffff0000u), bf16_t{});
         };
         auto exponentiate = [&]() {  // s becomes what is rounded to P; the sum of p
-            float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+            // Four at a time, summed and rounded while the next four are on their way: an
+            // addition right behind its exponential waits for it.
+            float p[8][4], sum[2][4];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int g = 0; g <= 8; ++g) {
+                if (g < 8) {
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(s[e][i]), p1 = __builtin_amdgcn_exp2f(s[e][i + 1]);
-                    sum[e][0] += p0;
-                    sum[e][1] += p1;
-                    pack(e, i, p0, p1);
+                    for (int x = 0; x < 4; ++x) p[g][x] = __builtin_amdgcn_exp2f(s[g >> 2][4 * (g & 3) + x]);
                 }
-            return (sum[0][0] + sum[0][1]) * out[0] + (sum[1][0] + sum[1][1]) * out[1];
+                if (g > 0) {
+                    const int w = g - 1, e = w >> 2;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) sum[e][x] = w & 3 ? sum[e][x] + p[w][x] : p[w][x];
+                    pack(e, 4 * (w & 3), p[w][0], p[w][1]);
+                    pack(e, 4 * (w & 3) + 2, p[w][2], p[w][3]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            return ((sum[0][0] + sum[0][1]) + (sum[0][2] + sum[0][3])) * out[0] +
+                   ((sum[1][0] + sum[1][1]) + (sum[1][2] + sum[1][3])) * out[1];
         };
         float sum = exponentiate();
         const bool fresh = m == -INFINITY && (seen[0] > 0 || seen[1] > 0);
@@ -1209,11 +1243,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             }
         }
         l += sum;
-        const int* nan = with_nan[4 * grp + (j & 3)];
-        int any_nan = nan[0];
-#pragma unroll
-        for (int i = 1; i < LOADERS; ++i) any_nan |= nan[i];
-        if (__builtin_amdgcn_readfirstlane(any_nan)) nan_values(j, seen);
+        if (__any(any_nan)) nan_values(j, seen);
     };
 
     // One M phase and what comes with it; the last tiles' load the last tile once more, into
@@ -1244,9 +1274,9 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         wait_vmem_le<2 * DMA>();  // tiles 0 and 1
         page_derive(pg);
         read_part(0);
-        check_part(0, part_nans());
+        check_part(0, part_nans(0));
         read_part(1);
-        check_part(1, part_nans());
+        check_part(1, part_nans(1));
         __syncthreads();
         m_phase(std::false_type{}, -1, 0, 0);
         // A barrier a tile: a SIMD's first wave passes it before, its second behind a product, so they
@@ -1263,20 +1293,29 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     wait_vmem_le<0>();  // no load into a ring is on its way
 
     l += __shfl_xor(l, 32);
-    uint16_t* dst = a.o + (int64_t)(r.first + row / a.G) * a.o_stride + (int64_t)(h * a.G + row % a.G) * D + 4 * hh;
-    auto store = [&](int t, int i, float z0, float z1, float z2, float z3) {  // channels 32 t + 8 i + 4 hh ..
-        u32x2 w;
-        w[0] = (uint32_t)elem<T>::from_f32(z0) | ((uint32_t)elem<T>::from_f32(z1) << 16);
-        w[1] = (uint32_t)elem<T>::from_f32(z2) | ((uint32_t)elem<T>::from_f32(z3) << 16);
-        if (live) *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * i) = w;
+    uint16_t* dst = a.o + (int64_t)(r.first + row / a.G) * a.o_stride + (int64_t)(h * a.G + row % a.G) * D + 8 * hh;
+    // Channels 32 t + 8 i + 4 hh .. of i and i + 1: the lane halves exchange, so that each
+    // stores 16 bytes, of i or of i + 1.
+    auto store = [&](int t, int i, const float (&z)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            w[x] = (uint32_t)elem<T>::from_f32(z[2 * x]) | ((uint32_t)elem<T>::from_f32(z[2 * x + 1]) << 16);
+        const auto lo = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+        const auto hi = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+        if (live) *reinterpret_cast<u32x4*>(dst + 32 * t + 8 * i) = u32x4{lo[0], hi[0], lo[1], hi[1]};
     };
     if constexpr (GROUPS == 1) {
         const float inv = m == -INFINITY ? 0.f : 1.0f / l;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                store(t, i, o[t][4 * i] * inv, o[t][4 * i + 1] * inv, o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv);
+            for (int i = 0; i < 4; i += 2) {
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = o[t][4 * i + e] * inv;
+                store(t, i, z);
+            }
         return;
     }
     __syncthreads();  // the rings are free
@@ -1304,15 +1343,15 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
 #pragma unroll
     for (int t = 0; t < DT / 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 y = take[(4 * t + i) * kWave];
-            float z[4];
+        for (int i = 0; i < 4; i += 2) {
+            const f32x4 y[2] = {take[(4 * t + i) * kWave], take[(4 * t + i + 1) * kWave]};
+            float z[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 8; ++e) {
                 const float mine = grp == 0 ? o[t][4 * i + e] : o[DT / 2 + t][4 * i + e];
-                z[e] = (mine * f + y[e] * g) * inv;
+                z[e] = (mine * f + y[e >> 2][e & 3] * g) * inv;
             }
-            store(grp * (DT / 2) + t, i, z[0], z[1], z[2], z[3]);
+            store(grp * (DT / 2) + t, i, z);
         }
 }
 
