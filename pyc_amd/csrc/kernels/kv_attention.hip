@@ -892,37 +892,55 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     if (n > 0)
         for (int j = 0; j < 3; ++j) issue(pg, min(j, n - 1), j);
     if constexpr (!SPLIT) {
-        float most = 0.f;
+        // The largest of the row, of the bits of |q|: bf16 in halves, 7f80 and more not finite.
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 top{0, 0};
 #pragma unroll
         for (int k = 0; k < K8; ++k)
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
+            for (int x = 0; x < 16; ++x)
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[k][x / 4][x % 4] & 0x7fff7fffu));
+        uint32_t most = max((uint32_t)top[0], (uint32_t)top[1]);
+        const bool finite = __all(most < 0x7f80u);
+        if (!finite) {
+            most = 0;
 #pragma unroll
-                for (int y = 0; y < 8; ++y) {
-                    const float v = fabsf(half_at<T>(w[k][x], y));
-                    most = v <= 3.402823466e38f ? fmaxf(most, v) : most;
+            for (int k = 0; k < K8; ++k)
+#pragma unroll
+                for (int x = 0; x < 32; ++x) {
+                    const uint32_t e = w[k][x / 8][x % 8 / 2] >> (16 * (x & 1)) & 0x7fffu;
+                    most = e < 0x7f80u ? max(most, e) : most;
                 }
-        most = fmaxf(most, __shfl_xor(most, 32));
-        q_scale = e4m3_scale(most);
+        }
+        most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+        q_scale = e4m3_scale(__uint_as_float(most << 16));
         const float inv = 1.0f / q_scale;
+        auto code = [&](auto check) {
 #pragma unroll
-        for (int k = 0; k < K8; ++k)
+            for (int k = 0; k < K8; ++k)
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {  // four channels
-                float v[4], rest[4];
+                for (int x = 0; x < 8; ++x) {  // four channels
+                    float v[4], rest[4];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const float e = half_at<T>(w[k][x / 2], 4 * (x & 1) + y);
-                    v[y] = fabsf(e) <= 3.402823466e38f ? e * inv : __builtin_nanf("");
+                    for (int y = 0; y < 4; ++y) {
+                        const float e = half_at<T>(w[k][x / 2], 4 * (x & 1) + y);
+                        v[y] = e * inv;
+                        if constexpr (decltype(check)::value) v[y] = fabsf(e) <= 3.402823466e38f ? v[y] : __builtin_nanf("");
+                    }
+                    const int hi8 = (int)pack_e4m3(v[0], v[1], v[2], v[3]);
+                    const auto h01 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi8, 16.f, false);
+                    const auto h23 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi8, 16.f, true);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) rest[y] = fmaf(v[y], 16.f, -(y < 2 ? h01[y] : h23[y - 2]));
+                    q8[k][0][x] = hi8;
+                    q8[k][1][x] = (int)pack_e4m3(rest[0], rest[1], rest[2], rest[3]);
                 }
-                const int hi8 = (int)pack_e4m3(v[0], v[1], v[2], v[3]);
-                rest[0] = v[0] - __builtin_amdgcn_cvt_f32_fp8(hi8, 0);
-                rest[1] = v[1] - __builtin_amdgcn_cvt_f32_fp8(hi8, 1);
-                rest[2] = v[2] - __builtin_amdgcn_cvt_f32_fp8(hi8, 2);
-                rest[3] = v[3] - __builtin_amdgcn_cvt_f32_fp8(hi8, 3);
-                q8[k][0][x] = hi8;
-                q8[k][1][x] = (int)pack_e4m3(16.f * rest[0], 16.f * rest[1], 16.f * rest[2], 16.f * rest[3]);
-            }
+        };
+        if (finite) code(std::false_type{});
+        else code(std::true_type{});
+        // here, while the tiles come, and not behind the barrier that waits for them
+#pragma unroll
+        for (int k = 0; k < K8; ++k) asm volatile("" : "+v"(q8[k][0]), "+v"(q8[k][1]));
     }
 
     f32x16 o[DT], s[2];
@@ -946,8 +964,9 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         }
         any_nan = with_nan[4 * grp + (j & 3)][lane % LOADERS];
     };
-    // Value fragments, read two steps ahead; a tile's first two before its M phase.
-    u32x4 vf[3][SHARED ? 2 : 1];
+    // Value fragments, read AHEAD steps ahead; a tile's first ones before its M phase.
+    constexpr int AHEAD = SHARED && !SPLIT ? 3 : 2;
+    u32x4 vf[AHEAD + 1][SHARED ? 2 : 1];
     // A tile's values as this lane reads them: half tile e, made here so that the addresses
     // are not held over the loop for every slot of the ring.
     auto v_base = [&](int j, const uint8_t* (&vs)[2]) {
@@ -961,8 +980,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     const int other = (l32 & 1) ? -16 : 16;  // from a fragment's first chunk to its second
     auto load_v = [&](const uint8_t* const (&vs)[2], int st) {
         const uint8_t* p = vs[st / KK] + 32 * (st % KK) * (SHARED ? 128 : 64);
-        vf[st % 3][0] = *reinterpret_cast<const u32x4*>(p);
-        if constexpr (SHARED) vf[st % 3][1] = *reinterpret_cast<const u32x4*>(p + other);
+        vf[st % (AHEAD + 1)][0] = *reinterpret_cast<const u32x4*>(p);
+        if constexpr (SHARED) vf[st % (AHEAD + 1)][1] = *reinterpret_cast<const u32x4*>(p + other);
     };
     auto put_values = [&](int j, int x, const u32x4& w) {  // this lane's chunk of codes into sh.values
         const int d = 16 * (wr + LOADERS * x) + lane / 4, c = 2 * swz(1, d, lane & 3);
@@ -1076,7 +1095,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         for (int st = 0; st < ST + 2; ++st) {
             if (st < ST) load_k(st);
             if constexpr (DP) {
-                if (st + 2 < ST) load_v(vs, st + 2);
+                if (st + AHEAD < ST) load_v(vs, st + AHEAD);
                 if (st == ST / 2) read_part(jp + 2);
             }
             if (st == ST / 2 + 1) take_scales(js);
@@ -1086,8 +1105,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                     if (st < ST) {
                         const int e = st / KK, k = st % KK;
                         u32x4 v0;
-                        if constexpr (SHARED) v0 = vf[st % 3][u];
-                        else v0 = fp8x8_to_half8(vf[st % 3][0][2 * u], vf[st % 3][0][2 * u + 1], bf16_t{});
+                        if constexpr (SHARED) v0 = vf[st % (AHEAD + 1)][u];
+                        else v0 = fp8x8_to_half8(vf[st % (AHEAD + 1)][0][2 * u], vf[st % (AHEAD + 1)][0][2 * u + 1], bf16_t{});
                         o[k] = mfma32x32x16(v0, hi[2 * e + u], o[k], bf16_t{});
                         if constexpr (SPLIT) o[k] = mfma32x32x16(v0, lo[2 * e + u], o[k], bf16_t{});
                     }
@@ -1267,8 +1286,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         v_phase(j);
         const uint8_t* vs[2];
         v_base(j, vs);
-        load_v(vs, 0);
-        load_v(vs, 1);
+#pragma unroll
+        for (int st = 0; st < AHEAD; ++st) load_v(vs, st);
     };
     if (n > 0) {
         wait_vmem_le<2 * DMA>();  // tiles 0 and 1
