@@ -703,7 +703,6 @@ __global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel
 constexpr int chunk_rows(int groups) { return 256 / groups; }
 constexpr int kChunkRing = 4;
 constexpr int kChunkThreads = 512;
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 __device__ inline f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x16& c, bf16_t) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
@@ -853,96 +852,25 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         for (int x = 0; x < 2 * DMA; ++x) issue_one(x, load_id(x, p.id, j), j, in);
     };
 
-    // bf16: q = r (h + l / 16) with r a power of two for the row and h and l e4m3: 4 + 4
-    // of its 8 bits, exact down to 2^-14 of the row's largest element, below
-    // that to 2^-23 of it. The scores are then products of codes as they are, at twice
-    // the rate, and K needs no conversion. f16 has 11 bits: K is converted.
-    constexpr int K8 = D / 64;  // 64-channel steps of the code product
-    u32x4 q[SPLIT ? 2 * KK : 1];
-    i32x8 q8[SPLIT ? 1 : K8][2];
-    float q_scale = 1.f;
     // What the first products wait for, in this order: the blocks' ids and Q together, then
-    // the scales and the tiles, and Q's codes while the tiles come.
-    u32x4 w[SPLIT ? 1 : K8][4];
+    // the scales and the tiles.
+    u32x4 q[2 * KK];
     Pages pg, nx;  // of the tile whose softmax is next; of the tiles 16 on
     pg.id = page_ids(0);
     {
         const int i = live ? row / a.G : 0, qh = live ? row % a.G : 0;
         const uint16_t* src = a.q + (int64_t)(r.first + i) * a.q_stride + (int64_t)(h * a.G + qh) * D;
-        if constexpr (SPLIT) {
 #pragma unroll
-            for (int k = 0; k < KK; ++k)
+        for (int k = 0; k < KK; ++k)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) q[2 * k + u] = *reinterpret_cast<const u32x4*>(src + 32 * k + 16 * hh + 8 * u);
+            for (int u = 0; u < 2; ++u) q[2 * k + u] = *reinterpret_cast<const u32x4*>(src + 32 * k + 16 * hh + 8 * u);
 #pragma unroll
-            for (int k = 0; k < 2 * KK; ++k) asm volatile("" : "+v"(q[k]));
-        } else {
-#pragma unroll
-            for (int k = 0; k < K8; ++k)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) w[k][x] = *reinterpret_cast<const u32x4*>(src + 64 * k + 32 * hh + 8 * x);
-#pragma unroll
-            for (int k = 0; k < K8; ++k)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) asm volatile("" : "+v"(w[k][x]));
-        }
+        for (int k = 0; k < 2 * KK; ++k) asm volatile("" : "+v"(q[k]));
     }
     page_scales(pg);
     nx = pg;
     if (n > 0)
         for (int j = 0; j < 3; ++j) issue(pg, min(j, n - 1), j);
-    if constexpr (!SPLIT) {
-        // The largest of the row, of the bits of |q|: bf16 in halves, 7f80 and more not finite.
-        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-        u16x2 top{0, 0};
-#pragma unroll
-        for (int k = 0; k < K8; ++k)
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[k][x / 4][x % 4] & 0x7fff7fffu));
-        uint32_t most = max((uint32_t)top[0], (uint32_t)top[1]);
-        const bool finite = __all(most < 0x7f80u);
-        if (!finite) {
-            most = 0;
-#pragma unroll
-            for (int k = 0; k < K8; ++k)
-#pragma unroll
-                for (int x = 0; x < 32; ++x) {
-                    const uint32_t e = w[k][x / 8][x % 8 / 2] >> (16 * (x & 1)) & 0x7fffu;
-                    most = e < 0x7f80u ? max(most, e) : most;
-                }
-        }
-        most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-        q_scale = e4m3_scale(__uint_as_float(most << 16));
-        const float inv = 1.0f / q_scale;
-        auto code = [&](auto check) {
-#pragma unroll
-            for (int k = 0; k < K8; ++k)
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {  // four channels
-                    float v[4], rest[4];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float e = half_at<T>(w[k][x / 2], 4 * (x & 1) + y);
-                        v[y] = e * inv;
-                        if constexpr (decltype(check)::value) v[y] = fabsf(e) <= 3.402823466e38f ? v[y] : __builtin_nanf("");
-                    }
-                    const int hi8 = (int)pack_e4m3(v[0], v[1], v[2], v[3]);
-                    const auto h01 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi8, 16.f, false);
-                    const auto h23 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi8, 16.f, true);
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) rest[y] = fmaf(v[y], 16.f, -(y < 2 ? h01[y] : h23[y - 2]));
-                    q8[k][0][x] = hi8;
-                    q8[k][1][x] = (int)pack_e4m3(rest[0], rest[1], rest[2], rest[3]);
-                }
-        };
-        if (finite) code(std::false_type{});
-        else code(std::true_type{});
-        // here, while the tiles come, and not behind the barrier that waits for them
-#pragma unroll
-        for (int k = 0; k < K8; ++k) asm volatile("" : "+v"(q8[k][0]), "+v"(q8[k][1]));
-    }
-
     f32x16 o[DT], s[2];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -1070,18 +998,9 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         const uint8_t* ks = ring + so_k;
         // K fragments are read two steps before their products, which are two steps behind
         // V's: a read takes longer than a step.
-        u32x4 kf[SPLIT ? 3 : 2][SPLIT ? 1 : 2];
+        u32x4 kf[3];
         auto load_k = [&](int st) {
-            if constexpr (SPLIT) {
-                kf[st % 3][0] = *reinterpret_cast<const u32x4*>(ks + (32 * (st / KK) + l32) * D +
-                                                                16 * swz(D == 64, l32, 2 * (st % KK) + hh));
-            } else if (st % 2 == 0) {
-                const int e = st / 2 / K8, k = st / 2 % K8;
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-                    kf[st / 2 % 2][y] = *reinterpret_cast<const u32x4*>(ks + (32 * e + l32) * D +
-                                                                        16 * swz(D == 64, l32, 4 * k + 2 * hh + y));
-            }
+            kf[st % 3] = *reinterpret_cast<const u32x4*>(ks + (32 * (st / KK) + l32) * D + 16 * swz(D == 64, l32, 2 * (st % KK) + hh));
         };
         int ids[2 * DMA];
         const uint8_t* vs[2];
@@ -1099,7 +1018,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                 if (st == ST / 2) read_part(jp + 2);
             }
             if (st == ST / 2 + 1) take_scales(js);
-            // O's two products of a step wait for each other: S goes between them.
+            // The two products of a step's O, and of its S, wait for each other: they take turns.
             auto pv = [&](int u) {
                 if constexpr (DP) {
                     if (st < ST) {
@@ -1112,28 +1031,19 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
                     }
                 }
             };
-            f32x16 zero;
+            auto qk = [&](int u) {
+                if (st < 2) return;
+                const int e = (st - 2) / KK, k = (st - 2) % KK;
+                const u32x4 kw = kf[(st - 2) % 3];
+                if (k == 0 && u == 0)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+                    for (int i = 0; i < 16; ++i) s[e][i] = 0.f;
+                s[e] = mfma32x32x16(fp8x8_to_half8(kw[2 * u], kw[2 * u + 1], T{}), q[2 * k + u], s[e], T{});
+            };
             pv(0);
-            if (st >= 2) {
-                const int ss = st - 2;
-                if constexpr (SPLIT) {
-                    const int e = ss / KK, k = ss % KK;
-                    const u32x4 kw = kf[ss % 3][0];
-                    s[e] = mfma32x32x16(fp8x8_to_half8(kw[0], kw[1], T{}), q[2 * k], k == 0 ? zero : s[e], T{});
-                    s[e] = mfma32x32x16(fp8x8_to_half8(kw[2], kw[3], T{}), q[2 * k + 1], s[e], T{});
-                } else {
-                    const int se = ss / 2 / K8, sk8 = ss / 2 % K8, piece = ss % 2;
-                    const u32x4 x = kf[ss / 2 % 2][0], y = kf[ss / 2 % 2][1];
-                    const i32x8 kw{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-                    // scales 2^0 and, for l, 2^-4 (exponent bytes 127 and 123)
-                    s[se] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                        kw, q8[sk8][piece], sk8 == 0 && piece == 0 ? zero : s[se], 0, 0, 0, 0x7f7f7f7f, 0,
-                        piece ? 0x7b7b7b7b : 0x7f7f7f7f);
-                }
-            }
+            qk(0);
             pv(1);
+            qk(1);
             if constexpr (DP) {
                 if (st == ST) bad = part_nans(jp + 2);
             }
@@ -1154,7 +1064,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         // p sv = 2^(x + log2 sv), and out of the chunk's sum once. Else p is
         // masked and multiplied.
         const bool plain = ((uint32_t)(pg.plain >> (4 * (j & 15))) & 15u) == 15u && key0 + 64 <= open;
-        const float ref = m == -INFINITY ? 0.f : m, factor = q_scale * a.scale_log2;
+        const float ref = m == -INFINITY ? 0.f : m, factor = a.scale_log2;
         float add[2], out[2], sv[2];
         int seen[2] = {16, 16};
 #pragma unroll

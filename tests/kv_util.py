@@ -124,10 +124,10 @@ def values(cache):
 # ---------------------------------------------------------------- attention
 
 
-def attention_ref(q, cache, table, lens, offsets, scale, max_q=1 << 30, out=None):
+def attention_ref(q, cache, table, lens, offsets, scale, max_q=1 << 30, out=None, only=None):
     """(o, bound, computed): float64 outputs; per output, how far a result of the
     types used may be off but for the output's own rounding; which rows of q the
-    call computes.
+    call computes. only: the tokens that are looked at (the others are not `computed`).
 
     With a_j = |v_j| and P = softmax: o = sum P v. The kernel's scores are off by
     at most ds = (D + 4) 2^-24 S (S = sum_d |q_d k_jd| scale, largest over j; fp32
@@ -154,6 +154,8 @@ def attention_ref(q, cache, table, lens, offsets, scale, max_q=1 << 30, out=None
         v = (c["v"][ids] * c["v_scale"][ids][..., None, None]).permute(1, 0, 3, 2).reshape(hk, -1, d)[:, :n_keys]
         for i in range(min(end - first, max_q)):
             t = first + i
+            if only is not None and t not in only:
+                continue
             done[t] = True
             see = max(0, min(n_keys, n_keys - (end - first) + i + 1))
             keep = there[:see]

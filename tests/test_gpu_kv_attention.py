@@ -52,11 +52,15 @@ class Call:
         torch.cuda.synchronize()
         return o.cpu()
 
-    def check(self, got, max_q=1 << 30, fill=7.0):
+    def check(self, got, max_q=1 << 30, fill=7.0, only=None):
         torch = self.torch
         ref, bound, done = kv_util.attention_ref(self.q, self.cache, self.table, self.lens, self.offsets, self.scale, max_q,
-                                                 torch.full(self.q.shape, fill))
+                                                 torch.full(self.q.shape, fill), only)
         g = got.double()
+        if only is not None:  # the rows looked at
+            g, ref, bound, done = g[done], ref[done], bound[done], done[done]
+            got = got[:0]
+            done = done[:0]
         same_nan = torch.equal(torch.isnan(g), torch.isnan(ref))
         assert same_nan, "NaN in other places"
         room = bound * (1 + HALF[self.dtype]) + HALF[self.dtype] * ref.abs() + 2.0 ** -24
@@ -114,6 +118,100 @@ def test_prompt_chunks(gpu, dtype, hq, hk, d, bs):
 
 def test_long_chunk(gpu):
     Call(gpu, "bf16", 8, 2, 128, 16, [1500, 900], [700, 513], seed=3).go()
+
+
+def _some(counts, seed, many=10):
+    """Some tokens of every request: the first and last two, and others."""
+    r, some, at = np.random.default_rng(seed), set(), 0
+    for n in counts:
+        pick = [0, 1, n - 2, n - 1] + r.integers(0, n, many).tolist() if n else []
+        some |= {at + int(i) for i in pick if 0 <= i < n}
+        at += n
+    return some
+
+
+# Enough rows that a part of them is 256 (more than 256 parts of 128), tables of more
+# than 32 tiles, and requests that end inside a part.
+WIDE = [(32, 8, 16, [4700, 2300], [1500, 1023]), (24, 8, 128, [4200, 1000], [1400, 999]),
+        (64, 64, 64, [700], [600]), (40, 8, 32, [3000, 500, 2200], [900, 500, 801])]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,bs,lens,counts", WIDE)
+def test_long_prompts(gpu, dtype, hq, hk, bs, lens, counts):
+    c = Call(gpu, dtype, hq, hk, 128, bs, lens, counts, seed=20 + bs)
+    c.check(c.run(), only=_some(counts, bs))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d,bs", [(64, 16), (64, 128), (128, 16), (128, 128)])
+def test_chunks_over_long_contexts(gpu, dtype, d, bs):
+    lens, counts = [4700, 5000, 2049], [300, 260, 257]
+    c = Call(gpu, dtype, 8, 2, d, bs, lens, counts, seed=30 + d + bs)
+    c.check(c.run(), only=_some(counts, d + bs, 20))
+
+
+# (heads, kv heads, lens, counts): the split kernel's two tilings, parts of 128 and of 256 rows
+KINDS = [(4, 2, [70, 200, 130], [1, 1, 1]), (8, 2, [70, 200, 130], [3, 9, 5]), (8, 2, [700, 300], [300, 200]),
+         (32, 8, [1500, 1300], [1200, 1000])]
+
+
+@pytest.mark.parametrize("hq,hk,lens,counts", KINDS)
+def test_scales_of_any_value(gpu, hq, hk, lens, counts):
+    """Scales that are no powers of two, negative, zero, and far from one; the blocks of
+    nobody hold NaN."""
+    torch = gpu
+    c = Call(torch, "bf16", hq, hk, 128, 16, lens, counts, seed=41)
+    n = c.blocks
+    g = torch.Generator().manual_seed(5)
+    for name in ("k_scale", "v_scale"):
+        c.cache[name] *= 0.5 + torch.rand((n, hk), generator=g)
+    at = c.table.flatten()
+    at = at[at >= 0].long()
+    c.cache["v_scale"][at[1::7]] = 0.0
+    c.cache["v_scale"][at[2::7]] *= -1.0
+    c.cache["v_scale"][at[3::7]] *= 2.0 ** -90
+    c.cache["k_scale"][at[4::7]] *= -1.0
+    c.cache["k_scale"][at[5::7]] = 0.0
+    c.cache["v_scale"][at[6::14]] *= 2.0 ** 70
+    nobody = sorted(set(range(n)) - set(at.tolist()))
+    for i in nobody:
+        c.cache["k"][i], c.cache["v"][i] = 0x7F, 0xFF
+        c.cache["k_scale"][i], c.cache["v_scale"][i] = float("nan"), float("-inf")
+    c.check(c.run(), only=_some(counts, 3))
+
+
+@pytest.mark.parametrize("hq,hk,lens,counts", KINDS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_queries_of_any_value(gpu, dtype, hq, hk, lens, counts):
+    """Rows of q with one large element, of zeros, of tiny ones, with NaN and infinities."""
+    torch = gpu
+    c = Call(torch, dtype, hq, hk, 128, 16, lens, counts, seed=42, gain=0.25)
+    n = c.q.shape[0]
+    row = lambda i: i * (n - 1) // 6
+    c.q[row(0), :, 17] = 300.0
+    c.q[row(1), 0] = 0.0
+    c.q[row(2), 1] *= 2.0 ** -13
+    if n > 6:
+        c.q[row(3), hq - 1, 5] = float("nan")
+        c.q[row(4), 0, 99] = float("inf")
+        c.q[row(5), 1, 3] = float("-inf")
+    ref = c.check(c.run(), only={row(i) for i in range(7)} | _some(counts, 4))
+    assert n <= 6 or int(torch.isnan(ref).sum()) >= 128
+
+
+@pytest.mark.parametrize("hq,hk,lens,counts", KINDS[1:])
+def test_nan_values_in_any_tile(gpu, hq, hk, lens, counts):
+    """NaN codes among the values all over the keys: only the rows that see them, only
+    their channels."""
+    torch = gpu
+    c = Call(torch, "bf16", hq, hk, 128, 16, lens, counts, seed=43)
+    for b in range(len(lens)):
+        for i, key in enumerate(range(lens[b] - counts[b] + 1, lens[b], 67)):
+            c.cache["v"][c.table[b, key // 16], i % hk, (37 * i) % 128, key % 16] = 0x7F if i & 1 else 0xFF
+    ref = c.check(c.run(), only=_some(counts, 5, 20))
+    nan = torch.isnan(ref)
+    assert bool(nan.any()) and not bool(nan.all())
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
