@@ -722,9 +722,13 @@ constexpr float kChunkSumMax = 16384.0f;
 
 template <int D, int GROUPS> struct ChunkShare {
     static constexpr int TILE = 64 * D;
-    __attribute__((aligned(1024))) uint8_t ring[GROUPS * kChunkRing * 2 * TILE];
-    // One group: the values as bf16, converted once by the wave that loaded them. Channel
-    // rows of 64 keys, 16-byte chunks at c ^ row % 8. Two groups have no room for this.
+    // One group: the codes go on as 16-bit numbers, converted once by the wave that loaded
+    // them, into `keys` (rows of D) and `values` (channel rows of 64 keys), 16-byte
+    // chunks at c ^ row % 8; two tiles of codes are enough then, a wave reads only its
+    // own. Two groups have no room for this: every wave converts what it multiplies.
+    static constexpr int RING = GROUPS == 1 ? 2 : kChunkRing;
+    __attribute__((aligned(1024))) uint8_t ring[GROUPS * RING * 2 * TILE];
+    __attribute__((aligned(1024))) uint16_t keys[GROUPS == 1 ? 2 * TILE : 1];
     __attribute__((aligned(1024))) uint16_t values[GROUPS == 1 ? kChunkRing * TILE : 1];
     // Which codes of a value tile are NaN, a bit each, where a wave's part of it (with_nan)
     // has any; [group][tile % 4]. In the ring these are 0: the product then says
@@ -744,7 +748,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     constexpr int TILE = 64 * D;          // bytes of one operand of a tile
     constexpr int DMA = TILE / (LOADERS * 1024);  // wave loads of an operand for each of them
     static_assert(DMA > 0, "each loads of both operands");
-    constexpr bool SHARED = GROUPS == 1;  // converted values in LDS
+    constexpr bool SHARED = GROUPS == 1;  // converted codes in LDS
+    constexpr int RING = ChunkShare<D, GROUPS>::RING;
     constexpr bool SPLIT = __is_same(T, f16_t);
     auto& ring = sh.ring;
     auto& nans = sh.nans;
@@ -816,7 +821,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     };
     // every row of the wave sees all keys below this
     const int open = w0 < r.rows ? min(r.len - r.n + w0 / a.G + 1, r.len) : r.len;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)&ring[0] + (uint32_t)(grp * kChunkRing * 2 * TILE);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)&ring[0] + (uint32_t)(grp * RING * 2 * TILE);
     // LDS row m of a half tile holds key 16 (m / 4 % 2) + 4 (m / 8) + m % 4 of it; rows
     // are swizzled by 16-byte chunks so that 16 lanes reading one chunk of 16 rows
     // touch every bank once (rows of 128 bytes: c ^ m / 2 % 8, of 64: c ^ m / 4 % 4).
@@ -842,7 +847,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     auto load_id = [&](int x, int ids, int j) { return __builtin_amdgcn_ds_bpermute(from[x] + 16 * (j & 15), ids); };
     const uint32_t odd = GROUPS == 1 && bs > 64 ? 64 : 0;  // keys
     auto issue_one = [&](int x, int id, int j, int in) {  // of tile j, from block id into tile in's slot
-        const uint32_t slot = lds0 + (uint32_t)((in % kChunkRing) * 2 * TILE + 1024 * (wr + LOADERS * (x % DMA)));
+        const uint32_t slot = lds0 + (uint32_t)((in % RING) * 2 * TILE + 1024 * (wr + LOADERS * (x % DMA)));
         const uint64_t src = at[x] + (uint64_t)(uint32_t)max(id, 0) * (x < DMA ? k_stride : v_stride) +
                              (j & 1 ? (x < DMA ? odd * D : odd) : 0u);
         lds_dma_b128((const void*)(uintptr_t)src, x < DMA ? slot : slot + TILE);
@@ -870,7 +875,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     page_scales(pg);
     nx = pg;
     if (n > 0)
-        for (int j = 0; j < 3; ++j) issue(pg, min(j, n - 1), j);
+        for (int j = 0; j < min(RING, 3); ++j) issue(pg, min(j, n - 1), j);
     f32x16 o[DT], s[2];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -898,7 +903,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     // A tile's values as this lane reads them: half tile e, made here so that the addresses
     // are not held over the loop for every slot of the ring.
     auto v_base = [&](int j, const uint8_t* (&vs)[2]) {
-        uint32_t so = (uint32_t)(SHARED ? j % kChunkRing * 2 * TILE : (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE);
+        uint32_t so = (uint32_t)(SHARED ? j % kChunkRing * 2 * TILE : (grp * RING + j % RING) * 2 * TILE + TILE);
         asm volatile("" : "+s"(so));
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -919,19 +924,33 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             *reinterpret_cast<u32x4*>(row + 8 * ((c + u) ^ (d & 7))) = fp8x8_to_half8(w[2 * u], w[2 * u + 1], bf16_t{});
     };
 
+    auto put_keys = [&](int j, int x, const u32x4& w) {  // into sh.keys
+        const int m = (wr + LOADERS * x) * (1024 / D) + lane / KC, c = 2 * swz(D == 64, m, lane % KC);
+        uint16_t* row = sh.keys + j % 2 * TILE + D * m;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<u32x4*>(row + 8 * ((c + u) ^ (m & 7))) = fp8x8_to_half8(w[2 * u], w[2 * u + 1], T{});
+    };
+
     // This wave's part of tile j's values, which has landed: NaN codes out of it. (The
     // tile's softmax is behind the next barrier.)
-    u32x4 part[DMA];
+    u32x4 part[DMA], key_part[SHARED ? DMA : 1];
     auto read_part = [&](int j) {
-        const uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
+        const uint8_t* mine = ring + (grp * RING + j % RING) * 2 * TILE + TILE + 16 * lane;
 #pragma unroll
-        for (int x = 0; x < DMA; ++x) part[x] = *reinterpret_cast<const u32x4*>(mine + 1024 * (wr + LOADERS * x));
+        for (int x = 0; x < DMA; ++x) {
+            part[x] = *reinterpret_cast<const u32x4*>(mine + 1024 * (wr + LOADERS * x));
+            if constexpr (SHARED) key_part[x] = *reinterpret_cast<const u32x4*>(mine - TILE + 1024 * (wr + LOADERS * x));
+        }
     };
     auto part_nans = [&](int j) {
         uint32_t bad = 0;
 #pragma unroll
         for (int x = 0; x < DMA; ++x) {
-            if constexpr (SHARED) put_values(j, x, part[x]);  // and again should one be NaN
+            if constexpr (SHARED) {
+                put_keys(j, x, key_part[x]);
+                put_values(j, x, part[x]);  // and again should one be NaN
+            }
 #pragma unroll
             for (int y = 0; y < 4; ++y) bad |= (part[x][y] & 0x7f7f7f7fu) + 0x01010101u;
         }
@@ -941,7 +960,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         const bool any = __any(bad != 0);
         if (lane == 0) with_nan[4 * grp + (j & 3)][wr] = any;
         if (!any) return;
-        uint8_t* mine = ring + (grp * kChunkRing + j % kChunkRing) * 2 * TILE + TILE + 16 * lane;
+        uint8_t* mine = ring + (grp * RING + j % RING) * 2 * TILE + TILE + 16 * lane;
 #pragma unroll
         for (int x = 0; x < DMA; ++x) {
             u32x4 w = part[x];
@@ -993,14 +1012,20 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         const int js = jp + 1;
         constexpr bool DP = decltype(dp_tag)::value;
         constexpr int ST = 2 * KK;
-        uint32_t so_k = (uint32_t)((grp * kChunkRing + js % kChunkRing) * 2 * TILE);
+        uint32_t so_k = (uint32_t)(SHARED ? js % 2 * 2 * TILE : (grp * RING + js % RING) * 2 * TILE);
         asm volatile("" : "+s"(so_k));
-        const uint8_t* ks = ring + so_k;
         // K fragments are read two steps before their products, which are two steps behind
         // V's: a read takes longer than a step.
-        u32x4 kf[3];
+        u32x4 kf[3][SHARED ? 2 : 1];
         auto load_k = [&](int st) {
-            kf[st % 3] = *reinterpret_cast<const u32x4*>(ks + (32 * (st / KK) + l32) * D + 16 * swz(D == 64, l32, 2 * (st % KK) + hh));
+            const int row = 32 * (st / KK) + l32, c = 2 * (st % KK) + hh;
+            if constexpr (SHARED) {
+                const uint8_t* p = (const uint8_t*)sh.keys + so_k + row * (2 * D) + 16 * ((2 * c) ^ (l32 & 7));
+                kf[st % 3][0] = *reinterpret_cast<const u32x4*>(p);
+                kf[st % 3][1] = *reinterpret_cast<const u32x4*>(p + other);
+            } else {
+                kf[st % 3][0] = *reinterpret_cast<const u32x4*>(ring + so_k + row * D + 16 * swz(D == 64, l32, c));
+            }
         };
         int ids[2 * DMA];
         const uint8_t* vs[2];
@@ -1034,11 +1059,13 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
             auto qk = [&](int u) {
                 if (st < 2) return;
                 const int e = (st - 2) / KK, k = (st - 2) % KK;
-                const u32x4 kw = kf[(st - 2) % 3];
+                u32x4 k0;
+                if constexpr (SHARED) k0 = kf[(st - 2) % 3][u];
+                else k0 = fp8x8_to_half8(kf[(st - 2) % 3][0][2 * u], kf[(st - 2) % 3][0][2 * u + 1], T{});
                 if (k == 0 && u == 0)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[e][i] = 0.f;
-                s[e] = mfma32x32x16(fp8x8_to_half8(kw[2 * u], kw[2 * u + 1], T{}), q[2 * k + u], s[e], T{});
+                s[e] = mfma32x32x16(k0, q[2 * k + u], s[e], T{});
             };
             pv(0);
             qk(0);
@@ -1200,14 +1227,19 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         for (int st = 0; st < AHEAD; ++st) load_v(vs, st);
     };
     if (n > 0) {
-        wait_vmem_le<2 * DMA>();  // tiles 0 and 1
+        wait_vmem_le<2 * DMA>();  // tile 0, of three also tile 1
         page_derive(pg);
         read_part(0);
         check_part(0, part_nans(0));
+        if constexpr (RING == 2) {  // tile 0's codes are read: its slot is tile 2's
+            issue(pg, min(2, n - 1), 2);
+            wait_vmem_le<2 * DMA>();
+        }
         read_part(1);
         check_part(1, part_nans(1));
         __syncthreads();
         m_phase(std::false_type{}, -1, 0, 0);
+        if constexpr (SHARED) __syncthreads();  // the next M phase overwrites tile 0's keys
         // A barrier a tile: a SIMD's first wave passes it before, its second behind a product, so they
         // stay half a tile apart and are free between. Behind it the tile that both
         // waited for and checked is there, and the slot of the tile before is free.
