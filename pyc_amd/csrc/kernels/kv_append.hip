@@ -18,6 +18,12 @@
 // codes. Keys go out as they came, 8 codes a lane; values are transposed in
 // LDS, so that a channel's 16 tokens leave as one 16-byte store, merged with the
 // codes that are there when the chunk is not all new.
+// HBM bounds it for prompts: 16000 tokens of 8 heads of 128 in bf16 take 25 us, 4.0 TB/s
+// of rows read once and codes written once (a copy reaches 5.1). Few tokens are
+// latency: 32 of them, 32 blocks, 4.6 us on the device, of which loads that wait
+// for each other (slots, scales, codes) are the most. A wave to a chunk, its rows held from
+// one read: a workgroup to a block and head, which read them twice, took 241 us for the
+// prompts (and 3.8 for the 32 tokens).
 #include "kv_cache.hpp"
 
 namespace pyc {

@@ -4,8 +4,11 @@
 // token i of the n that a request of `len` tokens brings sees keys j <= len - n + i;
 // head h reads kv head h / G, G = q heads / kv heads. Without a key: zero.
 //
-// One wave works on 16 rows (row r of a request and kv head: token r / G, head
-// r % G) and 64 keys at a time, on v_mfma_f32_16x16x32:
+// Rows are (token, head of the group): row r of a request and kv head is token r / G, head
+// r % G. Two kernels: the split kernel for requests of few rows, bound by reading the
+// cache, and the chunk kernels for many, bound by matrix and softmax work; a batch that
+// has both goes out in one launch. In the split kernel a wave works on 16 NT rows and 64
+// keys at a time, on v_mfma_f32_16x16x32:
 //   S^T = K Q^T: K's codes become 16-bit (exact) in registers, Q stays there.
 //   Which key a row of the A operand is, is free: row 4g' + i of product t is
 //   key 16 g' + 4 t + i, so that lane group g (lanes 16g .. 16g + 15) ends with
@@ -14,7 +17,10 @@
 //   O^T = V^T P^T: lane group g takes the 16 tokens of its chunk for one channel
 //   from the transposed values with one 16-byte load.
 // A block's value scale goes into P (p * sv), the sum of p stays without it.
-// Statistics and sums are fp32. P is rounded to 16 bits for the product: for bf16
+// Statistics and sums are fp32. (8-bit matrix products of codes, q as two of them, would
+// run at twice the rate for half the work, but add their 64 products with fewer
+// bits: scores near 170 came out off by 0.01. So both operands are 16-bit.) P is
+// rounded to 16 bits for the product: for bf16
 // output once (2^-8 of each p, below the output's own rounding once averaged);
 // for f16 output P is split into two bf16 parts (2^-16 left), as bf16 holds any
 // block's scale and f16 does not.
@@ -377,6 +383,14 @@ template <typename T, int D, int NT> struct AttnWave {
 // all of it; the workgroup joins what its waves have of one run, and where a run goes
 // on in other workgroups, the last of these to be done joins all. Up to 256 short runs
 // get a workgroup each instead: then no run crosses one.
+// Even pieces against one workgroup for a request and head: no CU waits for the longest
+// context, and two requests of 100000 keys use the card as 64 of 3000 do. Measured, 32
+// heads of 128 in bf16: 2 contexts of 100000 to 131072 keys, 8 kv heads, 83.5 us (5.2
+// TB/s, what a copy reaches); 64 of 300 to 6000, 32 kv heads, 216 us (5.4 TB/s); 32 of
+// 200 to 4096, 8 kv heads, 27 us (3.8 TB/s: what it takes to start, to find the work and to
+// join is 7 of them); one of 777, 10.3 us, which is latency: 0.8 for lengths and
+// their sums, 0.7 to find the piece, 2.7 for the tile's ids, scales and codes one after
+// the other, 1.2 for the join in LDS, 1 for the counter, and the launch.
 struct AttnSplit {
     int most_rows;
     float* part;     // two results of every workgroup: [16 NT][D] sums, [16 NT][2] maximum and sum
@@ -691,15 +705,25 @@ __global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel
 }
 
 // ---------------------------------------------------------------------------
-// Requests of many rows (prompt chunks): matrix work. A workgroup has 128 rows of a
-// request and kv head; its 8 waves are 4 times 32 rows and two groups that take the
-// tiles of 64 keys in turn and join at the end. On v_mfma_f32_32x32x16, as above:
-// S^T = K Q^T with the keys of a tile ordered so that a lane ends with 16 keys of one
-// chunk of each half tile, O^T += V^T P^T with P as it is. A group's tiles come by
-// LDS-DMA, as codes, into a ring of three. The two groups are one phase apart: while a
-// wave of one runs matrix instructions (phase M: the scores of its next tile and the
-// products of this one, and the conversion of both operands' codes), the wave of the
-// other that shares its SIMD runs its softmax (phase V).
+// Requests of many rows (prompt chunks): matrix work. A workgroup's 8 waves have 32 rows
+// each. On v_mfma_f32_32x32x16, as above: S^T = K Q^T with the keys of a tile of 64 ordered
+// so that a lane ends with 16 keys of one chunk of each half tile, O^T += V^T P^T with P as
+// it is. Tiles come by LDS-DMA, as codes, into a ring. A SIMD's two waves are one phase
+// apart: while one runs matrix instructions (phase M: the products of this tile and
+// the scores of the next), the other runs its softmax (phase V).
+// GROUPS 2: 128 rows, 4 waves for them, twice; the two groups take tiles in turn and join at
+// the end. GROUPS 1: 256 rows, all waves on the same tiles. A part costs 14 us that are
+// not its tiles (start, first loads, join), so 256 rows are better once 128 no longer
+// fit the card in one round (more than 256 parts), and worse before: over 4096 keys, 4
+// chunks of 256 tokens of 32 heads, 8 kv heads, take 90 us in parts of 128 rows and 126 in
+// parts of 256, 4 of 1024 tokens 283 and 243. With one group LDS has room for the tiles converted to 16
+// bits, once for the workgroup instead of once for each wave.
+// Measured, 32 heads of 128, 8 kv heads, bf16: 4 chunks of 2048 tokens over 3500 to 4100 keys
+// 370 us, 975 TFLOP/s (1.14 PFLOP/s over 16384 keys; a large library product reaches
+// 1.44). Of a tile's 4000 cycles the matrix unit is busy for 2048: phase M takes 1850
+// (its 34 16-byte reads a lane, for four waves, are 1100 cycles of LDS beside 1024 of
+// products), phase V 1700 (32 exponentials, 32 scalings, 32 additions, 16 roundings:
+// between the other wave's products a vector instruction issues about every 7 cycles).
 constexpr int chunk_rows(int groups) { return 256 / groups; }
 constexpr int kChunkRing = 4;
 constexpr int kChunkThreads = 512;
@@ -723,9 +747,9 @@ constexpr float kChunkSumMax = 16384.0f;
 template <int D, int GROUPS> struct ChunkShare {
     static constexpr int TILE = 64 * D;
     // One group: the codes go on as 16-bit numbers, converted once by the wave that loaded
-    // them, into `keys` (rows of D) and `values` (channel rows of 64 keys), 16-byte
-    // chunks at c ^ row % 8; two tiles of codes are enough then, a wave reads only its
-    // own. Two groups have no room for this: every wave converts what it multiplies.
+    // them, into `keys` (rows of D, 16-byte chunks at c ^ row % 16) and `values` (channel rows
+    // of 64 keys, chunks at c ^ row / 2 % 8: 16 lanes that read one chunk of 16 rows touch
+    // all 64 banks once); two tiles of codes are enough then, a wave reads only its own. Two groups have no room for this: every wave converts what it multiplies.
     static constexpr int RING = GROUPS == 1 ? 2 : kChunkRing;
     __attribute__((aligned(1024))) uint8_t ring[GROUPS * RING * 2 * TILE];
     __attribute__((aligned(1024))) uint16_t keys[GROUPS == 1 ? 2 * TILE : 1];
@@ -747,6 +771,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     constexpr int DT = D / 32;            // 32-channel tiles of O^T
     constexpr int TILE = 64 * D;          // bytes of one operand of a tile
     constexpr int DMA = TILE / (LOADERS * 1024);  // wave loads of an operand for each of them
+    static_assert(GROUPS == 2 || D == 128, "rows of 16 chunks");
     static_assert(DMA > 0, "each loads of both operands");
     constexpr bool SHARED = GROUPS == 1;  // converted codes in LDS
     constexpr int RING = ChunkShare<D, GROUPS>::RING;
@@ -907,21 +932,22 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         asm volatile("" : "+s"(so));
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-            if constexpr (SHARED) vs[e] = (const uint8_t*)sh.values + so + l32 * 128 + 16 * ((4 * e + 2 * hh) ^ (l32 & 7));
+            if constexpr (SHARED) vs[e] = (const uint8_t*)sh.values + so + l32 * 128 + 16 * ((4 * e + 2 * hh) ^ ((l32 >> 1) & 7));
             else vs[e] = ring + so + l32 * 64 + 16 * swz(1, l32, 2 * e + hh);
     };
-    const int other = (l32 & 1) ? -16 : 16;  // from a fragment's first chunk to its second
+    // from a fragment's first chunk to its second
+    const int other_v = (l32 & 2) ? -16 : 16, other_k = (l32 & 1) ? -16 : 16;
     auto load_v = [&](const uint8_t* const (&vs)[2], int st) {
         const uint8_t* p = vs[st / KK] + 32 * (st % KK) * (SHARED ? 128 : 64);
         vf[st % (AHEAD + 1)][0] = *reinterpret_cast<const u32x4*>(p);
-        if constexpr (SHARED) vf[st % (AHEAD + 1)][1] = *reinterpret_cast<const u32x4*>(p + other);
+        if constexpr (SHARED) vf[st % (AHEAD + 1)][1] = *reinterpret_cast<const u32x4*>(p + other_v);
     };
     auto put_values = [&](int j, int x, const u32x4& w) {  // this lane's chunk of codes into sh.values
         const int d = 16 * (wr + LOADERS * x) + lane / 4, c = 2 * swz(1, d, lane & 3);
         uint16_t* row = sh.values + j % kChunkRing * TILE + 64 * d;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-            *reinterpret_cast<u32x4*>(row + 8 * ((c + u) ^ (d & 7))) = fp8x8_to_half8(w[2 * u], w[2 * u + 1], bf16_t{});
+            *reinterpret_cast<u32x4*>(row + 8 * ((c + u) ^ ((d >> 1) & 7))) = fp8x8_to_half8(w[2 * u], w[2 * u + 1], bf16_t{});
     };
 
     auto put_keys = [&](int j, int x, const u32x4& w) {  // into sh.keys
@@ -929,7 +955,7 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         uint16_t* row = sh.keys + j % 2 * TILE + D * m;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-            *reinterpret_cast<u32x4*>(row + 8 * ((c + u) ^ (m & 7))) = fp8x8_to_half8(w[2 * u], w[2 * u + 1], T{});
+            *reinterpret_cast<u32x4*>(row + 8 * ((c + u) ^ (m & 15))) = fp8x8_to_half8(w[2 * u], w[2 * u + 1], T{});
     };
 
     // This wave's part of tile j's values, which has landed: NaN codes out of it. (The
@@ -1020,9 +1046,9 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         auto load_k = [&](int st) {
             const int row = 32 * (st / KK) + l32, c = 2 * (st % KK) + hh;
             if constexpr (SHARED) {
-                const uint8_t* p = (const uint8_t*)sh.keys + so_k + row * (2 * D) + 16 * ((2 * c) ^ (l32 & 7));
+                const uint8_t* p = (const uint8_t*)sh.keys + so_k + row * (2 * D) + 16 * ((2 * c) ^ (l32 & 15));
                 kf[st % 3][0] = *reinterpret_cast<const u32x4*>(p);
-                kf[st % 3][1] = *reinterpret_cast<const u32x4*>(p + other);
+                kf[st % 3][1] = *reinterpret_cast<const u32x4*>(p + other_k);
             } else {
                 kf[st % 3][0] = *reinterpret_cast<const u32x4*>(ring + so_k + row * D + 16 * swz(D == 64, l32, c));
             }
