@@ -713,10 +713,8 @@ __global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel
 // the scores of the next), the other runs its softmax (phase V).
 // GROUPS 2: 128 rows, 4 waves for them, twice; the two groups take tiles in turn and join at
 // the end. GROUPS 1: 256 rows, all waves on the same tiles. A part costs 14 us that are
-// not its tiles (start, first loads, join), so 256 rows are better once 128 no longer
-// fit the card in one round (more than 256 parts), and worse before: over 4096 keys, 4
-// chunks of 256 tokens of 32 heads, 8 kv heads, take 90 us in parts of 128 rows and 126 in
-// parts of 256, 4 of 1024 tokens 283 and 243. With one group LDS has room for the tiles converted to 16
+// not its tiles (start, first loads, join), so 256 rows are better where they save rounds of
+// workgroups, and worse where the card is not full (figures at the launch). With one group LDS has room for the tiles converted to 16
 // bits, once for the workgroup instead of once for each wave.
 // Measured, 32 heads of 128, 8 kv heads, bf16: 4 chunks of 2048 tokens over 3500 to 4100 keys
 // 370 us, 975 TFLOP/s (1.14 PFLOP/s over 16384 keys; a large library product reaches
@@ -1397,8 +1395,16 @@ template <typename T, int D> static void launch_attention(const AttnArgs& a, int
     // Parts: whole ones, and one more for each request that is large enough.
     const long all = (long)a.tokens * a.G, some = all / (sp.most_rows + 1);
     auto parts_of = [&](int groups) { return (all / chunk_rows(groups) + (some < a.B ? some : a.B)) * a.c.heads; };
+    // Rounds of workgroups if every request has max_q tokens. A round of 256 rows takes 1.6 to
+    // 1.85 times as long as one of 128. Measured (us, 128 rows against 256, 4 chunks over 4096 keys,
+    // 32 heads of 128, 8 kv heads): 256 tokens 90 / 130 (1 round / 1), 320 150 / 131 (2 / 1),
+    // 512 172 / 148 (2 / 1), 768 228 / 241 (3 / 2), 1024 290 / 267 (4 / 2).
+    auto rounds = [&](int groups) {
+        const long tiles = ((long)a.max_q * a.G + chunk_rows(groups) - 1) / chunk_rows(groups);
+        return (tiles * a.B * a.c.heads + kSplitGroups - 1) / kSplitGroups;
+    };
     if constexpr (D == 128)
-        if (chunks_only && parts_of(2) > kSplitGroups) {
+        if (chunks_only && 7 * rounds(1) <= 4 * rounds(2)) {
             hipLaunchKernelGGL((kv_chunks_kernel<T, D>), dim3((unsigned)parts_of(1)), dim3(kChunkThreads), 0, s, a);
             return;
         }

@@ -130,10 +130,10 @@ def _some(counts, seed, many=10):
     return some
 
 
-# Enough rows that a part of them is 256 (more than 256 parts of 128), tables of more
-# than 32 tiles, and requests that end inside a part.
-WIDE = [(32, 8, 16, [4700, 2300], [1500, 1023]), (24, 8, 128, [4200, 1000], [1400, 999]),
-        (64, 64, 64, [700], [600]), (40, 8, 32, [3000, 500, 2200], [900, 500, 801])]
+# Enough rows that a part of them is 256 (parts of 128 would take two rounds of 256
+# workgroups, these one), tables of more than 32 tiles, and requests that end inside a part.
+WIDE = [(32, 8, 16, [4700, 2300], [1024, 1003]), (24, 8, 128, [4200, 1000], [1300, 999]),
+        (64, 64, 64, [700], [600]), (40, 8, 32, [3000, 500, 2200], [500, 400, 470])]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -153,7 +153,7 @@ def test_chunks_over_long_contexts(gpu, dtype, d, bs):
 
 # (heads, kv heads, lens, counts): the split kernel's two tilings, parts of 128 and of 256 rows
 KINDS = [(4, 2, [70, 200, 130], [1, 1, 1]), (8, 2, [70, 200, 130], [3, 9, 5]), (8, 2, [700, 300], [300, 200]),
-         (32, 8, [1500, 1300], [1200, 1000])]
+         (32, 8, [1500, 1300], [1000, 900])]
 
 
 @pytest.mark.parametrize("hq,hk,lens,counts", KINDS)
