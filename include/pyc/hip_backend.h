@@ -262,7 +262,7 @@ int pyc_hip_kv_append_dispatch(
  * boundary, zero before its first call and left zeroed where that matters: for one
  * call at a time (calls that may overlap need one each). q_heads a multiple of
  * kv_heads; q, o on 16-byte boundaries, strides multiples of 8, o overlapping
- * nothing. 0 <= tokens < 2^24. Symbols "hip_kv_attention_bf16",
+ * nothing. 0 <= tokens < 2^24, tokens * q_heads / kv_heads < 2^31 - 255. Symbols "hip_kv_attention_bf16",
  * "hip_kv_attention_f16". 0, -1, -2 as above. */
 int pyc_hip_kv_attention_dispatch(
     const char* symbol, const pyc_hip_kv_cache* cache, int B, int tokens, int q_heads, int max_q, int max_len,

@@ -760,7 +760,7 @@ int pyc_hip_kv_attention_dispatch(const char* symbol, const pyc_hip_kv_cache* ca
     const hip_variant* var = find_variant(symbol, VK_KV_ATTN);
     size_t need;
     if (!var || !kv_cache_ok(cache) || B < 0 || tokens < 0 || tokens >= KV_MAX_TOKENS || q_heads <= 0 ||
-        q_heads % cache->kv_heads != 0 || max_len < 0) {
+        q_heads % cache->kv_heads != 0 || (int64_t)tokens * (q_heads / cache->kv_heads) > 0x7FFFFF00LL || max_len < 0) {
         return -1;
     }
     if (B == 0 || tokens == 0) {
@@ -771,7 +771,8 @@ int pyc_hip_kv_attention_dispatch(const char* symbol, const pyc_hip_kv_cache* ca
         return -1;
     }
     if (!table || width <= 0 || table_stride < width || (int64_t)width * cache->block_size > 0x7FFFFF00LL ||
-        (double)B * cache->kv_heads * width * cache->block_size >= 0x1p56 || !lens || !q_offsets || !(scale == scale) || !kv_rows_ok(q, q_stride, q_heads, cache->head_dim) ||
+        (double)B * cache->kv_heads * width * cache->block_size >= 0x1p56 || !lens || !q_offsets ||
+        !(scale == scale) || !kv_rows_ok(q, q_stride, q_heads, cache->head_dim) ||
         !kv_rows_ok(o, o_stride, q_heads, cache->head_dim)) {
         return -1;
     }

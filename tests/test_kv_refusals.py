@@ -65,7 +65,7 @@ def test_append_without_cache():
 
 @pytest.mark.parametrize("bad", [dict(symbol=b"hip_attention_bf16"), dict(symbol=None), dict(B=-1), dict(tokens=-1),
                                  dict(tokens=1 << 24), dict(hq=3), dict(hq=0), dict(max_q=0), dict(max_q=1 << 24),
-                                 dict(max_len=-1), dict(q=None), dict(q=P + 2), dict(qs=255), dict(qs=248),
+                                 dict(tokens=(1 << 24) - 1, hq=512, qs=1 << 15, os=1 << 15), dict(max_len=-1), dict(q=None), dict(q=P + 2), dict(qs=255), dict(qs=248),
                                  dict(table=None), dict(ts=7), dict(width=0), dict(ts=1 << 28, width=1 << 28),
                                  dict(lens=None), dict(offsets=None), dict(o=None), dict(o=P + 8), dict(os=128),
                                  dict(scale=float("nan")), dict(ws=None), dict(ws=P + 4), dict(ws_bytes=0)], ids=str)
