@@ -753,7 +753,7 @@ template <int D, int GROUPS> struct ChunkShare {
     __attribute__((aligned(1024))) uint16_t keys[GROUPS == 1 ? 2 * TILE : 1];
     __attribute__((aligned(1024))) uint16_t values[GROUPS == 1 ? kChunkRing * TILE : 1];
     // Which codes of a value tile are NaN, a bit each, where a wave's part of it (with_nan)
-    // has any; [group][tile % 4]. In the ring these are 0: the product then says
+    // has any; [group][tile % 4]. In the ring, or converted, these are 0: the product then says
     // nothing of them, and nan_values gives the NaN to the rows that see them.
     __attribute__((aligned(16))) uint16_t nans[4 * GROUPS][TILE / 16];
     __attribute__((aligned(16))) int with_nan[4 * GROUPS][8 / GROUPS];
@@ -1029,9 +1029,10 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
     };
 
     // One M phase: S of tile jp + 1 and O += P V of tile jp (if DP: from the second on); on
-    // its way the loads of tile ji are issued into the slot of tile jp + 3 (that of jp - 1),
-    // the part of tile jp + 2 that this wave loaded is checked, and the scales of jp + 1
-    // are taken.
+    // its way the loads of tile ji are issued into the slot of tile jp + 3 (that of jp - 1, which
+    // all are done with; with two slots that of jp + 1, whose codes this wave, their only
+    // reader, converted a tile ago), the part of tile jp + 2 that this wave loaded is checked
+    // and, with one group, converted, and the scales of jp + 1 are taken.
     auto m_phase = [&](auto dp_tag, int jp, int ids_of_ji, int ji) {
         const int js = jp + 1;
         constexpr bool DP = decltype(dp_tag)::value;
@@ -1266,7 +1267,8 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
         if constexpr (SHARED) __syncthreads();  // the next M phase overwrites tile 0's keys
         // A barrier a tile: a SIMD's first wave passes it before, its second behind a product, so they
         // stay half a tile apart and are free between. Behind it the tile that both
-        // waited for and checked is there, and the slot of the tile before is free.
+        // waited for and checked (and converted) is there, and the slot of the tile before
+        // is free: keys are read a phase before their values, so two tiles of them are enough.
         for (int k = 0; k < n; ++k) {
             v_step(k);
             if (phase == 0 && k > 0) __syncthreads();

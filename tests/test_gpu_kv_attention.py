@@ -151,6 +151,33 @@ def test_chunks_over_long_contexts(gpu, dtype, d, bs):
     c.check(c.run(), only=_some(counts, d + bs, 20))
 
 
+@pytest.mark.parametrize("hq,hk,d,lens,counts", [(32, 8, 128, [1500, 1300], [1000, 900]), (8, 2, 64, [700, 300], [300, 200]),
+                                                 (8, 2, 128, [900, 300, 2000], [200, 1, 1]), (8, 2, 128, [90, 3000], [1, 1])])
+def test_captured_calls_follow_lengths(gpu, hq, hk, d, lens, counts):
+    """A captured call of every kind, replayed with other lengths between eager work:
+    each replay is the eager call's result, bit for bit."""
+    torch = gpu
+    c = Call(torch, "bf16", hq, hk, d, 16, lens, counts, seed=50)
+    cache, q, table, offsets = c.handle(), c.q.cuda(), c.table.cuda(), c.offsets.cuda()
+    now, o = c.lens.cuda(), torch.zeros(c.q.shape, dtype=c.q.dtype, device="cuda")
+    work = pyc_amd.kv_attention_workspace(len(lens), hq, hk, d, c.max_q)
+    call = lambda out, ws: pyc_amd.kv_attention(q, cache, table, now, offsets, out, c.scale, c.max_q, workspace=ws)
+    call(o, work)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(o, work)
+    for shorter in (0, 1, 17, 0, 64):
+        now.copy_(torch.clamp(c.lens - shorter, min=0).cuda())
+        o.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = torch.full_like(o, 3.0)
+        call(eager, None)
+        torch.cuda.synchronize()
+        assert torch.equal(o, eager), shorter
+
+
 # (heads, kv heads, lens, counts): the split kernel's two tilings, parts of 128 and of 256 rows
 KINDS = [(4, 2, [70, 200, 130], [1, 1, 1]), (8, 2, [70, 200, 130], [3, 9, 5]), (8, 2, [700, 300], [300, 200]),
          (32, 8, [1500, 1300], [1000, 900])]
