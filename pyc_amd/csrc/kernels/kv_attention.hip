@@ -717,8 +717,8 @@ __global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel
 // workgroups, and worse where the card is not full (figures at the launch). With one group LDS has room for the tiles converted to 16
 // bits, once for the workgroup instead of once for each wave.
 // Measured, 32 heads of 128, 8 kv heads, bf16: 4 chunks of 2048 tokens over 3500 to 4100 keys
-// 370 us, 975 TFLOP/s (1.14 PFLOP/s over 16384 keys; a large library product reaches
-// 1.44). Of a tile's 4000 cycles the matrix unit is busy for 2048: phase M takes 1850
+// 370 to 383 us by the card, 0.94 to 0.98 PFLOP/s (1.09 to 1.14 over 16384 keys; a large
+// library product reaches 1.44). Of a tile's 4000 cycles the matrix unit is busy for 2048: phase M takes 1850
 // (its 34 16-byte reads a lane, for four waves, are 1100 cycles of LDS beside 1024 of
 // products), phase V 1700 (32 exponentials, 32 scalings, 32 additions, 16 roundings:
 // between the other wave's products a vector instruction issues about every 7 cycles).
