@@ -1369,12 +1369,14 @@ static int split_nt(long rows) { return rows <= 16 || rows > kSplitRows ? 1 : 2;
 static long split_most_rows(long rows) { return rows <= kSplitRows ? rows : 16; }
 static long split_run_tiles(long rows) { return (split_most_rows(rows) + 16 * split_nt(rows) - 1) / (16 * split_nt(rows)); }
 // A workspace is the workgroups' results, in room for the largest of any call, then the
-// counters: these stay zero between calls whatever the calls' shapes.
+// counters: these stay zero between calls whatever the calls' shapes. A call has as many as
+// it has run tiles; calls of up to `rows` rows have the most at 33 to 64.
+static long split_room_tiles(long rows) { return rows <= 32 ? 1 : split_run_tiles(kSplitRows); }
 constexpr size_t kSplitPartBytes = (size_t)2 * kSplitGroups * 32 * (128 + 2) * sizeof(float);
 
 template <typename T, int D> static void launch_attention(const AttnArgs& a, int max_q, void* workspace, int max_len,
                                                            hipStream_t s) {
-    const long rows = (long)max_q * a.G, run_tiles = split_run_tiles(rows);  // as the workspace was made
+    const long rows = (long)max_q * a.G, run_tiles = split_run_tiles(rows);
     const int nt = split_nt(rows), waves = split_waves(nt, D);
     AttnSplit sp;
     sp.most_rows = (int)split_most_rows(rows);
@@ -1421,7 +1423,7 @@ extern "C" size_t pyc_hip_kv_attention_workspace_bytes(int B, int hq, int hk, in
     using namespace pyc;
     const long rows = (long)max_q * (hq / hk);
     (void)d;
-    return kSplitPartBytes + ((size_t)B * hk * split_run_tiles(rows) * sizeof(uint32_t) + 15) / 16 * 16;
+    return kSplitPartBytes + ((size_t)B * hk * split_room_tiles(rows) * sizeof(uint32_t) + 15) / 16 * 16;
 }
 
 extern "C" int pyc_hip_kv_attention_launch(int is_bf16, const pyc_hip_kv_cache* cache, int B, int tokens, int hq,

@@ -404,6 +404,20 @@ def test_workspace_kept_and_made(gpu):
         c.check(a)
 
 
+def test_workspace_of_the_largest_step(gpu):
+    """One workspace, made for 2048 tokens a request, for steps of fewer: what a call
+    of the same shape with a workspace of its own gives, bit for bit, each time."""
+    torch = gpu
+    ws = pyc_amd.kv_attention_workspace(32, 32, 8, 128, 2048)
+    for n in (4, 12, 16, 17, 300, 9, 1):
+        lens = [n + 61 * i % 700 for i in range(32)]
+        counts = [n if i % 5 == 0 or n < 20 else 1 + i % 16 for i in range(32)]
+        c = Call(torch, "bf16", 32, 8, 128, 16, lens, counts, seed=60 + n)
+        a = c.run(workspace=ws)
+        assert torch.equal(a, c.run()) and torch.equal(a, c.run(workspace=ws)), n
+        c.check(a, only=set(list(_some(counts, n, 0))[::7]))
+
+
 def test_short_workspace_is_refused(gpu):
     torch = gpu
     c = Call(torch, "bf16", 8, 2, 64, 16, [80], [1], seed=19)

@@ -98,6 +98,17 @@ def test_workspace_sizes():
         assert f(*bad) == 0, bad
 
 
+@pytest.mark.parametrize("hq,hk", [(1, 1), (32, 8), (12, 12), (16, 1), (128, 8), (71, 1), (24, 8), (200, 2)])
+@pytest.mark.parametrize("batch,d", [(1, 64), (7, 128), (32, 128), (700, 64)])
+def test_workspace_of_a_larger_call_is_enough(hq, hk, batch, d):
+    """A workspace is for calls of up to its requests and tokens: its size never
+    falls as either grows, and a call takes one made for more."""
+    f = pyc_amd.lib().pyc_hip_kv_attention_workspace
+    sizes = [f(batch, hq, hk, d, n) for n in list(range(1, 100)) + [128, 300, 2048, 4096]]
+    assert all(0 < a <= b for a, b in zip(sizes, sizes[1:])), sizes
+    assert f(max(1, batch - 1), hq, hk, d, 2048) <= sizes[-1]
+
+
 def test_wrapper_refusals():
     """The Python wrappers refuse host tensors and tensors of other types and
     shapes before they reach the library."""
