@@ -1343,23 +1343,19 @@ __device__ inline void chunk_body(const AttnArgs& a, int from_rows, ChunkShare<D
 }
 
 // A batch with requests of many rows: the first `parts` workgroups take parts of these,
-// the others split what the rest of the batch reads, on the CUs that are left.
-template <typename T, int D>
+// those behind them split what the requests of up to sp.most_rows rows read (and end at
+// once where there are none). How many parts there are is known here only: the host counts
+// as many as there may be, and those that find none end as well.
+template <typename T, int D, int GROUPS>
 __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunk_kernel(AttnArgs a, AttnSplit sp, int parts) {
     static_assert(split_waves(1, 128) * kWave == kChunkThreads, "one workgroup size");
     union Share {
         SplitShare<D, 1> split;
-        ChunkShare<D, 2> chunk;
+        ChunkShare<D, GROUPS> chunk;
     };
     __shared__ Share sh;
-    if ((int)blockIdx.x < parts) chunk_body<T, D, 2>(a, sp.most_rows, sh.chunk, blockIdx.x);
+    if ((int)blockIdx.x < parts) chunk_body<T, D, GROUPS>(a, sp.most_rows, sh.chunk, blockIdx.x);
     else split_body<T, D, 1>(a, sp, sh.split, blockIdx.x - parts, gridDim.x - parts);
-}
-
-// A batch of long chunks only: parts of 256 rows.
-template <typename T, int D> __global__ void __launch_bounds__(kChunkThreads, 1) kv_chunks_kernel(AttnArgs a) {
-    __shared__ ChunkShare<D, 1> sh;
-    chunk_body<T, D, 1>(a, 0, sh, blockIdx.x);
 }
 
 // Rows of a request that the split kernel takes, 16 NT of them a wave: all up to 64 at
@@ -1393,12 +1389,15 @@ template <typename T, int D> static void launch_attention(const AttnArgs& a, int
         else hipLaunchKernelGGL((kv_split_kernel<T, D, 2>), dim3(split), dim3(waves * kWave), 0, s, a, sp);
         return;
     }
-    // Where most requests must have about max_q tokens, all are taken as chunks.
-    const bool chunks_only = 4.0 * a.tokens >= 3.0 * (double)a.B * max_q;
-    if (chunks_only) sp.most_rows = 0;
     // Parts: whole ones, and one more for each request that is large enough.
     const long all = (long)a.tokens * a.G, some = all / (sp.most_rows + 1);
     auto parts_of = [&](int groups) { return (all / chunk_rows(groups) + (some < a.B ? some : a.B)) * a.c.heads; };
+    // Requests of few rows are split in any batch, also where the rows of q would let all have
+    // max_q tokens: lengths are known on the device only, and a part walks all its keys alone.
+    // With parts alone in such calls, a token over 100000 keys beside three chunks of 2048 over 3800
+    // took 2855 us, now 342 (316 for the chunks and 40 for the token, each alone); 32 tokens over 3000
+    // keys in a q with room for 512 each 111, now 41 (36 in one of their size). Split workgroups
+    // without work cost a call of four such chunks nothing that can be seen (390).
     // Rounds of workgroups if every request has max_q tokens. A round of 256 rows takes 1.6 to
     // 1.85 times as long as one of 128. Measured (us, 128 rows against 256, 4 chunks over 4096 keys,
     // 32 heads of 128, 8 kv heads): 256 tokens 90 / 130 (1 round / 1), 320 150 / 131 (2 / 1),
@@ -1407,14 +1406,17 @@ template <typename T, int D> static void launch_attention(const AttnArgs& a, int
         const long tiles = ((long)a.max_q * a.G + chunk_rows(groups) - 1) / chunk_rows(groups);
         return (tiles * a.B * a.c.heads + kSplitGroups - 1) / kSplitGroups;
     };
+    const bool full = 4.0 * a.tokens >= 3.0 * (double)a.B * max_q;  // most requests may have about max_q
     if constexpr (D == 128)
-        if (chunks_only && 7 * rounds(1) <= 4 * rounds(2)) {
-            hipLaunchKernelGGL((kv_chunks_kernel<T, D>), dim3((unsigned)parts_of(1)), dim3(kChunkThreads), 0, s, a);
+        if (full && 7 * rounds(1) <= 4 * rounds(2)) {
+            const long parts = parts_of(1);
+            hipLaunchKernelGGL((kv_chunk_kernel<T, D, 1>), dim3((unsigned)(parts + split)), dim3(kChunkThreads), 0, s, a, sp,
+                               (int)parts);
             return;
         }
     const long parts = parts_of(2);
-    hipLaunchKernelGGL((kv_chunk_kernel<T, D>), dim3((unsigned)(parts + (chunks_only ? 0 : split))), dim3(kChunkThreads), 0,
-                       s, a, sp, (int)parts);
+    hipLaunchKernelGGL((kv_chunk_kernel<T, D, 2>), dim3((unsigned)(parts + split)), dim3(kChunkThreads), 0, s, a, sp,
+                       (int)parts);
 }
 
 }  // namespace pyc

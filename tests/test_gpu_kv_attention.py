@@ -448,3 +448,74 @@ def test_resources_match_the_code_object(gpu):
         assert r.device == 1 and r.lds_bytes == r.attr_lds_bytes and r.attr_max_threads >= r.threads, sym
         assert r.waves_per_simd == r.attr_blocks_per_cu * (r.threads // 64) / 4, (sym, r.waves_per_simd, r.attr_blocks_per_cu)
         assert r.attr_scratch_bytes == 0, sym
+
+
+def _us(torch, f, n=12):
+    """The shortest of n calls, with the GPU waited for."""
+    best = float("inf")
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        best = min(best, 1000.0 * a.elapsed_time(b))
+    return best
+
+
+class Timed:
+    """A batch's call on the device, with codes of any value below NaN. q may have more rows than the requests."""
+
+    def __init__(self, torch, lens, counts, max_q=None, rows=None, hq=32, hk=8, d=128, bs=16):
+        need = sum(kv_util.ceil_div(n, bs) for n in lens) + 1
+        g = torch.Generator(device="cuda").manual_seed(7)
+        k = torch.randint(0, 0x78, (need, hk, bs, d), dtype=torch.uint8, device="cuda", generator=g)
+        v = torch.randint(0, 0x78, (need, hk, d, bs), dtype=torch.uint8, device="cuda", generator=g)
+        s = torch.full((need, hk), 2.0 ** -9, device="cuda")
+        self.cache = pyc_amd.KvCache(k, v, s, s.clone())
+        self.table = torch.from_numpy(_tables(lens, bs, need, 7)).to(torch.int32).cuda()
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+        self.lens, self.offsets = i32(lens), i32([0] + np.cumsum(counts).tolist())
+        self.q = torch.randn((rows or sum(counts), hq, d), generator=g, device="cuda").to(torch.bfloat16)
+        self.o, self.max_q, self.scale = torch.empty_like(self.q), max_q or max(counts), d ** -0.5
+        self.work = pyc_amd.kv_attention_workspace(len(lens), hq, hk, d, self.max_q)
+
+    def __call__(self):
+        pyc_amd.kv_attention(self.q, self.cache, self.table, self.lens, self.offsets, self.o, self.scale, self.max_q,
+                             workspace=self.work)
+
+
+def test_a_token_beside_chunks_is_split(gpu):
+    """One token over a long context beside prompt chunks costs about what it does
+    alone: its keys are not walked by one workgroup. (Of one workgroup for each kv
+    head, 100000 keys took 2900 us, the chunks 320 and the token alone 40.)"""
+    chunks, token = [(3800, 2048)] * 3, [(100000, 1)]
+    times = []
+    for part in (chunks, token, chunks + token):
+        call = Timed(gpu, [n for n, _ in part], [m for _, m in part])
+        call()
+        times.append(_us(gpu, call))
+    assert times[2] < 2.0 * (times[0] + times[1]) + 100.0, times
+
+
+def test_decoding_in_a_step_captured_for_prompts(gpu):
+    """A step whose q has room for a prompt of every request, replayed where each
+    brings one token: near a call made for single tokens, with the same results up
+    to the order of sums, which bf16's rounding hides but for one step of it."""
+    torch = gpu
+    lens, counts = [40000 + 977 * i for i in range(6)], [1] * 6
+    plain, room = Timed(torch, lens, counts), Timed(torch, lens, counts, max_q=512, rows=6 * 512)
+    room.q[:6] = plain.q
+    plain()
+    room()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        room()
+    room.o.fill_(7.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    a, b = room.o[:6].double(), plain.o.double()
+    assert bool((room.o[6:] == 7.0).all())
+    assert bool(((a - b).abs() <= 2.0 ** -6 * b.abs() + 2.0 ** -6 * b.abs().max()).all())
+    assert _us(torch, graph.replay) < 2.0 * _us(torch, plain) + 100.0
