@@ -519,3 +519,73 @@ def test_decoding_in_a_step_captured_for_prompts(gpu):
     assert bool((room.o[6:] == 7.0).all())
     assert bool(((a - b).abs() <= 2.0 ** -6 * b.abs() + 2.0 ** -6 * b.abs().max()).all())
     assert _us(torch, graph.replay) < 2.0 * _us(torch, plain) + 100.0
+
+
+def test_chunks_among_many_requests(gpu):
+    """More requests than a wave has lanes, chunks among their first, the 64th, the
+    65th and the last ones, single tokens and requests without any between."""
+    r = np.random.default_rng(3)
+    lens, counts = r.integers(1, 90, 140).tolist(), [1] * 140
+    for i, n in ((0, 150), (63, 90), (64, 131), (129, 70), (139, 33)):
+        counts[i], lens[i] = n, n + 45 * (i % 3)
+    for i in (1, 65, 70, 138):
+        counts[i] = 0
+    for dtype, d in (("bf16", 128), ("f16", 64)):
+        c = Call(gpu, dtype, 8, 2, d, 16, lens, counts, seed=70 + d)
+        c.check(c.run(), only=_some(counts, d, 2))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 64), (8, 2, 128), (32, 8, 128)])
+def test_many_chunks(gpu, dtype, hq, hk, d):
+    """More chunks than a wave has lanes, in parts of 128 and (32 heads) 256 rows."""
+    r = np.random.default_rng(4)
+    counts = r.integers(90, 110, 70).tolist()
+    lens = [n + int(x) for n, x in zip(counts, r.integers(0, 200, 70))]
+    c = Call(gpu, dtype, hq, hk, d, 16, lens, counts, seed=80 + d)
+    some = _some(counts, d, 0)
+    c.check(c.run(), only=set(sorted(some)[::1 if hq == 8 else 7]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_draft_tokens_over_long_contexts(gpu, dtype, d):
+    """Requests of 17 to 64 rows whose keys several workgroups share."""
+    lens, counts = [6100, 3000, 70, 4097], [16, 5, 9, 13]
+    c = Call(gpu, dtype, 8, 2, d, 32, lens, counts, seed=90 + d)
+    c.check(c.run(), only=_some(counts, d, 3))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,lens,counts", KINDS)
+def test_rows_of_nobody_stay(gpu, dtype, hq, hk, lens, counts):
+    """Rows of q before the first request, behind the last and past max_q, in every
+    kind of batch: left as they were, to the bit; the others are as ever."""
+    torch = gpu
+    c = Call(torch, dtype, hq, hk, 128, 16, lens, counts, seed=44)
+    before = 5
+    c.q = torch.cat([c.q[:1].expand(before, -1, -1), c.q, c.q[:1].expand(70, -1, -1)])
+    c.offsets += before
+    most = max(counts) - (1 if max(counts) > 1 else 0)
+    got = c.run(max_q=most, fill=7.0)
+    mine = torch.zeros(c.q.shape[0], dtype=torch.bool)
+    for b, n in enumerate(counts):
+        mine[int(c.offsets[b]):int(c.offsets[b]) + min(n, most)] = True
+    assert bool((got[~mine] == 7.0).all())
+    some = {before + t for t in _some(counts, 6, 3)}
+    c.check(got, most, only={t for t in some if bool(mine[t])})
+
+
+def test_offsets_outside_the_rows(gpu):
+    """Offsets below 0 and past the rows of q, or falling, mean the nearest that there are."""
+    torch = gpu
+    c = Call(torch, "bf16", 4, 1, 64, 16, [48, 20, 33], [1, 1, 1], seed=15)
+    c.max_q = 4
+    c.offsets = torch.tensor([-5, 2, 1000, 900], dtype=torch.int32)
+    got = c.run()
+    c.offsets = torch.tensor([0, 2, 3, 3], dtype=torch.int32)
+    c.check(got, 4)
+    long = Call(torch, "bf16", 8, 2, 128, 16, [300, 200], [100, 90], seed=16)
+    want = long.run()
+    long.offsets = torch.tensor([-7, 100, 1 << 30], dtype=torch.int32)
+    assert torch.equal(long.run(), want)
