@@ -271,7 +271,7 @@ int pyc_hip_kv_attention_dispatch(
     void* workspace, size_t workspace_bytes, void* stream);
 
 /* Bytes of workspace that a call of up to B requests and max_q rows each needs
- * (0: bad arguments). Host only. */
+ * (0: bad arguments): never less for more of either. Host only. */
 size_t pyc_hip_kv_attention_workspace(int B, int q_heads, int kv_heads, int head_dim, int max_q);
 
 /* Device properties the bench and the registry report. */

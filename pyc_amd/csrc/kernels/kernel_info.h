@@ -52,7 +52,7 @@ enum { PYC_KI_W8_LDS = 0, PYC_KI_W8_REG = 1, PYC_KI_W8_CHAIN = 2 };
 int pyc_hip_kinfo_w8a16(int kid, pyc_hip_kinfo* out);
 /* eltwise.hip: GELU (kid 0) and the register-resident LayerNorm (kid 1) */
 int pyc_hip_kinfo_eltwise(int kid, int dtype, pyc_hip_kinfo* out);
-/* kv_plan.hip, kv_append.hip, kv_attention.hip (head dim 128) */
+/* kv_plan.hip, kv_append.hip, kv_attention.hip (head dim 128; of the attention kernels the one for single tokens) */
 int pyc_hip_kinfo_kv_plan(pyc_hip_kinfo* out);
 int pyc_hip_kinfo_kv_append(int is_bf16, pyc_hip_kinfo* out);
 int pyc_hip_kinfo_kv_attention(int is_bf16, pyc_hip_kinfo* out);

@@ -8,8 +8,8 @@
 //   code = e4m3(x * (1 / s)), round to nearest even; not finite -> NaN;
 //   where s > s_old the codes already there become e4m3(code * (s_old / s)).
 // Powers of two cost no precision in a floating-point code: x / s is exact, so
-// there is one rounding, the same for a token alone and in its prompt, and a
-// block whose scale grows loses only what falls below the code's normal range.
+// there is one rounding, at one block scale the same for a token alone and in its prompt, and
+// a block whose scale grows loses only what falls below the code's normal range.
 //
 // The tokens of one block stand together in the slot map; the workgroup that finds
 // the first of them owns the block for its heads. A wave has one chunk of 16 slots
@@ -21,7 +21,7 @@
 // HBM bounds it for prompts: 16000 tokens of 8 heads of 128 in bf16 take 21 us, 4.65 TB/s
 // of rows read once and codes written once (a copy reaches 5.1); with every element checked
 // and compared as a float they took 25, of them 18 vector instructions. Few tokens are
-// latency: 32 of them, 32 blocks, 4.6 us on the device, of which loads that wait
+// latency: 32 of them, 32 blocks, 4.1 us on the device, of which loads that wait
 // for each other (slots, scales, codes) are the most. A wave to a chunk, its rows held from
 // one read: a workgroup to a block and head, which read them twice, took 241 us for the
 // prompts (and 3.8 for the 32 tokens).
@@ -238,7 +238,9 @@ extern "C" int pyc_hip_kv_append_launch(int is_bf16, const pyc_hip_kv_cache* cac
     using namespace pyc;
     AppendArgs a{kv_cache_of(cache), tokens, 1, (const uint16_t*)k, (const uint16_t*)v, k_stride, v_stride, slots};
     // A workgroup for every row where that gives up to 16 k waves (most rows begin no
-    // block and their waves end at once), else for up to 16 rows in a row.
+    // block and their waves end at once), else for up to 16 rows in a row. With blocks of 64 three
+    // of four workgroups still find none, and the others read the slots a second time: 7 ragged
+    // chunks of 12 heads of 64 in f16, 8.2 us.
     const int S = a.c.bs / kChunk, waves = S > 4 ? S : 4, per = waves / S;
     const unsigned hy = (unsigned)((a.c.heads + per - 1) / per);
     while (a.span < kChunk && (double)tokens / a.span * hy * 2 * waves > 16384.0) a.span *= 2;

@@ -20,10 +20,12 @@
 // Statistics and sums are fp32. (8-bit matrix products of codes, q as two of them, would
 // run at twice the rate for half the work, but add their 64 products with fewer
 // bits: scores near 170 came out off by 0.01. So both operands are 16-bit.) P is
-// rounded to 16 bits for the product: for bf16
-// output once (2^-8 of each p, below the output's own rounding once averaged);
-// for f16 output P is split into two bf16 parts (2^-16 left), as bf16 holds any
-// block's scale and f16 does not.
+// rounded to 16 bits for the product: for bf16 output once (2^-8 of each p at most), which
+// adds about as much as the output's own rounding: 2.3e-3 of the result's norm against
+// 64 bits where 1.65e-3 is the output's alone. For f16 output P is split into two bf16
+// parts (2^-16 left), as bf16 holds any block's scale and f16 does not; the second product
+// takes 497 us where one takes 390 (4 chunks of 2048 tokens over 3800 keys) and 33.6 where
+// one takes 32.6 (32 single tokens), too much for the half bit it would give bf16.
 //
 // Masked places never reach a sum: scores are selected away, tokens behind
 // `len` (or of a block id outside the cache) have their value codes cleared, and
@@ -388,9 +390,11 @@ template <typename T, int D, int NT> struct AttnWave {
 // heads of 128 in bf16: 2 contexts of 100000 to 131072 keys, 8 kv heads, 83.5 us (5.2
 // TB/s, what a copy reaches); 64 of 300 to 6000, 32 kv heads, 216 us (5.4 TB/s); 32 of
 // 200 to 4096, 8 kv heads, 27 us (3.8 TB/s: what it takes to start, to find the work and to
-// join is 7 of them); one of 777, 10.3 us, which is latency: 0.8 for lengths and
-// their sums, 0.7 to find the piece, 2.7 for the tile's ids, scales and codes one after
-// the other, 1.2 for the join in LDS, 1 for the counter, and the launch.
+// join is 7 of them); one of 777, 10.3 us, which is latency: its 8 runs of 13 tiles are a
+// workgroup's each, up to two tiles to a wave, one after the other, behind loads that wait for
+// each other (lengths, ids, scales and codes), with a join in LDS and no counter. With 32
+// rows to a wave (NT 2; four heads to a kv head): 16 requests over 3000 to 3750 keys, 5 tokens
+// each, one run, 43 us; 16 tokens each, two runs, 70.
 struct AttnSplit {
     int most_rows;
     float* part;     // two results of every workgroup: [16 NT][D] sums, [16 NT][2] maximum and sum
@@ -717,7 +721,7 @@ __global__ void __launch_bounds__(split_waves(NT, D) * kWave, 1) kv_split_kernel
 // workgroups, and worse where the card is not full (figures at the launch). With one group LDS has room for the tiles converted to 16
 // bits, once for the workgroup instead of once for each wave.
 // Measured, 32 heads of 128, 8 kv heads, bf16: 4 chunks of 2048 tokens over 3500 to 4100 keys
-// 370 to 383 us by the card, 0.94 to 0.98 PFLOP/s (1.09 to 1.14 over 16384 keys; a large
+// 370 to 390 us by the card, 0.92 to 0.98 PFLOP/s (1.10 over 16384 keys; a large
 // library product reaches 1.44). Of a tile's 4000 cycles the matrix unit is busy for 2048: phase M takes 1850
 // (its 34 16-byte reads a lane, for four waves, are 1100 cycles of LDS beside 1024 of
 // products), phase V 1700 (32 exponentials, 32 scalings, 32 additions, 16 roundings:
@@ -1400,8 +1404,11 @@ template <typename T, int D> static void launch_attention(const AttnArgs& a, int
     // without work cost a call of four such chunks nothing that can be seen (390).
     // Rounds of workgroups if every request has max_q tokens. A round of 256 rows takes 1.6 to
     // 1.85 times as long as one of 128. Measured (us, 128 rows against 256, 4 chunks over 4096 keys,
-    // 32 heads of 128, 8 kv heads): 256 tokens 90 / 130 (1 round / 1), 320 150 / 131 (2 / 1),
-    // 512 172 / 148 (2 / 1), 768 228 / 241 (3 / 2), 1024 290 / 267 (4 / 2).
+    // 32 heads of 128, 8 kv heads, bf16): 256 tokens 78 / 112 (1 round / 1), 320 137 / 115 (2 / 1),
+    // 512 146 / 132 (2 / 1), 768 209 / 225 (3 / 2), 1024 267 / 246 (4 / 2); in f16 98 / 135,
+    // 167 / 137, 186 / 171, 267 / 281, 340 / 320. Of 80 shapes, half of them in f16 (1 to 8 requests of 256 to
+    // 2048 tokens, 5 to 32 kv heads) the rule took the slower side by more than 2 % in two (3 and 4 %:
+    // one request of 2048).
     auto rounds = [&](int groups) {
         const long tiles = ((long)a.max_q * a.G + chunk_rows(groups) - 1) / chunk_rows(groups);
         return (tiles * a.B * a.c.heads + kSplitGroups - 1) / kSplitGroups;

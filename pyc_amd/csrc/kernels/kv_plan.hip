@@ -15,8 +15,8 @@
 // move a wave at a time, a step whose requests bring a token each writes it from the
 // request's own thread, and many tokens get a launch over all CUs (from 4096 on: below,
 // the one workgroup has them sooner than a second launch starts). 32 requests of a token
-// each: 2.2 us on the device, 7.5 with the call; 1024 requests that bring 90000 tokens:
-// 8.7 and 4.5.
+// each: 2.1 us on the device, 7.5 with the call; 1024 requests that bring 55206 tokens:
+// 9.0 and 4.1 on the device, 13.1 with the call.
 #include "kv_cache.hpp"
 
 namespace pyc {
