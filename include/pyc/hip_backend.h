@@ -22,6 +22,10 @@ extern "C" {
 #define PYC_HIP_EPI_NONE 0
 #define PYC_HIP_EPI_BIAS 1 /* out[m,n] += bias[n] (fp32 bias) */
 #define PYC_HIP_EPI_RELU 2 /* out = max(out, 0) after bias */
+/* Products by expert and with 4-bit weights only, not with RELU: rows 0 .. N/2 - 1 of
+ * the weights are gates, the others values, and column c of out (N/2 of them) is
+ * silu(gate c) * value c, each with its bias. silu(g) = g / (1 + e^-g). */
+#define PYC_HIP_EPI_SILU_GATE 4
 
 /* Generalises reference gemm/kernel.cu:151-203 (pyc_cutlass_gemm_dispatch):
  * C[M,N] = epilogue(alpha * A[M,K] * op(B) + beta * C), fp32 accumulate.
@@ -274,6 +278,81 @@ int pyc_hip_kv_attention_dispatch(
  * (0: bad arguments): never less for more of either. Host only. */
 size_t pyc_hip_kv_attention_workspace(int B, int q_heads, int kv_heads, int head_dim, int max_q);
 
+/* Layers of experts (no reference counterpart: the reference's graph ops name no
+ * routing and its one matmul has one weight). Rows of tokens that go to the same expert
+ * stand together: expert e has rows offsets[e] .. offsets[e + 1] - 1.
+ *
+ * Routing. For each row of logits [tokens][experts] (rows logits_stride apart): the k
+ * largest, in descending order, ties to the lower expert: ids [tokens][k], and weights
+ * [tokens][k] fp32 = softmax over all experts, with normalize over the chosen ones. -infinity and
+ * NaN are never chosen and weigh nothing; a choice that there is none for has id -1 and
+ * weight 0 (padding: a row of -infinity). +infinity: all weight, in equal parts, on those that have it.
+ * With flat index f = t * k + j of choice j of token t:
+ *   offsets [experts + 1]  where each expert's rows begin, and how many there are,
+ *   rows [tokens * k]      the flat indexes by expert, ascending in each; -1 behind the last,
+ *   places [tokens * k]    where f stands in rows, -1 without an expert.
+ * 1 <= experts <= 1024, 1 <= k <= min(experts, 64), 0 <= tokens <= 2^22. workspace:
+ * pyc_hip_moe_route_workspace bytes on a 4-byte boundary, of any content, for one call at a time
+ * (calls that may overlap need one each); up to 64 tokens it may be NULL.
+ * Symbols "hip_moe_route_f32", "hip_moe_route_bf16", "hip_moe_route_f16". 0, -1 (bad
+ * argument, nothing launched), -2 (HIP error). */
+int pyc_hip_moe_route_dispatch(
+    const char* symbol, int tokens, int experts, int k, int normalize, const void* logits, int64_t logits_stride,
+    int32_t* ids, float* weights, int32_t* offsets, int32_t* rows, int32_t* places,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of a routing (0: bad arguments): never less for more tokens. Host only. */
+size_t pyc_hip_moe_route_workspace(int tokens, int experts, int k);
+
+/* out[t] = base[t] + sum_j weights[t][j] y[places[t][j]]: a token's experts' rows back onto it.
+ * y [rows][width], out and base [tokens][width] of the symbol's type (rows their strides
+ * apart, base NULL: 0), weights fp32 and places [tokens][k]. fp32 sums, base first, then j
+ * in order, one rounding. A place outside y (-1) counts as absent. out may be base; else it
+ * overlaps nothing. Any width and alignment; 16-byte rows are fastest. 1 <= k <= 64, tokens * width below 2^38.
+ * Symbols "hip_moe_combine_bf16", "hip_moe_combine_f16". 0, -1, -2 as above. */
+int pyc_hip_moe_combine_dispatch(
+    const char* symbol, int rows, int tokens, int k, int width, const void* y, int64_t y_stride,
+    const float* weights, const int32_t* places, const void* base, int64_t base_stride,
+    void* out, int64_t out_stride, void* stream);
+
+/* Products grouped by expert, of ragged sizes that the device knows:
+ *   y[p] = epi(x[src[p] / fan] w[e]^T + bias[e])   for offsets[e] <= p < offsets[e + 1],
+ * fp32 sums, one rounding. x [x_rows][K] (rows x_stride apart), w [experts][N][K] (experts w_stride
+ * elements apart, each dense), bias fp32 [experts][N] with PYC_HIP_EPI_BIAS; y [rows][N], with
+ * PYC_HIP_EPI_SILU_GATE [rows][N / 2] (rows y_stride apart). src NULL: row p of x; with the
+ * routing's rows and fan = k, a token's row goes to each of its experts. An index outside x reads a row of zeros.
+ * offsets are held to 0 .. rows and to never decrease; rows of y before the first and
+ * behind the last expert's stay as they are. Experts without rows are not read. y overlaps nothing.
+ * Any N, K, strides and 2-byte alignment; K, strides and bases in whole 16 bytes are fastest.
+ * 1 <= experts <= 1024, rows and x_rows up to 2^28, N and K up to 2^24.
+ * Symbols "hip_grouped_gemm_bf16", "hip_grouped_gemm_f16". 0, -1, -2 as above. */
+int pyc_hip_grouped_gemm_dispatch(
+    const char* symbol, int experts, int rows, int N, int K, const void* x, int64_t x_stride, int x_rows,
+    const int32_t* src, int fan, const int32_t* offsets, const void* w, int64_t w_stride,
+    const float* bias, int epilogue, void* y, int64_t y_stride, void* stream);
+
+/* Products with 4-bit weights: w[n][k] = (code - zero) * scale, with a scale of x's type and
+ * a zero point for each `group` (32, 64 or 128) k of a row:
+ *   codes [N][K / 2]  the even k in the low half of a byte, 0 .. 15,
+ *   scale [N][K / group], zeros [N][K / group] bytes, or NULL: 8.
+ *   y[M][N] = epi(x[M][K] w^T + bias), epilogues as above (bias fp32 [N]).
+ * Whole numbers times x are summed as they are, the scale comes in fp32: weights are
+ * never rounded. Finite x. Any M and N, K a multiple of group; x and codes on 16-byte boundaries, x_stride a
+ * multiple of 8. Symbols "hip_gemm_w4a16_bf16", "hip_gemm_w4a16_f16". 0, -1, -2 as above. */
+int pyc_hip_w4a16_gemm_dispatch(
+    const char* symbol, int M, int N, int K, int group, const void* x, int64_t x_stride,
+    const void* codes, const void* scale, const uint8_t* zeros, const float* bias, int epilogue,
+    void* y, int64_t y_stride, void* stream);
+
+/* The same by expert: codes [experts][N][K / 2] (experts codes_stride bytes apart, a multiple of 16),
+ * scale and zeros [experts][N][K / group] dense, bias [experts][N]; the rest as in
+ * pyc_hip_grouped_gemm_dispatch. Symbols "hip_grouped_gemm_w4a16_bf16", "hip_grouped_gemm_w4a16_f16". */
+int pyc_hip_w4a16_grouped_gemm_dispatch(
+    const char* symbol, int experts, int rows, int N, int K, int group, const void* x, int64_t x_stride, int x_rows,
+    const int32_t* src, int fan, const int32_t* offsets, const void* codes, int64_t codes_stride,
+    const void* scale, const uint8_t* zeros, const float* bias, int epilogue,
+    void* y, int64_t y_stride, void* stream);
+
 /* Device properties the bench and the registry report. */
 typedef struct {
     char gcn_arch[64];       /* e.g. "gfx950:sramecc+:xnack-" */
@@ -324,7 +403,8 @@ int pyc_hip_kernel_resources_query(const char* symbol, pyc_hip_kernel_resources*
 
 /* Number of kernel symbols compiled into this library for op_key
  * ("matmul", "attention", "conv2d", "matmul_w8a16", "matmul_w8a16_chain",
- * "gelu", "layernorm", "kv_plan", "kv_append", "kv_attention"), independent of the
+ * "gelu", "layernorm", "kv_plan", "kv_append", "kv_attention", "moe_route",
+ * "moe_combine", "grouped_gemm", "matmul_w4a16", "grouped_w4a16"), independent of the
  * registry's state. */
 int pyc_hip_kernel_symbol_count(const char* op_key);
 

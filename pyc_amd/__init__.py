@@ -66,6 +66,18 @@ def _declare(L: C.CDLL) -> None:
     L.pyc_hip_kv_attention_dispatch.restype = I
     L.pyc_hip_kv_attention_workspace.argtypes = [I, I, I, I, I]
     L.pyc_hip_kv_attention_workspace.restype = Z
+    L.pyc_hip_moe_route_dispatch.argtypes = [S, I, I, I, I, P, I64, P, P, P, P, P, P, Z, P]
+    L.pyc_hip_moe_route_dispatch.restype = I
+    L.pyc_hip_moe_route_workspace.argtypes = [I, I, I]
+    L.pyc_hip_moe_route_workspace.restype = Z
+    L.pyc_hip_moe_combine_dispatch.argtypes = [S, I, I, I, I, P, I64, P, P, P, I64, P, I64, P]
+    L.pyc_hip_moe_combine_dispatch.restype = I
+    L.pyc_hip_grouped_gemm_dispatch.argtypes = [S, I, I, I, I, P, I64, I, P, I, P, P, I64, P, I, P, I64, P]
+    L.pyc_hip_grouped_gemm_dispatch.restype = I
+    L.pyc_hip_w4a16_gemm_dispatch.argtypes = [S, I, I, I, I, P, I64, P, P, P, P, I, P, I64, P]
+    L.pyc_hip_w4a16_gemm_dispatch.restype = I
+    L.pyc_hip_w4a16_grouped_gemm_dispatch.argtypes = [S, I, I, I, I, I, P, I64, I, P, I, P, P, I64, P, P, P, I, P, I64, P]
+    L.pyc_hip_w4a16_grouped_gemm_dispatch.restype = I
     L.pyc_hip_device_query.argtypes = [C.POINTER(abi.DeviceInfo)]
     L.pyc_hip_device_query.restype = I
     L.pyc_hip_kernel_resources_query.argtypes = [S, C.POINTER(abi.KernelResources)]
@@ -414,6 +426,194 @@ def kv_attention(q, cache: KvCache, table, lens, q_offsets, o, scale: float, max
         o_stride, scale, workspace.data_ptr(), workspace.nbytes, at)
     if rc != 0:
         _check(rc, "kv attention")
+
+
+_moe_env = None  # (int32, float32, uint8, the current device's index, symbol suffixes of rows, of logits)
+
+
+def _make_moe_env():
+    import torch
+    global _moe_env
+    i32, current, half = _kv_env or _make_kv_env()
+    _moe_env = (i32, torch.float32, torch.uint8, current, half, {**half, torch.float32: b"f32"})
+    return _moe_env
+
+
+def _rows_of(what: str, t, width: int, dtype, device: int) -> int:
+    """Checks rows [n, width] of a type with dense elements on a device: their stride."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] != width or t.dtype is not dtype or t.get_device() != device or \
+            (stride[1] != 1 and width > 1):
+        _kv_refuse(what, f"rows are [n, {width}] of one type with dense elements, on the call's device")
+    return stride[0] if shape[0] > 1 else width
+
+
+def _dense_of(what: str, t, shape, dtype, device: int) -> int:
+    """Checks a dense tensor (None: 0): its address."""
+    if t is None:
+        return 0
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        _kv_refuse(what, f"an operand is not dense {dtype} {tuple(shape)} on the call's device")
+    return t.data_ptr()
+
+
+def _here(what: str, t, current) -> int:
+    device = t.get_device()
+    if device < 0 or device != current():
+        _kv_refuse(what, "the tensors are not on the current device")
+    return device
+
+
+def moe_route_workspace(tokens: int, experts: int, k: int):
+    """A workspace for moe_route calls of up to `tokens` tokens on the current device; for
+    one call at a time."""
+    import torch
+    n = lib().pyc_hip_moe_route_workspace(tokens, experts, k)
+    if n == 0:
+        raise PycError("moe route workspace: bad sizes")
+    return torch.empty(n, dtype=torch.uint8, device="cuda")
+
+
+def moe_route(logits, ids, weights, offsets, rows, places, normalize: bool = True, workspace=None, stream=None) -> None:
+    """The k experts of each token and the experts' order of rows
+    (pyc_hip_moe_route_dispatch): logits [T, E] float32, bf16 or f16; writes ids and
+    weights [T, k] (int32, float32), offsets [E + 1], rows and places [T * k] int32.
+    Without a workspace (moe_route_workspace) one is made where the call needs it."""
+    i32, f32, _, current, _, suffixes = _moe_env or _make_moe_env()
+    device = _here("moe route", logits, current)
+    suffix = suffixes.get(logits.dtype)
+    if suffix is None or logits.dim() != 2 or ids.dim() != 2:
+        _kv_refuse("moe route", "logits are float32, bf16 or f16 [tokens, experts], ids [tokens, k]")
+    (T, E), k = logits.shape, ids.shape[1]
+    stride = _rows_of("moe route", logits, E, logits.dtype, device)
+    i, w = _dense_of("moe route", ids, (T, k), i32, device), _dense_of("moe route", weights, (T, k), f32, device)
+    o, r = _dense_of("moe route", offsets, (E + 1,), i32, device), _dense_of("moe route", rows, (T * k,), i32, device)
+    p = _dense_of("moe route", places, (T * k,), i32, device)
+    at = _stream(stream)
+    if workspace is None and T > 64:
+        import contextlib
+
+        import torch
+        # made on the call's stream, so that it is other work's only after the call
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(torch.cuda.ExternalStream(at)):
+            workspace = moe_route_workspace(T, E, k)
+    elif workspace is not None and (workspace.get_device() != device or not workspace.is_contiguous()):
+        _kv_refuse("moe route", "the workspace is dense, on the call's device")
+    rc = (_lib or lib()).pyc_hip_moe_route_dispatch(
+        b"hip_moe_route_" + suffix, T, E, k, int(normalize), logits.data_ptr(), stride, i, w, o, r, p,
+        0 if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes, at)
+    if rc != 0:
+        _check(rc, "moe route")
+
+
+def moe_combine(y, weights, places, out, base=None, stream=None) -> None:
+    """out[t] = base[t] + sum_j weights[t, j] y[places[t * k + j]] (pyc_hip_moe_combine_dispatch):
+    y [rows, H], out and base [T, H] bf16 or f16, weights [T, k] float32, places
+    [T * k] int32 as moe_route leaves them. out may be base."""
+    i32, f32, _, current, half, _ = _moe_env or _make_moe_env()
+    device = _here("moe combine", out, current)
+    suffix = half.get(out.dtype)
+    if suffix is None or out.dim() != 2 or weights.dim() != 2:
+        _kv_refuse("moe combine", "out is bf16 or f16 [tokens, width], weights [tokens, k]")
+    (T, H), k = out.shape, weights.shape[1]
+    out_stride, y_stride = _rows_of("moe combine", out, H, out.dtype, device), _rows_of("moe combine", y, H, out.dtype, device)
+    base_stride = 0 if base is None else _rows_of("moe combine", base, H, out.dtype, device)
+    if base is not None and base.shape[0] != T:
+        _kv_refuse("moe combine", "base and out do not match")
+    rc = (_lib or lib()).pyc_hip_moe_combine_dispatch(
+        b"hip_moe_combine_" + suffix, y.shape[0], T, k, H, y.data_ptr(), y_stride,
+        _dense_of("moe combine", weights, (T, k), f32, device), _dense_of("moe combine", places, (T * k,), i32, device),
+        _ptr(base), base_stride, out.data_ptr(), out_stride, _stream(stream))
+    if rc != 0:
+        _check(rc, "moe combine")
+
+
+def _product(what: str, x, y, N: int, K: int, epilogue: int, env):
+    """Checks x [n, K] and y [rows, N, or N / 2 gated]: (suffix, device, x's stride, y's stride)."""
+    device = _here(what, x, env[3])
+    suffix = env[4].get(x.dtype)
+    if suffix is None:
+        _kv_refuse(what, "x is bf16 or f16")
+    if epilogue & 4 and N % 2:
+        _kv_refuse(what, "gated weights have an even number of rows")
+    return (suffix, device, _rows_of(what, x, K, x.dtype, device),
+            _rows_of(what, y, N // 2 if epilogue & 4 else N, x.dtype, device))
+
+
+def _experts(what: str, w, dtype, device: int) -> int:
+    """Checks expert weights [E, N, K]: elements from an expert to the next one."""
+    shape, stride = w.shape, w.stride()
+    if w.dtype is not dtype or w.get_device() != device or (stride[2] != 1 and shape[2] > 1) or \
+            (stride[1] != shape[2] and shape[1] > 1):
+        _kv_refuse(what, f"weights are {dtype} [experts, N, ..] with dense experts, on the call's device")
+    return stride[0] if shape[0] > 1 else shape[1] * shape[2]
+
+
+def grouped_gemm(x, w, offsets, y, rows=None, fan: int = 1, bias=None, epilogue: int = 0, stream=None) -> None:
+    """y[p] = epi(x[rows[p] // fan] w[e]^T + bias[e]) for offsets[e] <= p < offsets[e + 1]
+    (pyc_hip_grouped_gemm_dispatch): x [n, K], w [E, N, K] and y [rows, N] bf16 or f16, offsets
+    [E + 1] and rows int32 as moe_route leaves them (rows None: row p of x), bias [E, N]
+    float32. epilogue: 0, 2 (ReLU) or 4 (SiLU gate: y is [rows, N / 2])."""
+    env = _moe_env or _make_moe_env()
+    if w.dim() != 3 or y.dim() != 2:
+        _kv_refuse("grouped gemm", "weights are [experts, N, K], y [rows, columns]")
+    E, N, K = w.shape
+    suffix, device, x_stride, y_stride = _product("grouped gemm", x, y, N, K, epilogue, env)
+    i32, P = env[0], y.shape[0]
+    rc = (_lib or lib()).pyc_hip_grouped_gemm_dispatch(
+        b"hip_grouped_gemm_" + suffix, E, P, N, K, x.data_ptr(), x_stride, x.shape[0],
+        _dense_of("grouped gemm", rows, (P,), i32, device), fan, _dense_of("grouped gemm", offsets, (E + 1,), i32, device),
+        w.data_ptr(), _experts("grouped gemm", w, x.dtype, device), _dense_of("grouped gemm", bias, (E, N), env[1], device),
+        epilogue | (bias is not None), y.data_ptr(), y_stride, _stream(stream))
+    if rc != 0:
+        _check(rc, "grouped gemm")
+
+
+def w4a16_gemm(x, codes, scale, y, zeros=None, bias=None, epilogue: int = 0, stream=None) -> None:
+    """y = epi(x w^T + bias) with w = (code - zero) * scale (pyc_hip_w4a16_gemm_dispatch): x [M, K]
+    and y [M, N] bf16 or f16, codes [N, K / 2] uint8 (the even k in a byte's low half),
+    scale [N, K / group] of x's type, zeros [N, K / group] uint8 (None: 8), bias [N]
+    float32. epilogue as in grouped_gemm."""
+    env = _moe_env or _make_moe_env()
+    if codes.dim() != 2 or scale.dim() != 2 or y.dim() != 2:
+        _kv_refuse("w4a16 gemm", "codes are [N, K / 2], scale [N, K / group], y [M, columns]")
+    N, K, groups = codes.shape[0], 2 * codes.shape[1], scale.shape[1]
+    suffix, device, x_stride, y_stride = _product("w4a16 gemm", x, y, N, K, epilogue, env)
+    if x.shape[0] != y.shape[0] or groups == 0 or K % groups:
+        _kv_refuse("w4a16 gemm", "sizes do not match")
+    rc = (_lib or lib()).pyc_hip_w4a16_gemm_dispatch(
+        b"hip_gemm_w4a16_" + suffix, x.shape[0], N, K, K // groups, x.data_ptr(), x_stride,
+        _dense_of("w4a16 gemm", codes, (N, K // 2), env[2], device),
+        _dense_of("w4a16 gemm", scale, (N, groups), x.dtype, device),
+        _dense_of("w4a16 gemm", zeros, (N, groups), env[2], device),
+        _dense_of("w4a16 gemm", bias, (N,), env[1], device), epilogue | (bias is not None), y.data_ptr(), y_stride,
+        _stream(stream))
+    if rc != 0:
+        _check(rc, "w4a16 gemm")
+
+
+def w4a16_grouped_gemm(x, codes, scale, offsets, y, zeros=None, rows=None, fan: int = 1, bias=None, epilogue: int = 0,
+                       stream=None) -> None:
+    """grouped_gemm with the weights of w4a16_gemm (pyc_hip_w4a16_grouped_gemm_dispatch): codes
+    [E, N, K / 2], scale and zeros [E, N, K / group], bias [E, N]."""
+    env = _moe_env or _make_moe_env()
+    if codes.dim() != 3 or scale.dim() != 3 or y.dim() != 2:
+        _kv_refuse("w4a16 grouped gemm", "codes are [experts, N, K / 2], scale [experts, N, K / group], y [rows, columns]")
+    E, N, K, groups = codes.shape[0], codes.shape[1], 2 * codes.shape[2], scale.shape[2]
+    suffix, device, x_stride, y_stride = _product("w4a16 grouped gemm", x, y, N, K, epilogue, env)
+    if groups == 0 or K % groups:
+        _kv_refuse("w4a16 grouped gemm", "sizes do not match")
+    i32, P, g = env[0], y.shape[0], (E, N, groups)
+    rc = (_lib or lib()).pyc_hip_w4a16_grouped_gemm_dispatch(
+        b"hip_grouped_gemm_w4a16_" + suffix, E, P, N, K, K // groups, x.data_ptr(), x_stride, x.shape[0],
+        _dense_of("w4a16 grouped gemm", rows, (P,), i32, device), fan,
+        _dense_of("w4a16 grouped gemm", offsets, (E + 1,), i32, device), codes.data_ptr(),
+        _experts("w4a16 grouped gemm", codes, env[2], device), _dense_of("w4a16 grouped gemm", scale, g, x.dtype, device),
+        _dense_of("w4a16 grouped gemm", zeros, g, env[2], device),
+        _dense_of("w4a16 grouped gemm", bias, (E, N), env[1], device), epilogue | (bias is not None), y.data_ptr(),
+        y_stride, _stream(stream))
+    if rc != 0:
+        _check(rc, "w4a16 grouped gemm")
 
 
 def device_info() -> abi.DeviceInfo:

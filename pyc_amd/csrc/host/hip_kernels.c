@@ -19,6 +19,7 @@
 #include "pyc/hip_backend.h"
 #include "pyc/kernel_registry.h"
 #include "pyc_mutex.h"
+#include "../kernels/grouped_args.h"
 #include "../kernels/kernel_info.h"
 
 /* ---------------------------------------------------------------- launchers (.hip) */
@@ -75,11 +76,19 @@ int pyc_hip_kv_attention_launch(int is_bf16, const pyc_hip_kv_cache* cache, int 
                                 int max_len, const void* q, int64_t q_stride, const int32_t* table,
                                 int64_t table_stride, int width, const int32_t* lens, const int32_t* q_offsets,
                                 void* o, int64_t o_stride, float scale, void* workspace, void* stream);
+size_t pyc_hip_moe_route_workspace_bytes(int T, int E);
+int pyc_hip_moe_route_launch(int dtype, int T, int E, int k, int normalize, const void* logits, int64_t stride,
+                             int32_t* ids, float* weights, int32_t* offsets, int32_t* rows, int32_t* places,
+                             void* workspace, void* stream);
+int pyc_hip_moe_combine_launch(int is_bf16, int P, int T, int k, int H, const void* y, int64_t y_stride,
+                               const float* weights, const int32_t* places, const void* base, int64_t base_stride,
+                               void* out, int64_t out_stride, void* stream);
+int pyc_hip_grouped_launch(int is_bf16, int w4, const pyc_grouped* g, void* stream);
 
 /* ---------------------------------------------------------------- variant table */
 
 enum { VK_GEMM = 1, VK_ATTN = 2, VK_CONV = 3, VK_W8 = 4, VK_ELT = 5, VK_CHAIN = 6, VK_KV_PLAN = 7, VK_KV_APPEND = 8,
-       VK_KV_ATTN = 9 };
+       VK_KV_ATTN = 9, VK_ROUTE = 10, VK_COMBINE = 11, VK_GROUPED = 12, VK_W4 = 13, VK_W4_GROUPED = 14 };
 enum { VT_BF16 = 1, VT_F16 = 2, VT_F32 = 3 };
 /* conv2d paths (hip_variant.tile of a VK_CONV entry) */
 enum { CONV_AUTO = 0, CONV_PERSIST = -1, CONV_TILED = 1 };
@@ -154,6 +163,18 @@ static const hip_variant k_variants[] = {
     {"kv_append", "hip_kv_append_f16", VK_KV_APPEND, VT_F16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
     {"kv_attention", "hip_kv_attention_bf16", VK_KV_ATTN, VT_BF16, 0, 0, 0, 100, 3, PYC_KERNEL_WORKLOAD_ANY},
     {"kv_attention", "hip_kv_attention_f16", VK_KV_ATTN, VT_F16, 0, 0, 0, 100, 3, PYC_KERNEL_WORKLOAD_ANY},
+    /* layers of experts and 4-bit weights (no reference counterpart) */
+    {"moe_route", "hip_moe_route_f32", VK_ROUTE, VT_F32, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    {"moe_route", "hip_moe_route_bf16", VK_ROUTE, VT_BF16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    {"moe_route", "hip_moe_route_f16", VK_ROUTE, VT_F16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    {"moe_combine", "hip_moe_combine_bf16", VK_COMBINE, VT_BF16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    {"moe_combine", "hip_moe_combine_f16", VK_COMBINE, VT_F16, 0, 0, 0, 100, 1, PYC_KERNEL_WORKLOAD_ANY},
+    {"grouped_gemm", "hip_grouped_gemm_bf16", VK_GROUPED, VT_BF16, 1, 0, 0, 100, 3, PYC_KERNEL_WORKLOAD_ANY},
+    {"grouped_gemm", "hip_grouped_gemm_f16", VK_GROUPED, VT_F16, 1, 0, 0, 100, 3, PYC_KERNEL_WORKLOAD_ANY},
+    {"matmul_w4a16", "hip_gemm_w4a16_bf16", VK_W4, VT_BF16, 1, 0, 0, 100, 2, PYC_KERNEL_WORKLOAD_WIDE_SKINNY},
+    {"matmul_w4a16", "hip_gemm_w4a16_f16", VK_W4, VT_F16, 1, 0, 0, 100, 2, PYC_KERNEL_WORKLOAD_WIDE_SKINNY},
+    {"grouped_w4a16", "hip_grouped_gemm_w4a16_bf16", VK_W4_GROUPED, VT_BF16, 1, 0, 0, 100, 2, PYC_KERNEL_WORKLOAD_ANY},
+    {"grouped_w4a16", "hip_grouped_gemm_w4a16_f16", VK_W4_GROUPED, VT_F16, 1, 0, 0, 100, 2, PYC_KERNEL_WORKLOAD_ANY},
 };
 
 #define N_VARIANTS (sizeof(k_variants) / sizeof(k_variants[0]))
@@ -196,6 +217,15 @@ static int variant_kinfo(const hip_variant* v, pyc_hip_kinfo* ki) {
             return pyc_hip_kinfo_kv_append(bf, ki);
         case VK_KV_ATTN:
             return pyc_hip_kinfo_kv_attention(bf, ki);
+        case VK_ROUTE:
+            return pyc_hip_kinfo_moe_route(v->dtype == VT_F32 ? 0 : bf ? 1 : 2, ki);
+        case VK_COMBINE:
+            return pyc_hip_kinfo_moe_combine(bf, ki);
+        case VK_GROUPED:
+            return pyc_hip_kinfo_grouped(0, bf, ki);
+        case VK_W4:
+        case VK_W4_GROUPED:
+            return pyc_hip_kinfo_grouped(1, bf, ki);
         default:
             return -1;
     }
@@ -781,6 +811,131 @@ int pyc_hip_kv_attention_dispatch(const char* symbol, const pyc_hip_kv_cache* ca
                                        stream);
 }
 
+/* ---------------------------------------------------------------- layers of experts, 4-bit weights */
+
+enum { MOE_MAX_EXPERTS = 1024, MOE_MAX_K = 64, MOE_MAX_ROWS = 1 << 28, MOE_MAX_DIM = 1 << 24 };
+
+static int aligned(const void* p, size_t n) {
+    return p && ((uintptr_t)p & (n - 1)) == 0;
+}
+
+size_t pyc_hip_moe_route_workspace(int tokens, int experts, int k) {
+    if (tokens < 0 || tokens > MOE_MAX_ROWS / MOE_MAX_K || experts <= 0 || experts > MOE_MAX_EXPERTS || k <= 0 ||
+        k > MOE_MAX_K || k > experts) {
+        return 0;
+    }
+    return pyc_hip_moe_route_workspace_bytes(tokens, experts) + 16; /* never 0 */
+}
+
+int pyc_hip_moe_route_dispatch(const char* symbol, int tokens, int experts, int k, int normalize, const void* logits,
+                               int64_t logits_stride, int32_t* ids, float* weights, int32_t* offsets, int32_t* rows,
+                               int32_t* places, void* workspace, size_t workspace_bytes, void* stream) {
+    const hip_variant* v = find_variant(symbol, VK_ROUTE);
+    const size_t need = pyc_hip_moe_route_workspace(tokens, experts, k);
+    if (!v || need == 0 || !aligned(offsets, 4)) {
+        return -1;
+    }
+    if (tokens > 0 &&
+        (logits_stride < experts || !aligned(logits, v->dtype == VT_F32 ? 4 : 2) || !aligned(ids, 4) ||
+         !aligned(weights, 4) || !aligned(rows, 4) || !aligned(places, 4))) {
+        return -1;
+    }
+    if (need > 16 && (!aligned(workspace, 4) || workspace_bytes < need)) {
+        return -1;
+    }
+    return pyc_hip_moe_route_launch(v->dtype == VT_F32 ? 0 : v->dtype == VT_BF16 ? 1 : 2, tokens, experts, k, normalize != 0,
+                                    logits, logits_stride, ids, weights, offsets, rows, places, workspace, stream);
+}
+
+int pyc_hip_moe_combine_dispatch(const char* symbol, int rows, int tokens, int k, int width, const void* y, int64_t y_stride,
+                                 const float* weights, const int32_t* places, const void* base, int64_t base_stride,
+                                 void* out, int64_t out_stride, void* stream) {
+    const hip_variant* v = find_variant(symbol, VK_COMBINE);
+    if (!v || rows < 0 || rows > MOE_MAX_ROWS || tokens < 0 || tokens > MOE_MAX_ROWS / MOE_MAX_K || k <= 0 ||
+        k > MOE_MAX_K || width <= 0 || width > MOE_MAX_DIM) {
+        return -1;
+    }
+    if (tokens == 0) {
+        return 0;
+    }
+    if ((rows > 0 && (!aligned(y, 2) || y_stride < width)) || !aligned(weights, 4) || !aligned(places, 4) ||
+        (base && (!aligned(base, 2) || base_stride < width)) || !aligned(out, 2) || out_stride < width ||
+        (double)tokens * width >= 0x1p38) {
+        return -1;
+    }
+    return pyc_hip_moe_combine_launch(v->dtype == VT_BF16, rows, tokens, k, width, y, y_stride, weights, places, base,
+                                      base_stride, out, out_stride, stream);
+}
+
+/* What every product by expert refuses. */
+static int grouped_ok(const pyc_grouped* g) {
+    const int gate = g->epi & PYC_HIP_EPI_SILU_GATE;
+    if (g->E <= 0 || g->E > MOE_MAX_EXPERTS || g->P < 0 || g->P > MOE_MAX_ROWS || g->x_rows < 0 ||
+        g->x_rows > MOE_MAX_ROWS || g->N <= 0 || g->N > MOE_MAX_DIM || g->K <= 0 || g->K > MOE_MAX_DIM || g->fan <= 0) {
+        return 0;
+    }
+    if ((g->epi & ~(PYC_HIP_EPI_BIAS | PYC_HIP_EPI_RELU | PYC_HIP_EPI_SILU_GATE)) ||
+        (gate && ((g->epi & PYC_HIP_EPI_RELU) || g->N % 2)) || ((g->epi & PYC_HIP_EPI_BIAS) && !aligned(g->bias, 4))) {
+        return 0;
+    }
+    if (g->P == 0) {
+        return 1;
+    }
+    return (g->x_rows == 0 || (aligned(g->x, 2) && g->x_stride >= g->K)) && aligned(g->w, 2) && aligned(g->y, 2) &&
+           g->y_stride >= (gate ? g->N / 2 : g->N) && ((uintptr_t)g->rows & 3) == 0 && ((uintptr_t)g->offsets & 3) == 0;
+}
+
+int pyc_hip_grouped_gemm_dispatch(const char* symbol, int experts, int rows, int N, int K, const void* x, int64_t x_stride,
+                                  int x_rows, const int32_t* src, int fan, const int32_t* offsets, const void* w,
+                                  int64_t w_stride, const float* bias, int epilogue, void* y, int64_t y_stride,
+                                  void* stream) {
+    const hip_variant* v = find_variant(symbol, VK_GROUPED);
+    const pyc_grouped g = {(const uint16_t*)x, x_stride, x_rows, src, fan, offsets, experts, rows, w, w_stride, N, K,
+                           NULL, NULL, 0, bias, (uint16_t*)y, y_stride, epilogue};
+    if (!v || !grouped_ok(&g) || (experts > 1 && w_stride < (int64_t)N * K)) {
+        return -1;
+    }
+    if (rows == 0) {
+        return 0;
+    }
+    return offsets ? pyc_hip_grouped_launch(v->dtype == VT_BF16, 0, &g, stream) : -1;
+}
+
+static int w4_run(const hip_variant* v, const pyc_grouped* g, void* stream) {
+    if (!v || !grouped_ok(g) || (g->group != 32 && g->group != 64 && g->group != 128) || g->K % g->group != 0 ||
+        (g->E > 1 && (g->w_stride < (int64_t)g->N * (g->K / 2) || g->w_stride % 16 != 0))) {
+        return -1;
+    }
+    if (g->P == 0) {
+        return 0;
+    }
+    if (!aligned(g->w, 16) || !aligned(g->scale, 2) || (g->x_rows > 0 && (!aligned(g->x, 16) || g->x_stride % 8 != 0))) {
+        return -1;
+    }
+    return pyc_hip_grouped_launch(v->dtype == VT_BF16, 1, g, stream);
+}
+
+int pyc_hip_w4a16_gemm_dispatch(const char* symbol, int M, int N, int K, int group, const void* x, int64_t x_stride,
+                                const void* codes, const void* scale, const uint8_t* zeros, const float* bias,
+                                int epilogue, void* y, int64_t y_stride, void* stream) {
+    const pyc_grouped g = {(const uint16_t*)x, x_stride, M, NULL, 1, NULL, 1, M, codes, 0, N, K,
+                           (const uint16_t*)scale, zeros, group, bias, (uint16_t*)y, y_stride, epilogue};
+    return w4_run(find_variant(symbol, VK_W4), &g, stream);
+}
+
+int pyc_hip_w4a16_grouped_gemm_dispatch(const char* symbol, int experts, int rows, int N, int K, int group, const void* x,
+                                        int64_t x_stride, int x_rows, const int32_t* src, int fan,
+                                        const int32_t* offsets, const void* codes, int64_t codes_stride,
+                                        const void* scale, const uint8_t* zeros, const float* bias, int epilogue, void* y,
+                                        int64_t y_stride, void* stream) {
+    const pyc_grouped g = {(const uint16_t*)x, x_stride, x_rows, src, fan, offsets, experts, rows, codes, codes_stride, N, K,
+                           (const uint16_t*)scale, zeros, group, bias, (uint16_t*)y, y_stride, epilogue};
+    if (rows > 0 && !offsets) {
+        return -1;
+    }
+    return w4_run(find_variant(symbol, VK_W4_GROUPED), &g, stream);
+}
+
 /* ---------------------------------------------------------------- registry */
 
 static pyc_mutex g_registry_init_lock = PYC_MUTEX_INIT;
@@ -812,8 +967,9 @@ void pyc_cutlass_registry_init(void) {
                 d.estimated_occupancy = (double)ki.waves_per_simd / 8.0;
                 d.shared_mem_bytes = ki.lds_bytes;
             }
-            /* GELU/LayerNorm and the cache's plan and append: VALU only */
-            d.tensor_core_eligible = v->kind != VK_ELT && v->kind != VK_KV_PLAN && v->kind != VK_KV_APPEND;
+            /* GELU/LayerNorm, the cache's plan and append, the experts' routing and sum: VALU only */
+            d.tensor_core_eligible = v->kind != VK_ELT && v->kind != VK_KV_PLAN && v->kind != VK_KV_APPEND &&
+                                     v->kind != VK_ROUTE && v->kind != VK_COMBINE;
             d.reg_pressure_class = v->reg_class;
             d.preferred_workload_family = v->workload;
             d.preferred_hardware_family = PYC_KERNEL_HARDWARE_CDNA4;

@@ -1,0 +1,77 @@
+// grouped.hpp — what the products by expert share: their operands, the rows of an
+// expert, the row of x behind a row of y, and the epilogue.
+#pragma once
+
+#include "common.hpp"
+#include "grouped_args.h"
+
+namespace pyc {
+
+constexpr int kEpiBias = 1, kEpiRelu = 2, kEpiGate = 4;
+constexpr int kMaxExperts = 1024;
+
+typedef pyc_grouped Grouped;
+
+// Tile t of a grid whose tiles are `step` rows of one expert, expert after expert.
+// offsets are held to 0 .. P and to what came before, so that no row has two experts
+// whatever they say. Every wave finds its tile by itself: 64 experts at a time, a running
+// maximum and a sum over lanes.
+struct ExpertTile {
+    int e, begin, end;  // expert (-1: there is no tile t), the tile's first row, the expert's end
+};
+__device__ inline ExpertTile expert_tile(const Grouped& g, int t, int step, int lane) {
+    if (g.offsets == nullptr) {
+        const int b = t * step;
+        return b < g.P ? ExpertTile{0, b, g.P} : ExpertTile{-1, 0, 0};
+    }
+    int held = 0, before = 0;  // the largest offset so far, tiles so far
+    for (int e0 = 0; e0 < g.E; e0 += kWave) {
+        const int e = e0 + lane;
+        int b = e < g.E ? min(max(g.offsets[e], 0), g.P) : 0;
+        int end = e < g.E ? min(max(g.offsets[e + 1], 0), g.P) : 0;
+        b = max(b, held);
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) {
+            const int o = __shfl_up(b, d);
+            b = lane >= d ? max(b, o) : b;
+        }
+        end = max(end, b);
+        const int n = e < g.E ? (end - b + step - 1) / step : 0;
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) {
+            const int o = __shfl_up(sum, d);
+            sum = lane >= d ? sum + o : sum;
+        }
+        const uint64_t in = __ballot(t < before + sum);
+        if (in) {
+            const int l = __builtin_ctzll(in);
+            const int first = __builtin_amdgcn_readlane(b, l), last = __builtin_amdgcn_readlane(end, l);
+            const int tb = before + __builtin_amdgcn_readlane(sum - n, l);
+            return ExpertTile{e0 + l, first + (t - tb) * step, last};
+        }
+        before += __builtin_amdgcn_readlane(sum, kWave - 1);
+        held = __builtin_amdgcn_readlane(end, kWave - 1);
+    }
+    return ExpertTile{-1, 0, 0};
+}
+
+// Tiles there can be: every expert with rows begins one of its own.
+inline int64_t expert_tiles_most(int E, int P, int step) {
+    return (int64_t)P / step + (E < P ? E : P);
+}
+
+// The row of x behind row p of y, -1 (zeros) where the index is outside x.
+__device__ inline int source_row(const Grouped& g, int p) {
+    int r = p;
+    if (g.rows) {
+        r = g.rows[p];
+        r = r < 0 ? -1 : r / g.fan;
+    }
+    return r < g.x_rows ? r : -1;
+}
+
+// silu(g) * v = g v / (1 + e^-g), in fp32.
+__device__ inline float silu_gate(float g, float v) { return g / (1.0f + __expf(-g)) * v; }
+
+}  // namespace pyc

@@ -1,0 +1,270 @@
+// moe_route.hip — the k experts of each token, their weights, and the order that puts
+// the tokens of one expert together.
+//
+//   chosen_t   the k largest logits of row t, ties to the lower expert; -infinity and NaN
+//              are never chosen (a token may have fewer than k, or none: id -1, weight 0)
+//   weight     e^(l_i - m) / s, m the row's largest, s the sum over all experts or
+//              (normalize) over the chosen ones. m = +infinity: its limit, 1 at each
+//              +infinity and 0 elsewhere, before the division.
+//   offsets    where each expert's rows begin; rows[offsets[e] ..] its flat indexes
+//              t * k + j in ascending order, -1 behind the last expert's;
+//              places[t * k + j] the position of a flat index in rows, -1 without expert.
+//
+// A wave for a token, its logits in registers (E <= 1024: up to 16 a lane). One of the k
+// steps: the largest value by lanes, the lowest expert that has it by ballots, which
+// costs no more with ties. A token takes an expert once, so 32 tokens' choices are one
+// word of bits for each expert: setting bits needs no order, and the rank of a token
+// among its expert's is a count of lower bits. So no sum depends on the order of
+// atomics, and equal inputs give equal outputs.
+// Up to kOneTokens tokens one workgroup does it all; above, the first launch leaves each
+// 32 tokens' words in the workspace and the second adds up the words before its own.
+#include "common.hpp"
+
+namespace pyc {
+
+constexpr int kRouteThreads = 1024;
+constexpr int kRouteWaves = kRouteThreads / kWave;
+constexpr int kRouteBlock = 32;     // tokens to a word
+constexpr int kRouteExperts = 1024;
+constexpr int kOneBlocks = 2;       // blocks one workgroup does alone
+constexpr int kScatterBlocks = 8;   // blocks to a workgroup of the second launch
+
+struct Route {
+    const void* logits;
+    int64_t stride;
+    int T, E, k, normalize;
+    int32_t* ids;
+    float* weights;
+    int32_t* offsets;
+    int32_t* rows;
+    int32_t* places;
+    uint32_t* words;  // [blocks][E]
+};
+
+template <int DT> __device__ inline float route_logit(const void* p, int64_t i) {
+    if constexpr (DT == 0) return static_cast<const float*>(p)[i];
+    else if constexpr (DT == 1) return elem<bf16_t>::to_f32(static_cast<const uint16_t*>(p)[i]);
+    else return elem<f16_t>::to_f32(static_cast<const uint16_t*>(p)[i]);
+}
+
+__device__ inline float wave_max(float v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// One wave: token t's choices, its bit in the block's words (LDS).
+template <int DT, int NV> __device__ inline void route_token(const Route& r, int t, uint32_t* words, int lane) {
+    constexpr float kNone = -INFINITY;
+    float v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = i * kWave + lane;
+        const float l = e < r.E ? route_logit<DT>(r.logits, (int64_t)t * r.stride + e) : kNone;
+        v[i] = l == l ? l : kNone;
+    }
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = fmaxf(m, v[i]);
+    m = wave_max(m);
+    auto power = [&](float l) { return l == m ? 1.0f : expf(l - m); };  // m infinite: 1 or 0
+    float s = 0.f;
+    if (!r.normalize && m > kNone) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) s += v[i] > kNone ? power(v[i]) : 0.f;
+        s = wave_sum(s);
+    }
+    int mine = -1;       // lane j: choice j
+    float p = 0.f;
+    float top = m;
+    for (int j = 0; j < r.k && top > kNone; ++j) {
+        int best = -1;
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i) {
+            const uint64_t is = __ballot(v[i] == top);
+            best = is ? i * kWave + __builtin_ctzll(is) : best;
+        }
+        if (lane == j) {
+            mine = best;
+            p = power(top);
+        }
+        float left = kNone;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i] = i * kWave + lane == best ? kNone : v[i];
+            left = fmaxf(left, v[i]);
+        }
+        top = wave_max(left);
+    }
+    if (r.normalize) s = wave_sum(p);
+    if (lane < r.k) {
+        r.ids[(int64_t)t * r.k + lane] = mine;
+        r.weights[(int64_t)t * r.k + lane] = mine >= 0 ? p / s : 0.f;
+        if (mine >= 0) atomicOr(&words[mine], 1u << (t % kRouteBlock));
+    }
+}
+
+// Exclusive sums over the experts of n[e] (LDS, E of them) into first[], the total returned.
+__device__ inline int route_scan(const int* n, int* first, int E, int* part, int tid) {
+    const int v = tid < E ? n[tid] : 0;  // E <= the workgroup's threads
+    const int lane = tid & 63, wave = tid >> 6;
+    int sum = v;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_up(sum, d);
+        sum = lane >= d ? sum + o : sum;
+    }
+    if (lane == 63) part[wave] = sum;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kRouteWaves; ++w) {
+        before += w < wave ? part[w] : 0;
+        all += part[w];
+    }
+    if (tid < E) first[tid] = before + sum - v;
+    __syncthreads();
+    return all;
+}
+
+// Places and rows of the flat indexes of block b: `first[e]` positions of its experts'
+// rows come before the block's.
+__device__ inline void route_scatter(const Route& r, int b, const uint32_t* words, const int* first, int tid, int threads) {
+    const int t0 = b * kRouteBlock;
+    const int n = min(kRouteBlock, r.T - t0) * r.k;
+    for (int i = tid; i < n; i += threads) {
+        const int64_t f = (int64_t)t0 * r.k + i;
+        const int e = min(r.ids[f], r.E - 1);
+        int at = -1;
+        if (e >= 0) {
+            at = first[e] + __popc(words[e] & ((1u << (i / r.k)) - 1u));
+            // inside rows, whatever a second call on the same workspace left in the words
+            if ((unsigned)at < (unsigned)(r.T * r.k)) r.rows[at] = (int32_t)f;
+        }
+        r.places[f] = at;
+    }
+}
+
+template <int DT, int NV, bool ONE>
+__global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(Route r) {
+    constexpr int BLOCKS = ONE ? kOneBlocks : 1;
+    __shared__ uint32_t words[BLOCKS][NV * kWave];
+    __shared__ int count[NV * kWave], first[NV * kWave], part[kRouteWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int b0 = ONE ? 0 : blockIdx.x;
+    for (int i = tid; i < BLOCKS * NV * kWave; i += kRouteThreads) (&words[0][0])[i] = 0;
+    __syncthreads();
+    const int t0 = b0 * kRouteBlock, t1 = min(r.T, t0 + BLOCKS * kRouteBlock);
+    for (int t = t0 + wave; t < t1; t += kRouteWaves) route_token<DT, NV>(r, t, words[(t - t0) / kRouteBlock], lane);
+    __syncthreads();
+    if constexpr (ONE) {
+        if (tid < r.E) {
+            int n = 0;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) n += __popc(words[b][tid]);
+            count[tid] = n;
+        }
+        __syncthreads();
+        const int all = route_scan(count, first, r.E, part, tid);
+        if (tid < r.E) r.offsets[tid] = first[tid];
+        if (tid == 0) r.offsets[r.E] = all;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            if (b * kRouteBlock < r.T) route_scatter(r, b, words[b], first, tid, kRouteThreads);
+            __syncthreads();
+            if (tid < r.E) first[tid] += __popc(words[b][tid]);
+            __syncthreads();
+        }
+        for (int i = all + tid; i < r.T * r.k; i += kRouteThreads) r.rows[i] = -1;
+    } else {
+        for (int e = tid; e < r.E; e += kRouteThreads) r.words[(int64_t)b0 * r.E + e] = words[0][e];
+    }
+}
+
+__global__ void __launch_bounds__(kRouteThreads) moe_scatter_kernel(Route r, int blocks) {
+    __shared__ int count[kRouteExperts], before[kRouteExperts], first[kRouteExperts], part[kRouteWaves];
+    const int tid = threadIdx.x;
+    const int b0 = blockIdx.x * kScatterBlocks;
+    // threads per expert: as many as there are for it, each a share of the blocks
+    for (int e = tid; e < r.E; e += kRouteThreads) count[e] = before[e] = 0;
+    __syncthreads();
+    const int per = kRouteThreads / r.E;  // >= 1
+    if (tid < per * r.E) {
+        const int e = tid % r.E;
+        int n = 0, own = 0;
+        for (int b = tid / r.E; b < blocks; b += per) {
+            const int c = __popc(r.words[(int64_t)b * r.E + e]);
+            n += c;
+            own += b < b0 ? c : 0;
+        }
+        atomicAdd(&count[e], n);
+        atomicAdd(&before[e], own);
+    }
+    __syncthreads();
+    const int all = route_scan(count, first, r.E, part, tid);
+    if (blockIdx.x == 0) {
+        if (tid < r.E) r.offsets[tid] = first[tid];
+        if (tid == 0) r.offsets[r.E] = all;
+    }
+    if (tid < r.E) first[tid] += before[tid];
+    __syncthreads();
+    for (int b = b0; b < min(blocks, b0 + kScatterBlocks); ++b) {
+        const uint32_t* words = r.words + (int64_t)b * r.E;
+        route_scatter(r, b, words, first, tid, kRouteThreads);
+        __syncthreads();
+        if (tid < r.E) first[tid] += __popc(words[tid]);
+        __syncthreads();
+    }
+    for (int i = all + blockIdx.x * kRouteThreads + tid; i < r.T * r.k; i += gridDim.x * kRouteThreads) r.rows[i] = -1;
+}
+
+template <int DT, int NV> static int route_launch(const Route& r, hipStream_t s) {
+    const int blocks = (r.T + kRouteBlock - 1) / kRouteBlock;
+    if (blocks <= kOneBlocks) {
+        hipLaunchKernelGGL((moe_route_kernel<DT, NV, true>), dim3(1), dim3(kRouteThreads), 0, s, r);
+        return hipGetLastError() == hipSuccess ? 0 : -2;
+    }
+    hipLaunchKernelGGL((moe_route_kernel<DT, NV, false>), dim3(blocks), dim3(kRouteThreads), 0, s, r);
+    hipLaunchKernelGGL(moe_scatter_kernel, dim3((blocks + kScatterBlocks - 1) / kScatterBlocks), dim3(kRouteThreads), 0, s,
+                       r, blocks);
+    return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
+}  // namespace pyc
+
+// Workspace of a call: a word for each expert and 32 tokens where it takes two launches.
+extern "C" size_t pyc_hip_moe_route_workspace_bytes(int T, int E) {
+    const size_t blocks = ((size_t)T + pyc::kRouteBlock - 1) / pyc::kRouteBlock;
+    return blocks <= (size_t)pyc::kOneBlocks ? 0 : blocks * (size_t)E * 4;
+}
+
+extern "C" int pyc_hip_moe_route_launch(int dtype, int T, int E, int k, int normalize, const void* logits, int64_t stride,
+                                        int32_t* ids, float* weights, int32_t* offsets, int32_t* rows, int32_t* places,
+                                        void* workspace, void* stream) {
+    using namespace pyc;
+    const Route r{logits, stride, T, E, k, normalize, ids, weights, offsets, rows, places, (uint32_t*)workspace};
+    const hipStream_t s = (hipStream_t)stream;
+#define PYC_ROUTE(DT)                                       \
+    (E <= 64 ? route_launch<DT, 1>(r, s) : E <= 128 ? route_launch<DT, 2>(r, s) \
+     : E <= 256 ? route_launch<DT, 4>(r, s) : route_launch<DT, 16>(r, s))
+    return dtype == 0 ? PYC_ROUTE(0) : dtype == 1 ? PYC_ROUTE(1) : PYC_ROUTE(2);
+#undef PYC_ROUTE
+}
+
+extern "C" int pyc_hip_kinfo_moe_route(int dtype, pyc_hip_kinfo* out) {
+    using namespace pyc;
+    if (!out) return -1;
+    out->fn = dtype == 0   ? reinterpret_cast<const void*>(&moe_route_kernel<0, 2, false>)
+              : dtype == 1 ? reinterpret_cast<const void*>(&moe_route_kernel<1, 2, false>)
+                           : reinterpret_cast<const void*>(&moe_route_kernel<2, 2, false>);
+    out->name = "moe_route_kernel";
+    out->lds_bytes = 0;
+    out->threads = kRouteThreads;
+    out->waves_per_simd = 8;
+    return 0;
+}
