@@ -12,10 +12,32 @@ constexpr int kMaxExperts = 1024;
 
 typedef pyc_grouped Grouped;
 
+// Inclusive scans over the wave's lanes: four steps in each row of 16, then the rows' last lanes.
+template <int CTRL, int ROWS> __device__ inline int dpp_or(int old, int v) {
+    return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+__device__ inline int scan_add(int v) {
+    v += dpp_or<0x111, 0xf>(0, v);  // row_shr 1, 2, 4, 8
+    v += dpp_or<0x112, 0xf>(0, v);
+    v += dpp_or<0x114, 0xf>(0, v);
+    v += dpp_or<0x118, 0xf>(0, v);
+    v += dpp_or<0x142, 0xa>(0, v);  // lane 15 of a row into the next, rows 1 and 3
+    v += dpp_or<0x143, 0xc>(0, v);  // lane 31 into rows 2 and 3
+    return v;
+}
+__device__ inline int scan_max(int v) {  // of numbers >= 0
+    v = max(v, dpp_or<0x111, 0xf>(0, v));
+    v = max(v, dpp_or<0x112, 0xf>(0, v));
+    v = max(v, dpp_or<0x114, 0xf>(0, v));
+    v = max(v, dpp_or<0x118, 0xf>(0, v));
+    v = max(v, dpp_or<0x142, 0xa>(0, v));
+    v = max(v, dpp_or<0x143, 0xc>(0, v));
+    return v;
+}
+
 // Tile t of a grid whose tiles are `step` rows of one expert, expert after expert.
 // offsets are held to 0 .. P and to what came before, so that no row has two experts
-// whatever they say. Every wave finds its tile by itself: 64 experts at a time, a running
-// maximum and a sum over lanes.
+// whatever they say. Every wave finds its tile by itself, 64 experts at a time.
 struct ExpertTile {
     int e, begin, end;  // expert (-1: there is no tile t), the tile's first row, the expert's end
 };
@@ -27,28 +49,16 @@ __device__ inline ExpertTile expert_tile(const Grouped& g, int t, int step, int 
     int held = 0, before = 0;  // the largest offset so far, tiles so far
     for (int e0 = 0; e0 < g.E; e0 += kWave) {
         const int e = e0 + lane;
-        int b = e < g.E ? min(max(g.offsets[e], 0), g.P) : 0;
-        int end = e < g.E ? min(max(g.offsets[e + 1], 0), g.P) : 0;
-        b = max(b, held);
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-            const int o = __shfl_up(b, d);
-            b = lane >= d ? max(b, o) : b;
-        }
-        end = max(end, b);
-        const int n = e < g.E ? (end - b + step - 1) / step : 0;
-        int sum = n;
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-            const int o = __shfl_up(sum, d);
-            sum = lane >= d ? sum + o : sum;
-        }
+        const int b = scan_max(max(held, e < g.E ? min(g.offsets[e], g.P) : 0));
+        const int end = max(b, e < g.E ? min(g.offsets[e + 1], g.P) : 0);
+        const int n = (end - b + step - 1) / step;
+        const int sum = scan_add(n);
         const uint64_t in = __ballot(t < before + sum);
         if (in) {
             const int l = __builtin_ctzll(in);
             const int first = __builtin_amdgcn_readlane(b, l), last = __builtin_amdgcn_readlane(end, l);
             const int tb = before + __builtin_amdgcn_readlane(sum - n, l);
-            return ExpertTile{e0 + l, first + (t - tb) * step, last};
+            return ExpertTile{__builtin_amdgcn_readfirstlane(e0 + l), first + (t - tb) * step, last};
         }
         before += __builtin_amdgcn_readlane(sum, kWave - 1);
         held = __builtin_amdgcn_readlane(end, kWave - 1);

@@ -159,9 +159,13 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
 
 }  // namespace pyc
 
+extern "C" int pyc_hip_grouped_stream_takes(int w4, const pyc_grouped* g);
+extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, int w4, const pyc_grouped* g, void* stream);
+
 extern "C" int pyc_hip_grouped_launch(int is_bf16, int w4, const pyc_grouped* gp, void* stream) {
     using namespace pyc;
     const Grouped& g = *gp;
+    if ((int64_t)g.P <= 16 * (int64_t)g.E && pyc_hip_grouped_stream_takes(w4, gp)) return pyc_hip_grouped_stream_launch(is_bf16, w4, gp, stream);
     const int cols = g.epi & kEpiGate ? g.N / 2 : g.N, per = g.epi & kEpiGate ? kGenTile / 2 : kGenTile;
     const int tiles_n = (cols + per - 1) / per;
     const int64_t tiles = expert_tiles_most(g.offsets ? g.E : 1, g.P, kGenTile) * tiles_n;
