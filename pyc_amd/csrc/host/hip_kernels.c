@@ -222,10 +222,10 @@ static int variant_kinfo(const hip_variant* v, pyc_hip_kinfo* ki) {
         case VK_COMBINE:
             return pyc_hip_kinfo_moe_combine(bf, ki);
         case VK_GROUPED:
-            return pyc_hip_kinfo_grouped(0, bf, ki);
+            return pyc_hip_kinfo_grouped_ring(bf, ki);
         case VK_W4:
         case VK_W4_GROUPED:
-            return pyc_hip_kinfo_grouped(1, bf, ki);
+            return pyc_hip_kinfo_grouped_w4(bf, ki);
         default:
             return -1;
     }

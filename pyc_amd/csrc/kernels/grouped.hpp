@@ -81,7 +81,21 @@ __device__ inline int source_row(const Grouped& g, int p) {
     return r < g.x_rows ? r : -1;
 }
 
-// silu(g) * v = g v / (1 + e^-g), in fp32.
-__device__ inline float silu_gate(float g, float v) { return g / (1.0f + __expf(-g)) * v; }
+// w[i] of lane group g becomes w[g] of lane group i.
+__device__ inline void transpose4(u32x4& w) {
+    auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+    auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    w = u32x4{c[0], c[1], d[0], d[1]};
+}
+
+// v of the lane eight further on in each row of 16, around its end.
+__device__ inline float row_half_turn(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
+}
+
+// silu(g) * v = g v / (1 + e^-g), in fp32; the reciprocal is off by at most one of its steps.
+__device__ inline float silu_gate(float g, float v) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * v; }
 
 }  // namespace pyc

@@ -1,35 +1,52 @@
-// grouped_gemm.hip — products grouped by expert, any size and alignment.
+// grouped_gemm.hip — products grouped by expert: which kernel runs a call, and the one for any
+// size and alignment.
 //
 //   y[p] = epi(x[src(p)] W[e]^T + bias[e])   for offsets[e] <= p < offsets[e + 1]
 //
 // with W 16-bit values, or 4-bit codes with a scale (and zero point) for each group
-// along K. fp32 sums. A workgroup has 64 rows of one expert and 64 columns, four waves as
-// 2 x 2, operands through registers into LDS (16-byte chunk c of row r at c ^ (r % 8)). The
+// along K. fp32 sums. The general kernel: a workgroup has 64 rows of one expert and 64 columns, four waves as
+// 2 x 2, operands two steps ahead through registers into LDS (16-byte chunk c of row r at c ^ (r % 8)). The
 // rows of x are the first operand of the matrix instruction, so a lane's four results are
 // four rows of one column, and a column's scale is one value for each lane. Codes less
 // their zero point are whole numbers of at most 8 bits, exact in 16-bit values: each
 // 32 k of them (a group has 32, 64 or 128) are summed apart, then scaled into the sums
 // in fp32. Gated: fragments of a wave alternate, 16 gates and the 16 values of the same
-// columns, so that a lane has both.
+// columns, so that a lane has both. Rows at odd places are loaded as 16 unaligned bytes; what would
+// cross the end of its row is loaded up to there and shifted.
 #include "grouped.hpp"
 
 namespace pyc {
 
 constexpr int kGenTile = 64, kGenK = 64;
 
-// Eight elements from p, 0 behind `left` of them (p is not read there).
-__device__ inline u32x4 load_guarded(const uint16_t* p, int left, bool wide) {
-    if (wide && left >= 8) return *reinterpret_cast<const u32x4*>(p);
-    uint16_t e[8];
+// Elements c .. c + 7 of a row of K, 0 behind its end. `edge` (uniform): some lane's reach past it.
+__device__ inline u32x4 row_piece(const uint16_t* row, int c, int K, bool edge) {
+    u32x4 v = u32x4{0, 0, 0, 0};
+    if (!edge) {
+        __builtin_memcpy(&v, row + c, 16);
+    } else if (K >= 8) {
+        const int from = min(c, K - 8), sh = c - from;  // elements of it that come before c
+        __builtin_memcpy(&v, row + from, 16);
+        uint64_t lo = (uint64_t)v[0] | ((uint64_t)v[1] << 32), hi = (uint64_t)v[2] | ((uint64_t)v[3] << 32);
+        lo = sh >= 4 ? hi : lo;
+        hi = sh >= 4 ? 0 : hi;
+        const int b = 16 * (sh & 3);
+        lo = (lo >> b) | ((hi << 1) << (63 - b));
+        hi >>= b;
+        if (sh >= 8) lo = hi = 0;
+        v = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    } else {
+        uint16_t e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < left ? p[i] : (uint16_t)0;
-    return u32x4{e[0] | ((uint32_t)e[1] << 16), e[2] | ((uint32_t)e[3] << 16), e[4] | ((uint32_t)e[5] << 16),
-                 e[6] | ((uint32_t)e[7] << 16)};
+        for (int i = 0; i < 8; ++i) e[i] = c + i < K ? row[c + i] : (uint16_t)0;
+        __builtin_memcpy(&v, e, 16);
+    }
+    return v;
 }
 
 template <typename T, bool W4>
-__global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int tiles_n, int wide) {
-    __shared__ __attribute__((aligned(16))) uint16_t Xs[kGenTile * kGenK], Ws[kGenTile * kGenK];
+__global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int tiles_n) {
+    __shared__ __attribute__((aligned(16))) uint16_t Xs[2][kGenTile * kGenK], Ws[2][kGenTile * kGenK];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave >> 1, wn = wave & 1, lrow = lane & 15, lgrp = lane >> 4;
     const int tn = blockIdx.x % tiles_n;
@@ -48,13 +65,17 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
     // 16 of the 64 k
     const int row0 = tid >> 3, ch = tid & 7;
     const uint16_t* xr[2];
-    int wr[2];
+    const uint16_t* wr[2];
+    bool xin[2];
+    const int64_t ew = (int64_t)t.e * g.w_stride;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+        // rows that there are not are read from the first one; x's count as zeros, W's reach no result
         const int p = t.begin + row0 + 32 * i;
         const int r = p < t.end ? source_row(g, p) : -1;
-        xr[i] = r < 0 ? nullptr : g.x + (int64_t)r * g.x_stride;
-        wr[i] = weight_row(row0 + 32 * i);
+        xin[i] = r >= 0;
+        xr[i] = g.x_rows > 0 ? g.x + (int64_t)max(r, 0) * g.x_stride : static_cast<const uint16_t*>(g.w);
+        wr[i] = static_cast<const uint16_t*>(g.w) + ew + (int64_t)max(weight_row(row0 + 32 * i), 0) * g.K;
     }
     const int crow = weight_row(tid >> 2);
     auto slot = [](int r, int c) { return r * kGenK + ((c ^ (r & 7)) << 3); };
@@ -68,50 +89,55 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
 #pragma unroll
     for (int j = 0; j < 2; ++j) col[j] = weight_row(wn * 32 + j * 16 + lrow);
 
-    const int64_t ew = (int64_t)t.e * g.w_stride;
     const int groups = W4 ? g.K / g.group : 0;
-    for (int k0 = 0; k0 < g.K; k0 += kGenK) {
+    // a step's chunks as loaded: two steps ahead of the one that is multiplied
+    struct Step {
         u32x4 a[2], b[2];
+        uint64_t q;
+        int z;
+    };
+    auto load = [&](Step& s, int k0) {
+        const bool edge = k0 + kGenK > g.K;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int left = g.K - k0 - 8 * ch;
-            a[i] = xr[i] ? load_guarded(xr[i] + k0 + 8 * ch, left, wide & 1) : u32x4{0, 0, 0, 0};
-            if constexpr (!W4)
-                b[i] = wr[i] >= 0 ? load_guarded(static_cast<const uint16_t*>(g.w) + ew + (int64_t)wr[i] * g.K + k0 + 8 * ch,
-                                                 left, wide & 2)
-                                  : u32x4{0, 0, 0, 0};
+            s.a[i] = row_piece(xr[i], k0 + 8 * ch, g.K, edge);
+            if constexpr (!W4) s.b[i] = row_piece(wr[i], k0 + 8 * ch, g.K, edge);
         }
         if constexpr (W4) {
             const int k = k0 + 16 * (tid & 3);
-            uint64_t q = 0x8888888888888888ull;
-            int z = 8;
+            s.q = 0x8888888888888888ull;
+            s.z = 8;
             if (crow >= 0 && k < g.K) {
-                q = *reinterpret_cast<const uint64_t*>(static_cast<const uint8_t*>(g.w) + ew + (int64_t)crow * (g.K / 2) + k / 2);
-                if (g.zeros) z = g.zeros[((int64_t)t.e * g.N + crow) * groups + k / g.group];
+                s.q = *reinterpret_cast<const uint64_t*>(static_cast<const uint8_t*>(g.w) + ew + (int64_t)crow * (g.K / 2) + k / 2);
+                if (g.zeros) s.z = g.zeros[((int64_t)t.e * g.N + crow) * groups + k / g.group];
             }
+        }
+    };
+    auto store = [&](Step& s, int buf) {
+        if constexpr (W4) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int lo = (int)(q >> (32 * i + 8 * j)) & 15, hi = (int)(q >> (32 * i + 8 * j + 4)) & 15;
-                    b[i][j] = elem<T>::from_f32((float)(lo - z)) | ((uint32_t)elem<T>::from_f32((float)(hi - z)) << 16);
+                    const int lo = (int)(s.q >> (32 * i + 8 * j)) & 15, hi = (int)(s.q >> (32 * i + 8 * j + 4)) & 15;
+                    s.b[i][j] = elem<T>::from_f32((float)(lo - s.z)) | ((uint32_t)elem<T>::from_f32((float)(hi - s.z)) << 16);
                 }
         }
-        __syncthreads();  // the step before is read
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            *reinterpret_cast<u32x4*>(&Xs[slot(row0 + 32 * i, ch)]) = a[i];
-            if constexpr (W4) *reinterpret_cast<u32x4*>(&Ws[slot(tid >> 2, 2 * (tid & 3) + i)]) = b[i];
-            else *reinterpret_cast<u32x4*>(&Ws[slot(row0 + 32 * i, ch)]) = b[i];
+            *reinterpret_cast<u32x4*>(&Xs[buf][slot(row0 + 32 * i, ch)]) = xin[i] ? s.a[i] : u32x4{0, 0, 0, 0};
+            if constexpr (W4) *reinterpret_cast<u32x4*>(&Ws[buf][slot(tid >> 2, 2 * (tid & 3) + i)]) = s.b[i];
+            else *reinterpret_cast<u32x4*>(&Ws[buf][slot(row0 + 32 * i, ch)]) = s.b[i];
         }
-        __syncthreads();
+    };
+    auto multiply = [&](int k0, int buf) {
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             u32x4 fa[2], fb[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                fa[i] = *reinterpret_cast<const u32x4*>(&Xs[slot(wm * 32 + i * 16 + lrow, kk * 4 + lgrp)]);
-                fb[i] = *reinterpret_cast<const u32x4*>(&Ws[slot(wn * 32 + i * 16 + lrow, kk * 4 + lgrp)]);
+                fa[i] = *reinterpret_cast<const u32x4*>(&Xs[buf][slot(wm * 32 + i * 16 + lrow, kk * 4 + lgrp)]);
+                fb[i] = *reinterpret_cast<const u32x4*>(&Ws[buf][slot(wn * 32 + i * 16 + lrow, kk * 4 + lgrp)]);
             }
             if constexpr (W4) {
                 const int k = k0 + 32 * kk;
@@ -134,6 +160,19 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
                     for (int j = 0; j < 2; ++j) acc[i][j] = mfma16x16x32(fa[i], fb[j], acc[i][j], T{});
             }
         }
+    };
+    Step s0, s1;
+    load(s0, 0);
+    load(s1, kGenK);
+    for (int k0 = 0; k0 < g.K; k0 += 2 * kGenK) {  // k past K is zeros
+        store(s0, 0);
+        load(s0, k0 + 2 * kGenK);
+        __syncthreads();
+        multiply(k0, 0);
+        store(s1, 1);
+        load(s1, k0 + 3 * kGenK);
+        __syncthreads();
+        multiply(k0 + kGenK, 1);
     }
 
     float bias[2];
@@ -160,21 +199,56 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
 }  // namespace pyc
 
 extern "C" int pyc_hip_grouped_stream_takes(int w4, const pyc_grouped* g);
-extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, int w4, const pyc_grouped* g, void* stream);
+extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, const pyc_grouped* g, void* stream);
+extern "C" int pyc_hip_grouped_tile_takes(const pyc_grouped* g);
+extern "C" int pyc_hip_grouped_tile_launch(int is_bf16, const pyc_grouped* g, void* stream);
+extern "C" int pyc_hip_grouped_ring_launch(int is_bf16, const pyc_grouped* g, int fn, void* stream);
+extern "C" int pyc_hip_grouped_w4_tile_launch(int is_bf16, const pyc_grouped* g, int form, void* stream);
+
+// The kernel of a call, from what the host knows: rows in all, not whose they are. Measured on the MI355X
+// over experts of K x N with P rows in all, in us (other side behind the stroke):
+//  16-bit: the ring's tiles of 64 rows x 64 columns; of 128 columns where those fill the CUs twice (8 of
+//    4096 x 4096: P = 256 62 / 74, 1024 87 / 98); 256 x 256 tiles from some 200 rows an expert on, or
+//    100 in large calls (8 of 4096 x 4096: P = 2048 111 / 129, 1024 109 / 87; 64 of 2048 x 2816: P = 8192 207 / 292).
+//  4-bit: streamed up to 16 rows an expert (dense: 32); then the smallest tiles that are no more than 3 in
+//    two places (4096 x 11008: P = 64 27 / 34 streamed, 512 108 / 217 in tiles of 16 rows; 2048 x 1024: P = 512
+//    15 / 18 in tiles of 64), and 128 x 256 from 96 rows an expert on in large calls (4096 x
+//    11008: P = 256 99 / 57, 512 103 / 108; 32 of 4096 x 2816: P = 4096 222 / 287).
+// KIND: 0 the general kernel, 1 ring, 2 tiles, 3 stream, 4 4-bit tiles; arg: what its launch takes.
+extern "C" int pyc_hip_grouped_form(int w4, const pyc_grouped* g, int* arg) {
+    using namespace pyc;
+    const int64_t P = g->P, E = g->offsets ? g->E : 1, N = g->N;
+    *arg = 0;
+    if (!pyc_hip_grouped_stream_takes(w4, g)) return 0;
+    if (!w4) {
+        if (pyc_hip_grouped_tile_takes(g) && ((P >= 192 * E && P * N >= 1 << 23) || (P >= 96 * E && P * N >= 1 << 24))) return 2;
+        *arg = P * N >= 512 * 4096 ? 2 : 1;
+        return 1;
+    }
+    if (P <= 16 * E || P <= 32) return 3;
+    if (P >= 96 * E && P * N >= 170 * 128 * 256) return 4;
+    const int64_t blocks = (N + 63) / 64;
+    *arg = expert_tiles_most((int)E, g->P, 16) * blocks <= 384 ? 1 : expert_tiles_most((int)E, g->P, 32) * blocks <= 384 ? 2 : 4;
+    return 4;
+}
 
 extern "C" int pyc_hip_grouped_launch(int is_bf16, int w4, const pyc_grouped* gp, void* stream) {
     using namespace pyc;
     const Grouped& g = *gp;
-    if ((int64_t)g.P <= 16 * (int64_t)g.E && pyc_hip_grouped_stream_takes(w4, gp)) return pyc_hip_grouped_stream_launch(is_bf16, w4, gp, stream);
+    int arg;
+    switch (pyc_hip_grouped_form(w4, gp, &arg)) {
+        case 1: return pyc_hip_grouped_ring_launch(is_bf16, gp, arg, stream);
+        case 2: return pyc_hip_grouped_tile_launch(is_bf16, gp, stream);
+        case 3: return pyc_hip_grouped_stream_launch(is_bf16, gp, stream);
+        case 4: return pyc_hip_grouped_w4_tile_launch(is_bf16, gp, arg, stream);
+    }
     const int cols = g.epi & kEpiGate ? g.N / 2 : g.N, per = g.epi & kEpiGate ? kGenTile / 2 : kGenTile;
     const int tiles_n = (cols + per - 1) / per;
     const int64_t tiles = expert_tiles_most(g.offsets ? g.E : 1, g.P, kGenTile) * tiles_n;
     if (tiles > 0x7FFFFFFF) return -1;
-    const int wide = (g.x_stride % 8 == 0 && ((uintptr_t)g.x & 15) == 0 ? 1 : 0) |
-                     (g.K % 8 == 0 && g.w_stride % 8 == 0 && ((uintptr_t)g.w & 15) == 0 ? 2 : 0);
     const dim3 grid((unsigned)tiles), block(256);
     const hipStream_t s = (hipStream_t)stream;
-#define PYC_GENERAL(TY, W) hipLaunchKernelGGL((grouped_general_kernel<TY, W>), grid, block, 0, s, g, tiles_n, wide)
+#define PYC_GENERAL(TY, W) hipLaunchKernelGGL((grouped_general_kernel<TY, W>), grid, block, 0, s, g, tiles_n)
     if (w4) {
         if (is_bf16) PYC_GENERAL(bf16_t, true);
         else PYC_GENERAL(f16_t, true);
@@ -184,18 +258,4 @@ extern "C" int pyc_hip_grouped_launch(int is_bf16, int w4, const pyc_grouped* gp
     }
 #undef PYC_GENERAL
     return hipGetLastError() == hipSuccess ? 0 : -2;
-}
-
-extern "C" int pyc_hip_kinfo_grouped(int w4, int is_bf16, pyc_hip_kinfo* out) {
-    using namespace pyc;
-    if (!out) return -1;
-    out->fn = w4 ? (is_bf16 ? reinterpret_cast<const void*>(&grouped_general_kernel<bf16_t, true>)
-                            : reinterpret_cast<const void*>(&grouped_general_kernel<f16_t, true>))
-                 : (is_bf16 ? reinterpret_cast<const void*>(&grouped_general_kernel<bf16_t, false>)
-                            : reinterpret_cast<const void*>(&grouped_general_kernel<f16_t, false>));
-    out->name = "grouped_general_kernel";
-    out->lds_bytes = 2 * kGenTile * kGenK * 2;
-    out->threads = 256;
-    out->waves_per_simd = 8;
-    return 0;
 }

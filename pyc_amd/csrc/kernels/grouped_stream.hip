@@ -1,20 +1,26 @@
-// grouped_stream.hip — products by expert where an expert has few rows: single tokens and
-// decoding batches, with 16-bit weights or 4-bit ones. What bounds them is the stream of
-// the weights, every byte of which is used once.
+// grouped_stream.hip — products by expert with 4-bit weights where an expert has few rows: single
+// tokens and decoding batches. What bounds them is the stream of the weights, every byte of
+// which is used once, and the vector instructions that unpack them.
 //
-// A workgroup has 16 CF rows of one expert's W and up to 16 MT rows of x, over all of K: its
-// eight waves take every eighth chunk of 128 k and are added up through LDS at the end, in
-// a fixed order, so that a layer of a few thousand columns fills 256 CUs without a second
-// launch. W goes from memory into registers as the operand it is (16 rows of 64 bytes to an
-// instruction, two chunks in flight), through buffer descriptors: rows and k past the end,
-// rows of x that are not there and chunks past the last read zeros and cost no traffic.
+// A wave has 32 rows of one expert's W (two fragments; gated: of gates, and of the same
+// columns' values) and up to 16 rows of x. The eight waves of a workgroup take `ks` parts of
+// K for 8 / ks such column blocks: parts of the same columns take every ks-th chunk of 128 k
+// and are added up through LDS, in order, so that few columns still fill the CUs without a
+// second launch. W goes from memory into registers as the operand it is, several chunks ahead,
+// through buffer descriptors: rows and k past the end read zeros and cost no traffic.
+//
+// A load instruction costs a wave about 375 cycles here whatever it brings (x, scales and zero
+// points loaded beside W, 10 loads to a chunk: 3700 cycles a chunk). So a wave loads W alone: the rows of x
+// and the scales and zero points of the workgroup's columns go through LDS, as much of K at a
+// time as fits. Where x would take turns (each stops all waves), only the scales do, and x is
+// loaded beside W (23 tokens, 11008 x 4096: 42 us in turns, 25 beside).
+//
 // The rows of x are the first operand: a lane's results are four rows of one column of y, so
-// a column's scale is one value for each lane.
-//
-// 4-bit: a lane's 16 bytes are 32 k of a row, the four lanes of a row 128 k. A 4 x 4
+// a column's scale is one value for each lane. A lane's 16 bytes of W are 32 k of a row, the
+// four lanes of a row 128 k. A 4 x 4
 // transposition between the lanes and their four words (four swaps) gives each product 32
 // neighbouring k, so that groups of 32, 64 and 128 all work. A code c goes into the
-// mantissa of 16, as 16 + c exactly, two to an instruction and nearly for free; a group's sum is then
+// mantissa of 16, as 16 + c exactly, two to two instructions; a group's sum is then
 //   scale (sum x (16 + c) - (16 + zero) sum x),
 // all in fp32, with sum x from one more product by ones. (By conversion to whole numbers less
 // zero a pair takes three to four times the instructions. 128 + c, which needs a shift less, has
@@ -24,268 +30,256 @@
 namespace pyc {
 
 constexpr int kStreamWaves = 8;
-constexpr int kStreamK = 128;  // k of a chunk
+constexpr int kStreamThreads = kStreamWaves * kWave;
+constexpr int kStreamK = 128;               // k of a chunk
+// LDS: x, then scales and zero points as one word; the sums of the parts of K reuse x's. The smaller of each
+// pair keeps two workgroups to a CU; where there are no more workgroups than CUs, one may have it all.
+struct StreamLds {
+    int x, scales;  // bytes for x, words
+};
+constexpr StreamLds kStreamLds[2][2] = {{{63 * 1024, 4096}, {111 * 1024, 12032}}, {{16 * 1024, 15872}, {16 * 1024, 36352}}};
+constexpr size_t stream_lds_bytes(const StreamLds& l) { return l.x + 4 * l.scales; }
 constexpr uint32_t kPastEnd = 0xFFFFFFF0u;  // not below any descriptor's byte count
 
-// w[i] of lane group g becomes w[g] of lane group i.
-__device__ inline void transpose4(u32x4& w) {
-    auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-    auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-    auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
-    auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-    w = u32x4{c[0], c[1], d[0], d[1]};
-}
-
 // Eight codes as 16 + c, pairs k 0,4 1,5 2,6 3,7.
-__device__ inline u32x4 codes16(uint32_t w, bf16_t) {
-    constexpr uint32_t m = 0x00780078u, b = 0x41804180u;  // 16.0, 3 bits below its units
+__device__ inline u32x4 codes16(uint32_t w, uint32_t m, uint32_t b, bf16_t) {  // 3 bits below the units of 16.0
     return u32x4{((w << 3) & m) | b, ((w >> 1) & m) | b, ((w >> 5) & m) | b, ((w >> 9) & m) | b};
 }
-__device__ inline u32x4 codes16(uint32_t w, f16_t) {
-    constexpr uint32_t m = 0x03c003c0u, b = 0x4c004c00u;  // 16.0, 6 bits below its units
+__device__ inline u32x4 codes16(uint32_t w, uint32_t m, uint32_t b, f16_t) {  // 6 bits
     return u32x4{((w << 6) & m) | b, ((w << 2) & m) | b, ((w >> 2) & m) | b, ((w >> 6) & m) | b};
 }
+__device__ inline uint32_t codes16_mask(bf16_t) { return 0x00780078u; }
+__device__ inline uint32_t codes16_mask(f16_t) { return 0x03c003c0u; }
 __device__ inline u32x4 paired(const u32x4& x) {
     return u32x4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
                  __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
 }
-template <typename T> __device__ inline u32x4 ones() {
-    const uint32_t o = elem<T>::from_f32(1.0f) * 0x10001u;
-    return u32x4{o, o, o, o};
-}
 
-// G: k of a group (0: 16-bit weights)
-template <int G, int CF, int MT> struct Chunk {
-    static constexpr int kGroups = G ? kStreamK / G : 1;
-    u32x4 w[CF][G ? 1 : 4];
-    u32x4 x[MT][4];
-    uint64_t s[G ? CF : 1];  // the chunk's scales and zero points, the first ones lowest
-    uint32_t z[G ? CF : 1];
-};
+// G: k of a group. XD: x is loaded beside W. tiles_n: column blocks, wgs: workgroups they take.
+template <typename T, int G, bool XD>
+__global__ void __launch_bounds__(kStreamThreads, 4)
+grouped_stream_kernel(Grouped g, int tiles_n, int wgs, int ks, int x_lds, int words) {
+    constexpr int CF = 2;
+    constexpr int NG = kStreamK / G;       // groups to a chunk
+    constexpr int AHEAD = XD ? 2 : 4;      // chunks in registers
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ int64_t src[16];
+    static_assert(kStreamWaves * CF * kWave * 16 <= kStreamLds[1][0].x, "sums through x's LDS");
+    uint32_t* const sz = reinterpret_cast<uint32_t*>(smem + x_lds);  // [group][column of the workgroup]: scale, zero point << 16
 
-// `n` values of type V from v[at], the first one lowest; what lies behind v[last] reads 0.
-// One load at any alignment, moved back where it would pass the end (last >= n).
-template <typename R, int n, typename V> __device__ inline R load_values(const V* v, uint32_t at, uint32_t last) {
-    const uint32_t from = min(at, last - n);
-    R r = 0;
-    __builtin_memcpy(&r, v + from, n * sizeof(V));
-    if constexpr (n > 1) {
-        const uint32_t d = 8 * sizeof(V) * min(at - from, (uint32_t)(n - 1));
-        r >>= d;
-    }
-    return r;
-}
-
-template <typename T, int G, int CF, int MT>
-__global__ void __launch_bounds__(kStreamWaves * kWave, MT * CF <= 2 ? 4 : 2)
-grouped_stream_kernel(Grouped g, int tiles_n, int wgs, int ks) {
-    constexpr bool W4 = G != 0;
-    typedef Chunk<G, CF, MT> C;
-    __shared__ f32x4 red[kStreamWaves][MT][CF][kWave];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lrow = lane & 15, lgrp = lane >> 4;
-    const int kp = wave & (ks - 1);                                     // this wave's part of K
-    const int tn = (blockIdx.x % wgs) * (kStreamWaves / ks) + wave / ks;  // its columns
-    const ExpertTile t = expert_tile(g, blockIdx.x / wgs, 16 * MT, lane);
+    const int units = kStreamWaves / ks;                     // column blocks of the workgroup
+    const int kp = wave & (ks - 1), unit = wave / ks;        // this wave's part of K and block
+    const int tn0 = (blockIdx.x % wgs) * units, tn = tn0 + unit;
+    const ExpertTile t = expert_tile(g, blockIdx.x / wgs, 16, lane);
     if (t.e < 0) return;
+    const int rows = min(t.end - t.begin, 16);
     const bool gate = g.epi & kEpiGate;
     const int F = gate ? g.N / 2 : g.N;
-    const int half = gate ? CF / 2 : CF;  // fragments of columns of y
-    // the row of W behind column lrow of fragment f (N: none)
-    auto weight_row = [&](int f) {
-        const int c = (tn * half + (f < half ? f : f - half)) * 16 + lrow;
-        return c < F ? (f < half ? c : c + F) : g.N;
+    // the row of W behind column c (0 .. 31) of block b, g.N: none
+    auto weight_row = [&](int b, int c) __attribute__((always_inline)) {
+        const int y = gate ? b * 16 + (c & 15) : b * 32 + c;
+        return y < F ? (gate && c >= 16 ? y + F : y) : g.N;
     };
-
-    const uint32_t row_bytes = W4 ? (uint32_t)g.K / 2 : (uint32_t)g.K * 2;
-    const int groups = W4 ? g.K / (W4 ? G : 1) : 0;
     const int chunks = (g.K + kStreamK - 1) / kStreamK;
-    const int whole = g.K / kStreamK;
-    // A chunk's place is the scalar part of a load's offset, which the descriptor's check leaves out. So the
-    // last chunk, where K is no multiple of 128, has lane offsets of its own, past the end for k
-    // past K, and chunks behind it a descriptor of no bytes.
-    void* const wbase = const_cast<char*>(static_cast<const char*>(g.w)) + (int64_t)t.e * g.w_stride * (W4 ? 1 : 2);
+    const int groups = g.K / G;
+
+    // W: a chunk's place is the scalar part of a load's offset, which the descriptor's check leaves out. So the
+    // last chunk, where K is no multiple of 128, has lane offsets past the end for k past K, and
+    // chunks behind it a descriptor of no bytes.
+    const uint32_t row_bytes = (uint32_t)g.K / 2;
+    void* const wbase = const_cast<char*>(static_cast<const char*>(g.w)) + (int64_t)t.e * g.w_stride;
     const uint32_t wbytes = tn < tiles_n ? (uint32_t)g.N * row_bytes : 0u;
-    const uint32_t xbytes = (uint32_t)(((int64_t)(g.x_rows - 1) * g.x_stride + g.K) * 2);
-    const int left = g.K - whole * kStreamK;
-    uint32_t wo[CF], xo[MT], so[CF];
+    const int whole = g.K / kStreamK, left = g.K - whole * kStreamK;
+    uint32_t wo[CF];
 #pragma unroll
     for (int f = 0; f < CF; ++f) {
-        const int r = weight_row(f);
+        const int r = weight_row(tn, 16 * f + lrow);
         wo[f] = r < g.N ? (uint32_t)r * row_bytes + 16 * lgrp : kPastEnd;
-        so[f] = (uint32_t)min(r, g.N - 1) * (uint32_t)groups;
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int p = t.begin + 16 * m + lrow;
-        const int r = p < t.end ? source_row(g, p) : -1;
-        xo[m] = r < 0 ? kPastEnd : (uint32_t)((int64_t)r * g.x_stride * 2) + 16 * lgrp;
-    }
-    const uint16_t* scale = W4 ? g.scale + (int64_t)t.e * g.N * groups : nullptr;
-    // without zero points their loads take the scales' places, and what comes is not used: a branch
-    // around loads would make every wait one for all of them
-    const bool has_zeros = W4 && g.zeros != nullptr;
-    const uint8_t* zeros = !W4 ? nullptr : has_zeros ? g.zeros + (int64_t)t.e * g.N * groups : reinterpret_cast<const uint8_t*>(scale);
-
-    auto load = [&](C& c, int i) {
-        const auto wr = __builtin_amdgcn_make_buffer_rsrc(wbase, 0, i < chunks ? wbytes : 0u, 0x00020000);
-        const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.x), 0, i < chunks ? xbytes : 0u, 0x00020000);
-        const int end = i == whole ? left : kStreamK;  // k of the chunk that there are
-        const uint32_t at = (uint32_t)i * kStreamK;
-        auto get = [&](const __amdgpu_buffer_rsrc_t& r, uint32_t off, uint32_t s) {
-            return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, s, 0));
-        };
-#pragma unroll
-        for (int f = 0; f < CF; ++f) {
-            if constexpr (W4) {
-                c.w[f][0] = get(wr, 32 * lgrp < end ? wo[f] : kPastEnd, at / 2);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) c.w[f][j] = get(wr, 32 * j + 8 * lgrp < end ? wo[f] : kPastEnd, at * 2 + 64 * j);
-            }
-        }
-        if constexpr (W4) {
-#pragma unroll
-            for (int f = 0; f < CF; ++f) {
-                const uint32_t q = so[f] + (uint32_t)min(i, chunks - 1) * C::kGroups, all = (uint32_t)(g.N * groups);
-                c.s[f] = load_values<uint64_t, C::kGroups>(scale, q, all);
-                const uint32_t z = load_values<uint32_t, C::kGroups>(zeros, has_zeros ? q : 2 * q, has_zeros ? all : 2 * all);
-                c.z[f] = has_zeros ? z : 0x08080808u;
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) c.x[m][j] = get(xr, 32 * j + 8 * lgrp < end ? xo[m] : kPastEnd, at * 2 + 64 * j);
+    struct Chunk {
+        u32x4 w[CF], x[XD ? 4 : 1];
     };
-
-    f32x4 acc[MT][CF];
+    uint32_t xo = kPastEnd;  // XD: of the lane's row
+    uint32_t xbytes = 0;
+    if constexpr (XD) {
+        const int r = lrow < rows ? source_row(g, t.begin + lrow) : -1;
+        xo = r < 0 ? kPastEnd : (uint32_t)((int64_t)r * g.x_stride * 2) + 16 * lgrp;
+        xbytes = (uint32_t)(((int64_t)(g.x_rows - 1) * g.x_stride + g.K) * 2);
+    }
+    auto load = [&](Chunk& c, int i) __attribute__((always_inline)) {
+        const int end = i == whole ? left : kStreamK;  // k of the chunk that there are
+        const auto wr = __builtin_amdgcn_make_buffer_rsrc(wbase, 0, i < chunks ? wbytes : 0u, 0x00020000);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int f = 0; f < CF; ++f) acc[m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](C& c) {
-        if constexpr (W4) {
-            const u32x4 one = ones<T>();
-            f32x4 part[MT][CF], sum[MT];
-#pragma unroll
-            for (int f = 0; f < CF; ++f) transpose4(c.w[f][0]);
-#pragma unroll
-            for (int q = 0; q < C::kGroups; ++q) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    sum[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int f = 0; f < CF; ++f) part[m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-                }
-#pragma unroll
-                for (int j = q * (4 / C::kGroups); j < (q + 1) * (4 / C::kGroups); ++j) {
-                    u32x4 x[MT];
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        x[m] = paired(c.x[m][j]);
-                        sum[m] = mfma16x16x32(x[m], one, sum[m], T{});
-                    }
-#pragma unroll
-                    for (int f = 0; f < CF; ++f) {
-                        const u32x4 w = codes16(c.w[f][0][j], T{});
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) part[m][f] = mfma16x16x32(x[m], w, part[m][f], T{});
-                    }
-                    __builtin_amdgcn_sched_barrier(0);  // a slice at a time: unpacked ahead, codes take four times the registers
-                }
-#pragma unroll
-                for (int f = 0; f < CF; ++f) {
-                    const float s = elem<T>::to_f32((uint16_t)(c.s[f] >> (16 * q)));
-                    const float z = -16.0f - (float)((c.z[f] >> (8 * q)) & 255u);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            acc[m][f][r] = fmaf(s, fmaf(z, sum[m][r], part[m][f][r]), acc[m][f][r]);
-                }
-            }
-        } else {
+        for (int f = 0; f < CF; ++f)
+            c.w[f] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                   wr, 32 * lgrp < end ? wo[f] : kPastEnd, (uint32_t)i * (kStreamK / 2), 0));
+        if constexpr (XD) {
+            const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.x), 0, i < chunks ? xbytes : 0u, 0x00020000);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int f = 0; f < CF; ++f)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) acc[m][f] = mfma16x16x32(c.x[m][j], c.w[f][j], acc[m][f], T{});
+                c.x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                       xr, 32 * j + 8 * lgrp < end ? xo : kPastEnd, (uint32_t)i * (kStreamK * 2) + 64 * j, 0));
         }
     };
-    // two chunks in flight; each column block begins elsewhere in K
-    const int rot = (int)((((uint32_t)(tn + 37 * t.e) * 0x9E37u & 0xFFFFu) * (uint32_t)chunks) >> 16);
-    auto turned = [&](int i) { return i < chunks ? (i + rot < chunks ? i + rot : i + rot - chunks) : i; };
-    C a, b;
-    load(a, turned(kp));
-    __builtin_amdgcn_sched_barrier(0);  // the loop's waits count loads in this order
-    load(b, turned(kp + ks));
-    __builtin_amdgcn_sched_barrier(0);
+
+    // the first chunks go before x and scales where a wave streams many, behind them where all is over soon (a
+    // token through 4096 x 11008: 12.5 and 11.5 us; 16 by 4 of 32 experts, 4096 x 2816: 67 and 70 with 8 parts)
+    Chunk c[AHEAD];
+    auto load_first = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            __builtin_amdgcn_sched_barrier(0);  // the loop's waits count loads in this order
+            load(c[a], kp + a * ks);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (ks < kStreamWaves) load_first();
+
+    // As much of K at a time (a power of two of chunks to a wave) as x's rows and the scales leave room for;
+    // one is in any case: 16 rows of 8 chunks, 8 chunks' scales of a column block
+    int span = kStreamK * ks;
+    while (span < g.K && (XD || rows * (2 * span * 2 + 16) <= x_lds) && 2 * span / G * 32 * units <= words) span *= 2;
+    const int pitch = min(span, chunks * kStreamK) * 2 + 16;  // bytes of a row of x in LDS
+    // element offset of the row of x behind each row of the tile, -1: zeros
+    if (!XD && tid < rows) {
+        const int r = source_row(g, t.begin + tid);
+        src[tid] = r < 0 ? -1 : (int64_t)r * g.x_stride;
+    }
+    const uint16_t* const scale = g.scale + (int64_t)t.e * g.N * groups;
+    const uint8_t* const zeros = g.zeros ? g.zeros + (int64_t)t.e * g.N * groups : nullptr;
+    // four scales to a load where rows of them keep to 8 bytes
+    const bool quads = (groups & 3) == 0 && ((uintptr_t)scale & 7) == 0 && ((uintptr_t)zeros & 3) == 0;
+    const int columns = 32 * units;
+    auto stage = [&](int k0) __attribute__((always_inline)) {
+        if constexpr (!XD) {
+            const int n = min(span, g.K - k0), padded = min(span, chunks * kStreamK - k0);
+            const int shift = __builtin_ctz(span) - 3;  // pieces of 8 to a row
+            for (int p = tid; p < rows << shift; p += kStreamThreads) {
+                const int r = p >> shift, k = (p - (r << shift)) * 8;
+                if (k >= padded) continue;
+                const int64_t s = src[r];
+                u32x4 v = u32x4{0, 0, 0, 0};
+                if (k < n && s >= 0) v = *reinterpret_cast<const u32x4*>(g.x + s + k0 + k);
+                *reinterpret_cast<u32x4*>(smem + r * pitch + 2 * k) = paired(v);
+            }
+        }
+        const int gshift = __builtin_ctz(span / G), q0 = k0 / G;
+        if (quads) {
+            const int qs = gshift > 2 ? gshift - 2 : 0;
+            for (int p = tid; p < columns << qs; p += kStreamThreads) {
+                const int c = p >> qs, q = (p - (c << qs)) * 4, r = weight_row(tn0 + (c >> 5), c & 31);
+                if (q0 + q >= groups || r >= g.N) continue;
+                const uint64_t v = *reinterpret_cast<const uint64_t*>(scale + (int64_t)r * groups + q0 + q);
+                const uint32_t z = zeros ? *reinterpret_cast<const uint32_t*>(zeros + (int64_t)r * groups + q0 + q) : 0x08080808u;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (u < 1 << gshift) sz[(q + u) * columns + c] = (uint32_t)(uint16_t)(v >> (16 * u)) | (z >> (8 * u) & 255u) << 16;
+            }
+        } else {
+            for (int p = tid; p < columns << gshift; p += kStreamThreads) {
+                const int c = p >> gshift, q = p - (c << gshift), r = weight_row(tn0 + (c >> 5), c & 31);
+                if (q0 + q >= groups || r >= g.N) continue;
+                const int64_t at = (int64_t)r * groups + q0 + q;
+                sz[q * columns + c] = (uint32_t)scale[at] | (zeros ? (uint32_t)zeros[at] : 8u) << 16;
+            }
+        }
+    };
+
+    f32x4 acc[CF];
+#pragma unroll
+    for (int f = 0; f < CF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint32_t mask = codes16_mask(T{}), base16 = elem<T>::from_f32(16.0f) * 0x10001u;
+    asm volatile("" : "+v"(mask), "+v"(base16));  // in registers: and-or takes one constant at most
+    const u32x4 one = [] {
+        const uint32_t o = elem<T>::from_f32(1.0f) * 0x10001u;
+        return u32x4{o, o, o, o};
+    }();
+    // chunk i, k0: the first k in LDS. Rows of x that are not there read as the last one's: their results are not stored
+    auto multiply = [&](Chunk& c, int i, int k0) __attribute__((always_inline)) {
+        const int at = i * kStreamK - k0;
+        const uint8_t* const row = smem + min(lrow, rows - 1) * pitch + (at + 8 * lgrp) * 2;
+#pragma unroll
+        for (int f = 0; f < CF; ++f) transpose4(c.w[f]);
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+            f32x4 part[CF], sum = f32x4{0.f, 0.f, 0.f, 0.f};
+            float s[CF], z[CF];
+#pragma unroll
+            for (int f = 0; f < CF; ++f) {
+                part[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+                // what lies behind the last group was not brought
+                const uint32_t v = i * NG + q < groups ? sz[(at / G + q) * columns + 32 * unit + 16 * f + lrow] : 0u;
+                s[f] = elem<T>::to_f32((uint16_t)v);
+                z[f] = -16.0f - (float)(v >> 16);
+            }
+#pragma unroll
+            for (int j = q * (4 / NG); j < (q + 1) * (4 / NG); ++j) {
+                const u32x4 x = XD ? paired(c.x[XD ? j : 0]) : *reinterpret_cast<const u32x4*>(row + 64 * j);
+                sum = mfma16x16x32(x, one, sum, T{});
+#pragma unroll
+                for (int f = 0; f < CF; ++f) part[f] = mfma16x16x32(x, codes16(c.w[f][j], mask, base16, T{}), part[f], T{});
+            }
+#pragma unroll
+            for (int f = 0; f < CF; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[f][r] = fmaf(s[f], fmaf(z[f], sum[r], part[f][r]), acc[f][r]);
+        }
+    };
+
+    __syncthreads();  // src
+    stage(0);
+    if (ks == kStreamWaves) load_first();
+    __syncthreads();
+    // every wave has the same number of turns; chunks behind the last are not multiplied
+    const int turns = (chunks + ks - 1) / ks, turns_here = span / (kStreamK * ks);
+    int k0 = 0;
 #pragma unroll 1
-    for (int i = kp; i < chunks; i += 2 * ks) {
-        multiply(a);
-        __builtin_amdgcn_sched_barrier(0);
-        load(a, turned(i + 2 * ks));
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(b);
-        __builtin_amdgcn_sched_barrier(0);
-        load(b, turned(i + 3 * ks));
-        __builtin_amdgcn_sched_barrier(0);
+    for (int n = 0; n < turns; n += AHEAD) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const int i = kp + (n + a) * ks;
+            if (n + a > 0 && n + a < turns && ((n + a) & (turns_here - 1)) == 0) {
+                k0 += span;
+                __syncthreads();
+                stage(k0);
+                __syncthreads();
+            }
+            if (i < chunks) multiply(c[a], i, k0);
+            __builtin_amdgcn_sched_barrier(0);
+            load(c[a], i + AHEAD * ks);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 
     // the parts of K of the same columns, added up in order by the first of their waves
     if (ks > 1) {
+        f32x4* const red = reinterpret_cast<f32x4*>(smem);
+        __syncthreads();  // x has been read
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int f = 0; f < CF; ++f) red[wave][m][f][lane] = acc[m][f];
+        for (int f = 0; f < CF; ++f) red[(wave * CF + f) * kWave + lane] = acc[f];
         __syncthreads();
         if (kp) return;
         for (int w = 1; w < ks; ++w)
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int f = 0; f < CF; ++f) acc[m][f] += red[wave + w][m][f][lane];
+            for (int f = 0; f < CF; ++f) acc[f] += red[((wave + w) * CF + f) * kWave + lane];
     }
     if (g.epi & kEpiBias) {
 #pragma unroll
-        for (int f = 0; f < CF; ++f) {
-            const int r = weight_row(f);
-            const float b = g.bias[(int64_t)t.e * g.N + min(r, g.N - 1)];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][f] += b;
-        }
+        for (int f = 0; f < CF; ++f) acc[f] += g.bias[(int64_t)t.e * g.N + min(weight_row(tn, 16 * f + lrow), g.N - 1)];
     }
-    auto put = [&](int m, int f, f32x4 v) {
-        const int c = (tn * half + f) * 16 + lrow;
+    const bool relu = g.epi & kEpiRelu;
+#pragma unroll
+    for (int f = 0; f < CF; ++f) {
+        if (gate && f) break;
+        const int col = gate ? tn * 16 + lrow : tn * 32 + 16 * f + lrow;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int p = t.begin + 16 * m + 4 * lgrp + r;
-            if (p < t.end && c < F) g.y[(int64_t)p * g.y_stride + c] = elem<T>::from_f32(v[r]);
-        }
-    };
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (gate) {
-#pragma unroll
-            for (int f = 0; f < CF / 2; ++f) {
-                f32x4 v;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = silu_gate(acc[m][f][r], acc[m][f + CF / 2][r]);
-                put(m, f, v);
-            }
-        } else {
-#pragma unroll
-            for (int f = 0; f < CF; ++f) {
-                f32x4 v = acc[m][f];
-                if (g.epi & kEpiRelu) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = fmaxf(v[r], 0.f);
-                }
-                put(m, f, v);
-            }
+            const float v = gate ? silu_gate(acc[0][r], acc[1][r]) : relu ? fmaxf(acc[f][r], 0.f) : acc[f][r];
+            const int p = 4 * lgrp + r;
+            if (p < rows && col < F) g.y[(int64_t)(t.begin + p) * g.y_stride + col] = elem<T>::from_f32(v);
         }
     }
 }
@@ -299,34 +293,46 @@ extern "C" int pyc_hip_grouped_stream_takes(int w4, const pyc_grouped* g) {
         g->K % 8 || (g->E > 1 && g->w_stride % (w4 ? 16 : 8)))
         return 0;
     return ((int64_t)(g->x_rows - 1) * g->x_stride + g->K) * 2 <= most &&
-           (double)g->N * g->K * (w4 ? 0.5 : 2.0) <= (double)most && (!w4 || (int64_t)g->N * (g->K / g->group) >= 4);
+           (double)g->N * g->K * (w4 ? 0.5 : 2.0) <= (double)most;
 }
 
-extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, int w4, const pyc_grouped* gp, void* stream) {
+extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, const pyc_grouped* gp, void* stream) {
     using namespace pyc;
     const Grouped& g = *gp;
     const bool gate = g.epi & kEpiGate;
     const int cols = gate ? g.N / 2 : g.N, per = gate ? 16 : 32;
     const int tiles_n = (cols + per - 1) / per;
     const int64_t most = expert_tiles_most(g.offsets ? g.E : 1, g.P, 16);
-    // K in as many parts as give a wave to every place there is (16 to a CU), two at least (32 tokens by
-    // 8 of 64 experts, 2048 x 2816: 8 parts 158 us, 4 137, 2 139, 1 147)
+    // K in as many parts as give a wave to every place there is (16 to a CU), two at least (16 tokens by 4 of 32
+    // experts, 4096 x 2816: 8 parts 71 us, 4 58, 2 55)
     int ks = 8;
     while (ks > 2 && most * tiles_n * ks > 4096) ks /= 2;
     const int wgs = (tiles_n + kStreamWaves / ks - 1) / (kStreamWaves / ks);
     if (most * wgs > 0x7FFFFFFF) return -1;
     const hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)(most * wgs)), block(kStreamWaves * kWave);
-#define PYC_STREAM(G)                                                                                                  \
-    if ((w4 ? g.group : 0) == G) {                                                                                     \
-        if (is_bf16) hipLaunchKernelGGL((grouped_stream_kernel<bf16_t, G, 2, 1>), grid, block, 0, s, g, tiles_n, wgs, ks); \
-        else hipLaunchKernelGGL((grouped_stream_kernel<f16_t, G, 2, 1>), grid, block, 0, s, g, tiles_n, wgs, ks);          \
-        return hipGetLastError() == hipSuccess ? 0 : -2;                                                               \
+    const dim3 grid((unsigned)(most * wgs)), block(kStreamThreads);
+    // x beside W where LDS would take it in turns; by expert, of about twice the mean of rows
+    const int big = most * wgs <= 256;
+    const int64_t rows = g.offsets ? 2 * (int64_t)g.P / g.E + 2 : g.P;
+    const int xd = (rows < 16 ? rows : 16) * (2 * (int64_t)g.K + 16) > kStreamLds[0][big].x;
+    const StreamLds lds = kStreamLds[xd][big];
+    const size_t bytes = stream_lds_bytes(lds);
+#define PYC_STREAM_X(TY, G, XD) \
+    hipLaunchKernelGGL((grouped_stream_kernel<TY, G, XD>), grid, block, bytes, s, g, tiles_n, wgs, ks, lds.x, lds.scales)
+#define PYC_STREAM(G)                                   \
+    if (g.group == G) {                                 \
+        if (is_bf16) {                                  \
+            if (xd) PYC_STREAM_X(bf16_t, G, true);      \
+            else PYC_STREAM_X(bf16_t, G, false);        \
+        } else {                                        \
+            if (xd) PYC_STREAM_X(f16_t, G, true);       \
+            else PYC_STREAM_X(f16_t, G, false);         \
+        }                                               \
     }
-    PYC_STREAM(0)
     PYC_STREAM(32)
     PYC_STREAM(64)
     PYC_STREAM(128)
 #undef PYC_STREAM
-    return -1;
+#undef PYC_STREAM_X
+    return hipGetLastError() == hipSuccess ? 0 : -2;
 }

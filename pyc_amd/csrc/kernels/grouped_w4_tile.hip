@@ -1,0 +1,389 @@
+// grouped_w4_tile.hip — products of many rows with 4-bit weights, dense or by expert.
+//
+// 128 rows of one expert x 256 rows of its W per tile, eight waves of 64 x 64 (two to a SIMD: one
+// unpacks or scales while the other multiplies), K in steps of 128. x, codes, scales and
+// zero points of a step come by LDS-DMA into a ring of three, so that two steps are on their way
+// while one is used, and no wait for one kind of load drains the others. The formula is the one of
+// grouped_stream.hip: a code goes into the mantissa of 16, and for each group
+//   acc += scale (sum x (16 + code) - (16 + zero) sum x),
+// with sum x from products by ones. Weights are never rounded, which costs a second set of sums
+// and two vector instructions for each result and group: bound by those for groups of 32
+// and 64, by both kinds of instructions for groups of 128.
+//
+// Scales and zero points are 2-byte and 1-byte values at any alignment, LDS-DMA moves aligned
+// dwords: the dwords that hold a row's values of the step are fetched (1 to 3, 1 or 2), and the
+// values shifted out of them.
+#include <type_traits>
+
+#include "grouped.hpp"
+#include "lds_dma.hpp"
+
+namespace pyc {
+
+constexpr int kW4K = 128;
+constexpr uint32_t kW4PastEnd = 0xFFFFFFF0u;
+constexpr int w4_scale_dwords(int g) { return g == 128 ? 1 : g == 64 ? 2 : 3; }
+constexpr int w4_zero_dwords(int g) { return g == 128 ? 1 : 2; }
+// A tile: 16 FM rows to a wave, WM waves of them; four waves of 16 FN columns. A step in LDS: x, codes, dwords
+// of scales and zero points; as many steps as leave room for a second workgroup (of four waves)
+constexpr uint32_t w4_x_bytes(int wm, int fm) { return (uint32_t)wm * fm * 16 * kW4K * 2; }
+constexpr uint32_t w4_code_bytes(int fn) { return (uint32_t)64 * fn * kW4K / 2; }
+constexpr uint32_t w4_step_bytes(int g, int wm, int fn, int fm) {
+    return w4_x_bytes(wm, fm) + w4_code_bytes(fn) + (uint32_t)(w4_scale_dwords(g) + w4_zero_dwords(g)) * 64 * fn * 4;
+}
+constexpr int w4_steps(int g, int wm, int fn, int fm) {
+    const int n = (int)((wm == 1 ? 80 : 160) * 1024 / w4_step_bytes(g, wm, fn, fm));
+    return n < 8 ? n : 8;
+}
+
+// lane i's 4 bytes at offset voff land at lds_base + 4 * i
+__device__ inline void lds_dma_buf_b32(i32x4 rsrc, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds_base), "v"(voff), "s"(rsrc)
+                 : "memory", "m0");
+}
+
+// Eight codes as B + c in the order of x: pairs k 0,1 2,3 4,5 6,7. A byte has two codes; 3 bits up its
+// low one, 1 bit down its high one stand where the mantissa of B has its units.
+__device__ inline float code_base(bf16_t) { return 16.0f; }
+__device__ inline float code_base(f16_t) { return 128.0f; }
+template <typename T> __device__ inline u32x4 codes_in_order(uint32_t w, T) {
+    const uint32_t m = 0x00780078u, b = elem<T>::from_f32(code_base(T{})) * 0x10001u;
+    const uint32_t lo = w << 3, hi = w >> 1;
+    u32x4 r;
+    r[0] = (__builtin_amdgcn_perm(hi, lo, 0x0c040c00u) & m) | b;
+    r[1] = (__builtin_amdgcn_perm(hi, lo, 0x0c050c01u) & m) | b;
+    r[2] = (__builtin_amdgcn_perm(hi, lo, 0x0c060c02u) & m) | b;
+    r[3] = (__builtin_amdgcn_perm(hi, lo, 0x0c070c03u) & m) | b;
+    return r;
+}
+
+template <typename T, int G, bool GATE, int WM, int FN, int FMX>
+__global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g, int tiles_n, int wide) {
+    constexpr int NW = 4 * WM, ROWS = 16 * WM * FMX, COLS = 64 * FN;
+    constexpr int NG = kW4K / G;                                   // groups to a step
+    constexpr int NS = w4_scale_dwords(G), NZ = w4_zero_dwords(G);
+    constexpr int CL = FN / WM;                                    // loads of codes to a wave and step
+    constexpr int DW = FN * (NS + NZ), SZ = (DW + NW - 1) / NW;    // loads of dwords in all, to a wave
+    constexpr uint32_t X_BYTES = w4_x_bytes(WM, FMX), CODE_BYTES = w4_code_bytes(FN);
+    constexpr uint32_t STEP = w4_step_bytes(G, WM, FN, FMX);
+    constexpr int S = w4_steps(G, WM, FN, FMX);
+    constexpr int YC = GATE ? 8 * FN : 16 * FN;                    // columns of y to a wave
+    constexpr int PITCH = 4 * YC + 8;                              // results in LDS: a row of all waves' columns
+    static_assert(CL * WM == FN && S >= 3 && (uint32_t)(ROWS * PITCH * 2) <= S * STEP, "tile shape");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[S * STEP];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 2, wn = wave & 3;
+    const int lrow = lane & 15, lgrp = lane >> 4;
+    const int F = GATE ? g.N / 2 : g.N, groups = g.K / G;
+    const int steps = (g.K + kW4K - 1) / kW4K;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
+    const i32x4 x_rsrc = make_buf_rsrc(g.x, (uint32_t)(((int64_t)(g.x_rows - 1) * g.x_stride + g.K) * 2));
+
+    // row tiles there are
+    int row_tiles = 0;
+    if (g.offsets) {
+        int held = 0;
+        for (int e0 = 0; e0 < g.E; e0 += kWave) {
+            const int e = e0 + lane;
+            const int b = scan_max(max(held, e < g.E ? min(g.offsets[e], g.P) : 0));
+            const int end = max(b, e < g.E ? min(g.offsets[e + 1], g.P) : 0);
+            row_tiles += __builtin_amdgcn_readlane(scan_add((end - b + ROWS - 1) / ROWS), kWave - 1);
+            held = __builtin_amdgcn_readlane(end, kWave - 1);
+        }
+    } else {
+        row_tiles = (g.P + ROWS - 1) / ROWS;
+    }
+    // XCD x (workgroups b with b % 8 == x) has the x-th eighth of the tiles
+    const int64_t all = (int64_t)row_tiles * tiles_n;
+    const int xcd = blockIdx.x & 7, per = gridDim.x >> 3;
+    const int t_end = __builtin_amdgcn_readfirstlane((int)(all * (xcd + 1) / 8));
+    int t = __builtin_amdgcn_readfirstlane((int)(all * xcd / 8) + (int)(blockIdx.x >> 3));
+
+    for (; t < t_end; t += per) {
+        const ExpertTile et = expert_tile(g, t / tiles_n, ROWS, lane);
+        if (et.e < 0) break;
+        const int e = __builtin_amdgcn_readfirstlane(et.e), row0 = __builtin_amdgcn_readfirstlane(et.begin);
+        const int end = __builtin_amdgcn_readfirstlane(et.end);
+        const int col0 = (t - t / tiles_n * tiles_n) * (GATE ? COLS / 2 : COLS);
+        // the row of W in slot c of the tile, -1: none. A wave has 16 FN slots; gated, half gates and then the
+        // values of the same columns.
+        auto weight_row = [&](int c) __attribute__((always_inline)) {
+            if constexpr (GATE) {
+                const int y = col0 + c / (2 * YC) * YC + c % YC;
+                return y < F ? y + (c / YC & 1) * F : -1;
+            } else {
+                return col0 + c < F ? col0 + c : -1;
+            }
+        };
+        const char* const codes = static_cast<const char*>(g.w) + (int64_t)e * g.w_stride;
+        const i32x4 w_rsrc = make_buf_rsrc(codes, (uint32_t)((int64_t)g.N * (g.K / 2)));
+        const uintptr_t sa = (uintptr_t)(g.scale + (int64_t)e * g.N * groups);
+        const uintptr_t za = (uintptr_t)(g.zeros ? g.zeros + (int64_t)e * g.N * groups : nullptr);
+        const uint32_t s_mis = (uint32_t)(sa & 3) / 2, z_mis = (uint32_t)(za & 3);
+        const i32x4 s_rsrc = make_buf_rsrc((const void*)(sa & ~(uintptr_t)3), ((uint32_t)(g.N * groups) * 2 + 2 * s_mis + 3) & ~3u);
+        const i32x4 z_rsrc = make_buf_rsrc((const void*)(za & ~(uintptr_t)3), g.zeros ? ((uint32_t)(g.N * groups) + z_mis + 3) & ~3u : 0u);
+
+        auto run_tile = [&](auto fm) __attribute__((always_inline)) {
+            constexpr int FM = decltype(fm)::value;  // fragments of rows to a wave
+            constexpr int LOADS = FM + CL + SZ;       // to a wave and step
+            // x: load i of a wave has rows 4 (NW i + wave) + lane / 16, chunk lane % 16 holding logical chunk
+            // (lane % 16) ^ (row % 16); codes: load i rows 16 (CL wave + i) + lane / 4, chunk lane % 4
+            // holding (lane % 4) ^ (row / 4 % 4)
+            uint32_t xo[FM], co[CL], so[SZ];
+            const int xk = 8 * ((lane & 15) ^ ((4 * wave + lane / 16) & 15));  // first k of the lane's chunk
+            const int ck = 32 * ((lane & 3) ^ ((lane >> 4) & 3));
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const int p = row0 + 4 * (NW * i + wave) + lane / 16;
+                const int s = p < end ? source_row(g, p) : -1;
+                xo[i] = s < 0 ? kW4PastEnd : (uint32_t)((int64_t)s * g.x_stride * 2) + 2 * xk;
+            }
+#pragma unroll
+            for (int i = 0; i < CL; ++i) {
+                const int n = weight_row(16 * (CL * wave + i) + lane / 4);
+                co[i] = n < 0 ? kW4PastEnd : (uint32_t)n * (uint32_t)(g.K / 2) + ck / 2;
+            }
+            // dword load q: slots 64 (q % FN) + lane, dword q / FN, scales first; one too many is the last again
+#pragma unroll
+            for (int i = 0; i < SZ; ++i) {
+                const int q = min(wave * SZ + i, DW - 1);
+                const int n = weight_row(64 * (q % FN) + lane);
+                so[i] = n < 0 ? kW4PastEnd : (uint32_t)n * (uint32_t)groups + (q < FN * NS ? s_mis : z_mis);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i) asm volatile("" : "+v"(xo[i]));  // complete before the first load goes out
+#pragma unroll
+            for (int i = 0; i < CL; ++i) asm volatile("" : "+v"(co[i]));
+#pragma unroll
+            for (int i = 0; i < SZ; ++i) asm volatile("" : "+v"(so[i]));
+            auto issue = [&](int s, int slot) __attribute__((always_inline)) {
+                const uint32_t base = lds0 + (uint32_t)slot * STEP;
+                const int left = g.K - s * kW4K;  // k from this step on
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+                    lds_dma_buf_b128_u(x_rsrc, xk < left ? xo[i] : kW4PastEnd, (uint32_t)s * (kW4K * 2), base + (uint32_t)(NW * i + wave) * 1024);
+#pragma unroll
+                for (int i = 0; i < CL; ++i)
+                    lds_dma_buf_b128_u(w_rsrc, ck < left ? co[i] : kW4PastEnd, (uint32_t)s * (kW4K / 2),
+                                       base + X_BYTES + (uint32_t)(CL * wave + i) * 1024);
+#pragma unroll
+                for (int i = 0; i < SZ; ++i) {
+                    const int q = min(wave * SZ + i, DW - 1);
+                    const bool zero = q >= FN * NS;
+                    const uint32_t a = so[i] + (uint32_t)(s * NG);  // the first value's place
+                    const uint32_t off = zero ? ((a >> 2) + (uint32_t)(q / FN - NS)) * 4 : ((a >> 1) + (uint32_t)(q / FN)) * 4;
+                    lds_dma_buf_b32(zero ? z_rsrc : s_rsrc, so[i] == kW4PastEnd ? kW4PastEnd : off,
+                                    __builtin_amdgcn_readfirstlane(base + X_BYTES + CODE_BYTES + (uint32_t)q * 256));
+                }
+            };
+
+            f32x4 acc[FM][FN], part[FM][FN], sum[FM];
+            u32x4 fa[2][FM], cw[FN];
+            uint32_t sv[FN][2], zv[FN], sp[FN], zp[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int n = max(weight_row(16 * (FN * wn + j) + lrow), 0);
+                sp[j] = (uint32_t)n * (uint32_t)groups + s_mis;
+                zp[j] = (uint32_t)n * (uint32_t)groups + z_mis;
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            auto read_x = [&](int b, int slot, int ks) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+                    fa[b][i] = *reinterpret_cast<const u32x4*>(smem + slot * STEP + ((wm * FM + i) * 16 + lrow) * 256 +
+                                                               (((ks * 4 + lgrp) ^ lrow) << 4));
+            };
+            // a step's codes, scales and zero points, the latter as the step's values from the lowest bits on
+            auto read_w = [&](int s, int slot) __attribute__((always_inline)) {
+                const uint8_t* const c = smem + slot * STEP + X_BYTES + (16 * FN * wn + lrow) * 64 + ((lgrp ^ ((lrow >> 2) & 3)) << 4);
+                const uint32_t* const d = reinterpret_cast<const uint32_t*>(smem + slot * STEP + X_BYTES + CODE_BYTES) + 16 * FN * wn + lrow;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    cw[j] = *reinterpret_cast<const u32x4*>(c + j * 1024);
+                    const uint32_t ss = ((sp[j] + (uint32_t)(s * NG)) & 1) * 16, zs = ((zp[j] + (uint32_t)(s * NG)) & 3) * 8;
+                    const uint32_t d0 = d[16 * j], d1 = NS > 1 ? d[COLS + 16 * j] : 0;
+                    sv[j][0] = __builtin_amdgcn_alignbit(d1, d0, ss);
+                    if constexpr (NS > 2) sv[j][1] = __builtin_amdgcn_alignbit(d[2 * COLS + 16 * j], d1, ss);
+                    const uint32_t z0 = d[NS * COLS + 16 * j], z1 = NZ > 1 ? d[(NS + 1) * COLS + 16 * j] : 0;
+                    zv[j] = __builtin_amdgcn_alignbit(z1, z0, zs);
+                }
+            };
+
+#pragma unroll
+            for (int s = 0; s < S; ++s) issue(s, s);
+            wait_vmem_le<(S - 1) * LOADS>();
+            __syncthreads();
+            read_x(0, 0, 0);
+            read_w(0, 0);
+            const u32x4 one = [] {
+                const uint32_t o = elem<T>::from_f32(1.0f) * 0x10001u;
+                return u32x4{o, o, o, o};
+            }();
+            int slot = 0;
+#pragma unroll 1
+            for (int s = 0; s < steps; ++s) {
+                const int next = slot == S - 1 ? 0 : slot + 1;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) transpose4(cw[j]);
+                u32x4 c[FN];
+                uint32_t svn[FN][2], zvn[FN];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    c[j] = cw[j];
+                    svn[j][0] = sv[j][0];
+                    svn[j][1] = sv[j][1];
+                    zvn[j] = zv[j];
+                }
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    if (ks < 3) {
+                        read_x((ks + 1) & 1, slot, ks + 1);
+                    } else {
+                        // the next step has landed, and this one has been read by all
+                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                        wait_vmem_le<(S - 2) * LOADS>();
+                        __syncthreads();
+                        issue(s + S, slot);
+                        read_x(0, next, 0);
+                        read_w(s + 1, next);
+                    }
+                    const bool first = ks % (G / 32) == 0, last = (ks + 1) % (G / 32) == 0;
+                    if (first) {
+#pragma unroll
+                        for (int i = 0; i < FM; ++i) {
+                            sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int j = 0; j < FN; ++j) part[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) sum[i] = mfma16x16x32(fa[ks & 1][i], one, sum[i], T{});
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) {
+                        const u32x4 w = codes_in_order(c[j][ks], T{});
+#pragma unroll
+                        for (int i = 0; i < FM; ++i) part[i][j] = mfma16x16x32(fa[ks & 1][i], w, part[i][j], T{});
+                    }
+                    if (last) {
+                        const int q = ks / (G / 32);
+                        const bool there = s * NG + q < groups;  // what lies behind the row is another's
+#pragma unroll
+                        for (int j = 0; j < FN; ++j) {
+                            const uint32_t raw = q < 2 ? svn[j][0] : svn[j][1];
+                            const float f = there ? elem<T>::to_f32((uint16_t)(raw >> (16 * (q & 1)))) : 0.f;
+                            const float z = -code_base(T{}) - (g.zeros ? (float)((zvn[j] >> (8 * q)) & 255u) : 8.0f);
+#pragma unroll
+                            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    acc[i][j][r] = fmaf(f, fmaf(z, sum[i][r], part[i][j][r]), acc[i][j][r]);
+                        }
+                    }
+                }
+                slot = next;
+            }
+            wait_vmem_le<0>();
+            __syncthreads();  // the ring is free: results go through it
+
+            float bias[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int n = weight_row(16 * (FN * wn + j) + lrow);
+                bias[j] = (g.epi & kEpiBias) && n >= 0 ? g.bias[(int64_t)e * g.N + n] : 0.f;
+            }
+            const bool relu = g.epi & kEpiRelu;
+            uint16_t* const out = reinterpret_cast<uint16_t*>(smem);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < (YC + 15) / 16; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float v = acc[i][j][r] + bias[j];
+                        // gated: the value is FN / 2 fragments on, or eight lanes
+                        if constexpr (GATE) v = silu_gate(v, FN > 1 ? acc[i][(j + FN / 2) % FN][r] + bias[(j + FN / 2) % FN] : row_half_turn(v));
+                        else if (relu) v = fmaxf(v, 0.f);
+                        if (!GATE || FN > 1 || lrow < 8)
+                            out[(16 * (wm * FM + i) + 4 * lgrp + r) * PITCH + wn * YC + 16 * j + lrow] = elem<T>::from_f32(v);
+                    }
+            __syncthreads();
+            constexpr int CH = 4 * YC / 8;
+            for (int q = tid; q < min(end - row0, ROWS) * CH; q += 64 * NW) {
+                const int r = q / CH, ch = q % CH, col = col0 + 8 * ch;
+                if (col >= F) continue;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(out + r * PITCH + 8 * ch);
+                uint16_t* const y = g.y + (int64_t)(row0 + r) * g.y_stride + col;
+                if (wide && col + 8 <= F) {
+                    *reinterpret_cast<u32x4*>(y) = v;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (col + k < F) y[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+                }
+            }
+            __syncthreads();  // the next tile's loads go into the ring
+        };
+        const int rows = end - row0;
+        if (FMX > 2 && rows > 32 * WM) run_tile(std::integral_constant<int, FMX>{});
+        else if (FMX > 1 && rows > 16 * WM) run_tile(std::integral_constant<int, (FMX > 1 ? 2 : 1)>{});
+        else run_tile(std::integral_constant<int, 1>{});
+    }
+}
+
+}  // namespace pyc
+
+extern "C" int pyc_hip_grouped_stream_takes(int w4, const pyc_grouped* g);
+
+// form 0: tiles of 128 rows and 256 columns; 1, 2 and 4: of 16, 32 and 64 rows and 64 columns
+extern "C" int pyc_hip_grouped_w4_tile_launch(int is_bf16, const pyc_grouped* gp, int form, void* stream) {
+    using namespace pyc;
+    const Grouped& g = *gp;
+    const bool gate = g.epi & kEpiGate;
+    const int cols = gate ? g.N / 2 : g.N, per = (form ? 64 : 256) / (gate ? 2 : 1);
+    const int tiles_n = (cols + per - 1) / per;
+    if (expert_tiles_most(g.offsets ? g.E : 1, g.P, 16) * tiles_n > 0x7FFFFFFF) return -1;
+    const int wide = ((uintptr_t)g.y & 15) == 0 && (g.P == 1 || g.y_stride % 8 == 0);
+    const dim3 grid(form ? 512 : 256), block(form ? 256 : 512);
+    const hipStream_t s = (hipStream_t)stream;
+#define PYC_W4_FORM(TY, G, FORM, WM, FN, FMX)                                                                                   \
+    if (form == FORM) {                                                                                                         \
+        if (gate) hipLaunchKernelGGL((grouped_w4_tile_kernel<TY, G, true, WM, FN, FMX>), grid, block, 0, s, g, tiles_n, wide);  \
+        else hipLaunchKernelGGL((grouped_w4_tile_kernel<TY, G, false, WM, FN, FMX>), grid, block, 0, s, g, tiles_n, wide);      \
+    }
+#define PYC_W4_TILE(TY, G)              \
+    if (g.group == G) {                 \
+        PYC_W4_FORM(TY, G, 0, 2, 4, 4)  \
+        PYC_W4_FORM(TY, G, 1, 1, 1, 1)  \
+        PYC_W4_FORM(TY, G, 2, 1, 1, 2)  \
+        PYC_W4_FORM(TY, G, 4, 1, 1, 4)  \
+    }
+    if (is_bf16) {
+        PYC_W4_TILE(bf16_t, 32)
+        PYC_W4_TILE(bf16_t, 64)
+        PYC_W4_TILE(bf16_t, 128)
+    } else {
+        PYC_W4_TILE(f16_t, 32)
+        PYC_W4_TILE(f16_t, 64)
+        PYC_W4_TILE(f16_t, 128)
+    }
+#undef PYC_W4_TILE
+#undef PYC_W4_FORM
+    return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
+// The form of 64 rows and columns, groups of 128.
+extern "C" int pyc_hip_kinfo_grouped_w4(int is_bf16, pyc_hip_kinfo* out) {
+    using namespace pyc;
+    out->fn = is_bf16 ? reinterpret_cast<const void*>(&grouped_w4_tile_kernel<bf16_t, 128, false, 1, 1, 4>)
+                      : reinterpret_cast<const void*>(&grouped_w4_tile_kernel<f16_t, 128, false, 1, 1, 4>);
+    out->name = "grouped_w4_tile_kernel";
+    out->lds_bytes = (size_t)w4_steps(128, 1, 1, 4) * w4_step_bytes(128, 1, 1, 4);
+    out->threads = 256;
+    out->waves_per_simd = 2;
+    return 0;
+}

@@ -56,10 +56,12 @@ int pyc_hip_kinfo_eltwise(int kid, int dtype, pyc_hip_kinfo* out);
 int pyc_hip_kinfo_kv_plan(pyc_hip_kinfo* out);
 int pyc_hip_kinfo_kv_append(int is_bf16, pyc_hip_kinfo* out);
 int pyc_hip_kinfo_kv_attention(int is_bf16, pyc_hip_kinfo* out);
-/* moe_route.hip (dtype 0 f32, 1 bf16, 2 f16; 128 experts), moe_combine.hip, grouped_gemm.hip */
+/* moe_route.hip (dtype 0 f32, 1 bf16, 2 f16; 128 experts), moe_combine.hip, grouped_ring.hip and
+ * grouped_w4_tile.hip (the forms of 64 rows and columns) */
 int pyc_hip_kinfo_moe_route(int dtype, pyc_hip_kinfo* out);
 int pyc_hip_kinfo_moe_combine(int is_bf16, pyc_hip_kinfo* out);
-int pyc_hip_kinfo_grouped(int w4, int is_bf16, pyc_hip_kinfo* out);
+int pyc_hip_kinfo_grouped_ring(int is_bf16, pyc_hip_kinfo* out);
+int pyc_hip_kinfo_grouped_w4(int is_bf16, pyc_hip_kinfo* out);
 
 #ifdef __cplusplus
 }

@@ -54,7 +54,7 @@ class Layer:
         """(out, bound) in 64 bits."""
         torch = self.torch
         values = lambda w: (w.double(), None) if self.bits == 16 else (  # noqa: E731
-            lambda v: (v[0] * v[1], 80 * v[1].abs()))(moe_util.w4_values(*w))
+            lambda v: (v[0] * v[1], (80 if self.x.dtype == torch.bfloat16 else 288) * v[1].abs()))(moe_util.w4_values(*w))
         (w1, s1), (w2, s2) = values(self.w1), values(self.w2)
         r = moe_util.route_ref(self.logits, K, True)
         like = lambda n: torch.zeros((self.t * K, n), dtype=self.x.dtype)  # noqa: E731

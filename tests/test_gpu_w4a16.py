@@ -1,8 +1,10 @@
 """GPU: products with 4-bit weights (pyc_hip_w4a16_gemm_dispatch and its form by expert)
-against moe_util.product_ref in 64 bits. What stands for |w| in the sums' rounding is
-(64 + zero) |scale|: a kernel may sum x (16 + code), up to 31 |x|, and x (16 + zero)
-apart before it takes their difference, and scales of fp32 sums by groups add two roundings
-that the bound's K + 4 holds."""
+against moe_util.product_ref in 64 bits. What stands for |w| in the sums' rounding: a
+kernel may sum x (B + code) and x apart and take sum x (B + code) - (B + zero) sum x, with B up
+to 16 in bf16 and 128 in fp16. Every partial sum of the first is at most (B + 15) sum |x|,
+the second at most (B + zero) sum |x|, so the roundings are those of (2 B + 15 + zero)
+|scale| |x| (64 + zero >= that in bf16, 272 + zero in fp16); scaling the groups' sums adds two
+roundings that the bound's K + 4 holds."""
 import pytest
 
 import pyc_amd
@@ -24,7 +26,7 @@ def _check(torch, x, codes, scale, zeros, offsets, n_out, rows=None, fan=1, bias
     whole, s = moe_util.w4_values(codes, scale, zeros)
     z = 8.0 if zeros is None else zeros.double().repeat_interleave(whole.shape[2] // scale.shape[2], 2)
     y = torch.full((x.shape[0] if p is None else p, n_out), 7.0, dtype=x.dtype)
-    ref, bound = moe_util.product_ref(x, whole * s, offsets, y, rows, fan, bias, epi, spread=(64 + z) * s.abs())
+    ref, bound = moe_util.product_ref(x, whole * s, offsets, y, rows, fan, bias, epi, spread=((64 if x.dtype == torch.bfloat16 else 272) + z) * s.abs())
     d = y.cuda()
     if dense:
         pyc_amd.w4a16_gemm(x.cuda(), codes[0].cuda(), scale[0].cuda(), d, zeros=_cuda(None if zeros is None else zeros[0]),
