@@ -439,15 +439,8 @@ def _make_moe_env():
     return _moe_env
 
 
-def _rows_of(what: str, t, width: int, dtype, device: int) -> int:
-    """Checks rows [n, width] of a type with dense elements on a device: their stride."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or shape[1] != width or t.dtype is not dtype or t.get_device() != device or \
-            (stride[1] != 1 and width > 1):
-        _kv_refuse(what, f"rows are [n, {width}] of one type with dense elements, on the call's device")
-    return stride[0] if shape[0] > 1 else width
-
-
+# The checks below are written out in each wrapper: a call of a few microseconds is mostly
+# its host time, and one of these through helper functions took 2 us more.
 def _dense_of(what: str, t, shape, dtype, device: int) -> int:
     """Checks a dense tensor (None: 0): its address."""
     if t is None:
@@ -455,13 +448,6 @@ def _dense_of(what: str, t, shape, dtype, device: int) -> int:
     if t.shape != shape or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
         _kv_refuse(what, f"an operand is not dense {dtype} {tuple(shape)} on the call's device")
     return t.data_ptr()
-
-
-def _here(what: str, t, current) -> int:
-    device = t.get_device()
-    if device < 0 or device != current():
-        _kv_refuse(what, "the tensors are not on the current device")
-    return device
 
 
 def moe_route_workspace(tokens: int, experts: int, k: int):
@@ -480,15 +466,19 @@ def moe_route(logits, ids, weights, offsets, rows, places, normalize: bool = Tru
     weights [T, k] (int32, float32), offsets [E + 1], rows and places [T * k] int32.
     Without a workspace (moe_route_workspace) one is made where the call needs it."""
     i32, f32, _, current, _, suffixes = _moe_env or _make_moe_env()
-    device = _here("moe route", logits, current)
-    suffix = suffixes.get(logits.dtype)
-    if suffix is None or logits.dim() != 2 or ids.dim() != 2:
-        _kv_refuse("moe route", "logits are float32, bf16 or f16 [tokens, experts], ids [tokens, k]")
-    (T, E), k = logits.shape, ids.shape[1]
-    stride = _rows_of("moe route", logits, E, logits.dtype, device)
-    i, w = _dense_of("moe route", ids, (T, k), i32, device), _dense_of("moe route", weights, (T, k), f32, device)
-    o, r = _dense_of("moe route", offsets, (E + 1,), i32, device), _dense_of("moe route", rows, (T * k,), i32, device)
-    p = _dense_of("moe route", places, (T * k,), i32, device)
+    device, suffix, shape, stride = logits.get_device(), suffixes.get(logits.dtype), logits.shape, logits.stride()
+    if device < 0 or device != current():
+        _kv_refuse("moe route", "the tensors are not on the current device")
+    if suffix is None or len(shape) != 2 or ids.dim() != 2 or (stride[1] != 1 and shape[1] > 1):
+        _kv_refuse("moe route", "logits are float32, bf16 or f16 [tokens, experts] with dense rows, ids [tokens, k]")
+    (T, E), k = shape, ids.shape[1]
+    n = T * k
+    for t in (ids, offsets, rows, places):
+        if t.dtype is not i32 or t.get_device() != device or not t.is_contiguous():
+            _kv_refuse("moe route", "index tensors are dense int32 on the call's device")
+    if weights.dtype is not f32 or weights.get_device() != device or not weights.is_contiguous() or ids.shape[0] != T or \
+            weights.shape != ids.shape or offsets.numel() != E + 1 or rows.numel() != n or places.numel() != n:
+        _kv_refuse("moe route", "weights are dense float32 [tokens, k], offsets [experts + 1], rows and places [tokens * k]")
     at = _stream(stream)
     if workspace is None and T > 64:
         import contextlib
@@ -500,7 +490,8 @@ def moe_route(logits, ids, weights, offsets, rows, places, normalize: bool = Tru
     elif workspace is not None and (workspace.get_device() != device or not workspace.is_contiguous()):
         _kv_refuse("moe route", "the workspace is dense, on the call's device")
     rc = (_lib or lib()).pyc_hip_moe_route_dispatch(
-        b"hip_moe_route_" + suffix, T, E, k, int(normalize), logits.data_ptr(), stride, i, w, o, r, p,
+        b"hip_moe_route_" + suffix, T, E, k, normalize, logits.data_ptr(), stride[0] if T > 1 else E, ids.data_ptr(),
+        weights.data_ptr(), offsets.data_ptr(), rows.data_ptr(), places.data_ptr(),
         0 if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes, at)
     if rc != 0:
         _check(rc, "moe route")
@@ -511,42 +502,30 @@ def moe_combine(y, weights, places, out, base=None, stream=None) -> None:
     y [rows, H], out and base [T, H] bf16 or f16, weights [T, k] float32, places
     [T * k] int32 as moe_route leaves them. out may be base."""
     i32, f32, _, current, half, _ = _moe_env or _make_moe_env()
-    device = _here("moe combine", out, current)
-    suffix = half.get(out.dtype)
-    if suffix is None or out.dim() != 2 or weights.dim() != 2:
-        _kv_refuse("moe combine", "out is bf16 or f16 [tokens, width], weights [tokens, k]")
-    (T, H), k = out.shape, weights.shape[1]
-    out_stride, y_stride = _rows_of("moe combine", out, H, out.dtype, device), _rows_of("moe combine", y, H, out.dtype, device)
-    base_stride = 0 if base is None else _rows_of("moe combine", base, H, out.dtype, device)
-    if base is not None and base.shape[0] != T:
-        _kv_refuse("moe combine", "base and out do not match")
+    dtype, device, shape, stride, yshape, ystride = out.dtype, out.get_device(), out.shape, out.stride(), y.shape, y.stride()
+    suffix = half.get(dtype)
+    if device < 0 or device != current():
+        _kv_refuse("moe combine", "the tensors are not on the current device")
+    if suffix is None or len(shape) != 2 or len(yshape) != 2 or yshape[1] != shape[1] or y.dtype is not dtype or \
+            y.get_device() != device or ((stride[1] != 1 or ystride[1] != 1) and shape[1] > 1):
+        _kv_refuse("moe combine", "y [rows, width] and out [tokens, width] are bf16 or f16 with dense rows, on one device")
+    T, H = shape
+    wshape = weights.shape
+    if weights.dtype is not f32 or weights.get_device() != device or not weights.is_contiguous() or len(wshape) != 2 or \
+            wshape[0] != T or places.dtype is not i32 or places.get_device() != device or not places.is_contiguous() or \
+            places.numel() != T * wshape[1]:
+        _kv_refuse("moe combine", "weights are dense float32 [tokens, k], places dense int32 [tokens * k], on the call's device")
+    at, base_stride = 0, 0
+    if base is not None:
+        bstride = base.stride()
+        if base.shape != shape or base.dtype is not dtype or base.get_device() != device or (bstride[1] != 1 and H > 1):
+            _kv_refuse("moe combine", "base is as out")
+        at, base_stride = base.data_ptr(), bstride[0] if T > 1 else H
     rc = (_lib or lib()).pyc_hip_moe_combine_dispatch(
-        b"hip_moe_combine_" + suffix, y.shape[0], T, k, H, y.data_ptr(), y_stride,
-        _dense_of("moe combine", weights, (T, k), f32, device), _dense_of("moe combine", places, (T * k,), i32, device),
-        _ptr(base), base_stride, out.data_ptr(), out_stride, _stream(stream))
+        b"hip_moe_combine_" + suffix, yshape[0], T, wshape[1], H, y.data_ptr(), ystride[0] if yshape[0] > 1 else H,
+        weights.data_ptr(), places.data_ptr(), at, base_stride, out.data_ptr(), stride[0] if T > 1 else H, _stream(stream))
     if rc != 0:
         _check(rc, "moe combine")
-
-
-def _product(what: str, x, y, N: int, K: int, epilogue: int, env):
-    """Checks x [n, K] and y [rows, N, or N / 2 gated]: (suffix, device, x's stride, y's stride)."""
-    device = _here(what, x, env[3])
-    suffix = env[4].get(x.dtype)
-    if suffix is None:
-        _kv_refuse(what, "x is bf16 or f16")
-    if epilogue & 4 and N % 2:
-        _kv_refuse(what, "gated weights have an even number of rows")
-    return (suffix, device, _rows_of(what, x, K, x.dtype, device),
-            _rows_of(what, y, N // 2 if epilogue & 4 else N, x.dtype, device))
-
-
-def _experts(what: str, w, dtype, device: int) -> int:
-    """Checks expert weights [E, N, K]: elements from an expert to the next one."""
-    shape, stride = w.shape, w.stride()
-    if w.dtype is not dtype or w.get_device() != device or (stride[2] != 1 and shape[2] > 1) or \
-            (stride[1] != shape[2] and shape[1] > 1):
-        _kv_refuse(what, f"weights are {dtype} [experts, N, ..] with dense experts, on the call's device")
-    return stride[0] if shape[0] > 1 else shape[1] * shape[2]
 
 
 def grouped_gemm(x, w, offsets, y, rows=None, fan: int = 1, bias=None, epilogue: int = 0, stream=None) -> None:
@@ -554,19 +533,49 @@ def grouped_gemm(x, w, offsets, y, rows=None, fan: int = 1, bias=None, epilogue:
     (pyc_hip_grouped_gemm_dispatch): x [n, K], w [E, N, K] and y [rows, N] bf16 or f16, offsets
     [E + 1] and rows int32 as moe_route leaves them (rows None: row p of x), bias [E, N]
     float32. epilogue: 0, 2 (ReLU) or 4 (SiLU gate: y is [rows, N / 2])."""
-    env = _moe_env or _make_moe_env()
-    if w.dim() != 3 or y.dim() != 2:
-        _kv_refuse("grouped gemm", "weights are [experts, N, K], y [rows, columns]")
-    E, N, K = w.shape
-    suffix, device, x_stride, y_stride = _product("grouped gemm", x, y, N, K, epilogue, env)
-    i32, P = env[0], y.shape[0]
+    i32, f32, _, current, half, _ = _moe_env or _make_moe_env()
+    dtype, device, xshape, wshape, yshape = x.dtype, x.get_device(), x.shape, w.shape, y.shape
+    xstride, wstride, ystride, suffix = x.stride(), w.stride(), y.stride(), half.get(dtype)
+    if device < 0 or device != current():
+        _kv_refuse("grouped gemm", "the tensors are not on the current device")
+    if suffix is None or len(wshape) != 3 or len(xshape) != 2 or len(yshape) != 2 or w.dtype is not dtype or \
+            y.dtype is not dtype or w.get_device() != device or y.get_device() != device:
+        _kv_refuse("grouped gemm", "x [n, K], w [experts, N, K] and y [rows, columns] are bf16 or f16, on one device")
+    E, N, K = wshape
+    P, C = yshape
+    if xshape[1] != K or C != (N // 2 if epilogue & 4 else N) or (epilogue & 4 and N % 2):
+        _kv_refuse("grouped gemm", "sizes do not match")
+    if (K > 1 and (xstride[1] != 1 or wstride[2] != 1)) or (C > 1 and ystride[1] != 1) or (N > 1 and wstride[1] != K):
+        _kv_refuse("grouped gemm", "rows and experts' weights are dense")
+    if offsets.dtype is not i32 or offsets.get_device() != device or not offsets.is_contiguous() or offsets.numel() != E + 1:
+        _kv_refuse("grouped gemm", "offsets are dense int32 [experts + 1] on the call's device")
     rc = (_lib or lib()).pyc_hip_grouped_gemm_dispatch(
-        b"hip_grouped_gemm_" + suffix, E, P, N, K, x.data_ptr(), x_stride, x.shape[0],
-        _dense_of("grouped gemm", rows, (P,), i32, device), fan, _dense_of("grouped gemm", offsets, (E + 1,), i32, device),
-        w.data_ptr(), _experts("grouped gemm", w, x.dtype, device), _dense_of("grouped gemm", bias, (E, N), env[1], device),
-        epilogue | (bias is not None), y.data_ptr(), y_stride, _stream(stream))
+        b"hip_grouped_gemm_" + suffix, E, P, N, K, x.data_ptr(), xstride[0] if xshape[0] > 1 else K, xshape[0],
+        rows if rows is None else _dense_of("grouped gemm", rows, (P,), i32, device), fan, offsets.data_ptr(), w.data_ptr(),
+        wstride[0] if E > 1 else N * K, bias if bias is None else _dense_of("grouped gemm", bias, (E, N), f32, device),
+        epilogue | (bias is not None), y.data_ptr(), ystride[0] if P > 1 else C, _stream(stream))
     if rc != 0:
         _check(rc, "grouped gemm")
+
+
+def _w4_sizes(what: str, x, y, codes, scale, epilogue: int, env, by_expert: int):
+    """What both products with 4-bit weights check of x, y, codes [.., N, K / 2] and scale [.., N, K / group]."""
+    dtype, device, xshape, yshape, cshape, sshape = x.dtype, x.get_device(), x.shape, y.shape, codes.shape, scale.shape
+    xstride, ystride, suffix = x.stride(), y.stride(), env[4].get(dtype)
+    if device < 0 or device != env[3]():
+        _kv_refuse(what, "the tensors are not on the current device")
+    if suffix is None or len(cshape) != 2 + by_expert or len(sshape) != 2 + by_expert or len(xshape) != 2 or \
+            len(yshape) != 2 or y.dtype is not dtype or scale.dtype is not dtype or codes.dtype is not env[2] or \
+            y.get_device() != device or codes.get_device() != device or scale.get_device() != device:
+        _kv_refuse(what, "x, y and scale are bf16 or f16, codes uint8, with the dimensions of this call, on one device")
+    N, K, groups, C = cshape[-2], 2 * cshape[-1], sshape[-1], yshape[1]
+    if xshape[1] != K or sshape[-2] != N or sshape[0] != cshape[0] or groups == 0 or K % groups or \
+            C != (N // 2 if epilogue & 4 else N) or (epilogue & 4 and N % 2):
+        _kv_refuse(what, "sizes do not match")
+    if (K > 1 and xstride[1] != 1) or (C > 1 and ystride[1] != 1) or not scale.is_contiguous():
+        _kv_refuse(what, "rows and scales are dense")
+    return (suffix, device, N, K, groups, yshape[0], xshape[0], xstride[0] if xshape[0] > 1 else K,
+            ystride[0] if yshape[0] > 1 else C)
 
 
 def w4a16_gemm(x, codes, scale, y, zeros=None, bias=None, epilogue: int = 0, stream=None) -> None:
@@ -575,19 +584,14 @@ def w4a16_gemm(x, codes, scale, y, zeros=None, bias=None, epilogue: int = 0, str
     scale [N, K / group] of x's type, zeros [N, K / group] uint8 (None: 8), bias [N]
     float32. epilogue as in grouped_gemm."""
     env = _moe_env or _make_moe_env()
-    if codes.dim() != 2 or scale.dim() != 2 or y.dim() != 2:
-        _kv_refuse("w4a16 gemm", "codes are [N, K / 2], scale [N, K / group], y [M, columns]")
-    N, K, groups = codes.shape[0], 2 * codes.shape[1], scale.shape[1]
-    suffix, device, x_stride, y_stride = _product("w4a16 gemm", x, y, N, K, epilogue, env)
-    if x.shape[0] != y.shape[0] or groups == 0 or K % groups:
-        _kv_refuse("w4a16 gemm", "sizes do not match")
+    suffix, device, N, K, groups, M, n, x_stride, y_stride = _w4_sizes("w4a16 gemm", x, y, codes, scale, epilogue, env, 0)
+    if n != M or not codes.is_contiguous():
+        _kv_refuse("w4a16 gemm", "x and y have a row for each token, codes are dense")
     rc = (_lib or lib()).pyc_hip_w4a16_gemm_dispatch(
-        b"hip_gemm_w4a16_" + suffix, x.shape[0], N, K, K // groups, x.data_ptr(), x_stride,
-        _dense_of("w4a16 gemm", codes, (N, K // 2), env[2], device),
-        _dense_of("w4a16 gemm", scale, (N, groups), x.dtype, device),
-        _dense_of("w4a16 gemm", zeros, (N, groups), env[2], device),
-        _dense_of("w4a16 gemm", bias, (N,), env[1], device), epilogue | (bias is not None), y.data_ptr(), y_stride,
-        _stream(stream))
+        b"hip_gemm_w4a16_" + suffix, M, N, K, K // groups, x.data_ptr(), x_stride, codes.data_ptr(), scale.data_ptr(),
+        zeros if zeros is None else _dense_of("w4a16 gemm", zeros, (N, groups), env[2], device),
+        bias if bias is None else _dense_of("w4a16 gemm", bias, (N,), env[1], device), epilogue | (bias is not None),
+        y.data_ptr(), y_stride, _stream(stream))
     if rc != 0:
         _check(rc, "w4a16 gemm")
 
@@ -597,21 +601,20 @@ def w4a16_grouped_gemm(x, codes, scale, offsets, y, zeros=None, rows=None, fan: 
     """grouped_gemm with the weights of w4a16_gemm (pyc_hip_w4a16_grouped_gemm_dispatch): codes
     [E, N, K / 2], scale and zeros [E, N, K / group], bias [E, N]."""
     env = _moe_env or _make_moe_env()
-    if codes.dim() != 3 or scale.dim() != 3 or y.dim() != 2:
-        _kv_refuse("w4a16 grouped gemm", "codes are [experts, N, K / 2], scale [experts, N, K / group], y [rows, columns]")
-    E, N, K, groups = codes.shape[0], codes.shape[1], 2 * codes.shape[2], scale.shape[2]
-    suffix, device, x_stride, y_stride = _product("w4a16 grouped gemm", x, y, N, K, epilogue, env)
-    if groups == 0 or K % groups:
-        _kv_refuse("w4a16 grouped gemm", "sizes do not match")
-    i32, P, g = env[0], y.shape[0], (E, N, groups)
+    suffix, device, N, K, groups, P, n, x_stride, y_stride = _w4_sizes("w4a16 grouped gemm", x, y, codes, scale, epilogue,
+                                                                       env, 1)
+    E, stride, i32 = codes.shape[0], codes.stride(), env[0]
+    if (stride[2] != 1 and K > 2) or (stride[1] != K // 2 and N > 1):
+        _kv_refuse("w4a16 grouped gemm", "an expert's codes are dense")
+    if offsets.dtype is not i32 or offsets.get_device() != device or not offsets.is_contiguous() or offsets.numel() != E + 1:
+        _kv_refuse("w4a16 grouped gemm", "offsets are dense int32 [experts + 1] on the call's device")
     rc = (_lib or lib()).pyc_hip_w4a16_grouped_gemm_dispatch(
-        b"hip_grouped_gemm_w4a16_" + suffix, E, P, N, K, K // groups, x.data_ptr(), x_stride, x.shape[0],
-        _dense_of("w4a16 grouped gemm", rows, (P,), i32, device), fan,
-        _dense_of("w4a16 grouped gemm", offsets, (E + 1,), i32, device), codes.data_ptr(),
-        _experts("w4a16 grouped gemm", codes, env[2], device), _dense_of("w4a16 grouped gemm", scale, g, x.dtype, device),
-        _dense_of("w4a16 grouped gemm", zeros, g, env[2], device),
-        _dense_of("w4a16 grouped gemm", bias, (E, N), env[1], device), epilogue | (bias is not None), y.data_ptr(),
-        y_stride, _stream(stream))
+        b"hip_grouped_gemm_w4a16_" + suffix, E, P, N, K, K // groups, x.data_ptr(), x_stride, n,
+        rows if rows is None else _dense_of("w4a16 grouped gemm", rows, (P,), i32, device), fan, offsets.data_ptr(),
+        codes.data_ptr(), stride[0] if E > 1 else N * (K // 2), scale.data_ptr(),
+        zeros if zeros is None else _dense_of("w4a16 grouped gemm", zeros, (E, N, groups), env[2], device),
+        bias if bias is None else _dense_of("w4a16 grouped gemm", bias, (E, N), env[1], device),
+        epilogue | (bias is not None), y.data_ptr(), y_stride, _stream(stream))
     if rc != 0:
         _check(rc, "w4a16 grouped gemm")
 
