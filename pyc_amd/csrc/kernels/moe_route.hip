@@ -16,8 +16,14 @@
 // word of bits for each expert: setting bits needs no order, and the rank of a token
 // among its expert's is a count of lower bits. So no sum depends on the order of
 // atomics, and equal inputs give equal outputs.
-// Up to kOneTokens tokens one workgroup does it all; above, the first launch leaves each
+// Up to 64 tokens one workgroup does it all; above, the first launch leaves each
 // 32 tokens' words in the workspace and the second adds up the words before its own.
+//
+// Bound by latency: the logits are read once (2 MB of 8200 tokens by 128 experts, under
+// 1 us), the k steps of a token follow on each other, and the second launch waits for the
+// first. Times of a call, cold logits: 8200 tokens by 128 experts, 8 chosen 16.7 us (27.0
+// with the wave's maximum through LDS and eight blocks to every workgroup of the second
+// launch); 32 tokens by 64 experts 8.8 us, most of it the host's.
 #include "common.hpp"
 
 namespace pyc {
@@ -27,7 +33,7 @@ constexpr int kRouteWaves = kRouteThreads / kWave;
 constexpr int kRouteBlock = 32;     // tokens to a word
 constexpr int kRouteExperts = 1024;
 constexpr int kOneBlocks = 2;       // blocks one workgroup does alone
-constexpr int kScatterBlocks = 8;   // blocks to a workgroup of the second launch
+constexpr int kScatterMost = 8;     // blocks to a workgroup of the second launch, at most
 
 struct Route {
     const void* logits;
@@ -47,15 +53,28 @@ template <int DT> __device__ inline float route_logit(const void* p, int64_t i) 
     else return elem<f16_t>::to_f32(static_cast<const uint16_t*>(p)[i]);
 }
 
+// Over the wave's lanes, by DPP: four steps in each row of 16, then the rows' last lanes; lane 63 has it.
+template <int CTRL, int ROWS> __device__ inline float dpp_f(float old, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ inline float last_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
 __device__ inline float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    v = fmaxf(v, dpp_f<0x111, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x112, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x114, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x118, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x142, 0xa>(v, v));
+    v = fmaxf(v, dpp_f<0x143, 0xc>(v, v));
+    return last_lane(v);
 }
 __device__ inline float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    v += dpp_f<0x111, 0xf>(0.f, v);
+    v += dpp_f<0x112, 0xf>(0.f, v);
+    v += dpp_f<0x114, 0xf>(0.f, v);
+    v += dpp_f<0x118, 0xf>(0.f, v);
+    v += dpp_f<0x142, 0xa>(0.f, v);
+    v += dpp_f<0x143, 0xc>(0.f, v);
+    return last_lane(v);
 }
 
 // One wave: token t's choices, its bit in the block's words (LDS).
@@ -132,29 +151,22 @@ __device__ inline int route_scan(const int* n, int* first, int E, int* part, int
     return all;
 }
 
-// Places and rows of the flat indexes of block b: `first[e]` positions of its experts'
-// rows come before the block's.
-__device__ inline void route_scatter(const Route& r, int b, const uint32_t* words, const int* first, int tid, int threads) {
-    const int t0 = b * kRouteBlock;
-    const int n = min(kRouteBlock, r.T - t0) * r.k;
-    for (int i = tid; i < n; i += threads) {
-        const int64_t f = (int64_t)t0 * r.k + i;
-        const int e = min(r.ids[f], r.E - 1);
-        int at = -1;
-        if (e >= 0) {
-            at = first[e] + __popc(words[e] & ((1u << (i / r.k)) - 1u));
-            // inside rows, whatever a second call on the same workspace left in the words
-            if ((unsigned)at < (unsigned)(r.T * r.k)) r.rows[at] = (int32_t)f;
-        }
-        r.places[f] = at;
+// Place and row of flat index f, of token t of its block of 32, whose words and first positions are given.
+__device__ inline void route_place(const Route& r, int64_t f, const uint32_t* words, const int* first, int t) {
+    const int e = min(r.ids[f], r.E - 1);
+    int at = -1;
+    if (e >= 0) {
+        at = first[e] + __popc(words[e] & ((1u << t) - 1u));
+        // inside rows, whatever a second call on the same workspace left in the words
+        if ((unsigned)at < (unsigned)(r.T * r.k)) r.rows[at] = (int32_t)f;
     }
+    r.places[f] = at;
 }
 
 template <int DT, int NV, bool ONE>
 __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(Route r) {
     constexpr int BLOCKS = ONE ? kOneBlocks : 1;
     __shared__ uint32_t words[BLOCKS][NV * kWave];
-    __shared__ int count[NV * kWave], first[NV * kWave], part[kRouteWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int b0 = ONE ? 0 : blockIdx.x;
     for (int i = tid; i < BLOCKS * NV * kWave; i += kRouteThreads) (&words[0][0])[i] = 0;
@@ -163,6 +175,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(Route r) {
     for (int t = t0 + wave; t < t1; t += kRouteWaves) route_token<DT, NV>(r, t, words[(t - t0) / kRouteBlock], lane);
     __syncthreads();
     if constexpr (ONE) {
+        __shared__ int count[NV * kWave], first[BLOCKS][NV * kWave], part[kRouteWaves];
         if (tid < r.E) {
             int n = 0;
 #pragma unroll
@@ -170,15 +183,18 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(Route r) {
             count[tid] = n;
         }
         __syncthreads();
-        const int all = route_scan(count, first, r.E, part, tid);
-        if (tid < r.E) r.offsets[tid] = first[tid];
-        if (tid == 0) r.offsets[r.E] = all;
+        const int all = route_scan(count, first[0], r.E, part, tid);
+        if (tid < r.E) {
+            r.offsets[tid] = first[0][tid];
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-            if (b * kRouteBlock < r.T) route_scatter(r, b, words[b], first, tid, kRouteThreads);
-            __syncthreads();
-            if (tid < r.E) first[tid] += __popc(words[b][tid]);
-            __syncthreads();
+            for (int b = 1; b < BLOCKS; ++b) first[b][tid] = first[b - 1][tid] + __popc(words[b - 1][tid]);
+        }
+        if (tid == 0) r.offsets[r.E] = all;
+        __syncthreads();
+        const int each = kRouteBlock * r.k;
+        for (int i = tid; i < r.T * r.k; i += kRouteThreads) {
+            const int b = i / each;
+            route_place(r, i, words[b], first[b], (i - b * each) / r.k);
         }
         for (int i = all + tid; i < r.T * r.k; i += kRouteThreads) r.rows[i] = -1;
     } else {
@@ -186,39 +202,55 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(Route r) {
     }
 }
 
-__global__ void __launch_bounds__(kRouteThreads) moe_scatter_kernel(Route r, int blocks) {
-    __shared__ int count[kRouteExperts], before[kRouteExperts], first[kRouteExperts], part[kRouteWaves];
+// nb blocks to a workgroup. Every workgroup adds up all blocks' words by itself: they are few and in L2, and
+// a third launch would take longer.
+__global__ void __launch_bounds__(kRouteThreads) moe_scatter_kernel(Route r, int blocks, int nb) {
+    __shared__ uint32_t own[kScatterMost][kRouteExperts];
+    __shared__ int first[kScatterMost + 1][kRouteExperts];
+    __shared__ int count[kRouteExperts], before[kRouteExperts], part[kRouteWaves];
     const int tid = threadIdx.x;
-    const int b0 = blockIdx.x * kScatterBlocks;
-    // threads per expert: as many as there are for it, each a share of the blocks
+    const int b0 = blockIdx.x * nb, mine = min(nb, blocks - b0);
     for (int e = tid; e < r.E; e += kRouteThreads) count[e] = before[e] = 0;
+    for (int i = tid; i < mine * r.E; i += kRouteThreads) own[i / r.E][i % r.E] = r.words[(int64_t)b0 * r.E + i];
     __syncthreads();
-    const int per = kRouteThreads / r.E;  // >= 1
+    const int per = kRouteThreads / r.E;  // threads to an expert, each a share of the blocks
     if (tid < per * r.E) {
         const int e = tid % r.E;
-        int n = 0, own = 0;
-        for (int b = tid / r.E; b < blocks; b += per) {
-            const int c = __popc(r.words[(int64_t)b * r.E + e]);
-            n += c;
-            own += b < b0 ? c : 0;
+        int n = 0, low = 0;
+        for (int b = tid / r.E; b < blocks; b += 8 * per) {
+            uint32_t w[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) w[u] = r.words[(int64_t)min(b + u * per, blocks - 1) * r.E + e];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int c = b + u * per < blocks ? __popc(w[u]) : 0;
+                n += c;
+                low += b + u * per < b0 ? c : 0;
+            }
         }
         atomicAdd(&count[e], n);
-        atomicAdd(&before[e], own);
+        atomicAdd(&before[e], low);
     }
     __syncthreads();
-    const int all = route_scan(count, first, r.E, part, tid);
+    const int all = route_scan(count, first[0], r.E, part, tid);
     if (blockIdx.x == 0) {
-        if (tid < r.E) r.offsets[tid] = first[tid];
+        if (tid < r.E) r.offsets[tid] = first[0][tid];
         if (tid == 0) r.offsets[r.E] = all;
     }
-    if (tid < r.E) first[tid] += before[tid];
     __syncthreads();
-    for (int b = b0; b < min(blocks, b0 + kScatterBlocks); ++b) {
-        const uint32_t* words = r.words + (int64_t)b * r.E;
-        route_scatter(r, b, words, first, tid, kRouteThreads);
-        __syncthreads();
-        if (tid < r.E) first[tid] += __popc(words[tid]);
-        __syncthreads();
+    if (tid < r.E) {
+        int at = first[0][tid] + before[tid];
+        for (int b = 0; b < mine; ++b) {
+            first[b][tid] = at;
+            at += __popc(own[b][tid]);
+        }
+    }
+    __syncthreads();
+    const int each = kRouteBlock * r.k;
+    const int n = min(mine * each, (r.T - b0 * kRouteBlock) * r.k);
+    for (int i = tid; i < n; i += kRouteThreads) {
+        const int b = i / each, t = (i - b * each) / r.k;
+        route_place(r, (int64_t)b0 * each + i, own[b], first[b], t);
     }
     for (int i = all + blockIdx.x * kRouteThreads + tid; i < r.T * r.k; i += gridDim.x * kRouteThreads) r.rows[i] = -1;
 }
@@ -230,8 +262,9 @@ template <int DT, int NV> static int route_launch(const Route& r, hipStream_t s)
         return hipGetLastError() == hipSuccess ? 0 : -2;
     }
     hipLaunchKernelGGL((moe_route_kernel<DT, NV, false>), dim3(blocks), dim3(kRouteThreads), 0, s, r);
-    hipLaunchKernelGGL(moe_scatter_kernel, dim3((blocks + kScatterBlocks - 1) / kScatterBlocks), dim3(kRouteThreads), 0, s,
-                       r, blocks);
+    // two blocks to a workgroup; eight where the words that each of them reads are many
+    const int nb = (int64_t)blocks * r.E <= 65536 ? 2 : kScatterMost;
+    hipLaunchKernelGGL(moe_scatter_kernel, dim3((blocks + nb - 1) / nb), dim3(kRouteThreads), 0, s, r, blocks, nb);
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
@@ -263,7 +296,7 @@ extern "C" int pyc_hip_kinfo_moe_route(int dtype, pyc_hip_kinfo* out) {
               : dtype == 1 ? reinterpret_cast<const void*>(&moe_route_kernel<1, 2, false>)
                            : reinterpret_cast<const void*>(&moe_route_kernel<2, 2, false>);
     out->name = "moe_route_kernel";
-    out->lds_bytes = 0;
+    out->lds_bytes = 2 * kWave * 4;
     out->threads = kRouteThreads;
     out->waves_per_simd = 8;
     return 0;
