@@ -308,7 +308,7 @@ size_t pyc_hip_moe_route_workspace(int tokens, int experts, int k);
  * y [rows][width], out and base [tokens][width] of the symbol's type (rows their strides
  * apart, base NULL: 0), weights fp32 and places [tokens][k]. fp32 sums, base first, then j
  * in order, one rounding. A place outside y (-1) counts as absent. out may be base; else it
- * overlaps nothing. Any width and alignment; 16-byte rows are fastest. 1 <= k <= 64, tokens * width below 2^38.
+ * overlaps nothing. Any width and alignment; 16-byte rows are fastest. 1 <= k <= 64, tokens * width below 2^32.
  * Symbols "hip_moe_combine_bf16", "hip_moe_combine_f16". 0, -1, -2 as above. */
 int pyc_hip_moe_combine_dispatch(
     const char* symbol, int rows, int tokens, int k, int width, const void* y, int64_t y_stride,

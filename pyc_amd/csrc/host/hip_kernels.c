@@ -860,7 +860,7 @@ int pyc_hip_moe_combine_dispatch(const char* symbol, int rows, int tokens, int k
     }
     if ((rows > 0 && (!aligned(y, 2) || y_stride < width)) || !aligned(weights, 4) || !aligned(places, 4) ||
         (base && (!aligned(base, 2) || base_stride < width)) || !aligned(out, 2) || out_stride < width ||
-        (double)tokens * width >= 0x1p38) {
+        (int64_t)tokens * width >= ((int64_t)1 << 32)) {
         return -1;
     }
     return pyc_hip_moe_combine_launch(v->dtype == VT_BF16, rows, tokens, k, width, y, y_stride, weights, places, base,

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
         const int p = t.begin + row0 + 32 * i;
         const int r = p < t.end ? source_row(g, p) : -1;
         xin[i] = r >= 0;
-        xr[i] = g.x_rows > 0 ? g.x + (int64_t)max(r, 0) * g.x_stride : static_cast<const uint16_t*>(g.w);
+        xr[i] = g.x + (int64_t)max(r, 0) * g.x_stride;
         wr[i] = static_cast<const uint16_t*>(g.w) + ew + (int64_t)max(weight_row(row0 + 32 * i), 0) * g.K;
     }
     const int crow = weight_row(tid >> 2);
@@ -96,11 +96,12 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
         uint64_t q;
         int z;
     };
+    const int xk = g.x_rows > 0 ? g.K : 0;  // without rows nothing of x is read
     auto load = [&](Step& s, int k0) {
         const bool edge = k0 + kGenK > g.K;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            s.a[i] = row_piece(xr[i], k0 + 8 * ch, g.K, edge);
+            s.a[i] = row_piece(xr[i], k0 + 8 * ch, xk, edge || xk == 0);
             if constexpr (!W4) s.b[i] = row_piece(wr[i], k0 + 8 * ch, g.K, edge);
         }
         if constexpr (W4) {
@@ -245,7 +246,7 @@ extern "C" int pyc_hip_grouped_launch(int is_bf16, int w4, const pyc_grouped* gp
     const int cols = g.epi & kEpiGate ? g.N / 2 : g.N, per = g.epi & kEpiGate ? kGenTile / 2 : kGenTile;
     const int tiles_n = (cols + per - 1) / per;
     const int64_t tiles = expert_tiles_most(g.offsets ? g.E : 1, g.P, kGenTile) * tiles_n;
-    if (tiles > 0x7FFFFFFF) return -1;
+    if (tiles > kMostThreads / 256) return -1;
     const dim3 grid((unsigned)tiles), block(256);
     const hipStream_t s = (hipStream_t)stream;
 #define PYC_GENERAL(TY, W) hipLaunchKernelGGL((grouped_general_kernel<TY, W>), grid, block, 0, s, g, tiles_n)

@@ -161,7 +161,7 @@ extern "C" int pyc_hip_grouped_ring_launch(int is_bf16, const pyc_grouped* gp, i
     const int cols = gate ? g.N / 2 : g.N, per = gate ? 32 * fn : 64 * fn;
     const int tiles_n = (cols + per - 1) / per;
     const int64_t tiles = expert_tiles_most(g.offsets ? g.E : 1, g.P, kRingRows) * tiles_n;
-    if (tiles > 0x7FFFFFFF) return -1;
+    if (tiles > kMostThreads / 256) return -1;
     const int wide = ((uintptr_t)g.y & 15) == 0 && (g.P == 1 || g.y_stride % 8 == 0);
     const dim3 grid((unsigned)tiles), block(256);
     const hipStream_t s = (hipStream_t)stream;

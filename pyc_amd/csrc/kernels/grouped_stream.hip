@@ -308,7 +308,7 @@ extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, const pyc_grouped* gp,
     int ks = 8;
     while (ks > 2 && most * tiles_n * ks > 4096) ks /= 2;
     const int wgs = (tiles_n + kStreamWaves / ks - 1) / (kStreamWaves / ks);
-    if (most * wgs > 0x7FFFFFFF) return -1;
+    if (most * wgs > kMostThreads / kStreamThreads) return -1;
     const hipStream_t s = (hipStream_t)stream;
     const dim3 grid((unsigned)(most * wgs)), block(kStreamThreads);
     // x beside W where LDS would take it in turns; by expert, of about twice the mean of rows

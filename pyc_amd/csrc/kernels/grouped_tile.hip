@@ -372,7 +372,7 @@ extern "C" int pyc_hip_grouped_tile_launch(int is_bf16, const pyc_grouped* gp, v
     const bool gate = g.epi & kEpiGate, tail = g.K % kTileK != 0;
     const int cols = gate ? g.N / 2 : g.N, per = gate ? 128 : 256;
     const int tiles_n = (cols + per - 1) / per;
-    if (expert_tiles_most(g.offsets ? g.E : 1, g.P, kTile) * tiles_n > 0x7FFFFFFF) return -1;
+    if (expert_tiles_most(g.offsets ? g.E : 1, g.P, kTile) * tiles_n > 0x7FFF0000) return -1;
     const dim3 grid(256), block(256);
     const hipStream_t s = (hipStream_t)stream;
 #define PYC_TILE(G, TL)                                                                                       \

@@ -346,7 +346,7 @@ extern "C" int pyc_hip_grouped_w4_tile_launch(int is_bf16, const pyc_grouped* gp
     const bool gate = g.epi & kEpiGate;
     const int cols = gate ? g.N / 2 : g.N, per = (form ? 64 : 256) / (gate ? 2 : 1);
     const int tiles_n = (cols + per - 1) / per;
-    if (expert_tiles_most(g.offsets ? g.E : 1, g.P, 16) * tiles_n > 0x7FFFFFFF) return -1;
+    if (expert_tiles_most(g.offsets ? g.E : 1, g.P, 16) * tiles_n > 0x7FFF0000) return -1;
     const int wide = ((uintptr_t)g.y & 15) == 0 && (g.P == 1 || g.y_stride % 8 == 0);
     const dim3 grid(form ? 512 : 256), block(form ? 256 : 512);
     const hipStream_t s = (hipStream_t)stream;

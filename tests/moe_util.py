@@ -1,9 +1,12 @@
 """The operators of a layer of experts and of 4-bit weights restated plainly, in
 64 bits on the CPU, inputs for their tests, and how far results may be off."""
+import ctypes
 import math
 
 import numpy as np
 import torch
+
+import pyc_amd
 
 DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}  # half a step of the type, relative
@@ -96,30 +99,78 @@ def product_ref(x, w, offsets, y, rows=None, fan=1, bias=None, epi=0, spread=Non
     (|g| + 8) U each way; ReLU does not widen. Then the output's own rounding."""
     out, bound = y.double().clone(), torch.zeros(y.shape, dtype=torch.float64)
     ends = held(offsets, y.shape[0])
-    xd = x.double()
     for e in range(w.shape[0]):
-        for p in range(ends[e], ends[e + 1]):
-            r = p
-            if rows is not None:
-                r = int(rows[p]) // fan if int(rows[p]) >= 0 else -1
-            row = xd[r] if 0 <= r < x.shape[0] else torch.zeros(w.shape[2], dtype=torch.float64)
-            h = w[e] @ row
-            s = (w[e].abs() if spread is None else spread[e]) @ row.abs()
-            if bias is not None:
-                h = h + bias[e].double()
-                s = s + bias[e].double().abs()
-            d = (w.shape[2] + 4) * U * s
-            if epi & RELU:
-                h = h.clamp(min=0)
-            if epi & GATE:
-                n = h.shape[0] // 2
-                g, v, dg, dv = h[:n], h[n:], d[:n], d[n:]
-                f = g / (1.0 + torch.exp(-g))
-                h = f * v
-                d = 1.1 * (v.abs() + dv) * dg + f.abs() * dv + (g.abs() + 8) * U * h.abs()
-            out[p] = h
-            bound[p] = rounded(h, d, y.dtype)
+        p0, p1 = ends[e], ends[e + 1]
+        if p0 == p1:
+            continue
+        src = torch.arange(p0, p1)
+        if rows is not None:
+            r = torch.as_tensor(rows)[p0:p1].long()
+            src = torch.where(r >= 0, torch.div(r, fan, rounding_mode="floor"), -1)
+        xd = torch.zeros((p1 - p0, w.shape[2]), dtype=torch.float64)
+        there = (src >= 0) & (src < x.shape[0])
+        xd[there] = x[src[there]].double()
+        we = w[e]
+        h = xd @ we.T
+        s = xd.abs() @ (we.abs() if spread is None else spread[e]).T
+        if bias is not None:
+            h = h + bias[e].double()
+            s = s + bias[e].double().abs()
+        d = (w.shape[2] + 4) * U * s
+        if epi & RELU:
+            h = h.clamp(min=0)
+        if epi & GATE:
+            n = h.shape[1] // 2
+            g, v, dg, dv = h[:, :n], h[:, n:], d[:, :n], d[:, n:]
+            f = g / (1.0 + torch.exp(-g))
+            h = f * v
+            d = 1.1 * (v.abs() + dv) * dg + f.abs() * dv + (g.abs() + 8) * U * h.abs()
+        out[p0:p1] = h
+        bound[p0:p1] = rounded(h, d, y.dtype)
     return out, bound
+
+
+class Weights4:
+    """Weights of 4-bit codes, an expert at a time, as product_ref takes them; spread: what stands for |w|
+    in the sums' rounding where sum x (B + code) and sum x are taken apart, at B = 16 (bf16) and 128 (fp16)."""
+
+    def __init__(self, codes, scale, zeros, spread=0):
+        self.parts, self.spread = (codes, scale, zeros), spread
+        self.shape = (codes.shape[0], codes.shape[1], 2 * codes.shape[2])
+
+    def __getitem__(self, e):
+        codes, scale, zeros = self.parts
+        z = None if zeros is None else zeros[e:e + 1]
+        whole, s = w4_values(codes[e:e + 1], scale[e:e + 1], z)
+        if not self.spread:
+            return (whole * s)[0]
+        zero = 8.0 if z is None else z.double().repeat_interleave(self.shape[2] // scale.shape[2], 2)
+        return ((self.spread + zero) * s.abs())[0]
+
+
+# ---------------------------------------------------------------- which kernel runs a product
+
+
+class GroupedArgs(ctypes.Structure):
+    """pyc_grouped of csrc/kernels/grouped_args.h."""
+    _fields_ = [("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("x_rows", ctypes.c_int), ("rows", ctypes.c_void_p),
+                ("fan", ctypes.c_int), ("offsets", ctypes.c_void_p), ("E", ctypes.c_int), ("P", ctypes.c_int),
+                ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64), ("N", ctypes.c_int), ("K", ctypes.c_int),
+                ("scale", ctypes.c_void_p), ("zeros", ctypes.c_void_p), ("group", ctypes.c_int), ("bias", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64), ("epi", ctypes.c_int)]
+
+
+def form(w4, experts, rows, n, k, epi=0, x_rows=None, x_stride=None, dense=False, at=0x10000):
+    """(kernel, its argument) of a call on 16-byte boundaries (at: another address of x): 0 general, 1 ring,
+    2 tiles, 3 stream, 4 4-bit tiles."""
+    out = n // 2 if epi & GATE else n
+    g = GroupedArgs(at, k if x_stride is None else x_stride, rows if x_rows is None else x_rows, None, 1,
+                    None if dense else 0x10000, experts, rows, 0x10000, n * (k // 2 if w4 else k), n, k, None, None, 0, None,
+                    0x10000, out, epi)
+    arg = ctypes.c_int(-1)
+    f = pyc_amd.lib().pyc_hip_grouped_form
+    f.argtypes = [ctypes.c_int, ctypes.POINTER(GroupedArgs), ctypes.POINTER(ctypes.c_int)]
+    return f(int(w4), ctypes.byref(g), ctypes.byref(arg)), arg.value
 
 
 def check(got, ref, bound):

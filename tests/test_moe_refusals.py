@@ -57,6 +57,7 @@ def test_route_refusals(bad):
                                  dict(width=0), dict(width=(1 << 24) + 1), dict(y=None), dict(y=P + 1), dict(ys=63),
                                  dict(weights=None), dict(weights=P + 2), dict(places=None), dict(base=P + 1), dict(bs=60),
                                  dict(out=None), dict(out=P + 1), dict(os=10),
+                                 dict(tokens=1 << 16, width=1 << 16, ys=1 << 16, bs=1 << 16, os=1 << 16),
                                  dict(tokens=1 << 22, width=1 << 16, ys=1 << 16, bs=1 << 16, os=1 << 16)], ids=str)
 def test_combine_refusals(bad):
     assert _combine(**bad) == -1
