@@ -44,18 +44,14 @@ __device__ inline void lds_dma_buf_b32(i32x4 rsrc, uint32_t voff, uint32_t lds_b
                  : "memory", "m0");
 }
 
-// Eight codes as B + c in the order of x: pairs k 0,1 2,3 4,5 6,7. A byte has two codes; 3 bits up its
-// low one, 1 bit down its high one stand where the mantissa of B has its units.
+// Eight codes as B + c in the order of x: pairs k 0,1 2,3 4,5 6,7. A byte has two codes; the units of B are
+// 3 bits up in its mantissa, so byte * (2^3 + 2^15) has both in place, one to each half. m: 0x00780078, b: B twice.
 __device__ inline float code_base(bf16_t) { return 16.0f; }
 __device__ inline float code_base(f16_t) { return 128.0f; }
-template <typename T> __device__ inline u32x4 codes_in_order(uint32_t w, T) {
-    const uint32_t m = 0x00780078u, b = elem<T>::from_f32(code_base(T{})) * 0x10001u;
-    const uint32_t lo = w << 3, hi = w >> 1;
+__device__ inline u32x4 codes_in_order(uint32_t w, uint32_t m, uint32_t b) {
     u32x4 r;
-    r[0] = (__builtin_amdgcn_perm(hi, lo, 0x0c040c00u) & m) | b;
-    r[1] = (__builtin_amdgcn_perm(hi, lo, 0x0c050c01u) & m) | b;
-    r[2] = (__builtin_amdgcn_perm(hi, lo, 0x0c060c02u) & m) | b;
-    r[3] = (__builtin_amdgcn_perm(hi, lo, 0x0c070c03u) & m) | b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (((w >> (8 * i)) & 255u) * 0x8008u & m) | b;
     return r;
 }
 
@@ -160,38 +156,44 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
             for (int i = 0; i < CL; ++i) asm volatile("" : "+v"(co[i]));
 #pragma unroll
             for (int i = 0; i < SZ; ++i) asm volatile("" : "+v"(so[i]));
-            auto issue = [&](int s, int slot) __attribute__((always_inline)) {
+            // load i of a wave for step s
+            auto issue = [&](int i, int s, int slot) __attribute__((always_inline)) {
                 const uint32_t base = lds0 + (uint32_t)slot * STEP;
                 const int left = g.K - s * kW4K;  // k from this step on
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-                    lds_dma_buf_b128_u(x_rsrc, xk < left ? xo[i] : kW4PastEnd, (uint32_t)s * (kW4K * 2), base + (uint32_t)(NW * i + wave) * 1024);
-#pragma unroll
-                for (int i = 0; i < CL; ++i)
-                    lds_dma_buf_b128_u(w_rsrc, ck < left ? co[i] : kW4PastEnd, (uint32_t)s * (kW4K / 2),
-                                       base + X_BYTES + (uint32_t)(CL * wave + i) * 1024);
-#pragma unroll
-                for (int i = 0; i < SZ; ++i) {
-                    const int q = min(wave * SZ + i, DW - 1);
+                if (i < FM) {
+                    lds_dma_buf_b128_u(x_rsrc, xk < left ? xo[i < FM ? i : 0] : kW4PastEnd, (uint32_t)s * (kW4K * 2),
+                                       base + (uint32_t)(NW * i + wave) * 1024);
+                } else if (i < FM + CL) {
+                    const int j = i - FM;
+                    lds_dma_buf_b128_u(w_rsrc, ck < left ? co[j < CL ? j : 0] : kW4PastEnd, (uint32_t)s * (kW4K / 2),
+                                       base + X_BYTES + (uint32_t)(CL * wave + j) * 1024);
+                } else {
+                    const int j = i - FM - CL, q = min(wave * SZ + j, DW - 1);
                     const bool zero = q >= FN * NS;
-                    const uint32_t a = so[i] + (uint32_t)(s * NG);  // the first value's place
+                    const uint32_t o = so[j < SZ ? j : 0], a = o + (uint32_t)(s * NG);  // the first value's place
                     const uint32_t off = zero ? ((a >> 2) + (uint32_t)(q / FN - NS)) * 4 : ((a >> 1) + (uint32_t)(q / FN)) * 4;
-                    lds_dma_buf_b32(zero ? z_rsrc : s_rsrc, so[i] == kW4PastEnd ? kW4PastEnd : off,
+                    lds_dma_buf_b32(zero ? z_rsrc : s_rsrc, o == kW4PastEnd ? kW4PastEnd : off,
                                     __builtin_amdgcn_readfirstlane(base + X_BYTES + CODE_BYTES + (uint32_t)q * 256));
                 }
             };
 
             f32x4 acc[FM][FN], part[FM][FN], sum[FM];
+            constexpr int NV = NG > 2 ? 2 : 1, HALVES = GATE && FN > 1 ? 2 : 1;
             u32x4 fa[2][FM], cw[FN];
-            uint32_t sv[FN][2], zv[FN], sp[FN], zp[FN];
+            uint32_t sv[FN][NV], zv[FN];
+            // how far into its dword a slot's first scale and zero point of step 0 stand, in bits (above the lowest five:
+            // whole dwords). Slots 16 rows of W apart agree; gated, a wave's gates do and its values do.
+            uint32_t sp[HALVES], zp[HALVES];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const int n = max(weight_row(16 * (FN * wn + j) + lrow), 0);
-                sp[j] = (uint32_t)n * (uint32_t)groups + s_mis;
-                zp[j] = (uint32_t)n * (uint32_t)groups + z_mis;
+            for (int h = 0; h < HALVES; ++h) {
+                const int n = max(weight_row(16 * FN * wn + YC * h + lrow), 0);
+                sp[h] = ((uint32_t)n * (uint32_t)groups + s_mis) * 16;
+                zp[h] = ((uint32_t)n * (uint32_t)groups + z_mis) * 8;
+            }
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
 #pragma unroll
                 for (int i = 0; i < FM; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
             auto read_x = [&](int b, int slot, int ks) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
@@ -205,18 +207,21 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
                     cw[j] = *reinterpret_cast<const u32x4*>(c + j * 1024);
-                    const uint32_t ss = ((sp[j] + (uint32_t)(s * NG)) & 1) * 16, zs = ((zp[j] + (uint32_t)(s * NG)) & 3) * 8;
+                    const int h = j * HALVES / FN;
+                    const uint32_t ss = sp[h] + (uint32_t)(s * NG * 16), zs = zp[h] + (uint32_t)(s * NG * 8);  // alignbit takes five bits
                     const uint32_t d0 = d[16 * j], d1 = NS > 1 ? d[COLS + 16 * j] : 0;
                     sv[j][0] = __builtin_amdgcn_alignbit(d1, d0, ss);
-                    if constexpr (NS > 2) sv[j][1] = __builtin_amdgcn_alignbit(d[2 * COLS + 16 * j], d1, ss);
+                    if constexpr (NS > 2) sv[j][NV - 1] = __builtin_amdgcn_alignbit(d[2 * COLS + 16 * j], d1, ss);
                     const uint32_t z0 = d[NS * COLS + 16 * j], z1 = NZ > 1 ? d[(NS + 1) * COLS + 16 * j] : 0;
                     zv[j] = __builtin_amdgcn_alignbit(z1, z0, zs);
                 }
             };
 
 #pragma unroll
-            for (int s = 0; s < S; ++s) issue(s, s);
-            wait_vmem_le<(S - 1) * LOADS>();
+            for (int s = 0; s < S - 1; ++s)
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) issue(i, s, s);
+            wait_vmem_le<(S - 2) * LOADS>();
             __syncthreads();
             read_x(0, 0, 0);
             read_w(0, 0);
@@ -224,23 +229,27 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                 const uint32_t o = elem<T>::from_f32(1.0f) * 0x10001u;
                 return u32x4{o, o, o, o};
             }();
-            int slot = 0;
+            uint32_t mask = 0x00780078u, base = elem<T>::from_f32(code_base(T{})) * 0x10001u;
+            asm volatile("" : "+v"(mask), "+v"(base));  // in registers: and-or takes one constant at most
+            int slot = 0, into = S - 1;
 #pragma unroll 1
             for (int s = 0; s < steps; ++s) {
                 const int next = slot == S - 1 ? 0 : slot + 1;
 #pragma unroll
                 for (int j = 0; j < FN; ++j) transpose4(cw[j]);
-                u32x4 c[FN];
-                uint32_t svn[FN][2], zvn[FN];
-#pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    c[j] = cw[j];
-                    svn[j][0] = sv[j][0];
-                    svn[j][1] = sv[j][1];
-                    zvn[j] = zv[j];
-                }
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
+                    const bool first = ks % (G / 32) == 0, last = (ks + 1) % (G / 32) == 0;
+                    float f[FN], z[FN];
+                    uint32_t c[FN];
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) {
+                        const int q = ks / (G / 32);
+                        const bool there = NG == 1 || s * NG + q < groups;  // what lies behind the row is another's
+                        f[j] = there ? elem<T>::to_f32((uint16_t)(sv[j][q < 2 ? 0 : NV - 1] >> (16 * (q & 1)))) : 0.f;
+                        z[j] = -code_base(T{}) - (g.zeros ? (float)((zv[j] >> (8 * q)) & 255u) : 8.0f);
+                        c[j] = cw[j][ks];
+                    }
                     if (ks < 3) {
                         read_x((ks + 1) & 1, slot, ks + 1);
                     } else {
@@ -248,11 +257,9 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         wait_vmem_le<(S - 2) * LOADS>();
                         __syncthreads();
-                        issue(s + S, slot);
                         read_x(0, next, 0);
                         read_w(s + 1, next);
                     }
-                    const bool first = ks % (G / 32) == 0, last = (ks + 1) % (G / 32) == 0;
                     if (first) {
 #pragma unroll
                         for (int i = 0; i < FM; ++i) {
@@ -265,26 +272,28 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                     for (int i = 0; i < FM; ++i) sum[i] = mfma16x16x32(fa[ks & 1][i], one, sum[i], T{});
 #pragma unroll
                     for (int j = 0; j < FN; ++j) {
-                        const u32x4 w = codes_in_order(c[j][ks], T{});
+                        const u32x4 w = codes_in_order(c[j], mask, base);
 #pragma unroll
                         for (int i = 0; i < FM; ++i) part[i][j] = mfma16x16x32(fa[ks & 1][i], w, part[i][j], T{});
+                        // the loads of the step that takes the place of the one before, a few between the products
+                        if (ks < 3) {
+                            constexpr int PLACES = 3 * FN;
+                            const int q = ks * FN + j;
+#pragma unroll
+                            for (int i = q * LOADS / PLACES; i < (q + 1) * LOADS / PLACES; ++i) issue(i, s + S - 1, into);
+                        }
                     }
                     if (last) {
-                        const int q = ks / (G / 32);
-                        const bool there = s * NG + q < groups;  // what lies behind the row is another's
 #pragma unroll
-                        for (int j = 0; j < FN; ++j) {
-                            const uint32_t raw = q < 2 ? svn[j][0] : svn[j][1];
-                            const float f = there ? elem<T>::to_f32((uint16_t)(raw >> (16 * (q & 1)))) : 0.f;
-                            const float z = -code_base(T{}) - (g.zeros ? (float)((zvn[j] >> (8 * q)) & 255u) : 8.0f);
+                        for (int j = 0; j < FN; ++j)
 #pragma unroll
                             for (int i = 0; i < FM; ++i)
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
-                                    acc[i][j][r] = fmaf(f, fmaf(z, sum[i][r], part[i][j][r]), acc[i][j][r]);
-                        }
+                                    acc[i][j][r] = fmaf(f[j], fmaf(z[j], sum[i][r], part[i][j][r]), acc[i][j][r]);
                     }
                 }
+                into = slot;
                 slot = next;
             }
             wait_vmem_le<0>();
