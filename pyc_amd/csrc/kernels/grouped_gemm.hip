@@ -211,10 +211,12 @@ extern "C" int pyc_hip_grouped_w4_tile_launch(int is_bf16, const pyc_grouped* g,
 //  16-bit: the ring's tiles of 64 rows x 64 columns; of 128 columns where those fill the CUs twice (8 of
 //    4096 x 4096: P = 256 62 / 74, 1024 87 / 98); 256 x 256 tiles from some 200 rows an expert on, or
 //    100 in large calls (8 of 4096 x 4096: P = 2048 111 / 129, 1024 109 / 87; 64 of 2048 x 2816: P = 8192 207 / 292).
-//  4-bit: streamed up to 16 rows an expert (dense: 32); then the smallest tiles that are no more than 3 in
-//    two places (4096 x 11008: P = 64 27 / 34 streamed, 512 108 / 217 in tiles of 16 rows; 2048 x 1024: P = 512
-//    15 / 18 in tiles of 64), and 128 x 256 from 96 rows an expert on in large calls (4096 x
-//    11008: P = 256 99 / 57, 512 103 / 108; 32 of 4096 x 2816: P = 4096 222 / 287).
+//  4-bit: streamed up to 6 rows an expert (32 of 4096 x 2816: P = 128 60 / 67 in tiles, 256 75 / 71), or where
+//    columns are so few that only parts of K fill the CUs (11008 x 4096: P = 32 27 / 53, 64 48 / 57, 128 81 / 63; 4096 x
+//    11008: P = 16 16.5 / 14.8, 24 25 / 19); then the smallest tiles that are no more than 3 in two places (4096 x 11008: P = 48
+//    25 / 29 in tiles of 16 rows, 128 33 / 54; 11008 x 4096: P = 128 63 / 80 in tiles of 64), and 128 x 256 from 96
+//    rows an expert on where they fill half of the CUs (4096 x 11008: P = 256 66 / 53, 512 69 / 101; 32 of 4096 x
+//    2816: P = 4096 189 / 263; 8 of 2048 x 2048: P = 2048 41 / 46).
 // KIND: 0 the general kernel, 1 ring, 2 tiles, 3 stream, 4 4-bit tiles; arg: what its launch takes.
 extern "C" int pyc_hip_grouped_form(int w4, const pyc_grouped* g, int* arg) {
     using namespace pyc;
@@ -226,10 +228,11 @@ extern "C" int pyc_hip_grouped_form(int w4, const pyc_grouped* g, int* arg) {
         *arg = P * N >= 512 * 4096 ? 2 : 1;
         return 1;
     }
-    if (P <= 16 * E || P <= 32) return 3;
-    if (P >= 96 * E && P * N >= 170 * 128 * 256) return 4;
+    auto tiles = [&](int rows) { return g->offsets ? expert_tiles_most((int)E, g->P, rows) : (P + rows - 1) / rows; };
+    if (P <= 6 * E || tiles(16) * N <= 16384) return 3;
+    if (P >= 96 * E && P * N >= 128 * 128 * 256) return 4;
     const int64_t blocks = (N + 63) / 64;
-    *arg = expert_tiles_most((int)E, g->P, 16) * blocks <= 384 ? 1 : expert_tiles_most((int)E, g->P, 32) * blocks <= 384 ? 2 : 4;
+    *arg = tiles(16) * blocks <= 384 ? 1 : tiles(32) * blocks <= 384 ? 2 : 4;
     return 4;
 }
 

@@ -4,11 +4,16 @@
 // unpacks or scales while the other multiplies), K in steps of 128. x, codes, scales and
 // zero points of a step come by LDS-DMA into a ring of three, so that two steps are on their way
 // while one is used, and no wait for one kind of load drains the others. The formula is the one of
-// grouped_stream.hip: a code goes into the mantissa of 16, and for each group
-//   acc += scale (sum x (16 + code) - (16 + zero) sum x),
+// grouped_stream.hip: a code goes into the mantissa of B = 16 (fp16: 128), and for each group
+//   acc += scale (sum x (B + code) - (B + zero) sum x),
 // with sum x from products by ones. Weights are never rounded, which costs a second set of sums
-// and two vector instructions for each result and group: bound by those for groups of 32
-// and 64, by both kinds of instructions for groups of 128.
+// and two vector instructions for each result and group. Bound by the vector instructions: to 80
+// matrix instructions a wave issues 337 in a step of 128 (128 of them unpack, 128 scale), 3340 cycles for
+// the two waves of a SIMD where the matrix units need 2560. A step takes some 4900, a tile 10 us for its
+// start and end. 1999 x 11008 x 4096 with groups of 128: 223 us, 0.81 PFLOP/s (groups of 64 about 1.15 times
+// that, of 32 1.5 times). Measured and not kept: all loads of a step at once (310 us with the values of a step kept in
+// registers throughout); scaling a group among the next one's products (239); the two waves of a SIMD half a step
+// apart, which leaves loads one step instead of two (241); two workgroups of 64 rows a CU (267).
 //
 // Scales and zero points are 2-byte and 1-byte values at any alignment, LDS-DMA moves aligned
 // dwords: the dwords that hold a row's values of the step are fetched (1 to 3, 1 or 2), and the

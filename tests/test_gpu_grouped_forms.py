@@ -18,7 +18,7 @@ SIXTEEN = [(2, 0, [700, 324], 8192, [64, 72]), (2, 0, RAGGED, 16416, [64, 200]),
            (0, 0, [30, 0, 64, 200, 3], 1000, [63, 129, 20])]
 # (kernel, argument, rows of each expert, N, depths by group); a single expert: the dense product too
 FOUR = [(4, 0, [300, 65, 10, 325], 8200, {32: [96], 64: [448], 128: [128, 640]}), (4, 0, [700], 8192, {32: [416], 64: [64], 128: [384]}),
-        (4, 1, [200], 1200, {32: [32, 544], 64: [192], 128: [1152]}), (4, 1, [90, 0, 107, 3], 1000, {32: [480], 64: [320], 128: [256]}),
+        (4, 1, [200], 1264, {32: [32, 544], 64: [192], 128: [1152]}), (4, 1, [90, 0, 107, 3], 1040, {32: [480], 64: [320], 128: [256]}),
         (4, 2, [200], 2000, {32: [160], 64: [576], 128: [384]}), (4, 2, [90, 0, 107, 3], 2000, {32: [96], 64: [128], 128: [512]}),
         (4, 4, [200], 3600, {32: [352], 64: [64], 128: [256]}), (4, 4, [90, 0, 107, 3], 3600, {32: [96], 64: [192], 128: [256]}),
         # streamed: x through LDS in one turn and in several, beside the weights; scales in turns
