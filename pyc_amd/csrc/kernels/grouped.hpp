@@ -2,6 +2,8 @@
 // expert, the row of x behind a row of y, and the epilogue.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 #include "grouped_args.h"
 
@@ -89,6 +91,20 @@ __device__ inline void transpose4(u32x4& w) {
     auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
     auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
     w = u32x4{c[0], c[1], d[0], d[1]};
+}
+
+// Eight codes as 16 + c, exact in either type, pairs k 0,1 2,3 4,5 6,7. A byte has two codes; the units of 16 are s
+// bits up in its mantissa (bf16: 3, fp16: 6), so byte * (2^s + 2^(s + 12)) has one code in place in each half: a
+// multiplication (which takes a byte of a register as it is) and an and-or for each pair. b: 16 twice, m: the codes' bits;
+// both best in registers.
+__device__ inline uint32_t codes16_mask(bf16_t) { return 0x00780078u; }
+__device__ inline uint32_t codes16_mask(f16_t) { return 0x03c003c0u; }
+template <typename T> __device__ inline u32x4 codes16(uint32_t w, uint32_t m, uint32_t b, T) {
+    constexpr uint32_t f = std::is_same_v<T, bf16_t> ? 0x8008u : 0x40040u;
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (((w >> (8 * i)) & 255u) * f & m) | b;
+    return r;
 }
 
 // v of the lane eight further on in each row of 16, around its end.

@@ -23,8 +23,7 @@
 // mantissa of 16, as 16 + c exactly, two to two instructions; a group's sum is then
 //   scale (sum x (16 + c) - (16 + zero) sum x),
 // all in fp32, with sum x from one more product by ones. (By conversion to whole numbers less
-// zero a pair takes three to four times the instructions. 128 + c, which needs a shift less, has
-// six times the cancellation.) Pairs come out as k 0,4 1,5 2,6 3,7, so x is put in that order.
+// zero a pair takes three to four times the instructions.)
 #include "grouped.hpp"
 
 namespace pyc {
@@ -40,20 +39,6 @@ struct StreamLds {
 constexpr StreamLds kStreamLds[2][2] = {{{63 * 1024, 4096}, {111 * 1024, 12032}}, {{16 * 1024, 15872}, {16 * 1024, 36352}}};
 constexpr size_t stream_lds_bytes(const StreamLds& l) { return l.x + 4 * l.scales; }
 constexpr uint32_t kPastEnd = 0xFFFFFFF0u;  // not below any descriptor's byte count
-
-// Eight codes as 16 + c, pairs k 0,4 1,5 2,6 3,7.
-__device__ inline u32x4 codes16(uint32_t w, uint32_t m, uint32_t b, bf16_t) {  // 3 bits below the units of 16.0
-    return u32x4{((w << 3) & m) | b, ((w >> 1) & m) | b, ((w >> 5) & m) | b, ((w >> 9) & m) | b};
-}
-__device__ inline u32x4 codes16(uint32_t w, uint32_t m, uint32_t b, f16_t) {  // 6 bits
-    return u32x4{((w << 6) & m) | b, ((w << 2) & m) | b, ((w >> 2) & m) | b, ((w >> 6) & m) | b};
-}
-__device__ inline uint32_t codes16_mask(bf16_t) { return 0x00780078u; }
-__device__ inline uint32_t codes16_mask(f16_t) { return 0x03c003c0u; }
-__device__ inline u32x4 paired(const u32x4& x) {
-    return u32x4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
-                 __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
-}
 
 // G: k of a group. XD: x is loaded beside W. tiles_n: column blocks, wgs: workgroups they take.
 template <typename T, int G, bool XD>
@@ -163,7 +148,7 @@ grouped_stream_kernel(Grouped g, int tiles_n, int wgs, int ks, int x_lds, int wo
                 const int64_t s = src[r];
                 u32x4 v = u32x4{0, 0, 0, 0};
                 if (k < n && s >= 0) v = *reinterpret_cast<const u32x4*>(g.x + s + k0 + k);
-                *reinterpret_cast<u32x4*>(smem + r * pitch + 2 * k) = paired(v);
+                *reinterpret_cast<u32x4*>(smem + r * pitch + 2 * k) = v;
             }
         }
         const int gshift = __builtin_ctz(span / G), q0 = k0 / G;
@@ -217,7 +202,7 @@ grouped_stream_kernel(Grouped g, int tiles_n, int wgs, int ks, int x_lds, int wo
             }
 #pragma unroll
             for (int j = q * (4 / NG); j < (q + 1) * (4 / NG); ++j) {
-                const u32x4 x = XD ? paired(c.x[XD ? j : 0]) : *reinterpret_cast<const u32x4*>(row + 64 * j);
+                const u32x4 x = XD ? c.x[XD ? j : 0] : *reinterpret_cast<const u32x4*>(row + 64 * j);
                 sum = mfma16x16x32(x, one, sum, T{});
 #pragma unroll
                 for (int f = 0; f < CF; ++f) part[f] = mfma16x16x32(x, codes16(c.w[f][j], mask, base16, T{}), part[f], T{});

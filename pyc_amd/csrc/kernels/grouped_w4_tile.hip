@@ -4,15 +4,14 @@
 // unpacks or scales while the other multiplies), K in steps of 128. x, codes, scales and
 // zero points of a step come by LDS-DMA into a ring of three, so that two steps are on their way
 // while one is used, and no wait for one kind of load drains the others. The formula is the one of
-// grouped_stream.hip: a code goes into the mantissa of B = 16 (fp16: 128), and for each group
-//   acc += scale (sum x (B + code) - (B + zero) sum x),
+// grouped_stream.hip: a code goes into the mantissa of 16, and for each group
+//   acc += scale (sum x (16 + code) - (16 + zero) sum x),
 // with sum x from products by ones. Weights are never rounded, which costs a second set of sums
 // and two vector instructions for each result and group. Bound by the vector instructions: to 80
 // matrix instructions a wave issues 337 in a step of 128 (128 of them unpack, 128 scale), 3340 cycles for
 // the two waves of a SIMD where the matrix units need 2560. A step takes some 4900, a tile 10 us for its
 // start and end. 1999 x 11008 x 4096 with groups of 128: 223 us, 0.81 PFLOP/s (groups of 64 about 1.15 times
-// that, of 32 1.5 times). Measured and not kept: all loads of a step at once (310 us with the values of a step kept in
-// registers throughout); scaling a group among the next one's products (239); the two waves of a SIMD half a step
+// that, of 32 1.5 times). Measured and not kept: scaling a group among the next one's products (239); the two waves of a SIMD half a step
 // apart, which leaves loads one step instead of two (241); two workgroups of 64 rows a CU (267).
 //
 // Scales and zero points are 2-byte and 1-byte values at any alignment, LDS-DMA moves aligned
@@ -47,17 +46,6 @@ __device__ inline void lds_dma_buf_b32(i32x4 rsrc, uint32_t voff, uint32_t lds_b
                  :
                  : "s"(lds_base), "v"(voff), "s"(rsrc)
                  : "memory", "m0");
-}
-
-// Eight codes as B + c in the order of x: pairs k 0,1 2,3 4,5 6,7. A byte has two codes; the units of B are
-// 3 bits up in its mantissa, so byte * (2^3 + 2^15) has both in place, one to each half. m: 0x00780078, b: B twice.
-__device__ inline float code_base(bf16_t) { return 16.0f; }
-__device__ inline float code_base(f16_t) { return 128.0f; }
-__device__ inline u32x4 codes_in_order(uint32_t w, uint32_t m, uint32_t b) {
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (((w >> (8 * i)) & 255u) * 0x8008u & m) | b;
-    return r;
 }
 
 template <typename T, int G, bool GATE, int WM, int FN, int FMX>
@@ -234,7 +222,7 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                 const uint32_t o = elem<T>::from_f32(1.0f) * 0x10001u;
                 return u32x4{o, o, o, o};
             }();
-            uint32_t mask = 0x00780078u, base = elem<T>::from_f32(code_base(T{})) * 0x10001u;
+            uint32_t mask = codes16_mask(T{}), base = elem<T>::from_f32(16.0f) * 0x10001u;
             asm volatile("" : "+v"(mask), "+v"(base));  // in registers: and-or takes one constant at most
             int slot = 0, into = S - 1;
 #pragma unroll 1
@@ -252,7 +240,7 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                         const int q = ks / (G / 32);
                         const bool there = NG == 1 || s * NG + q < groups;  // what lies behind the row is another's
                         f[j] = there ? elem<T>::to_f32((uint16_t)(sv[j][q < 2 ? 0 : NV - 1] >> (16 * (q & 1)))) : 0.f;
-                        z[j] = -code_base(T{}) - (g.zeros ? (float)((zv[j] >> (8 * q)) & 255u) : 8.0f);
+                        z[j] = -16.0f - (g.zeros ? (float)((zv[j] >> (8 * q)) & 255u) : 8.0f);
                         c[j] = cw[j][ks];
                     }
                     if (ks < 3) {
@@ -277,7 +265,7 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                     for (int i = 0; i < FM; ++i) sum[i] = mfma16x16x32(fa[ks & 1][i], one, sum[i], T{});
 #pragma unroll
                     for (int j = 0; j < FN; ++j) {
-                        const u32x4 w = codes_in_order(c[j], mask, base);
+                        const u32x4 w = codes16(c[j], mask, base, T{});
 #pragma unroll
                         for (int i = 0; i < FM; ++i) part[i][j] = mfma16x16x32(fa[ks & 1][i], w, part[i][j], T{});
                         // the loads of the step that takes the place of the one before, a few between the products
