@@ -108,6 +108,6 @@ extern "C" int pyc_hip_kinfo_moe_combine(int is_bf16, pyc_hip_kinfo* out) {
     out->name = "moe_combine_kernel";
     out->lds_bytes = 0;
     out->threads = kCombineThreads;
-    out->waves_per_simd = 8;
+    out->waves_per_simd = 6;
     return 0;
 }
