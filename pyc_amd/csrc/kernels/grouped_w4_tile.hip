@@ -4,15 +4,17 @@
 // unpacks or scales while the other multiplies), K in steps of 128. x, codes, scales and
 // zero points of a step come by LDS-DMA into a ring of three, so that two steps are on their way
 // while one is used, and no wait for one kind of load drains the others. The formula is the one of
-// grouped_stream.hip: a code goes into the mantissa of 16, and for each group
-//   acc += scale (sum x (16 + code) - (16 + zero) sum x),
-// with sum x from products by ones. Weights are never rounded, which costs a second set of sums
-// and two vector instructions for each result and group. Bound by the vector instructions: to 80
-// matrix instructions a wave issues 337 in a step of 128 (128 of them unpack, 128 scale), 3340 cycles for
-// the two waves of a SIMD where the matrix units need 2560. A step takes some 4900, a tile 10 us for its
-// start and end. 1999 x 11008 x 4096 with groups of 128: 223 us, 0.81 PFLOP/s (groups of 64 about 1.15 times
-// that, of 32 1.5 times). Measured and not kept: scaling a group among the next one's products (239); the two waves of a SIMD half a step
-// apart, which leaves loads one step instead of two (241); two workgroups of 64 rows a CU (267).
+// grouped_stream.hip: a code goes into the mantissa of 16, and the groups' sums are
+//   sum_g scale_g (sum x (16 + code)) - sum_g scale_g (16 + zero_g) (sum x),
+// with sum x from products by ones. The second part is a product itself, over groups: a matrix
+// instruction in fp32 takes four groups of it, in place of a vector instruction for each result
+// and group (groups of 32 690 -> 663 us, of 64 536 -> 514, of 128 448 -> 444; 2048 x 11008 x 8192). Weights are
+// never rounded, which costs a second set of sums, a vector instruction for each result and group, and the sums of x,
+// a fifth of the matrix instructions. What bounds it: both kinds of instructions, about half of the cycles each
+// at the 2.0 GHz that the card holds under them, and the ends of tiles, 10 us each.
+// 1999 x 11008 x 4096 with groups of 128: 223 us, 0.81 PFLOP/s (groups of 64 about 1.13 times that, of 32 1.4
+// times). Measured and not kept: scaling a group among the next one's products (239); the two waves of a SIMD half a
+// step apart, which leaves loads one step instead of two (241); two workgroups of 64 rows a CU (267).
 //
 // Scales and zero points are 2-byte and 1-byte values at any alignment, LDS-DMA moves aligned
 // dwords: the dwords that hold a row's values of the step are fetched (1 to 3, 1 or 2), and the
@@ -224,6 +226,18 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
             }();
             uint32_t mask = codes16_mask(T{}), base = elem<T>::from_f32(16.0f) * 0x10001u;
             asm volatile("" : "+v"(mask), "+v"(base));  // in registers: and-or takes one constant at most
+            // sums of x (lane: row lrow) and scales times -(16 + zero) of the last four groups, one to a lane group
+            float sa[FM], sb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) sa[i] = 0.f;
+#pragma unroll
+            for (int j = 0; j < FN; ++j) sb[j] = 0.f;
+            auto zero_points = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sa[i], sb[j], acc[i][j], 0, 0, 0);
+            };
             int slot = 0, into = S - 1;
 #pragma unroll 1
             for (int s = 0; s < steps; ++s) {
@@ -233,14 +247,14 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
                     const bool first = ks % (G / 32) == 0, last = (ks + 1) % (G / 32) == 0;
-                    float f[FN], z[FN];
+                    float f[FN], fz[FN];
                     uint32_t c[FN];
 #pragma unroll
                     for (int j = 0; j < FN; ++j) {
                         const int q = ks / (G / 32);
                         const bool there = NG == 1 || s * NG + q < groups;  // what lies behind the row is another's
                         f[j] = there ? elem<T>::to_f32((uint16_t)(sv[j][q < 2 ? 0 : NV - 1] >> (16 * (q & 1)))) : 0.f;
-                        z[j] = -16.0f - (g.zeros ? (float)((zv[j] >> (8 * q)) & 255u) : 8.0f);
+                        fz[j] = f[j] * (-16.0f - (g.zeros ? (float)((zv[j] >> (8 * q)) & 255u) : 8.0f));
                         c[j] = cw[j][ks];
                     }
                     if (ks < 3) {
@@ -262,7 +276,7 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < FM; ++i) sum[i] = mfma16x16x32(fa[ks & 1][i], one, sum[i], T{});
+                    for (int i = 0; i < FM; ++i) sum[i] = mfma16x16x32(one, fa[ks & 1][i], sum[i], T{});
 #pragma unroll
                     for (int j = 0; j < FN; ++j) {
                         const u32x4 w = codes16(c[j], mask, base, T{});
@@ -277,17 +291,29 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                         }
                     }
                     if (last) {
+                        const int turn = (s * NG + ks / (G / 32)) & 3;
 #pragma unroll
-                        for (int j = 0; j < FN; ++j)
+                        for (int j = 0; j < FN; ++j) {
+                            sb[j] = lgrp == turn ? fz[j] : sb[j];
 #pragma unroll
                             for (int i = 0; i < FM; ++i)
 #pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    acc[i][j][r] = fmaf(f[j], fmaf(z[j], sum[i][r], part[i][j][r]), acc[i][j][r]);
+                                for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(f[j], part[i][j][r], acc[i][j][r]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < FM; ++i) sa[i] = lgrp == turn ? sum[i][0] : sa[i];
+                        if (turn == 3) zero_points();
                     }
                 }
                 into = slot;
                 slot = next;
+            }
+            if (const int rest = steps * NG & 3; rest) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i) sa[i] = lgrp < rest ? sa[i] : 0.f;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) sb[j] = lgrp < rest ? sb[j] : 0.f;
+                zero_points();
             }
             wait_vmem_le<0>();
             __syncthreads();  // the ring is free: results go through it
