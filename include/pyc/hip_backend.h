@@ -337,8 +337,8 @@ int pyc_hip_grouped_gemm_dispatch(
  *   scale [N][K / group], zeros [N][K / group] bytes, or NULL: 8.
  *   y[M][N] = epi(x[M][K] w^T + bias), epilogues as above (bias fp32 [N]).
  * Whole numbers times x are summed as they are, the scale comes in fp32: weights are
- * never rounded. Finite x. Any M and N, K a multiple of group; x and codes on 16-byte boundaries, x_stride a
- * multiple of 8. Symbols "hip_gemm_w4a16_bf16", "hip_gemm_w4a16_f16". 0, -1, -2 as above. */
+ * never rounded. x finite, the sums of |x| and |scale x| along K below 2^122 (those of x (16 + code) and of
+ * x (16 + zero) are taken apart). Any M and N, K a multiple of group; x and codes on 16-byte boundaries, x_stride a multiple of 8. Symbols "hip_gemm_w4a16_bf16", "hip_gemm_w4a16_f16". 0, -1, -2 as above. */
 int pyc_hip_w4a16_gemm_dispatch(
     const char* symbol, int M, int N, int K, int group, const void* x, int64_t x_stride,
     const void* codes, const void* scale, const uint8_t* zeros, const float* bias, int epilogue,

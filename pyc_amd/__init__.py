@@ -532,7 +532,7 @@ def grouped_gemm(x, w, offsets, y, rows=None, fan: int = 1, bias=None, epilogue:
     """y[p] = epi(x[rows[p] // fan] w[e]^T + bias[e]) for offsets[e] <= p < offsets[e + 1]
     (pyc_hip_grouped_gemm_dispatch): x [n, K], w [E, N, K] and y [rows, N] bf16 or f16, offsets
     [E + 1] and rows int32 as moe_route leaves them (rows None: row p of x), bias [E, N]
-    float32. epilogue: 0, 2 (ReLU) or 4 (SiLU gate: y is [rows, N / 2])."""
+    float32. epilogue: 0, abi.EPI_RELU or abi.EPI_SILU_GATE (y is [rows, N / 2])."""
     i32, f32, _, current, half, _ = _moe_env or _make_moe_env()
     dtype, device, xshape, wshape, yshape = x.dtype, x.get_device(), x.shape, w.shape, y.shape
     xstride, wstride, ystride, suffix = x.stride(), w.stride(), y.stride(), half.get(dtype)

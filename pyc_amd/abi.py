@@ -31,7 +31,7 @@ HW_ANY, HW_GENERIC, HW_ADA, HW_HOPPER, HW_CDNA4 = range(5)
 MODE_BALANCED, MODE_MEMORY_FIRST, MODE_UTILIZATION_FIRST = range(3)
 STATUS_OK, STATUS_INVALID_ARGUMENT, STATUS_VERIFY_FAILED, STATUS_COMPILE_FAILED, STATUS_RUNTIME_FAILED = range(5)
 DISPATCH_OK, DISPATCH_FALLBACK, DISPATCH_ERROR = range(3)
-EPI_NONE, EPI_BIAS, EPI_RELU = 0, 1, 2
+EPI_NONE, EPI_BIAS, EPI_RELU, EPI_SILU_GATE = 0, 1, 2, 4
 
 
 class Shape(C.Structure):
