@@ -10,7 +10,7 @@
 //              t * k + j in ascending order, -1 behind the last expert's;
 //              places[t * k + j] the position of a flat index in rows, -1 without expert.
 //
-// A wave for a token, its logits in registers (E <= 1024: up to 16 a lane). One of the k
+// A wave for two tokens, their logits in registers (E <= 1024: up to 16 a lane). One of the k
 // steps: the largest value by lanes, the lowest expert that has it by ballots, which
 // costs no more with ties. A token takes an expert once, so 32 tokens' choices are one
 // word of bits for each expert: setting bits needs no order, and the rank of a token
@@ -20,10 +20,11 @@
 // 32 tokens' words in the workspace and the second adds up the words before its own.
 //
 // Bound by latency: the logits are read once (2 MB of 8200 tokens by 128 experts, under
-// 1 us), the k steps of a token follow on each other, and the second launch waits for the
-// first. Times of a call, cold logits: 8200 tokens by 128 experts, 8 chosen 16.7 us (27.0
-// with the wave's maximum through LDS and eight blocks to every workgroup of the second
-// launch); 32 tokens by 64 experts 8.8 us, most of it the host's.
+// 1 us), the k choices of a token follow on each other (a wave makes those of two tokens side by
+// side), and the second launch waits for the first. 32 tokens by 64 experts, 8 chosen: 7.8 us a
+// call, 7.6 on the device (8.8 one token after the other, ids read back from memory). 8200 tokens by
+// 128 experts 17 us, 10 and 7 on the device (27 with the wave's maximum through LDS and eight
+// blocks to every workgroup of the second launch).
 #include "common.hpp"
 
 namespace pyc {
@@ -77,54 +78,88 @@ __device__ inline float wave_sum(float v) {
     return last_lane(v);
 }
 
-// One wave: token t's choices, its bit in the block's words (LDS).
-template <int DT, int NV> __device__ inline void route_token(const Route& r, int t, uint32_t* words, int lane) {
+// One wave: the choices of tokens t and t + kRouteWaves (below t1), side by side, for each depends on the one before;
+// their bits in the words of blocks (LDS), and the ids there too where `kept` is given.
+template <int DT, int NV>
+__device__ inline void route_tokens(const Route& r, int t, int t1, uint32_t* words, int16_t* kept, int lane) {
     constexpr float kNone = -INFINITY;
-    float v[NV];
+    constexpr int NT = 2;
+    float v[NT][NV], m[NT], s[NT], p[NT], top[NT];
+    int mine[NT];  // lane j: choice j
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int e = i * kWave + lane;
-        const float l = e < r.E ? route_logit<DT>(r.logits, (int64_t)t * r.stride + e) : kNone;
-        v[i] = l == l ? l : kNone;
-    }
-    float m = v[0];
-#pragma unroll
-    for (int i = 1; i < NV; ++i) m = fmaxf(m, v[i]);
-    m = wave_max(m);
-    auto power = [&](float l) { return l == m ? 1.0f : expf(l - m); };  // m infinite: 1 or 0
-    float s = 0.f;
-    if (!r.normalize && m > kNone) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) s += v[i] > kNone ? power(v[i]) : 0.f;
-        s = wave_sum(s);
-    }
-    int mine = -1;       // lane j: choice j
-    float p = 0.f;
-    float top = m;
-    for (int j = 0; j < r.k && top > kNone; ++j) {
-        int best = -1;
-#pragma unroll
-        for (int i = NV - 1; i >= 0; --i) {
-            const uint64_t is = __ballot(v[i] == top);
-            best = is ? i * kWave + __builtin_ctzll(is) : best;
-        }
-        if (lane == j) {
-            mine = best;
-            p = power(top);
-        }
-        float left = kNone;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            v[i] = i * kWave + lane == best ? kNone : v[i];
-            left = fmaxf(left, v[i]);
+            const int e = i * kWave + lane, tn = min(t + n * kRouteWaves, t1 - 1);
+            v[n][i] = route_logit<DT>(r.logits, (int64_t)tn * r.stride + min(e, r.E - 1));
         }
-        top = wave_max(left);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const float l = v[n][i];
+            v[n][i] = i * kWave + lane < r.E && l == l ? l : kNone;
+        }
+        m[n] = v[n][0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) m[n] = fmaxf(m[n], v[n][i]);
     }
-    if (r.normalize) s = wave_sum(p);
-    if (lane < r.k) {
-        r.ids[(int64_t)t * r.k + lane] = mine;
-        r.weights[(int64_t)t * r.k + lane] = mine >= 0 ? p / s : 0.f;
-        if (mine >= 0) atomicOr(&words[mine], 1u << (t % kRouteBlock));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) top[n] = m[n] = wave_max(m[n]);
+    auto power = [&](int n, float l) { return l == m[n] ? 1.0f : expf(l - m[n]); };  // m infinite: 1 or 0
+    if (!r.normalize) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            s[n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) s[n] += v[n][i] > kNone ? power(n, v[n][i]) : 0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n] = wave_sum(s[n]);
+    }
+    float chosen[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        mine[n] = -1;
+        chosen[n] = kNone;
+    }
+    for (int j = 0; j < r.k; ++j) {
+        float left[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            int best = -1;
+#pragma unroll
+            for (int i = NV - 1; i >= 0; --i) {
+                const uint64_t is = __ballot(v[n][i] == top[n] && top[n] > kNone);
+                best = is ? i * kWave + __builtin_ctzll(is) : best;
+            }
+            mine[n] = lane == j ? best : mine[n];
+            chosen[n] = lane == j ? top[n] : chosen[n];
+            left[n] = kNone;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                v[n][i] = i * kWave + lane == best ? kNone : v[n][i];
+                left[n] = fmaxf(left[n], v[n][i]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) top[n] = wave_max(left[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) p[n] = mine[n] >= 0 ? power(n, chosen[n]) : 0.f;
+    if (r.normalize) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n] = wave_sum(p[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int tn = t + n * kRouteWaves;
+        if (tn < t1 && lane < r.k) {
+            r.ids[(int64_t)tn * r.k + lane] = mine[n];
+            r.weights[(int64_t)tn * r.k + lane] = mine[n] >= 0 ? p[n] / s[n] : 0.f;
+            if (mine[n] >= 0) atomicOr(&words[mine[n]], 1u << (tn % kRouteBlock));
+            if (kept) kept[tn * r.k + lane] = (int16_t)mine[n];
+        }
     }
 }
 
@@ -151,9 +186,8 @@ __device__ inline int route_scan(const int* n, int* first, int E, int* part, int
     return all;
 }
 
-// Place and row of flat index f, of token t of its block of 32, whose words and first positions are given.
-__device__ inline void route_place(const Route& r, int64_t f, const uint32_t* words, const int* first, int t) {
-    const int e = min(r.ids[f], r.E - 1);
+// Place and row of flat index f, which chose e, of token t of its block of 32, whose words and first positions are given.
+__device__ inline void route_place(const Route& r, int64_t f, int e, const uint32_t* words, const int* first, int t) {
     int at = -1;
     if (e >= 0) {
         at = first[e] + __popc(words[e] & ((1u << t) - 1u));
@@ -172,7 +206,12 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(Route r) {
     for (int i = tid; i < BLOCKS * NV * kWave; i += kRouteThreads) (&words[0][0])[i] = 0;
     __syncthreads();
     const int t0 = b0 * kRouteBlock, t1 = min(r.T, t0 + BLOCKS * kRouteBlock);
-    for (int t = t0 + wave; t < t1; t += kRouteWaves) route_token<DT, NV>(r, t, words[(t - t0) / kRouteBlock], lane);
+    __shared__ int16_t kept[ONE ? kOneBlocks * kRouteBlock * kWave : 1];  // k <= 64
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        const int t = t0 + b * kRouteBlock + wave;
+        if (t < t1) route_tokens<DT, NV>(r, t, t1, words[b], ONE ? kept : nullptr, lane);
+    }
     __syncthreads();
     if constexpr (ONE) {
         __shared__ int count[NV * kWave], first[BLOCKS][NV * kWave], part[kRouteWaves];
@@ -194,7 +233,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(Route r) {
         const int each = kRouteBlock * r.k;
         for (int i = tid; i < r.T * r.k; i += kRouteThreads) {
             const int b = i / each;
-            route_place(r, i, words[b], first[b], (i - b * each) / r.k);
+            route_place(r, i, kept[i], words[b], first[b], (i - b * each) / r.k);
         }
         for (int i = all + tid; i < r.T * r.k; i += kRouteThreads) r.rows[i] = -1;
     } else {
@@ -211,6 +250,9 @@ __global__ void __launch_bounds__(kRouteThreads) moe_scatter_kernel(Route r, int
     const int tid = threadIdx.x;
     const int b0 = blockIdx.x * nb, mine = min(nb, blocks - b0);
     for (int e = tid; e < r.E; e += kRouteThreads) count[e] = before[e] = 0;
+    const int each = kRouteBlock * r.k;
+    const int n = min(mine * each, (r.T - b0 * kRouteBlock) * r.k);
+    int e0 = tid < n ? r.ids[(int64_t)b0 * each + tid] : -1;  // on its way from the start
     for (int i = tid; i < mine * r.E; i += kRouteThreads) own[i / r.E][i % r.E] = r.words[(int64_t)b0 * r.E + i];
     __syncthreads();
     const int per = kRouteThreads / r.E;  // threads to an expert, each a share of the blocks
@@ -246,11 +288,10 @@ __global__ void __launch_bounds__(kRouteThreads) moe_scatter_kernel(Route r, int
         }
     }
     __syncthreads();
-    const int each = kRouteBlock * r.k;
-    const int n = min(mine * each, (r.T - b0 * kRouteBlock) * r.k);
     for (int i = tid; i < n; i += kRouteThreads) {
         const int b = i / each, t = (i - b * each) / r.k;
-        route_place(r, (int64_t)b0 * each + i, own[b], first[b], t);
+        route_place(r, (int64_t)b0 * each + i, min(e0, r.E - 1), own[b], first[b], t);
+        if (i + kRouteThreads < n) e0 = r.ids[(int64_t)b0 * each + i + kRouteThreads];
     }
     for (int i = all + blockIdx.x * kRouteThreads + tid; i < r.T * r.k; i += gridDim.x * kRouteThreads) r.rows[i] = -1;
 }
