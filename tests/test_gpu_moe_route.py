@@ -130,3 +130,10 @@ def test_stream_workspace_and_repeats(gpu):
             assert gpu.equal(o[n], first[n]), n
     o = _run(gpu, xd, 4, True, stream=side.cuda_stream)
     assert gpu.equal(o["rows"], first["rows"])
+
+
+@pytest.mark.parametrize("t,e,k", [(2100, 1024, 20), (130, 100, 64), (2081, 1000, 1)])
+def test_many_words(gpu, t, e, k):
+    """So many words of bits that a workgroup of the second launch takes eight blocks; more choices than its threads."""
+    x = (gpu.randn((t, e), generator=gpu.Generator().manual_seed(t)) * 2).bfloat16()
+    _check(_run(gpu, x.cuda(), k, True), x, k, True)
