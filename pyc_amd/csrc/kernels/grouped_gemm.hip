@@ -12,7 +12,9 @@
 // 32 k of them (a group has 32, 64 or 128) are summed apart, then scaled into the sums
 // in fp32. Gated: fragments of a wave alternate, 16 gates and the 16 values of the same
 // columns, so that a lane has both. Rows at odd places are loaded as 16 unaligned bytes; what would
-// cross the end of its row is loaded up to there and shifted.
+// cross the end of its row is loaded up to there and shifted. Bound by its loads, two 16-byte pieces of each operand to
+// a thread and step: 256 rows of 64 experts of 2048 x 2816 with x off 16 bytes 196 us (aligned, in the ring, 136), 2048 of
+// 8 of 4096 x 4096 210 (in tiles 139).
 #include "grouped.hpp"
 
 namespace pyc {

@@ -15,6 +15,10 @@
 // time as fits. Where x would take turns (each stops all waves), only the scales do, and x is
 // loaded beside W (23 tokens, 11008 x 4096: 42 us in turns, 25 beside).
 //
+// One token through 4096 x 11008: 10.9 us (85 by the general kernel); 16 tokens by 4 of 32 experts of 4096 x 2816:
+// 50 us, 3.9 TB/s (218). Measured and not kept: x and scales loaded four pieces ahead of their way into LDS (12.6 and
+// 56), 16 waves and parts of K (23 tokens, 11008 x 4096: 25 as with eight).
+//
 // The rows of x are the first operand: a lane's results are four rows of one column of y, so
 // a column's scale is one value for each lane. A lane's 16 bytes of W are 32 k of a row, the
 // four lanes of a row 128 k. A 4 x 4

@@ -254,3 +254,23 @@ def test_replayed_with_other_routing(gpu, w4):
         want, bound = moe_util.product_ref(x, ref, offsets, torch.full((p, n), 7.0, dtype=x.dtype), rows.tolist(), spread=spread)
         moe_util.check(y, want, bound)
         assert (y[:offsets[0]] == 7).all() and (y[offsets[-1]:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,k", [(32, 96), (64, 192), (128, 384)])
+@pytest.mark.parametrize("rows,n", [(3, 2056), (200, 1264), (200, 2000), (200, 3600), (700, 8192)])
+def test_four_bits_beside_values_that_are_not_finite(gpu, rows, n, group, k):
+    """Infinite and NaN scales of every other row of W, of an expert without rows, and NaN in rows of x of no expert
+    change no bit of the other columns: streamed, in tiles of 16, 32, 64 and 128 rows."""
+    g = gpu.Generator().manual_seed(n)
+    codes, scale, zeros = moe_util.random_w4(2, n, k, group, "bf16", 3, True)
+    x = gpu.randn((rows + 4, k), generator=g).bfloat16()
+    bad, xbad = scale.clone(), x.clone()
+    bad[0, 1::4], bad[0, 3::4], bad[1] = math.inf, math.nan, math.inf
+    xbad[rows:] = math.nan
+    c, z, o = codes.cuda(), zeros.cuda(), _i32(gpu, [0, rows, rows])
+    y = [gpu.full((rows + 4, n), 7.0, dtype=x.dtype, device="cuda") for _ in range(2)]
+    pyc_amd.w4a16_grouped_gemm(x.cuda(), c, scale.cuda(), o, y[0], zeros=z)
+    pyc_amd.w4a16_grouped_gemm(xbad.cuda(), c, bad.cuda(), o, y[1], zeros=z)
+    assert gpu.isfinite(y[0]).all() and gpu.equal(y[0][:, 0::2], y[1][:, 0::2])
+    assert not gpu.isfinite(y[1][:rows, 1::2]).any() and (y[1][rows:] == 7).all()
