@@ -44,10 +44,10 @@ constexpr StreamLds kStreamLds[2][2] = {{{63 * 1024, 4096}, {111 * 1024, 12032}}
 constexpr size_t stream_lds_bytes(const StreamLds& l) { return l.x + 4 * l.scales; }
 constexpr uint32_t kPastEnd = 0xFFFFFFF0u;  // not below any descriptor's byte count
 
-// G: k of a group. XD: x is loaded beside W. tiles_n: column blocks, wgs: workgroups they take.
+// G: k of a group. XD: x is loaded beside W. wgs: workgroups that the column blocks take.
 template <typename T, int G, bool XD>
 __global__ void __launch_bounds__(kStreamThreads, 4)
-grouped_stream_kernel(Grouped g, int tiles_n, int wgs, int ks, int x_lds, int words) {
+grouped_stream_kernel(Grouped g, int wgs, int ks, int x_lds, int words) {
     constexpr int CF = 2;
     constexpr int NG = kStreamK / G;       // groups to a chunk
     constexpr int AHEAD = XD ? 2 : 4;      // chunks in registers
@@ -75,13 +75,11 @@ grouped_stream_kernel(Grouped g, int tiles_n, int wgs, int ks, int x_lds, int wo
     const int chunks = (g.K + kStreamK - 1) / kStreamK;
     const int groups = g.K / G;
 
-    // W: a chunk's place is the scalar part of a load's offset, which the descriptor's check leaves out. So the
-    // last chunk, where K is no multiple of 128, has lane offsets past the end for k past K, and
-    // chunks behind it a descriptor of no bytes.
+    // W: a chunk's place is the scalar part of a load's offset, which the descriptor's check leaves out. So k past
+    // K, of the last chunk where K is no multiple of 128 and of all chunks behind it, have lane offsets past the end.
     const uint32_t row_bytes = (uint32_t)g.K / 2;
     void* const wbase = const_cast<char*>(static_cast<const char*>(g.w)) + (int64_t)t.e * g.w_stride;
-    const uint32_t wbytes = tn < tiles_n ? (uint32_t)g.N * row_bytes : 0u;
-    const int whole = g.K / kStreamK, left = g.K - whole * kStreamK;
+    const auto wr = __builtin_amdgcn_make_buffer_rsrc(wbase, 0, (uint32_t)g.N * row_bytes, 0x00020000);
     uint32_t wo[CF];
 #pragma unroll
     for (int f = 0; f < CF; ++f) {
@@ -99,14 +97,13 @@ grouped_stream_kernel(Grouped g, int tiles_n, int wgs, int ks, int x_lds, int wo
         xbytes = (uint32_t)(((int64_t)(g.x_rows - 1) * g.x_stride + g.K) * 2);
     }
     auto load = [&](Chunk& c, int i) __attribute__((always_inline)) {
-        const int end = i == whole ? left : kStreamK;  // k of the chunk that there are
-        const auto wr = __builtin_amdgcn_make_buffer_rsrc(wbase, 0, i < chunks ? wbytes : 0u, 0x00020000);
+        const int end = g.K - i * kStreamK;  // k from this chunk on
 #pragma unroll
         for (int f = 0; f < CF; ++f)
             c.w[f] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                                    wr, 32 * lgrp < end ? wo[f] : kPastEnd, (uint32_t)i * (kStreamK / 2), 0));
         if constexpr (XD) {
-            const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.x), 0, i < chunks ? xbytes : 0u, 0x00020000);
+            const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.x), 0, xbytes, 0x00020000);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 c.x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
@@ -307,7 +304,7 @@ extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, const pyc_grouped* gp,
     const StreamLds lds = kStreamLds[xd][big];
     const size_t bytes = stream_lds_bytes(lds);
 #define PYC_STREAM_X(TY, G, XD) \
-    hipLaunchKernelGGL((grouped_stream_kernel<TY, G, XD>), grid, block, bytes, s, g, tiles_n, wgs, ks, lds.x, lds.scales)
+    hipLaunchKernelGGL((grouped_stream_kernel<TY, G, XD>), grid, block, bytes, s, g, wgs, ks, lds.x, lds.scales)
 #define PYC_STREAM(G)                                   \
     if (g.group == G) {                                 \
         if (is_bf16) {                                  \
