@@ -19,6 +19,7 @@ typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4;
 typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
 
 constexpr int kWave = 64;
+constexpr int64_t kMostThreads = 0xFFFFFFFF;  // threads of a launch
 
 // Element traits: storage type is always a 16-bit pattern for the half types.
 template <typename T> struct elem;

@@ -11,7 +11,6 @@ namespace pyc {
 
 constexpr int kEpiBias = 1, kEpiRelu = 2, kEpiGate = 4;
 constexpr int kMaxExperts = 1024;
-constexpr int64_t kMostThreads = 0xFFFFFFFF;  // threads of a launch
 
 typedef pyc_grouped Grouped;
 

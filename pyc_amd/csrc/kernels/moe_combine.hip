@@ -87,7 +87,15 @@ extern "C" int pyc_hip_moe_combine_launch(int is_bf16, int P, int T, int k, int 
     const bool wide = ((H | y_stride | out_stride | (base ? base_stride : 0)) & 7) == 0 &&
                       (((uintptr_t)y | (uintptr_t)out | (uintptr_t)base) & 15) == 0;
     const int chunks = wide ? H / 8 : H;
-    const dim3 grid((unsigned)(((int64_t)T * chunks + kCombineThreads - 1) / kCombineThreads));
+    const int64_t blocks = ((int64_t)T * chunks + kCombineThreads - 1) / kCombineThreads;
+    if (blocks > kMostThreads / kCombineThreads) {  // more threads than a launch has: half of the tokens each (one alone never is)
+        const int n = T / 2;
+        const int rc = pyc_hip_moe_combine_launch(is_bf16, P, n, k, H, y, y_stride, weights, places, base, base_stride, out, out_stride, stream);
+        return rc ? rc : pyc_hip_moe_combine_launch(is_bf16, P, T - n, k, H, y, y_stride, weights + (int64_t)n * k, places + (int64_t)n * k,
+                                                    base ? c.base + n * base_stride : nullptr, base_stride, c.out + n * out_stride,
+                                                    out_stride, stream);
+    }
+    const dim3 grid((unsigned)blocks);
     const hipStream_t s = (hipStream_t)stream;
     const bool one = chunks % kWave == 0;
 #define PYC_COMBINE(TY)                                                                                                     \
