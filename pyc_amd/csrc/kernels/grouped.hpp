@@ -73,6 +73,14 @@ inline int64_t expert_tiles_most(int E, int P, int step) {
     return (int64_t)P / step + (E < P ? E : P);
 }
 
+// `all` workgroups in as few launches as hold their threads: launch(the first one's place, grid).
+template <typename F> inline int grouped_launches(int64_t all, int threads, F launch) {
+    if (all > 0x7FFF0000) return -1;
+    const int64_t most = kMostThreads / threads;
+    for (int64_t at = 0; at < all; at += most) launch((uint32_t)at, dim3((unsigned)(all - at < most ? all - at : most)));
+    return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
 // The row of x behind row p of y, -1 (zeros) where the index is outside x.
 __device__ inline int source_row(const Grouped& g, int p) {
     int r = p;

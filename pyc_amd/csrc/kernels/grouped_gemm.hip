@@ -47,12 +47,13 @@ __device__ inline u32x4 row_piece(const uint16_t* row, int c, int K, bool edge) 
 }
 
 template <typename T, bool W4>
-__global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int tiles_n) {
+__global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int tiles_n, uint32_t tile0) {
     __shared__ __attribute__((aligned(16))) uint16_t Xs[2][kGenTile * kGenK], Ws[2][kGenTile * kGenK];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave >> 1, wn = wave & 1, lrow = lane & 15, lgrp = lane >> 4;
-    const int tn = blockIdx.x % tiles_n;
-    const ExpertTile t = expert_tile(g, blockIdx.x / tiles_n, kGenTile, lane);
+    const uint32_t tile = tile0 + blockIdx.x;
+    const int tn = tile % tiles_n;
+    const ExpertTile t = expert_tile(g, tile / tiles_n, kGenTile, lane);
     if (t.e < 0) return;
     const bool gate = g.epi & kEpiGate;
     const int F = gate ? g.N / 2 : g.N;                    // columns of y
@@ -251,17 +252,16 @@ extern "C" int pyc_hip_grouped_launch(int is_bf16, int w4, const pyc_grouped* gp
     const int cols = g.epi & kEpiGate ? g.N / 2 : g.N, per = g.epi & kEpiGate ? kGenTile / 2 : kGenTile;
     const int tiles_n = (cols + per - 1) / per;
     const int64_t tiles = expert_tiles_most(g.offsets ? g.E : 1, g.P, kGenTile) * tiles_n;
-    if (tiles > kMostThreads / 256) return -1;
-    const dim3 grid((unsigned)tiles), block(256);
     const hipStream_t s = (hipStream_t)stream;
-#define PYC_GENERAL(TY, W) hipLaunchKernelGGL((grouped_general_kernel<TY, W>), grid, block, 0, s, g, tiles_n)
-    if (w4) {
-        if (is_bf16) PYC_GENERAL(bf16_t, true);
-        else PYC_GENERAL(f16_t, true);
-    } else {
-        if (is_bf16) PYC_GENERAL(bf16_t, false);
-        else PYC_GENERAL(f16_t, false);
-    }
+    return grouped_launches(tiles, 256, [&](uint32_t tile0, dim3 grid) {
+#define PYC_GENERAL(TY, W) hipLaunchKernelGGL((grouped_general_kernel<TY, W>), grid, dim3(256), 0, s, g, tiles_n, tile0)
+        if (w4) {
+            if (is_bf16) PYC_GENERAL(bf16_t, true);
+            else PYC_GENERAL(f16_t, true);
+        } else {
+            if (is_bf16) PYC_GENERAL(bf16_t, false);
+            else PYC_GENERAL(f16_t, false);
+        }
 #undef PYC_GENERAL
-    return hipGetLastError() == hipSuccess ? 0 : -2;
+    });
 }

@@ -22,7 +22,7 @@ constexpr int ring_stage_bytes(int fn) { return (kRingRows + 64 * fn) * kRingK *
 constexpr int ring_stages(int fn) { return fn == 1 ? 5 : 3; }
 
 template <typename T, int FN, bool GATE>
-__global__ void __launch_bounds__(256, 2) grouped_ring_kernel(Grouped g, int tiles_n, int wide) {
+__global__ void __launch_bounds__(256, 2) grouped_ring_kernel(Grouped g, int tiles_n, int wide, uint32_t tile0) {
     constexpr int BN = 64 * FN, S = ring_stages(FN);
     constexpr uint32_t STAGE = ring_stage_bytes(FN), A_BYTES = kRingRows * kRingK * 2;
     constexpr int LA = 2, LB = 2 * FN, LOADS = LA + LB;  // 1 KB loads to a wave and stage
@@ -32,10 +32,11 @@ __global__ void __launch_bounds__(256, 2) grouped_ring_kernel(Grouped g, int til
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lrow = lane & 15, lgrp = lane >> 4;
     const int F = GATE ? g.N / 2 : g.N;
-    const ExpertTile t = expert_tile(g, blockIdx.x / tiles_n, kRingRows, lane);
+    const uint32_t tile = tile0 + blockIdx.x;
+    const ExpertTile t = expert_tile(g, tile / tiles_n, kRingRows, lane);
     if (t.e < 0) return;
     const int rows = min(t.end - t.begin, kRingRows);
-    const int col0 = (blockIdx.x % tiles_n) * (GATE ? BN / 2 : BN);
+    const int col0 = (int)(tile % tiles_n) * (GATE ? BN / 2 : BN);
     // the row of W in slot c of the tile (-1: none): a wave's 16 FN; gated, half gates and then their values
     auto weight_row = [&](int c) __attribute__((always_inline)) {
         if constexpr (GATE) {
@@ -163,19 +164,20 @@ extern "C" int pyc_hip_grouped_ring_launch(int is_bf16, const pyc_grouped* gp, i
     const int cols = gate ? g.N / 2 : g.N, per = gate ? 32 * fn : 64 * fn;
     const int tiles_n = (cols + per - 1) / per;
     const int64_t tiles = expert_tiles_most(g.offsets ? g.E : 1, g.P, kRingRows) * tiles_n;
-    if (tiles > kMostThreads / 256) return -1;
     const int wide = ((uintptr_t)g.y & 15) == 0 && (g.P == 1 || g.y_stride % 8 == 0);
-    const dim3 grid((unsigned)tiles), block(256);
     const hipStream_t s = (hipStream_t)stream;
-#define PYC_RING(TY)                                                                                          \
-    if (gate && fn == 2) hipLaunchKernelGGL((grouped_ring_kernel<TY, 2, true>), grid, block, 0, s, g, tiles_n, wide); \
-    else if (gate) hipLaunchKernelGGL((grouped_ring_kernel<TY, 1, true>), grid, block, 0, s, g, tiles_n, wide); \
-    else if (fn == 2) hipLaunchKernelGGL((grouped_ring_kernel<TY, 2, false>), grid, block, 0, s, g, tiles_n, wide); \
-    else hipLaunchKernelGGL((grouped_ring_kernel<TY, 1, false>), grid, block, 0, s, g, tiles_n, wide)
-    if (is_bf16) PYC_RING(bf16_t);
-    else PYC_RING(f16_t);
+    return grouped_launches(tiles, 256, [&](uint32_t tile0, dim3 grid) {
+#define PYC_RING(TY, FN, GATE) hipLaunchKernelGGL((grouped_ring_kernel<TY, FN, GATE>), grid, dim3(256), 0, s, g, tiles_n, wide, tile0)
+#define PYC_RING_TYPE(TY)                         \
+    if (gate && fn == 2) PYC_RING(TY, 2, true);   \
+    else if (gate) PYC_RING(TY, 1, true);         \
+    else if (fn == 2) PYC_RING(TY, 2, false);     \
+    else PYC_RING(TY, 1, false)
+        if (is_bf16) PYC_RING_TYPE(bf16_t);
+        else PYC_RING_TYPE(f16_t);
+#undef PYC_RING_TYPE
 #undef PYC_RING
-    return hipGetLastError() == hipSuccess ? 0 : -2;
+    });
 }
 
 // The form of 64 columns.

@@ -47,7 +47,7 @@ constexpr uint32_t kPastEnd = 0xFFFFFFF0u;  // not below any descriptor's byte c
 // G: k of a group. XD: x is loaded beside W. wgs: workgroups that the column blocks take.
 template <typename T, int G, bool XD>
 __global__ void __launch_bounds__(kStreamThreads, 4)
-grouped_stream_kernel(Grouped g, int wgs, int ks, int x_lds, int words) {
+grouped_stream_kernel(Grouped g, int wgs, int ks, int x_lds, int words, uint32_t wg0) {
     constexpr int CF = 2;
     constexpr int NG = kStreamK / G;       // groups to a chunk
     constexpr int AHEAD = XD ? 2 : 4;      // chunks in registers
@@ -61,8 +61,9 @@ grouped_stream_kernel(Grouped g, int wgs, int ks, int x_lds, int words) {
     const int lrow = lane & 15, lgrp = lane >> 4;
     const int units = kStreamWaves / ks;                     // column blocks of the workgroup
     const int kp = wave & (ks - 1), unit = wave / ks;        // this wave's part of K and block
-    const int tn0 = (blockIdx.x % wgs) * units, tn = tn0 + unit;
-    const ExpertTile t = expert_tile(g, blockIdx.x / wgs, 16, lane);
+    const uint32_t wg = wg0 + blockIdx.x;
+    const int tn0 = (int)(wg % wgs) * units, tn = tn0 + unit;
+    const ExpertTile t = expert_tile(g, wg / wgs, 16, lane);
     if (t.e < 0) return;
     const int rows = min(t.end - t.begin, 16);
     const bool gate = g.epi & kEpiGate;
@@ -294,17 +295,16 @@ extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, const pyc_grouped* gp,
     int ks = 8;
     while (ks > 2 && most * tiles_n * ks > 4096) ks /= 2;
     const int wgs = (tiles_n + kStreamWaves / ks - 1) / (kStreamWaves / ks);
-    if (most * wgs > kMostThreads / kStreamThreads) return -1;
     const hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)(most * wgs)), block(kStreamThreads);
     // x beside W where LDS would take it in turns; by expert, of about twice the mean of rows
     const int big = most * wgs <= 256;
     const int64_t rows = g.offsets ? 2 * (int64_t)g.P / g.E + 2 : g.P;
     const int xd = (rows < 16 ? rows : 16) * (2 * (int64_t)g.K + 16) > kStreamLds[0][big].x;
     const StreamLds lds = kStreamLds[xd][big];
     const size_t bytes = stream_lds_bytes(lds);
+    return grouped_launches(most * wgs, kStreamThreads, [&](uint32_t wg0, dim3 grid) {
 #define PYC_STREAM_X(TY, G, XD) \
-    hipLaunchKernelGGL((grouped_stream_kernel<TY, G, XD>), grid, block, bytes, s, g, wgs, ks, lds.x, lds.scales)
+    hipLaunchKernelGGL((grouped_stream_kernel<TY, G, XD>), grid, dim3(kStreamThreads), bytes, s, g, wgs, ks, lds.x, lds.scales, wg0)
 #define PYC_STREAM(G)                                   \
     if (g.group == G) {                                 \
         if (is_bf16) {                                  \
@@ -315,10 +315,10 @@ extern "C" int pyc_hip_grouped_stream_launch(int is_bf16, const pyc_grouped* gp,
             else PYC_STREAM_X(f16_t, G, false);         \
         }                                               \
     }
-    PYC_STREAM(32)
-    PYC_STREAM(64)
-    PYC_STREAM(128)
+        PYC_STREAM(32)
+        PYC_STREAM(64)
+        PYC_STREAM(128)
 #undef PYC_STREAM
 #undef PYC_STREAM_X
-    return hipGetLastError() == hipSuccess ? 0 : -2;
+    });
 }

@@ -5,6 +5,7 @@ import torch
 
 import pyc_amd
 from tests import moe_util
+from tests import moe_util
 
 MOST = (1 << 32) - 1  # threads of a launch
 
@@ -39,3 +40,38 @@ def test_sum_of_most_threads(gpu):
     pyc_amd.moe_combine(y, w, places, out, base=base)
     for a in range(0, tokens, 8192):
         assert torch.equal(out[a:a + 8192], want(a, a + 8192).bfloat16()), a
+# (kernel, bits, N, K): 1024 experts of a row each
+PRODUCTS = [(0, 16, 1 << 20, 1), (1, 16, 1 << 21, 8), (3, 4, 1 << 20, 32)]
+
+
+@pytest.mark.parametrize("kind,bits,n,k", PRODUCTS)
+def test_which_kernel(kind, bits, n, k):
+    got, arg = moe_util.form(bits == 4, 1024, 1024, n, k)
+    assert got == kind
+    columns, rows, threads = {0: (64, 64, 256), 1: (64 * arg, 64, 256), 3: (4 * 32, 16, 512)}[kind]
+    assert (1024 + 1024 // rows) * (n // columns) * threads > MOST
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,bits,n,k", PRODUCTS)
+def test_products_of_most_workgroups(gpu, kind, bits, n, k):
+    e, dtype = 1024, torch.float16
+    x = _ints((e, k), -2, 3, dtype, 1)
+    offsets = _i32(list(range(e + 1)))
+    y = torch.full((e, n), 77.0, dtype=dtype, device="cuda")
+    per = torch.arange(e, device="cuda") % 5 - 2  # what an expert adds to all of its weights
+    if bits == 16:
+        first = _ints((n, k), -2, 3, dtype, 2)
+        w = torch.empty((e, n, k), dtype=dtype, device="cuda")
+        for i in range(0, e, 64):
+            w[i:i + 64] = first + per[i:i + 64, None, None].to(dtype)
+        pyc_amd.grouped_gemm(x, w, offsets, y)
+        values = first.float()
+    else:
+        codes = torch.randint(0, 256, (n, k // 2), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda", dtype=torch.uint8)
+        scale = torch.ones((e, n, k // 32), dtype=dtype, device="cuda")
+        zeros = (8 - per).to(torch.uint8)[:, None, None].expand(e, n, k // 32).contiguous()
+        pyc_amd.w4a16_grouped_gemm(x, codes.expand(e, n, k // 2).contiguous(), scale, offsets, y, zeros=zeros)
+        values = torch.stack([codes & 15, codes >> 4], -1).reshape(n, k).float() - 8
+    total = x.float().sum(1)
+    _same(y, lambda a, b: x[a:b].float() @ values.t() + (per[a:b] * total[a:b])[:, None])
