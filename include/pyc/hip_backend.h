@@ -21,7 +21,8 @@ extern "C" {
 /* GEMM epilogue flags: applied to the fp32 accumulator before the store. */
 #define PYC_HIP_EPI_NONE 0
 #define PYC_HIP_EPI_BIAS 1 /* out[m,n] += bias[n] (fp32 bias) */
-#define PYC_HIP_EPI_RELU 2 /* out = max(out, 0) after bias */
+#define PYC_HIP_EPI_RELU 2 /* out = max(out, 0) after bias. NaN: 0, but from the products by expert
+                            * and with 4-bit weights NaN */
 /* Products by expert and with 4-bit weights only, not with RELU: rows 0 .. N/2 - 1 of
  * the weights are gates, the others values, and column c of out (N/2 of them) is
  * silu(gate c) * value c, each with its bias. silu(g) = g / (1 + e^-g). */

@@ -119,6 +119,9 @@ __device__ inline float row_half_turn(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
 }
 
+// max(v, 0), NaN of NaN (a maximum instruction would take 0).
+__device__ inline float relu_of(float v) { return v < 0.f ? 0.f : v; }
+
 // silu(g) * v = g v / (1 + e^-g), in fp32; the reciprocal is off by at most one of its steps.
 __device__ inline float silu_gate(float g, float v) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * v; }
 

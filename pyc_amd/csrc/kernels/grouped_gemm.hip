@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
                 if (col[0] >= 0) y[col[0]] = elem<T>::from_f32(silu_gate(v0, v1));
             } else {
                 const bool relu = g.epi & kEpiRelu;
-                if (col[0] >= 0) y[col[0]] = elem<T>::from_f32(relu ? fmaxf(v0, 0.f) : v0);
-                if (col[1] >= 0) y[col[1]] = elem<T>::from_f32(relu ? fmaxf(v1, 0.f) : v1);
+                if (col[0] >= 0) y[col[0]] = elem<T>::from_f32(relu ? relu_of(v0) : v0);
+                if (col[1] >= 0) y[col[1]] = elem<T>::from_f32(relu ? relu_of(v1) : v1);
             }
         }
 }

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(256, 2) grouped_ring_kernel(Grouped g, int til
                     float v = acc[i][j][r] + bias[j];
                     // gated: the value is in the other fragment, or eight lanes on
                     if constexpr (GATE) v = silu_gate(v, FN == 2 ? acc[i][FN - 1][r] + bias[FN - 1] : row_half_turn(v));
-                    else if (relu) v = fmaxf(v, 0.f);
+                    else if (relu) v = relu_of(v);
                     if (!GATE || FN == 2 || lrow < 8)
                         out[(16 * i + 4 * lgrp + r) * PITCH + wave * YC + 16 * j + lrow] = elem<T>::from_f32(v);
                 }

@@ -264,7 +264,7 @@ grouped_stream_kernel(Grouped g, int wgs, int ks, int x_lds, int words, uint32_t
         const int col = gate ? tn * 16 + lrow : tn * 32 + 16 * f + lrow;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float v = gate ? silu_gate(acc[0][r], acc[1][r]) : relu ? fmaxf(acc[f][r], 0.f) : acc[f][r];
+            const float v = gate ? silu_gate(acc[0][r], acc[1][r]) : relu ? relu_of(acc[f][r]) : acc[f][r];
             const int p = 4 * lgrp + r;
             if (p < rows && col < F) g.y[(int64_t)(t.begin + p) * g.y_stride + col] = elem<T>::from_f32(v);
         }

@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(256, 1) grouped_tile_kernel(Grouped g, int til
                 for (int q = 0; q < 4; ++q) {
                     v[q] = acc[i][j][q] + (&bv[j].x)[q];
                     if constexpr (GATE) v[q] = silu_gate(v[q], acc[i][j + 1][q] + (&bv[j + 1].x)[q]);
-                    else if (relu) v[q] = fmaxf(v[q], 0.f);
+                    else if (relu) v[q] = relu_of(v[q]);
                 }
                 uint2 packed;
                 packed.x = (uint32_t)elem<T>::from_f32(v[0]) | ((uint32_t)elem<T>::from_f32(v[1]) << 16);

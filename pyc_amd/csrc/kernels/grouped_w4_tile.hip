@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
                         float v = acc[i][j][r] + bias[j];
                         // gated: the value is FN / 2 fragments on, or eight lanes
                         if constexpr (GATE) v = silu_gate(v, FN > 1 ? acc[i][(j + FN / 2) % FN][r] + bias[(j + FN / 2) % FN] : row_half_turn(v));
-                        else if (relu) v = fmaxf(v, 0.f);
+                        else if (relu) v = relu_of(v);
                         if (!GATE || FN > 1 || lrow < 8)
                             out[(16 * (wm * FM + i) + 4 * lgrp + r) * PITCH + wn * YC + 16 * j + lrow] = elem<T>::from_f32(v);
                     }
