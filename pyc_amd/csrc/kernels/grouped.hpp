@@ -39,7 +39,8 @@ __device__ inline int scan_max(int v) {  // of numbers >= 0
 
 // Tile t of a grid whose tiles are `step` rows of one expert, expert after expert.
 // offsets are held to 0 .. P and to what came before, so that no row has two experts
-// whatever they say. Every wave finds its tile by itself, 64 experts at a time.
+// whatever they say. Every wave finds its tile by itself, 64 experts at a time, lanes behind
+// the last expert with none of its rows (no branch: see source_row).
 struct ExpertTile {
     int e, begin, end;  // expert (-1: there is no tile t), the tile's first row, the expert's end
 };
@@ -51,8 +52,8 @@ __device__ inline ExpertTile expert_tile(const Grouped& g, int t, int step, int 
     int held = 0, before = 0;  // the largest offset so far, tiles so far
     for (int e0 = 0; e0 < g.E; e0 += kWave) {
         const int e = e0 + lane;
-        const int b = scan_max(max(held, e < g.E ? min(g.offsets[e], g.P) : 0));
-        const int end = max(b, e < g.E ? min(g.offsets[e + 1], g.P) : 0);
+        const int b = scan_max(max(held, min(g.offsets[min(e, g.E)], g.P)));
+        const int end = max(b, min(g.offsets[min(e + 1, g.E)], g.P));
         const int n = (end - b + step - 1) / step;
         const int sum = scan_add(n);
         const uint64_t in = __ballot(t < before + sum);
@@ -81,15 +82,32 @@ template <typename F> inline int grouped_launches(int64_t all, int threads, F la
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
-// The row of x behind row p of y, -1 (zeros) where the index is outside x.
-__device__ inline int source_row(const Grouped& g, int p) {
+// The row of x behind row p of y, -1 (zeros) where the index is outside x or p is not below end (the expert's, at least
+// one). All lanes do the same, for some that there is no row for read another one's index: where lanes go apart among
+// as many values as a tile's, the compiler has put copies of registers at the join before all of them were back.
+__device__ inline int source_row(const Grouped& g, int p, int end) {
     int r = p;
-    if (g.rows) {
-        r = g.rows[p];
-        r = r < 0 ? -1 : r / g.fan;
+    bool in = p < end;
+    if (g.rows) {  // the same for all
+        r = g.rows[min(p, end - 1)];
+        in &= r >= 0;
+        r = (int)((unsigned)max(r, 0) / (unsigned)g.fan);
     }
-    return r < g.x_rows ? r : -1;
+    return (in & (r < g.x_rows)) ? r : -1;
 }
+
+// Bias of row n of expert e's W, 0 for row -1 and without a bias: the range check of a descriptor takes the place of a
+// branch that lanes take apart (an expert's biases are at most 2^26 bytes).
+struct ExpertBias {
+    __amdgpu_buffer_rsrc_t rsrc;
+    bool there;  // the same for all lanes
+    __device__ ExpertBias(const Grouped& g, int e)
+        : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(g.bias) + (int64_t)e * g.N, 0, (uint32_t)g.N * 4u, 0x00020000)),
+          there(g.epi & kEpiBias) {}
+    __device__ float operator[](int n) const {
+        return there ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, (uint32_t)n * 4u, 0, 0)) : 0.f;
+    }
+};
 
 // w[i] of lane group g becomes w[g] of lane group i.
 __device__ inline void transpose4(u32x4& w) {

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
     for (int i = 0; i < 2; ++i) {
         // rows that there are not are read from the first one; x's count as zeros, W's reach no result
         const int p = t.begin + row0 + 32 * i;
-        const int r = p < t.end ? source_row(g, p) : -1;
+        const int r = source_row(g, p, t.end);
         xin[i] = r >= 0;
         xr[i] = g.x + (int64_t)max(r, 0) * g.x_stride;
         wr[i] = static_cast<const uint16_t*>(g.w) + ew + (int64_t)max(weight_row(row0 + 32 * i), 0) * g.K;
@@ -179,9 +179,8 @@ __global__ void __launch_bounds__(256) grouped_general_kernel(Grouped g, int til
         multiply(k0 + kGenK, 1);
     }
 
-    float bias[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) bias[j] = (g.epi & kEpiBias) && col[j] >= 0 ? g.bias[(int64_t)t.e * g.N + col[j]] : 0.f;
+    const ExpertBias expert_bias(g, t.e);
+    const float bias[2] = {expert_bias[col[0]], expert_bias[col[1]]};
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll

@@ -61,7 +61,8 @@ __global__ void __launch_bounds__(256, 2) grouped_ring_kernel(Grouped g, int til
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
         const int p = t.begin + 8 * (LA * wave + i) + lane / 8;
-        const int r = p < t.end ? source_row(g, p) : -1;
+        // a wave without rows does not wait for an index
+        const int r = t.begin + 8 * LA * wave < t.end ? source_row(g, p, t.end) : -1;
         voff[i] = r < 0 ? kRingPastEnd : (uint32_t)((int64_t)r * g.x_stride * 2) + 16 * lch;
     }
 #pragma unroll
@@ -111,12 +112,10 @@ __global__ void __launch_bounds__(256, 2) grouped_ring_kernel(Grouped g, int til
         wait_vmem_le<0>();
         __syncthreads();  // the ring is free: results go through it
 
+        const ExpertBias expert_bias(g, t.e);
         float bias[FN];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int n = weight_row(16 * (FN * wave + j) + lrow);
-            bias[j] = (g.epi & kEpiBias) && n >= 0 ? g.bias[(int64_t)t.e * g.N + n] : 0.f;
-        }
+        for (int j = 0; j < FN; ++j) bias[j] = expert_bias[weight_row(16 * (FN * wave + j) + lrow)];
         const bool relu = g.epi & kEpiRelu;
         constexpr int PITCH = 4 * YC + 8;  // all waves' columns of a row
         uint16_t* const out = reinterpret_cast<uint16_t*>(smem);

@@ -93,7 +93,7 @@ grouped_stream_kernel(Grouped g, int wgs, int ks, int x_lds, int words, uint32_t
     uint32_t xo = kPastEnd;  // XD: of the lane's row
     uint32_t xbytes = 0;
     if constexpr (XD) {
-        const int r = lrow < rows ? source_row(g, t.begin + lrow) : -1;
+        const int r = source_row(g, t.begin + lrow, t.begin + rows);
         xo = r < 0 ? kPastEnd : (uint32_t)((int64_t)r * g.x_stride * 2) + 16 * lgrp;
         xbytes = (uint32_t)(((int64_t)(g.x_rows - 1) * g.x_stride + g.K) * 2);
     }
@@ -132,7 +132,7 @@ grouped_stream_kernel(Grouped g, int wgs, int ks, int x_lds, int words, uint32_t
     const int pitch = min(span, chunks * kStreamK) * 2 + 16;  // bytes of a row of x in LDS
     // element offset of the row of x behind each row of the tile, -1: zeros
     if (!XD && tid < rows) {
-        const int r = source_row(g, t.begin + tid);
+        const int r = source_row(g, t.begin + tid, t.end);
         src[tid] = r < 0 ? -1 : (int64_t)r * g.x_stride;
     }
     const uint16_t* const scale = g.scale + (int64_t)t.e * g.N * groups;

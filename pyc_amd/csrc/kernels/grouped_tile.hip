@@ -65,10 +65,10 @@ __global__ void __launch_bounds__(256, 1) grouped_tile_kernel(Grouped g, int til
         for (int e0 = 0; e0 < g.E; e0 += kWave) {
             const int e = e0 + lane;
             const bool in = e < g.E;
-            const int lo = g.offsets ? (in ? min(g.offsets[e], g.P) : 0) : 0;
-            const int hi = g.offsets ? (in ? min(g.offsets[e + 1], g.P) : 0) : g.P;
+            const int lo = g.offsets ? min(g.offsets[min(e, g.E)], g.P) : in ? 0 : g.P;
+            const int hi = g.offsets ? min(g.offsets[min(e + 1, g.E)], g.P) : g.P;
             const int b = scan_max(max(held, lo));
-            const int end = in ? max(b, hi) : b;
+            const int end = max(b, hi);
             const int h = (end - b + kTile / 2 - 1) / kTile, l = end - b > h * kTile ? 1 : 0;
             const int sh = scan_add(h), sl = scan_add(l);
             if (in) {
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(256, 1) grouped_tile_kernel(Grouped g, int til
     // offset of x's row behind row r of y, for thread r of the workgroup's 256
     auto source = [&](const Tile& c) __attribute__((always_inline)) {
         const int p = c.row + tid;
-        const int r = p < c.end ? source_row(g, p) : -1;
+        const int r = source_row(g, p, c.end);
         return r < 0 ? kTilePastEnd : (uint32_t)((int64_t)r * g.x_stride * 2);
     };
     auto set_tile = [&](const Tile& c) __attribute__((always_inline)) {
@@ -224,9 +224,9 @@ __global__ void __launch_bounds__(256, 1) grouped_tile_kernel(Grouped g, int til
         const int tn = t + per;
         more = tn < t_end;
         const Tile next = tile_of(more ? tn : t);
-        const int np = next.row + tid;
-        const bool nin = np < next.end;
-        const int nidx = g.rows && nin ? g.rows[np] : 0;
+        const int np = min(next.row + tid, next.end - 1);
+        const bool nin = next.row + tid < next.end;
+        const int nidx = g.rows ? g.rows[np] : 0;
         auto read_a = [&](int h, int f, uint32_t buf) {
             return *reinterpret_cast<const u32x4*>(a_rd[h] + buf + (wm * FM + f) * 16 * BK);
         };
@@ -291,9 +291,8 @@ __global__ void __launch_bounds__(256, 1) grouped_tile_kernel(Grouped g, int til
         }
         wait_vmem_le<0>();
         {
-            int r = -1;
-            if (nin) r = !g.rows ? np : nidx < 0 ? -1 : nidx / g.fan;
-            src[tid] = r < 0 || r >= g.x_rows ? kTilePastEnd : (uint32_t)((int64_t)r * g.x_stride * 2);
+            const int r = g.rows ? (int)((unsigned)max(nidx, 0) / (unsigned)g.fan) : np;
+            src[tid] = (nin & (nidx >= 0) & (r < g.x_rows)) ? (uint32_t)((int64_t)r * g.x_stride * 2) : kTilePastEnd;
         }
         __syncthreads();  // the stages are free, the next tile's rows are there
 

@@ -80,8 +80,8 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
         int held = 0;
         for (int e0 = 0; e0 < g.E; e0 += kWave) {
             const int e = e0 + lane;
-            const int b = scan_max(max(held, e < g.E ? min(g.offsets[e], g.P) : 0));
-            const int end = max(b, e < g.E ? min(g.offsets[e + 1], g.P) : 0);
+            const int b = scan_max(max(held, min(g.offsets[min(e, g.E)], g.P)));
+            const int end = max(b, min(g.offsets[min(e + 1, g.E)], g.P));
             row_tiles += __builtin_amdgcn_readlane(scan_add((end - b + ROWS - 1) / ROWS), kWave - 1);
             held = __builtin_amdgcn_readlane(end, kWave - 1);
         }
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
                 const int p = row0 + 4 * (NW * i + wave) + lane / 16;
-                const int s = p < end ? source_row(g, p) : -1;
+                const int s = source_row(g, p, end);
                 xo[i] = s < 0 ? kW4PastEnd : (uint32_t)((int64_t)s * g.x_stride * 2) + 2 * xk;
             }
 #pragma unroll
@@ -318,12 +318,10 @@ __global__ void __launch_bounds__(256 * WM, 2) grouped_w4_tile_kernel(Grouped g,
             wait_vmem_le<0>();
             __syncthreads();  // the ring is free: results go through it
 
+            const ExpertBias expert_bias(g, e);
             float bias[FN];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const int n = weight_row(16 * (FN * wn + j) + lrow);
-                bias[j] = (g.epi & kEpiBias) && n >= 0 ? g.bias[(int64_t)e * g.N + n] : 0.f;
-            }
+            for (int j = 0; j < FN; ++j) bias[j] = expert_bias[weight_row(16 * (FN * wn + j) + lrow)];
             const bool relu = g.epi & kEpiRelu;
             uint16_t* const out = reinterpret_cast<uint16_t*>(smem);
 #pragma unroll
