@@ -25,7 +25,8 @@ extern "C" {
                             * and with 4-bit weights NaN */
 /* Products by expert and with 4-bit weights only, not with RELU: rows 0 .. N/2 - 1 of
  * the weights are gates, the others values, and column c of out (N/2 of them) is
- * silu(gate c) * value c, each with its bias. silu(g) = g / (1 + e^-g). */
+ * silu(gate c) * value c, each with its bias. silu(g) = g / (1 + e^-g), 0 where e^-g leaves
+ * fp32 (g below -88.7). */
 #define PYC_HIP_EPI_SILU_GATE 4
 
 /* Generalises reference gemm/kernel.cu:151-203 (pyc_cutlass_gemm_dispatch):

@@ -140,7 +140,11 @@ __device__ inline float row_half_turn(float v) {
 // max(v, 0), NaN of NaN (a maximum instruction would take 0).
 __device__ inline float relu_of(float v) { return v < 0.f ? 0.f : v; }
 
-// silu(g) * v = g v / (1 + e^-g), in fp32; the reciprocal is off by at most one of its steps.
-__device__ inline float silu_gate(float g, float v) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * v; }
+// silu(g) * v = g v / (1 + e^-g), in fp32. All of it is taken in quarters: 1 + e^-g comes to 2^128 at g = -88.7,
+// and the reciprocal instruction keeps no result below 2^-126. So it is off by at most one of its steps wherever
+// e^-g is a number; below, silu(g) (under 3e-37 in size) counts as 0.
+__device__ inline float silu_gate(float g, float v) {
+    return 0.25f * g * __builtin_amdgcn_rcpf(fmaf(0.25f, __expf(-g), 0.25f)) * v;
+}
 
 }  // namespace pyc

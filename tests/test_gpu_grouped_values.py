@@ -1,5 +1,5 @@
 """GPU: values at the ends of what the products by expert take, in every kernel of theirs: NaN and
-infinity through ReLU."""
+infinity through ReLU, gates where e^-g comes near the end of fp32."""
 import math
 
 import pytest
@@ -7,7 +7,7 @@ import torch
 
 import pyc_amd
 from tests import moe_util
-from tests.moe_util import DT, GATE, RELU
+from tests.moe_util import DT, GATE, RELU, U
 
 # (kernel, argument, rows of each expert, N, K) and, 4-bit, the group
 SIXTEEN = [(0, 0, [30, 0, 64, 3], 1008, 63), (1, 1, [30, 0, 64, 3], 1008, 64), (1, 2, [300, 20, 270], 4112, 64),
@@ -62,3 +62,46 @@ def test_relu_keeps_nan(gpu, bits, kind, arg, counts, n, k, group, dtype):
     assert (y[1][:, 3::8] == math.inf).all() and (y[1][:, 6::8] == 0).all()
     for c in (1, 2, 4, 7):
         assert torch.equal(y[0][:, c::8], y[1][:, c::8])
+
+
+def _gates(n):
+    """n gates: all over -100 .. 100, more of them where 1 + e^-g is past 2^126, and odd ones."""
+    odd = [0.0, -0.0, 1e-30, -1e-30, 2.0 ** -126, -(2.0 ** -126), 1e4, -1e4, 3e37, -3e37]
+    a = torch.linspace(-100, 100, (n - len(odd)) // 2, dtype=torch.float64)
+    b = torch.linspace(-88.9, -87.0, n - len(odd) - a.numel(), dtype=torch.float64)
+    return torch.cat([a, b, torch.tensor(odd, dtype=torch.float64)]).float()
+
+
+def _gate_ref(g, v, dtype):
+    """silu(g) v, and how far it may be off: (|g| + 8) U of itself and the output's rounding. Where e^-g
+    leaves fp32, below -88.722, silu(g) counts as 0."""
+    g, v = g.double(), v.double()
+    f = g / (1.0 + torch.exp(-g)) * v
+    d = (g.abs() + 8) * U * f.abs()
+    return f, moe_util.rounded(f, torch.where(g < -88.722, f.abs(), d), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bits,kind,arg,counts,n,k,group", ALL)
+def test_gates_near_the_end_of_fp32(gpu, bits, kind, arg, counts, n, k, group, dtype):
+    """Gates and values by the bias alone (weights of zero). Large values, so that silu of -88 shows."""
+    e, f = len(counts), n // 2
+    gates = _gates(f)
+    x = torch.randint(-2, 3, (sum(counts), k), generator=torch.Generator().manual_seed(n)).to(DT[dtype]).cuda()
+    w = torch.zeros((e, n, k), dtype=DT[dtype], device="cuda") if bits == 16 else [
+        torch.full((e, n, k // 2), 0x88, dtype=torch.uint8, device="cuda"), torch.ones((e, n, k // group), dtype=DT[dtype], device="cuda")]
+    for value in (1.0, -3.0, 1e36):
+        values = torch.where(gates > 80, 1.0, value)  # large ones for small results only
+        bias = torch.cat([gates, values]).expand(e, n).contiguous().cuda()
+        y = torch.full((sum(counts), f), 7.0, dtype=x.dtype, device="cuda")
+        _call(bits, x, w, counts, y, bias=bias, epilogue=GATE)
+        ref, bound = _gate_ref(gates, values, x.dtype)
+        moe_util.check(y, ref.expand(sum(counts), f), bound.expand(sum(counts), f))
+
+
+def test_gate_restatement_by_hand():
+    g, v = torch.tensor([-88.0, -87.4, 0.0, 2.0]), torch.full((4,), 1e36)
+    f, d = _gate_ref(g, v, torch.bfloat16)
+    assert abs(float(f[0]) - -88.0 * math.exp(-88.0) * float(v[0])) < 1e-12
+    assert float(d[0]) < abs(float(f[0])) * 2.0 ** -7 and float(d[1]) < abs(float(f[1])) * 2.0 ** -7  # 0 would not pass
