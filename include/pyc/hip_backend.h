@@ -293,7 +293,8 @@ size_t pyc_hip_kv_attention_workspace(int B, int q_heads, int kv_heads, int head
  *   offsets [experts + 1]  where each expert's rows begin, and how many there are,
  *   rows [tokens * k]      the flat indexes by expert, ascending in each; -1 behind the last,
  *   places [tokens * k]    where f stands in rows, -1 without an expert.
- * 1 <= experts <= 1024, 1 <= k <= min(experts, 64), 0 <= tokens <= 2^22. workspace:
+ * 1 <= experts <= 1024, 1 <= k <= min(experts, 64), 0 <= tokens <= 2^22; above about 2^17 tokens the time
+ * grows with their square (2^20 by 128 experts: 5.4 ms). workspace:
  * pyc_hip_moe_route_workspace bytes on a 4-byte boundary, of any content, for one call at a time
  * (calls that may overlap need one each); up to 64 tokens it may be NULL.
  * Symbols "hip_moe_route_f32", "hip_moe_route_bf16", "hip_moe_route_f16". 0, -1 (bad

@@ -241,8 +241,9 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(Route r) {
     }
 }
 
-// nb blocks to a workgroup. Every workgroup adds up all blocks' words by itself: they are few and in L2, and
-// a third launch would take longer.
+// nb blocks to a workgroup. Every workgroup adds up all blocks' words by itself, which up to 65536 tokens costs less than
+// a third launch: the words (1 MB by 128 experts) stay in L2. That work grows with the square of the tokens and takes over
+// from 2^18 on (by 128 experts, 8 chosen: 2^16 tokens 75 us, 2^17 172, 2^18 479, 2^20 5.4 ms).
 __global__ void __launch_bounds__(kRouteThreads) moe_scatter_kernel(Route r, int blocks, int nb) {
     __shared__ uint32_t own[kScatterMost][kRouteExperts];
     __shared__ int first[kScatterMost + 1][kRouteExperts];
