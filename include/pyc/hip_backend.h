@@ -385,7 +385,9 @@ int pyc_hip_autotune_conv2d(
 
 /* Resources of the kernel a registered symbol launches (at the large shapes
  * its registry entry describes; shape-chosen symbols may launch another kernel
- * for small shapes). The registry's shared_mem_bytes and
+ * for small shapes). The products by expert and with 4-bit weights are described by their
+ * forms of 64 rows and columns; calls of many rows launch tiles of 256 x 256 or 128 x 256, which
+ * take nearly all LDS of a CU and one or two waves a SIMD. The registry's shared_mem_bytes and
  * estimated_occupancy (waves_per_simd / 8) are the compiled-in figures;
  * with a HIP device present the attr_* fields are read from the loaded code
  * object (hipFuncGetAttributes, hipOccupancyMaxActiveBlocksPerMultiprocessor)

@@ -19,6 +19,8 @@
 // Scales and zero points are 2-byte and 1-byte values at any alignment, LDS-DMA moves aligned
 // dwords: the dwords that hold a row's values of the step are fetched (1 to 3, 1 or 2), and the
 // values shifted out of them.
+//
+// The 128 x 256 form's registers are full: 8 to 26 values of a tile's start and end lie in scratch, none of the loop over K.
 #include <type_traits>
 
 #include "grouped.hpp"
