@@ -12,9 +12,9 @@
 // 32 k of them (a group has 32, 64 or 128) are summed apart, then scaled into the sums
 // in fp32. Gated: fragments of a wave alternate, 16 gates and the 16 values of the same
 // columns, so that a lane has both. Rows at odd places are loaded as 16 unaligned bytes; what would
-// cross the end of its row is loaded up to there and shifted. Bound by its loads, two 16-byte pieces of each operand to
-// a thread and step: 256 rows of 64 experts of 2048 x 2816 with x off 16 bytes 196 us (aligned, in the ring, 136), 2048 of
-// 8 of 4096 x 4096 210 (in tiles 139).
+// cross the end of its row is loaded up to there and shifted. Bound by the L1, which 16 unaligned bytes cost more than one
+// access: 2048 rows of 8 experts of 4096 x 4096 with x off 16 bytes take 447 thousand a CU in 444 thousand cycles,
+// 194 us (aligned, in tiles, 112); 256 rows of 64 of 2048 x 2816 191 (in the ring 131).
 #include "grouped.hpp"
 
 namespace pyc {
@@ -214,8 +214,9 @@ extern "C" int pyc_hip_grouped_w4_tile_launch(int is_bf16, const pyc_grouped* g,
 //    4096 x 4096: P = 256 62 / 74, 1024 87 / 98); 256 x 256 tiles from some 200 rows an expert on, or
 //    100 in large calls (8 of 4096 x 4096: P = 2048 111 / 129, 1024 109 / 87; 64 of 2048 x 2816: P = 8192 207 / 292).
 //  4-bit: streamed up to 6 rows an expert (32 of 4096 x 2816: P = 128 60 / 67 in tiles, 256 75 / 71), or where
-//    columns are so few that only parts of K fill the CUs (11008 x 4096: P = 32 27 / 53, 64 48 / 57, 128 81 / 63; 4096 x
-//    11008: P = 16 16.5 / 14.8, 24 25 / 19); then the smallest tiles that are no more than 3 in two places (4096 x 11008: P = 48
+//    columns are so few that only parts of K fill the CUs (11008 x 4096: P = 32 27 / 53, 64 48 / 57, 128 81 / 63), which
+//    takes in wide products of up to 16 rows (4096 x 11008: P = 8 13.2 / 14.5, 12 14.8 / 14.6, 16 15.7 / 14.7, but 24
+//    23.5 / 19.6); then the smallest tiles that are no more than 3 in two places (4096 x 11008: P = 48
 //    25 / 29 in tiles of 16 rows, 128 33 / 54; 11008 x 4096: P = 128 63 / 80 in tiles of 64), and 128 x 256 from 96
 //    rows an expert on where they fill half of the CUs (4096 x 11008: P = 256 66 / 53, 512 69 / 101; 32 of 4096 x
 //    2816: P = 4096 189 / 263; 8 of 2048 x 2048: P = 2048 41 / 46).

@@ -1,6 +1,7 @@
 // grouped_stream.hip — products by expert with 4-bit weights where an expert has few rows: single
 // tokens and decoding batches. What bounds them is the stream of the weights, every byte of
-// which is used once, and the vector instructions that unpack them.
+// which is used once, and with it the waits of the two or three waves a SIMD has for it, between the vector
+// instructions that unpack them (a third of the cycles of a token through 4096 x 11008, 40 % of 23 through 11008 x 4096).
 //
 // A wave has 32 rows of one expert's W (two fragments; gated: of gates, and of the same
 // columns' values) and up to 16 rows of x. The eight waves of a workgroup take `ks` parts of
@@ -9,15 +10,17 @@
 // second launch. W goes from memory into registers as the operand it is, several chunks ahead,
 // through buffer descriptors: rows and k past the end read zeros and cost no traffic.
 //
-// A load instruction costs a wave about 375 cycles here whatever it brings (x, scales and zero
-// points loaded beside W, 10 loads to a chunk: 3700 cycles a chunk). So a wave loads W alone: the rows of x
+// With x, scales and zero points loaded beside W a wave took 3700 cycles for a chunk and its 10 loads (one token
+// through 4096 x 11008: 19 us). So a wave loads W alone: the rows of x
 // and the scales and zero points of the workgroup's columns go through LDS, as much of K at a
 // time as fits. Where x would take turns (each stops all waves), only the scales do, and x is
 // loaded beside W (23 tokens, 11008 x 4096: 42 us in turns, 25 beside).
 //
 // One token through 4096 x 11008: 10.9 us (85 by the general kernel); 16 tokens by 4 of 32 experts of 4096 x 2816:
-// 50 us, 3.9 TB/s (218). Measured and not kept: x and scales loaded four pieces ahead of their way into LDS (12.6 and
-// 56), 16 waves and parts of K (23 tokens, 11008 x 4096: 25 as with eight).
+// 50 us, 3.9 TB/s (218). 23 tokens, 11008 x 4096, groups of 32: 25 us, 11 of them for each half of the depth (two
+// workgroups read and unpack W for the two row tiles); 22 with groups of 128. Measured and not kept: x and scales
+// loaded four pieces ahead of their way into LDS (12.6 and 56), 16 waves and parts of K (23 tokens, 11008 x 4096: 25 as
+// with eight).
 //
 // The rows of x are the first operand: a lane's results are four rows of one column of y, so
 // a column's scale is one value for each lane. A lane's 16 bytes of W are 32 k of a row, the

@@ -16,8 +16,8 @@
 //    buffer's end, which read zeros; rows past the end are stored nowhere the same way.
 //  * Gated: 16 rows of gates and 16 of values alternate in the tile, so a lane holds
 //    both of a column and 128 columns go out.
-// 4096 tokens by 2 of 8 experts of 4096 x 22016, gated: 1280 us, 1.15 PFLOP/s, the matrix units busy 63 % of
-// the cycles (1336 with tiles of 256 rows only, 1315 with the two lists, then a quotient's reciprocal).
+// 4096 tokens by 2 of 8 experts of 4096 x 22016, gated: 1270 to 1320 us over cards, 1.12 to 1.16 PFLOP/s, the matrix
+// units busy 63 % of the cycles (on one card 1285; 1336 with tiles of 256 rows only, 1315 with the two lists, then a quotient's reciprocal).
 // Its registers are full: 16 to 37 values of a tile's start and end lie in scratch, none of the loop over K.
 #include <type_traits>
 

@@ -5,7 +5,8 @@
 // Bound by memory: k rows read for one written. A thread has 16 bytes of a row (eight
 // columns) and loads its k pieces before it adds any. Where a wave lies in one token (width
 // a multiple of 512) its places and weights come by scalar loads. A call with 8200 tokens by
-// 8 rows of 2048 columns: 63 us (74 with vector loads of them), 4.8 TB/s; a large copy reaches 5.1.
+// 8 rows of 2048 columns: 63 us (74 with vector loads of them), 4.8 TB/s; a large copy reaches 5.1. Rows off 16
+// bytes take a thread and 2-byte loads for each column: 225 us, of waiting for 128 bytes to a wave's load.
 #include "common.hpp"
 
 namespace pyc {
