@@ -13,7 +13,7 @@
 // a fifth of the matrix instructions. What bounds it: both kinds of instructions, about half of the cycles each at the
 // 2.0 GHz that the card holds under them, which overlap little (a barrier a step keeps the two waves of a SIMD in
 // phase), and the ends of tiles, 10 us each, where all loads and stores are waited for.
-// 1999 x 11008 x 4096 with groups of 128: 222 to 236 us over cards, 0.76 to 0.81 PFLOP/s (groups of 64 1.18 times that,
+// 1999 x 11008 x 4096 with groups of 128: 222 to 238 us over cards, 0.76 to 0.81 PFLOP/s (groups of 64 1.18 times that,
 // of 32 1.55 times). Measured and not kept: scaling a group among the next one's products (239); the two waves of a SIMD half a
 // step apart, which leaves loads one step instead of two (241); two workgroups of 64 rows a CU (267).
 //
